@@ -702,6 +702,57 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
                          uint16_t* grad_student, const void* workspace, size_t workspace_bytes,
                          int64_t rows, int64_t dim, void* stream);
 
+/* ---- decoding over a paged key-value cache ------------------------------------------- */
+/* A cache is a pool of num_pages pages of page_size tokens (a power of two, 16..1024); one layer's
+ * pages are k_cache bf16 [num_pages, kv_heads, head_dim / 8, page_size, 8] (value d of a token at
+ * [d / 8][token][d % 8]) and v_cache bf16 [num_pages, kv_heads, page_size, head_dim]. Page w of
+ * request b, block_table[b, w] (int32 [batch, width]), holds its tokens w page_size .. ; a slot is
+ * page * page_size + offset. num_pages * page_size, width * page_size, batch * width <= 2^30.
+ * There is no counterpart in the reference, which generates through the HF cache of its models.
+ *
+ * One scheduler step. Request b has lens[b] tokens, keeps the first keep[b] of them (NULL: all)
+ * and adds new_tokens[b] (values out of range are clamped). Its pages past the kept tokens are
+ * pushed onto the stack free_pages [num_pages] (free_count[0] pages before the call), then the
+ * pages for its new tokens are taken off the top, in order of b, and written into block_table, as
+ * long as the stack and the table's width last. lens_out [batch]: the tokens that it has room for
+ * then, keep + new unless pages ran out. The step's token rows follow each other in order of b:
+ * request b has the rows starts[b] .. starts[b + 1] - 1 (starts [batch + 1]; rows past the given
+ * `rows` are cut off), with their positions [rows] and slots [rows] (-1: no room). Rows behind the
+ * last request's get slot -1 and position 0. free_count_out[0]: the pages left. lens_out and
+ * free_count_out may be lens and free_count themselves. */
+int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_tokens,
+                   int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
+                   int32_t* slots, int32_t* positions, int32_t* starts, int32_t* lens_out,
+                   int32_t* free_count_out, int64_t batch, int64_t width, int64_t num_pages,
+                   int64_t rows, int page_size, void* stream);
+/* The rows of a step on their way into the cache: q bf16 [tokens, heads, head_dim], k, v bf16
+ * [tokens, kv_heads, head_dim], consecutive tokens ld_q, ld_k, ld_v elements apart (multiples of 8:
+ * the three may lie side by side in one projection's output), head_dim 64, 128 or 256.
+ * Per-head RMSNorm of q and k with q_weight, k_weight bf16 [head_dim] (both NULL: none), then the
+ * rotation of plz_rope_fwd at the token's position (cos, sin fp32 [max_positions, head_dim]), in
+ * fp32 with one rounding; q_out bf16 [tokens, heads, head_dim], k and v into slots[t] of the cache.
+ * A token whose slot is outside the cache (-1) is stored nowhere; one whose position is outside the
+ * tables neither, and its q_out is NaN. Two tokens of a call must not share a slot. */
+int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t ld_q,
+                         int64_t ld_k, int64_t ld_v, const uint16_t* q_weight,
+                         const uint16_t* k_weight, const float* cos_table, const float* sin_table,
+                         const int32_t* positions, const int32_t* slots, uint16_t* q_out,
+                         uint16_t* k_cache, uint16_t* v_cache, int64_t tokens, int heads,
+                         int kv_heads, int head_dim, int64_t max_positions, int64_t num_pages,
+                         int page_size, float eps, void* stream);
+/* Attention of one new token a request over its lens[b] cached tokens (its own among them): q bf16
+ * [batch, heads, head_dim] (rows ld_q elements apart), o bf16 [batch, heads, head_dim], lse fp32
+ * [batch, heads] = log-sum-exp of the scaled scores; heads % kv_heads == 0, head_dim 64, 128 or
+ * 256. lens[b] <= 0: o = 0, lse = -inf. A request whose length passes width * page_size, or that
+ * needs a page outside [0, num_pages), gives NaN in both; nothing is read past the cache. Values in
+ * the cache behind a request's last token do not matter. Deterministic. */
+size_t plz_paged_attn_workspace(int64_t batch, int heads, int kv_heads, int head_dim);
+int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
+                   const uint16_t* v_cache, const int32_t* block_table, const int32_t* lens,
+                   uint16_t* o, float* lse, void* workspace, size_t workspace_bytes, int64_t batch,
+                   int64_t width, int heads, int kv_heads, int head_dim, int64_t num_pages,
+                   int page_size, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

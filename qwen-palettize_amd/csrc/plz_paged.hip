@@ -1,0 +1,347 @@
+// The paged key-value cache of a decoding batch: who holds which page, and what goes into it.
+//
+// A cache is a pool of pages of P tokens (P a power of two, 16..1024). One layer's pages are
+//   k_cache bf16 [num_pages, kv_heads, D / 8, P, 8]   value d of a token at [d / 8][token][d % 8]
+//   v_cache bf16 [num_pages, kv_heads, P, D]
+// (the order of K: plz_paged_attn.hip). Page w of request b, block_table[b, w], holds its tokens
+// w P .. w P + P - 1; a token's slot is page * P + its offset. The pages that no request holds are
+// a stack: free_pages[0 .. free_count).
+//
+//   paged_step        one scheduler step: pages handed back and taken, block table, slots and
+//                     positions of the step's token rows, all from the requests' lengths
+//   paged_rope_write  per-head RMSNorm and rotation of the rows' q and k, q written out, k and v
+//                     written into their slots
+#include "plz_common.h"
+#include "palettize_hip.h"
+
+namespace plz {
+namespace paged {
+
+// ---- one scheduler step -------------------------------------------------------------------
+// With L = lens[b], k = min(keep[b], L) tokens kept, a = new_tokens[b], pages(n) = ceil(n / P):
+//   request b hands back its pages pages(k) .. pages(L) - 1 (pushed in order of b), then takes
+//   want_b = pages(min(k + a, W P)) - pages(k) pages off the top, in order of b, while they last:
+//   given_b = clamp(pool - sum_{b' < b} want_b', 0, want_b)
+//   lens_out[b] = min(k + a, (pages(k) + given_b) P): what has room; token i of b, row starts[b] + i,
+//   has position k + i and the slot of that position, -1 where there is no room.
+// Everything is a prefix sum over the requests, then independent work a page and a token, which
+// find their request by binary search in the sums. One workgroup walks the requests in chunks of
+// its threads, twice: the pages handed back have to be on the stack before any is taken.
+constexpr int ST = 1024;  // threads, and requests a chunk
+
+struct StepArgs {
+  const int32_t *lens, *keep, *add;
+  int32_t *table, *stack;
+  const int32_t* count;
+  int32_t *slots, *pos, *starts, *lens_out, *count_out;
+  int B, W, F, rows, shift;  // shift = log2 P
+};
+
+// Inclusive sum over the workgroup's threads (no overflow by the entry point's limits); part: one
+// word a wave.
+__device__ __forceinline__ int block_scan(int v, int* part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(v, off);
+    if (lane >= off) v += u;
+  }
+  __syncthreads();  // part's last readers are done
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += part[w];
+  return v;
+}
+
+// The last i in [0, n) with start[i] <= j (start ascending, start[0] <= j)
+__device__ __forceinline__ int find_row(const int* start, int n, int j) {
+  int lo = 0;
+  for (int len = n; len > 1;) {
+    const int half = len >> 1;
+    if (start[lo + half] <= j) {
+      lo += half;
+      len -= half;
+    } else {
+      len = half;
+    }
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// a + b, at most cap, for 0 <= a, b <= cap <= 2^30
+__device__ __forceinline__ int add_cap(int a, int b, int cap) { return min(a + b, cap); }
+
+__device__ __forceinline__ int block_scan_cap(int v, int cap, int* part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(v, off);
+    if (lane >= off) v = add_cap(v, u, cap);
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v = add_cap(v, part[w], cap);
+  return v;
+}
+
+__global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
+  __shared__ int part[ST / 64];
+  __shared__ int s_tok[ST], s_page[ST], s_keep[ST], s_hold[ST], s_len[ST], s_last[2];
+  const int tid = threadIdx.x, P1 = (1 << g.shift) - 1, cap = g.W << g.shift;
+  const int count = clampi(*g.count, 0, g.F);
+  // pages handed back
+  int back = 0;  // by the chunks before
+  for (int b0 = 0; b0 < g.B; b0 += ST) {
+    const int b = b0 + tid, nb = min(ST, g.B - b0);
+    int n = 0;
+    if (b < g.B) {
+      const int L = clampi(g.lens[b], 0, cap), k = g.keep ? clampi(g.keep[b], 0, L) : L;
+      const int hold = (k + P1) >> g.shift;
+      n = ((L + P1) >> g.shift) - hold;
+      s_hold[tid] = hold;
+    }
+    const int end = block_scan(n, part);
+    s_page[tid] = end - n;
+    if (tid == ST - 1) s_last[0] = end;
+    __syncthreads();
+    const int total = s_last[0];
+    for (int j = tid; j < total; j += ST) {
+      const int r = find_row(s_page, nb, j), at = count + back + j;
+      if (at < g.F) g.stack[at] = g.table[(int64_t)(b0 + r) * g.W + s_hold[r] + j - s_page[r]];
+    }
+    back += total;
+    __syncthreads();
+  }
+  const int pool = min(count + back, g.F);
+  // pages taken, lengths, rows
+  int tok0 = 0, want0 = 0;  // rows used and pages asked for by the chunks before
+  for (int b0 = 0; b0 < g.B; b0 += ST) {
+    const int b = b0 + tid, nb = min(ST, g.B - b0);
+    int L = 0, k = 0, a = 0;
+    if (b < g.B) {
+      L = clampi(g.lens[b], 0, cap);
+      k = g.keep ? clampi(g.keep[b], 0, L) : L;
+      a = clampi(g.add[b], 0, g.rows);
+    }
+    const int tok_end = add_cap(tok0, block_scan_cap(a, g.rows, part), g.rows);
+    // the row before: the previous thread's end
+    s_tok[tid] = tok_end;
+    __syncthreads();
+    const int tok = tid ? s_tok[tid - 1] : tok0;
+    a = tok_end - tok;
+    const int hold = (k + P1) >> g.shift;
+    const int full = (int)min((int64_t)k + a, (int64_t)cap);
+    const int want = ((full + P1) >> g.shift) - hold;
+    const int want_end = want0 + block_scan(want, part);
+    const int before = want_end - want;
+    const int given = clampi(pool - before, 0, want);
+    const int len = min(full, (hold + given) << g.shift);
+    __syncthreads();  // s_tok has been read
+    s_tok[tid] = tok;
+    s_page[tid] = before;
+    s_keep[tid] = k;
+    s_hold[tid] = hold;
+    s_len[tid] = len;
+    if (tid == ST - 1) {
+      s_last[0] = tok_end;
+      s_last[1] = want_end;
+    }
+    if (b < g.B) {
+      g.lens_out[b] = len;
+      g.starts[b + 1] = tok_end;
+    }
+    __syncthreads();
+    const int tok1 = s_last[0], want1 = s_last[1];
+    for (int j = want0 + tid; j < min(want1, pool); j += ST) {
+      const int r = find_row(s_page, nb, j);
+      g.table[(int64_t)(b0 + r) * g.W + s_hold[r] + j - s_page[r]] = g.stack[pool - 1 - j];
+    }
+    for (int t = tok0 + tid; t < tok1; t += ST) {
+      const int r = find_row(s_tok, nb, t), pos = s_keep[r] + t - s_tok[r];
+      int slot = -1;
+      if (pos < s_len[r]) {
+        const int w = pos >> g.shift;
+        const int page = w < s_hold[r] ? g.table[(int64_t)(b0 + r) * g.W + w]
+                                       : g.stack[pool - 1 - (s_page[r] + w - s_hold[r])];
+        if (page >= 0 && page < g.F) slot = (page << g.shift) + (pos & P1);
+      }
+      g.slots[t] = slot;
+      g.pos[t] = pos;
+    }
+    tok0 = tok1;
+    want0 = want1;
+    __syncthreads();
+  }
+  for (int t = tok0 + tid; t < g.rows; t += ST) {
+    g.slots[t] = -1;
+    g.pos[t] = 0;
+  }
+  if (tid == 0) {
+    g.starts[0] = 0;
+    *g.count_out = pool - min(pool, want0);
+  }
+}
+
+// ---- norm, rotation, write --------------------------------------------------------------------
+// A row (token t, head) of D values: n = x rsqrt(mean(x^2) + eps) w (w NULL: n = x), then
+//   y_j = n_j cos[p, j] - n_{j + D/2} sin[p, j]  (j < D/2),   n_j cos[p, j] + n_{j - D/2} sin[p, j]
+// at the token's position p, all in fp32 and rounded once to bf16 (the training layers' norm and
+// rotation round the normalised and the weighted value too, as the modules that they stand for do:
+// here there is no such module to match). D / 8 lanes a row, 8 values a lane; the partner of value
+// j is in lane l ^ (D / 16).
+struct WriteArgs {
+  const uint16_t *q, *k, *v, *qw, *kw;
+  const float *cosv, *sinv;
+  const int32_t *pos, *slots;
+  uint16_t *q_out, *kc, *vc;
+  int64_t T, ldq, ldk, ldv;
+  int H, Hkv, max_pos, shift;
+  int64_t slots_end;  // num_pages * P
+  float eps;
+};
+
+template <int LPR>
+__global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
+  constexpr int D = 8 * LPR, RPW = 64 / LPR, TB = 4 * RPW;  // tokens a workgroup
+  const int lane = threadIdx.x & 63, l = lane % LPR;
+  const int64_t t = (int64_t)blockIdx.x * TB + (threadIdx.x >> 6) * RPW + lane / LPR;
+  const int head = blockIdx.y;  // 0..H-1 q, then Hkv k, then Hkv v
+  const bool valid = t < g.T;
+  const int64_t tt = valid ? t : 0;
+  const int slot = g.slots[tt], p = g.pos[tt];
+  const bool placed = p >= 0 && p < g.max_pos;  // else nothing is stored, and q is NaN
+  const bool stored = valid && placed && slot >= 0 && slot < g.slots_end;
+  const int kind = head < g.H ? 0 : head < g.H + g.Hkv ? 1 : 2;
+  const int h = kind == 0 ? head : kind == 1 ? head - g.H : head - g.H - g.Hkv;
+  const uint16_t* src = kind == 0 ? g.q + tt * g.ldq : kind == 1 ? g.k + tt * g.ldk : g.v + tt * g.ldv;
+  const uint4 xv = reinterpret_cast<const uint4*>(src + (int64_t)h * D)[l];
+  const int64_t page = stored ? slot >> g.shift : 0;
+  const int64_t at = stored ? slot & ((1 << g.shift) - 1) : 0;
+  const int64_t block = page * g.Hkv + h;  // of D * P values
+  if (kind == 2) {
+    if (stored) reinterpret_cast<uint4*>(g.vc)[((block << g.shift) + at) * LPR + l] = xv;
+    return;
+  }
+  float f[8];
+  unpack8(xv, f);
+  const uint16_t* wt = kind == 0 ? g.qw : g.kw;
+  if (wt) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+#pragma unroll
+    for (int off = LPR / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
+    const float r = rsqrtf(ss * (1.f / D) + g.eps);
+    float w[8];
+    unpack8(reinterpret_cast<const uint4*>(wt)[l], w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
+  }
+  const int64_t row = (int64_t)(placed ? p : 0) * D + 8 * l;
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float other = __shfl_xor(f[j], LPR / 2);
+    const float c = g.cosv[row + j], s = g.sinv[row + j];
+    o[j] = l < LPR / 2 ? f[j] * c - other * s : f[j] * c + other * s;
+    if (!placed) o[j] = __builtin_nanf("");
+  }
+  const uint4 out = pack8(o);
+  if (kind == 0) {
+    if (valid) reinterpret_cast<uint4*>(g.q_out + (tt * g.H + h) * D)[l] = out;
+  } else if (stored) {
+    reinterpret_cast<uint4*>(g.kc)[((block * LPR + l) << g.shift) + at] = out;
+  }
+}
+
+static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace paged
+}  // namespace plz
+
+using namespace plz;
+using namespace plz::paged;
+
+extern "C" {
+
+int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_tokens,
+                   int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
+                   int32_t* slots, int32_t* positions, int32_t* starts, int32_t* lens_out,
+                   int32_t* free_count_out, int64_t batch, int64_t width, int64_t num_pages,
+                   int64_t rows, int page_size, void* stream) {
+  PLZ_REQUIRE(batch >= 0 && width >= 0 && num_pages >= 0 && rows >= 0,
+              "plz_paged_step: negative shape");
+  PLZ_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+              "plz_paged_step: page_size must be a power of two of 16 to 1024, got %d", page_size);
+  const int64_t lim = (int64_t)1 << 30;
+  PLZ_REQUIRE(batch <= lim && width <= lim && num_pages <= lim && rows <= lim &&
+                  batch * width <= lim && width * page_size <= lim &&
+                  num_pages * page_size <= lim,
+              "plz_paged_step: batch x width, width x page_size, num_pages x page_size and rows "
+              "go up to 2^30");
+  PLZ_REQUIRE(free_count && free_count_out && starts && (num_pages == 0 || free_pages) &&
+                  (batch == 0 || (lens && new_tokens && lens_out)) &&
+                  (batch * width == 0 || block_table) && (rows == 0 || (slots && positions)),
+              "plz_paged_step: null pointer");
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  const StepArgs g{lens,  keep,   new_tokens, block_table,    free_pages, free_count, slots,
+                   positions, starts, lens_out,   free_count_out, (int)batch, (int)width,
+                   (int)num_pages, (int)rows, shift};
+  hipLaunchKernelGGL(step_kernel, dim3(1), dim3(ST), 0, (hipStream_t)stream, g);
+  return check_launch("plz_paged_step");
+}
+
+int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t ld_q,
+                         int64_t ld_k, int64_t ld_v, const uint16_t* q_weight,
+                         const uint16_t* k_weight, const float* cos_table, const float* sin_table,
+                         const int32_t* positions, const int32_t* slots, uint16_t* q_out,
+                         uint16_t* k_cache, uint16_t* v_cache, int64_t tokens, int heads,
+                         int kv_heads, int head_dim, int64_t max_positions, int64_t num_pages,
+                         int page_size, float eps, void* stream) {
+  const char* const what = "plz_paged_rope_write";
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+    set_error("%s: head_dim %d is not supported (64, 128 or 256)", what, head_dim);
+    return PLZ_EUNSUPPORTED;
+  }
+  PLZ_REQUIRE(tokens >= 0 && heads > 0 && kv_heads > 0 && max_positions > 0 && num_pages > 0,
+              "%s: need tokens >= 0 and heads, kv_heads, positions and pages", what);
+  PLZ_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+              "%s: page_size must be a power of two of 16 to 1024, got %d", what, page_size);
+  const int64_t lim = (int64_t)1 << 30;
+  PLZ_REQUIRE(tokens <= lim && heads <= 16384 && kv_heads <= 16384 && max_positions <= lim &&
+                  num_pages <= lim && num_pages * page_size <= lim,
+              "%s: tokens, positions and num_pages x page_size go up to 2^30, heads to 16384", what);
+  if (tokens == 0) return PLZ_OK;
+  PLZ_REQUIRE(ld_q >= (int64_t)heads * head_dim && ld_k >= (int64_t)kv_heads * head_dim &&
+                  ld_v >= (int64_t)kv_heads * head_dim && ld_q % 8 == 0 && ld_k % 8 == 0 &&
+                  ld_v % 8 == 0,
+              "%s: a row pitch is a multiple of 8 and at least the heads' width", what);
+  PLZ_REQUIRE((q_weight == nullptr) == (k_weight == nullptr),
+              "%s: q_weight and k_weight go together", what);
+  PLZ_REQUIRE(q && k && v && cos_table && sin_table && positions && slots && q_out && k_cache &&
+                  v_cache,
+              "%s: null pointer", what);
+  PLZ_REQUIRE(a16(q) && a16(k) && a16(v) && a16(q_weight) && a16(k_weight) && a16(cos_table) &&
+                  a16(sin_table) && a16(q_out) && a16(k_cache) && a16(v_cache),
+              "%s: operands must be 16-byte aligned", what);
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  const WriteArgs g{q,     k,      v,   q_weight, k_weight, cos_table, sin_table, positions,
+                    slots, q_out, k_cache, v_cache, tokens, ld_q, ld_k, ld_v,
+                    heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps};
+  const int lpr = head_dim / 8, tb = 4 * (64 / lpr);
+  const dim3 grid((unsigned)((tokens + tb - 1) / tb), (unsigned)(heads + 2 * kv_heads));
+  if (lpr == 8)
+    hipLaunchKernelGGL((rope_write_kernel<8>), grid, dim3(256), 0, (hipStream_t)stream, g);
+  else if (lpr == 16)
+    hipLaunchKernelGGL((rope_write_kernel<16>), grid, dim3(256), 0, (hipStream_t)stream, g);
+  else
+    hipLaunchKernelGGL((rope_write_kernel<32>), grid, dim3(256), 0, (hipStream_t)stream, g);
+  return check_launch(what);
+}
+
+}  // extern "C"

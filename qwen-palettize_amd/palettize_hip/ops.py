@@ -1164,3 +1164,160 @@ def attn_bwd(q, k, v, o, lse, grad_o, scale=None):
     call("plz_attn_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(grad_o), _ptr(lse), _ptr(gq),
          _ptr(gk), _ptr(gv), _ptr(ws), _numel(ws), B, S, Hq, Hkv, D, scale, _stream(q))
     return gq, gk, gv
+
+
+# ---- decoding over a paged key-value cache -----------------------------------------------------
+def _on(t, others, name, *args):
+    """call() on the device of t, with its current stream last; every tensor of others is on it."""
+    dev = t.get_device()
+    for x in others:
+        if x is not None and x.get_device() != dev:
+            raise ValueError(f"{name}: the tensors are on different devices")
+    if torch._C._cuda_getDevice() == dev:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _ints(t, name, *shape):
+    """An int32 GPU tensor of that shape."""
+    _need(t, name, torch.int32, len(shape))
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    return t
+
+
+def paged_cache(num_pages, page_size, kv_heads, head_dim, device):
+    """(k_cache, v_cache) of one layer, zeros: bf16 [num_pages, kv_heads, head_dim / 8, page_size, 8]
+    and [num_pages, kv_heads, page_size, head_dim]."""
+    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two of 16 to 1024, got {page_size}")
+    if head_dim not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+    kw = dict(dtype=torch.bfloat16, device=device)
+    return (torch.zeros(num_pages, kv_heads, head_dim // 8, page_size, 8, **kw),
+            torch.zeros(num_pages, kv_heads, page_size, head_dim, **kw))
+
+
+def _paged_caches(k_cache, v_cache):
+    """(num_pages, kv_heads, page_size, head_dim) of a layer's cache."""
+    _need(k_cache, "k_cache", torch.bfloat16, 5)
+    _need(v_cache, "v_cache", torch.bfloat16, 4)
+    n, hkv, P, D = v_cache.shape
+    if tuple(k_cache.shape) != (n, hkv, D // 8, P, 8) or D % 8:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must be "
+                         "[pages, kv_heads, head_dim / 8, page_size, 8] and "
+                         "[pages, kv_heads, page_size, head_dim]")
+    return n, hkv, P, D
+
+
+def _token_rows(t, name, heads=None, dim=None):
+    """The pitch of bf16 rows [tokens, heads, head_dim] whose heads are dense (a slice of a
+    projection's output is fine)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not _on_gpu(t):
+        raise RuntimeError(f"{name} must be a GPU tensor (palettize_hip has no CPU path)")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be 3-D, got shape {tuple(t.shape)}")
+    T, H, D = t.shape
+    if (heads is not None and H != heads) or (dim is not None and D != dim):
+        raise ValueError(f"{name} {tuple(t.shape)} does not match {heads or H} heads of {dim or D}")
+    st, sh, sd = t.stride()
+    if (sd != 1 and D > 1) or (sh != D and H > 1):
+        raise ValueError(f"the heads of {name} must be dense")
+    return st if T > 1 else H * D
+
+
+def paged_step(lens, new_tokens, block_table, free_pages, free_count, page_size, keep=None,
+               rows=None, lens_out=None, free_count_out=None):
+    """One scheduler step of a paged cache: pages handed back and taken, and where the step's
+    tokens go (plz_paged_step).
+
+    lens, new_tokens, keep (optional) int32 [B]: the tokens each request has, adds and keeps of what
+    it has (None: all; 0 ends a request and frees its row). block_table int32 [B, W] and free_pages
+    int32 [num_pages], the stack of the pages that nobody holds, are updated in place; free_count
+    int32 [1] of them are valid. rows: the size of the token buffer (default B: one token each).
+    Returns (slots [rows], positions [rows], starts [B + 1], lens [B], free_count [1]); lens_out and
+    free_count_out receive the last two (lens and free_count themselves may be given). A request
+    that finds no page keeps the tokens that have room, and the others get slot -1."""
+    _need(lens, "lens", torch.int32, 1)
+    B = lens.shape[0]
+    _ints(new_tokens, "new_tokens", B)
+    if keep is not None:
+        _ints(keep, "keep", B)
+    _need(block_table, "block_table", torch.int32, 2)
+    if block_table.shape[0] != B:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
+    _need(free_pages, "free_pages", torch.int32, 1)
+    _ints(free_count, "free_count", 1)
+    rows = B if rows is None else int(rows)
+    if rows < 0:
+        raise ValueError(f"rows must not be negative, got {rows}")
+    dev = lens.device
+    out = torch.empty(2 * rows + 2 * B + 2, dtype=torch.int32, device=dev)
+    slots, positions, starts, own_lens, own_count = out.split((rows, rows, B + 1, B, 1))
+    lens_out = own_lens if lens_out is None else _ints(lens_out, "lens_out", B)
+    free_count_out = (own_count if free_count_out is None
+                      else _ints(free_count_out, "free_count_out", 1))
+    _on(lens, (new_tokens, keep, block_table, free_pages, free_count, lens_out, free_count_out),
+        "plz_paged_step", _ptr(lens), _ptr(keep), _ptr(new_tokens), _ptr(block_table),
+        _ptr(free_pages), _ptr(free_count), _ptr(slots), _ptr(positions), _ptr(starts),
+        _ptr(lens_out), _ptr(free_count_out), B, block_table.shape[1], free_pages.shape[0], rows,
+        int(page_size))
+    return slots, positions, starts, lens_out, free_count_out
+
+
+def paged_rope_write(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_weight=None,
+                     k_weight=None, eps=1e-6):
+    """q [T, H, D], k, v [T, Hkv, D] (bf16, dense heads, any row pitch that is a multiple of 8)
+    through per-head RMSNorm (q_weight, k_weight bf16 [D], or neither) and the rotation at each
+    token's position (cos, sin fp32 [max_positions, D]): returns q [T, H, D]; k and v go into
+    slots [T] of the cache in place (plz_paged_rope_write). Tokens with slot -1 are stored nowhere."""
+    n, hkv, P, D = _paged_caches(k_cache, v_cache)
+    ldq = _token_rows(q, "q", None, D)
+    T, H = q.shape[0], q.shape[1]
+    ldk, ldv = _token_rows(k, "k", hkv, D), _token_rows(v, "v", hkv, D)
+    if k.shape[0] != T or v.shape[0] != T:
+        raise ValueError("q / k / v have different numbers of tokens")
+    for t, nm in ((cos, "cos"), (sin, "sin")):
+        _need(t, nm, torch.float32, 2)
+    if cos.shape != sin.shape or cos.shape[1] != D:
+        raise ValueError(f"cos and sin must be [positions, {D}]")
+    _ints(positions, "positions", T)
+    _ints(slots, "slots", T)
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight must be given together")
+    if q_weight is not None:
+        _norm_weight(q_weight, D)
+        _norm_weight(k_weight, D)
+    out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+    _on(q, (k, v, cos, sin, positions, slots, k_cache, v_cache, q_weight, k_weight),
+        "plz_paged_rope_write", _ptr(q), _ptr(k), _ptr(v), ldq, ldk, ldv, _ptr(q_weight),
+        _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots), _ptr(out),
+        _ptr(k_cache), _ptr(v_cache), T, H, hkv, D, cos.shape[0], n, P, float(eps))
+    return out
+
+
+def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
+    """Attention of one new token a request over its cached tokens: q [B, H, D] (bf16, dense heads),
+    block_table int32 [B, W], lens int32 [B] (the new token's own included) -> (o [B, H, D] bf16,
+    lse [B, H] fp32) (plz_paged_attn). Requests without tokens give 0 and -inf."""
+    n, hkv, P, D = _paged_caches(k_cache, v_cache)
+    ldq = _token_rows(q, "q", None, D)
+    B, H = q.shape[0], q.shape[1]
+    _need(block_table, "block_table", torch.int32, 2)
+    if block_table.shape[0] != B:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
+    _ints(lens, "lens", B)
+    scale = D ** -0.5 if scale is None else float(scale)
+    o = torch.empty((B, H, D), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=q.device)
+    ws = _opt_workspace(query("plz_paged_attn_workspace", B, H, hkv, D), q.device)
+    _on(q, (k_cache, v_cache, block_table, lens), "plz_paged_attn", _ptr(q), ldq, _ptr(k_cache),
+        _ptr(v_cache), _ptr(block_table), _ptr(lens), _ptr(o), _ptr(lse), _ptr(ws), _numel(ws), B,
+        block_table.shape[1], H, hkv, D, n, P, scale)
+    return o, lse

@@ -3,6 +3,7 @@ call reaches a GPU), and the references that the GPU tests use against each othe
 import importlib.util
 import os
 import random
+import subprocess
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ import torch
 import paged_ref
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FAKE = 4096  # an aligned address that is never read: a check fails first
 
 
@@ -82,7 +84,8 @@ def _attn_args(lib, **kw):
     (dict(heads=0), 1, b"heads"), (dict(kv=0), 1, b"heads"), (dict(heads=9), 1, b"multiple"),
     (dict(pages=0), 1, b"pages"), (dict(page=17), 1, b"power of two"), (dict(page=8), 1, b"power"),
     (dict(batch=65537), 1, b"65536"), (dict(width=1 << 27), 1, b"2^30"),
-    (dict(pages=1 << 27), 1, b"2^30"), (dict(scale=0.0), 1, b"scale"),
+    (dict(pages=1 << 27), 1, b"2^30"), (dict(batch=1 << 16, width=1 << 16), 1, b"2^35"),
+    (dict(scale=0.0), 1, b"scale"),
     (dict(scale=float("nan")), 1, b"scale"), (dict(ldq=1000), 1, b"pitch"),
     (dict(ldq=1028), 1, b"pitch"), (dict(q=None), 1, b"null"), (dict(lens=None), 1, b"null"),
     (dict(table=None), 1, b"null"), (dict(o=None), 1, b"null"), (dict(lse=None), 1, b"null"),
@@ -230,6 +233,29 @@ def test_calls_run_on_their_tensors_device(monkeypatch):
         o._on(t, (t, None), "plz_paged_attn", 7)
     assert log == [(("plz_paged_attn", 7, 100), 0), (("plz_paged_attn", 7, 101), 1)]
     assert current == [0]
+
+
+def test_attn_needs_its_workspace(lib):
+    need = lib.plz_paged_attn_workspace(3, 8, 2, 128)
+    assert need > 0
+    for kw in (dict(ws=None), dict(nws=need - 1), dict(ws=FAKE + 8)):
+        assert lib.plz_paged_attn(*_attn_args(lib, **kw)) == 4
+        assert b"workspace" in lib.plz_last_error()
+    for args in ((0, 8, 2, 128), (3, 0, 2, 128), (3, 8, 0, 128), (3, 9, 2, 128), (3, 8, 2, 0)):
+        assert lib.plz_paged_attn_workspace(*args) == 0
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not available")
+def test_tokens_are_dealt_once(tmp_path):
+    exe = tmp_path / "paged_check"
+    cmd = [HIPCC, "--offload-arch=gfx950", "-O1", "-g", "-std=c++17",
+           "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "qwen-palettize_amd", "csrc"),
+           os.path.join(ROOT, "tests", "native", "paged_check.hip"), "-o", str(exe)]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, (r.stdout + r.stderr)[-3000:]
+    assert "checks passed" in r.stdout
 
 
 # ---- the references against each other -------------------------------------------------------------

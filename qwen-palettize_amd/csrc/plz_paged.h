@@ -16,20 +16,30 @@ __host__ __device__ __forceinline__ int tiles_of(int len, int cap) {
   return len <= 0 || len > cap ? 0 : (len + TILE - 1) / TILE;
 }
 
-// The tiles of all requests, one behind the other (`total` of them), are cut into `parts` runs of equal
-// length, one a workgroup: a long request is shared by many, a workgroup takes several short ones.
-// No run is shorter than one tile a wave (`waves`).
-__host__ __device__ __forceinline__ int run_count(int total, int parts, int waves) {
-  const int n = (total + waves - 1) / waves;
-  return n < parts ? n : parts;
+// The tiles of all requests, one behind the other (`total` of them), are cut into runs of equal length
+// (the first `rem` one tile longer), one a wave: a long request is shared by many waves, a wave takes
+// several short ones. Runs are numbered through the workgroups, `waves` in each.
+struct Deal {
+  int runs, q, rem;
+};
+__host__ __device__ __forceinline__ Deal deal(int total, int most) {
+  const int runs = total < most ? total : most;
+  const int q = runs > 0 ? total / runs : 0;
+  return Deal{runs, q, total - q * runs};
 }
-__host__ __device__ __forceinline__ int run_begin(int total, int runs, int w) {
-  return (int)((int64_t)total * w / runs);
+__host__ __device__ __forceinline__ int run_begin(Deal d, int i) {
+  return i * d.q + (i < d.rem ? i : d.rem);
 }
-// the run that holds tile p: the largest w with run_begin(w) <= p
-__host__ __device__ __forceinline__ int run_of(int total, int runs, int p) {
-  return (int)((((int64_t)p + 1) * runs + total - 1) / total) - 1;
+// the run that holds tile p
+__host__ __device__ __forceinline__ int run_of(Deal d, int p) {
+  const int longer = d.rem * (d.q + 1);
+  return p < longer ? p / (d.q + 1) : d.rem + (p - longer) / d.q;
 }
+
+// What a run has of a request: from tile 0 or from later on (CARRIED, then it is the run's first), to
+// its last tile or not. Parts that are not whole are left for others to join: the part of a carried
+// request in place 0, that of one which begins here and ends elsewhere in place 1.
+__host__ __device__ __forceinline__ int place_of(bool carried) { return carried ? 0 : 1; }
 
 }  // namespace paged
 }  // namespace plz

@@ -21,9 +21,10 @@
 // error as the output's own rounding, and the matrix pipe has the room. The running maximum of a head
 // moves only when a tile exceeds it by more than 2^8.
 //
-// The four waves of a workgroup share a run of tiles (plz_paged.h) and join through LDS; runs that
-// share a request leave their maximum, sum and unscaled output in the workspace, and a second kernel
-// joins those in the order of the runs.
+// Each wave has a run of tiles (plz_paged.h) and goes through its requests without a word to the
+// others; the next request's length, pages and queries are on their way while it is at this one. Only
+// what a run has of a request that it does not have whole is joined: through LDS among the waves of a
+// workgroup, through the workspace among workgroups, by a second kernel, both in the order of the runs.
 #include "plz_paged.h"
 #include "palettize_hip.h"
 
@@ -40,21 +41,21 @@ struct AttnArgs {
   const int32_t *table, *lens;
   uint16_t* o;
   float *lse, *part;
-  int2* shared;  // [parts]: of run w, {the request that it begins and does not finish or -1, its last run}
+  int2* open;  // [parts] of workgroup w: {the request that it begins and does not finish or -1, the
+               // workgroup that does}
   int64_t ldq;
   int B, W, Hq, Hkv, G, tiles_h, parts, num_pages, shift;  // tiles_h = head tiles a kv head
   float scale_log2;
 };
 
-// one partial result: heads x D values, then the heads' maxima (log2 units) and sums
-__host__ __device__ __forceinline__ int64_t part_floats(int heads, int D) {
-  return ((int64_t)heads * (D + 2) + 3) / 4 * 4;
+// A partial result: heads x D values, then the heads' maxima (log2 units) and sums
+__host__ __device__ __forceinline__ int part_floats(int heads, int D) {
+  return (heads * (D + 2) + 3) / 4 * 4;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Tiles of the requests before request `b0` of this thread's share (k consecutive requests from
-// threadIdx.x * k), and of all: inclusive sums over the workgroup.
+// Exclusive sum of v over the workgroup's threads, and the total
 __device__ __forceinline__ int scan_tiles(int v, int* part, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int s = v;
@@ -75,18 +76,23 @@ __device__ __forceinline__ int scan_tiles(int v, int* part, int& total) {
   return before + s - v;
 }
 
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+enum { HAS_CARRIED = 1, CARRIED_ENDS = 2, HAS_OPEN = 4 };  // a wave's parts
+
 template <int D>
 __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnArgs g) {
   constexpr int KS = D / 32, VEC = D / 16, VDW = VEC / 2;
-  __shared__ int s_part[NW], s_empty[NW], s_at[2];
-  __shared__ float s_m[NW][HT], s_l[NW][HT];
-  __shared__ float s_o[NW][HT][D];
+  extern __shared__ f32x4 s_res[];  // partial results, [wave][place]
+  __shared__ int s_part[NW], s_empty[NW], s_b[NW], s_first[NW], s_has[NW], s_req[NW][2], s_last[NW];
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int P = 1 << g.shift, cap = g.W << g.shift;
 
-  // this workgroup's run of tiles, kv head and head tile; the head tiles of one run (the same K and
-  // V) sit side by side on one XCD (id % 8)
+  // the head tiles of one workgroup number (the same K and V) sit side by side on one XCD (id % 8)
   int w, hk, ht;
   {
     const int id = (int)blockIdx.x, per = 8 * g.tiles_h, pair = id / per * 8 + id % 8;
@@ -96,6 +102,10 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   }
   if (w >= g.parts) return;  // the last eighth's padding
   const int h0 = ht * HT, nh = min(g.G - h0, HT);  // heads hk G + h0 .. + nh - 1
+  const int slot = part_floats(min(g.G, HT), D);
+  float* const res = reinterpret_cast<float*>(s_res) + wave * 2 * slot;
+
+  // every request's tiles, and where the workgroup's runs begin among them
   const int per_thread = (g.B + NT - 1) / NT, b0 = threadIdx.x * per_thread;
   int mine = 0;
   bool none = false;
@@ -104,92 +114,80 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     mine += n;
     none |= n == 0;
   }
-  if (lane == 0) s_empty[wave] = 0;
-  if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) s_empty[wave] = 1;
+  none = __builtin_amdgcn_ballot_w64(none) != 0;
+  if (lane == 0) {
+    s_empty[wave] = none;
+    s_has[wave] = 0;
+  }
   int total;
-  int pre = scan_tiles(mine, s_part, total);
-  const int runs = run_count(total, g.parts, NW);
-  int open = -1, open_last = 0;  // the request that this run begins and does not finish, its last run
-  if (w < runs) {
-  const int r0 = run_begin(total, runs, w), r1 = run_begin(total, runs, w + 1);
-  if (pre <= r0 && r0 < pre + mine) {
-    int b = b0;
-    for (;; ++b) {
-      const int n = tiles_of(g.lens[b], cap);
-      if (r0 < pre + n) break;
-      pre += n;
+  const int pre = scan_tiles(mine, s_part, total);
+  const Deal runs = deal(total, g.parts * NW);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int at = run_begin(runs, w * NW + i);
+    if (pre <= at && at < pre + mine) {
+      int b = b0, before = pre;
+      for (; b < g.B - 1; ++b) {  // the bound: lens may change under a caller's race, not past it
+        const int n = tiles_of(g.lens[b], cap);
+        if (at < before + n) break;
+        before += n;
+      }
+      s_b[i] = b;
+      s_first[i] = before;
     }
-    s_at[0] = b;
-    s_at[1] = pre;
   }
   __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(s_at[0]);
-  int first = __builtin_amdgcn_readfirstlane(s_at[1]);  // request b's first tile among all
-  const uint32_t koff = (uint32_t)(grp * P + col) * 16;
-  const uint32_t voff = (uint32_t)(4 * grp * D + col * VEC) * 2;
-  const int64_t page_bytes = (int64_t)D * 2 << g.shift;  // of one kv head
 
-  for (;; ++b) {
-    const int len = g.lens[b], n = tiles_of(len, cap);
-    if (n == 0) continue;
-    const int t0 = max(r0 - first, 0), t1 = min(r1 - first, n);
-    const int32_t* row = g.table + (int64_t)b * g.W;
+  if (w * NW + wave < runs.runs) {
+    const int r0 = run_begin(runs, w * NW + wave), r1 = run_begin(runs, w * NW + wave + 1);
+    int b = __builtin_amdgcn_readfirstlane(s_b[wave]);
+    int first = __builtin_amdgcn_readfirstlane(s_first[wave]);  // its first tile among all
+    int len = g.lens[b], n = tiles_of(len, cap);
+    const uint32_t koff = (uint32_t)(grp * P + col) * 16;
+    const uint32_t voff = (uint32_t)(4 * grp * D + col * VEC) * 2;
+    const int64_t page_bytes = (int64_t)D * 2 << g.shift;  // of one kv head
 
-    // the heads' queries (columns past nh: zeros)
-    bf16x8 qf[KS];
-    {
-      const uint16_t* qp = g.q + b * g.ldq + (int64_t)(hk * g.G + h0 + min(col, nh - 1)) * D + 8 * grp;
+    // lane 2 j + half: the page of that half of tile t + j of request `req`
+    auto fetch_pages = [&](int req, int t, int tokens, int tiles) {
+      const int tile = t + (lane >> 1);
+      int tok = tile * TILE + (lane & 1) * 16;
+      if (tok >= tokens) tok -= 16;  // a second half without tokens: the first one's page
+      return tile < tiles ? g.table[(int64_t)req * g.W + (tok >> g.shift)] : 0;
+    };
+    // pages outside the cache become page 0, which exists; whether there were any
+    auto check_pages = [&](int& pages) {
+      const bool out = (uint32_t)pages >= (uint32_t)g.num_pages;
+      if (out) pages = 0;
+      return __builtin_amdgcn_ballot_w64(out) != 0;
+    };
+    u32x4 kr[2][KS], qf[KS], qn[KS];
+    uint32_t vr[8][VDW];
+    auto load_q = [&](int req, u32x4(&to)[KS]) {  // columns past nh: zeros
+      const uint16_t* qp =
+          g.q + req * g.ldq + (int64_t)(hk * g.G + h0 + min(col, nh - 1)) * D + 8 * grp;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        uint4 x = *reinterpret_cast<const uint4*>(qp + 32 * s);
-        if (col >= nh) x = make_uint4(0, 0, 0, 0);
-        qf[s] = __builtin_bit_cast(bf16x8, x);
+        to[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
+        if (col >= nh) to[s] = u32x4{};
       }
-    }
-    f32x4 acc[VEC];
-    float mrun, neg, lrun;  // maximum (log2 units), -maximum (0 for -inf), this lane's sum
-    bool bad = false;
-
-    u32x4 kr[2][KS];
-    uint32_t vr[8][VDW];
-    int pages = 0;  // lane 2 j + half: the page of half of this wave's j-th tile from jbase
-    int jbase = 0;
-    auto fetch_pages = [&](int j0) {
-      jbase = j0;
-      const int tile = t0 + wave + NW * (j0 + (lane >> 1));
-      int tok = tile * TILE + (lane & 1) * 16;
-      if (tok >= len) tok -= 16;  // a second half without tokens: the first one's page
-      pages = 0;
-      if (tile < t1) {
-        pages = row[tok >> g.shift];
-        if ((uint32_t)pages >= (uint32_t)g.num_pages) {
-          bad = true;
-          pages = 0;
-        }
-      }
-      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
     };
-    auto load_k = [&](int j) {
-      const int tok = (t0 + wave + NW * j) * TILE;
+    auto load_k = [&](int page0, int page1, int tile) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int page = __builtin_amdgcn_readlane(pages, 2 * (j - jbase) + half);
-        const int at = (tok + 16 * half) & (P - 1);
         const char* base = reinterpret_cast<const char*>(g.kc) +
-                           ((int64_t)page * g.Hkv + hk) * page_bytes + (int64_t)at * 16;
+                           ((int64_t)(half ? page1 : page0) * g.Hkv + hk) * page_bytes +
+                           (int64_t)((tile * TILE + 16 * half) & (P - 1)) * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
           kr[half][s] = *reinterpret_cast<const u32x4*>(base + (int64_t)s * 64 * P + koff);
       }
     };
-    auto load_v = [&](int j) {
-      const int tok = (t0 + wave + NW * j) * TILE;
+    auto load_v = [&](int page0, int page1, int tile) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int page = __builtin_amdgcn_readlane(pages, 2 * (j - jbase) + half);
-        const int at = (tok + 16 * half) & (P - 1);
         const char* base = reinterpret_cast<const char*>(g.vc) +
-                           ((int64_t)page * g.Hkv + hk) * page_bytes + (int64_t)at * D * 2;
+                           ((int64_t)(half ? page1 : page0) * g.Hkv + hk) * page_bytes +
+                           (int64_t)((tile * TILE + 16 * half) & (P - 1)) * D * 2;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           uint32_t(&d)[VDW] = vr[4 * half + t];
@@ -207,50 +205,109 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         }
       }
     };
-
-    const int nj = (t1 - t0 - wave + NW - 1) / NW;  // this wave's tiles (<= 0: none)
-    // once; where that leaves NaN (an infinite value times the two pieces of its weight, of which the
-    // second may be 0 or of the other sign) again with the first pieces alone, for those outputs
-    for (bool coarse = false;; coarse = true) {
-    mrun = -INFINITY;
-    neg = lrun = 0.f;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = f32x4{};
-    if (nj > 0) {
-      fetch_pages(0);
-      load_k(0);
-      load_v(0);
-    }
-    for (int j = 0; j < nj; ++j) {
-      const int left = len - (t0 + wave + NW * j) * TILE;  // tokens from the tile's first on
+    f32x4 acc[VEC];
+    // the tile's scores (log2 units) of this lane's 8 tokens; `left` tokens remain in the request
+    auto scores = [&](float(&x)[8]) {
       f32x4 st[2] = {f32x4{}, f32x4{}};
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-          st[half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[half][s]),
-                                                             qf[s], st[half], 0, 0, 0);
-      const bool more = j + 1 < nj;
-      // V of this tile is still on its way: its pages are not needed again
+        for (int half = 0; half < 2; ++half) st[half] = mfma16(kr[half][s], qf[s], st[half]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * g.scale_log2;
+    };
+    auto mask = [&](float(&x)[8], int left) {
+      if (left >= TILE) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (16 * (e >> 2) + 4 * grp + (e & 3) >= left) {
+          x[e] = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < VDW; ++i) vr[e][i] = 0;  // weight 0, but 0 x NaN is not
+        }
+    };
+    // acc += V^T p for one or two pieces of p
+    auto weigh = [&](u32x4 hi, u32x4 lo, bool both) {
+#pragma unroll
+      for (int i = 0; i < VDW; ++i) {
+        u32x4 even, odd;  // values 2 i and 2 i + 1 of the 8 tokens
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          even[t] = perm(vr[2 * t + 1][i], vr[2 * t][i], 0x05040100u);
+          odd[t] = perm(vr[2 * t + 1][i], vr[2 * t][i], 0x07060302u);
+        }
+        acc[2 * i] = mfma16(even, hi, acc[2 * i]);
+        acc[2 * i + 1] = mfma16(odd, hi, acc[2 * i + 1]);
+        if (both) {
+          acc[2 * i] = mfma16(even, lo, acc[2 * i]);
+          acc[2 * i + 1] = mfma16(odd, lo, acc[2 * i + 1]);
+        }
+      }
+    };
+    // value (4 grp + r) VEC + i of head col is acc[i][r]
+    auto put = [&](float* to) {
+      if (col < nh) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < VEC; i += 4)
+            *reinterpret_cast<f32x4*>(to + col * D + (4 * grp + r) * VEC + i) =
+                f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+      }
+    };
+
+    int t = r0 - first, t0 = t, pos = r0;  // tile of the request, its first one here; tile among all
+    int page_t = t, pages = fetch_pages(b, t, len, n);
+    load_q(b, qf);
+    bool bad = check_pages(pages), bad_next = false;
+    int b_next = 0, len_next = 0, n_next = 0, pages_next = 0;
+    auto look_ahead = [&]() {  // the next request with tokens, if the run goes on to it
+      if (first + n >= r1) return;
+      for (b_next = min(b + 1, g.B - 1);; ++b_next) {
+        len_next = g.lens[b_next];
+        n_next = tiles_of(len_next, cap);
+        if (n_next > 0 || b_next == g.B - 1) break;
+      }
+      pages_next = fetch_pages(b_next, 0, len_next, n_next);
+      load_q(b_next, qn);
+    };
+    {
+      const int page0 = __builtin_amdgcn_readlane(pages, 0), page1 = __builtin_amdgcn_readlane(pages, 1);
+      load_k(page0, page1, t);
+      load_v(page0, page1, t);
+    }
+    look_ahead();
+    float mrun = -INFINITY, neg = 0.f, lrun = 0.f;  // maximum (log2 units), -maximum or 0, own sum
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = f32x4{};
+
+    for (;;) {
+      float x[8];
+      scores(x);
+      // K of the next tile into the registers that are free now
+      const bool more = pos + 1 < r1, same = t + 1 < n;
+      int page0 = 0, page1 = 0, t_next = 0;
       if (more) {
-        if (j + 1 - jbase == 32) fetch_pages(j + 1);
-        load_k(j + 1);
-      }
-      if (left < TILE) {  // the last tile of the request
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (16 * (e >> 2) + 4 * grp + (e & 3) >= left) {
-            st[e >> 2][e & 3] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < VDW; ++i) vr[e][i] = 0;  // weight 0, but 0 x NaN is not
+        if (same) {
+          t_next = t + 1;
+          if (t_next - page_t == 32) {
+            page_t = t_next;
+            pages = fetch_pages(b, t_next, len, n);
+            bad |= check_pages(pages);
           }
+          page0 = __builtin_amdgcn_readlane(pages, 2 * (t_next - page_t));
+          page1 = __builtin_amdgcn_readlane(pages, 2 * (t_next - page_t) + 1);
+        } else {
+          bad_next = check_pages(pages_next);
+          page0 = __builtin_amdgcn_readlane(pages_next, 0);
+          page1 = __builtin_amdgcn_readlane(pages_next, 1);
+        }
+        load_k(page0, page1, t_next);
       }
-      float x[8], mx = -INFINITY;
+      mask(x, len - t * TILE);
+      float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = st[e >> 2][e & 3] * g.scale_log2;
-        mx = fmaxf(mx, x[e]);
-      }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
       if (__builtin_amdgcn_ballot_w64(mx > mrun + 8.f) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -272,73 +329,129 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         lo[e / 2] = f2bf2(p0 - __builtin_bit_cast(float, h << 16),
                           p1 - __builtin_bit_cast(float, h & 0xffff0000u));
       }
-      const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, lo);
-#pragma unroll
-      for (int i = 0; i < VDW; ++i) {
-        u32x4 even, odd;  // values 2 i and 2 i + 1 of the 8 tokens
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          even[t] = perm(vr[2 * t + 1][i], vr[2 * t][i], 0x05040100u);
-          odd[t] = perm(vr[2 * t + 1][i], vr[2 * t][i], 0x07060302u);
-        }
-        const bf16x8 ve = __builtin_bit_cast(bf16x8, even), vo = __builtin_bit_cast(bf16x8, odd);
-        acc[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, ph, acc[2 * i], 0, 0, 0);
-        acc[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, ph, acc[2 * i + 1], 0, 0, 0);
-        if (!coarse) {
-          acc[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, pl, acc[2 * i], 0, 0, 0);
-          acc[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, pl, acc[2 * i + 1], 0, 0, 0);
-        }
+      weigh(hi, lo, true);
+      if (more) load_v(page0, page1, t_next);
+      ++pos;
+      if (more && same) {
+        t = t_next;
+        continue;
       }
-      if (more) load_v(j + 1);
-    }
 
-    // the wave's results: value (4 grp + r) VEC + i of head col is acc[i][r]
-    lrun += __shfl_xor(lrun, 16);
-    lrun += __shfl_xor(lrun, 32);
-    bool nan = false;
-    if (col < nh) {
-      if (grp == 0) {
-        s_m[wave][col] = mrun;
-        s_l[wave][col] = bad ? __builtin_nanf("") : lrun;
-      }
+      // the request ends, here or for this run
+      const bool carried = t0 > 0, whole = !carried && !same;
+      lrun += __shfl_xor(lrun, 16);
+      lrun += __shfl_xor(lrun, 32);
+      float any = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int i = 0; i < VEC; ++i) any += acc[i][0] + acc[i][1] + acc[i][2] + acc[i][3];
+      float* const to = res + place_of(carried) * slot;
+      if (__builtin_amdgcn_ballot_w64(any != any && col < nh) != 0) {
+        // An infinite value times the two pieces of its weight is NaN where the second is 0 or of the
+        // other sign. For the outputs that are NaN, once more with the first pieces alone.
+        put(to);
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-          f32x4* to = reinterpret_cast<f32x4*>(&s_o[wave][col][(4 * grp + r) * VEC + i]);
-          f32x4 x = {acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
-          if (coarse) {
-            const f32x4 fine = *to;
+        for (int i = 0; i < VEC; ++i) acc[i] = f32x4{};
+        for (int tt = t0; tt <= t; ++tt) {
+          int again = fetch_pages(b, tt, len, n);
+          check_pages(again);
+          const int p0 = __builtin_amdgcn_readlane(again, 0), p1 = __builtin_amdgcn_readlane(again, 1);
+          load_k(p0, p1, tt);
+          load_v(p0, p1, tt);
+          scores(x);
+          mask(x, len - tt * TILE);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x[c] = fine[c] == fine[c] ? fine[c] : x[c];
-          }
-          *to = x;
-          const float any = x[0] + x[1] + x[2] + x[3];
-          nan |= any != any;
+          for (int e = 0; e < 8; e += 2)
+            hi[e / 2] = f2bf2(exp2_fast(x[e] + neg), exp2_fast(x[e + 1] + neg));
+          weigh(hi, hi, false);
         }
+        if (col < nh) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float fine = to[col * D + (4 * grp + r) * VEC + i];
+              if (fine == fine) acc[i][r] = fine;
+            }
+        }
+        if (more) {
+          load_k(page0, page1, t_next);
+          load_v(page0, page1, t_next);
+        }
+      }
+      if (bad) lrun = __builtin_nanf("");
+      if (whole) {
+        if (col < nh) {
+          const float inv = 1.f / lrun;
+          const int64_t at = (int64_t)b * g.Hq + hk * g.G + h0 + col;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4)
+              *reinterpret_cast<u32x2*>(g.o + at * D + (4 * grp + r) * VEC + i) =
+                  u32x2{f2bf2(acc[i][r] * inv, acc[i + 1][r] * inv),
+                        f2bf2(acc[i + 2][r] * inv, acc[i + 3][r] * inv)};
+          if (grp == 0) g.lse[at] = ((mrun == -INFINITY ? 0.f : mrun) + log2f(lrun)) * kLn2;
+        }
+      } else {
+        put(to);
+        if (grp == 0 && col < nh) {
+          to[nh * D + col] = mrun;
+          to[nh * D + nh + col] = lrun;
+        }
+        if (lane == 0) {
+          s_has[wave] |= carried ? HAS_CARRIED | (same ? 0 : CARRIED_ENDS) : HAS_OPEN;
+          s_req[wave][place_of(carried)] = b;
+          if (!carried) s_last[wave] = run_of(runs, first + n - 1) / NW;
+        }
+      }
+      if (!more) break;
+      first += n;
+      b = b_next, len = len_next, n = n_next;
+      pages = pages_next, bad = bad_next;
+      page_t = t = t0 = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[s] = qn[s];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] = f32x4{};
+      mrun = -INFINITY;
+      neg = lrun = 0.f;
+      look_ahead();
     }
-    if (coarse || __builtin_amdgcn_ballot_w64(nan) == 0) break;
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == n;
-    if (t0 == 0 && !whole) {
+  }
+  __syncthreads();
+
+  // join the waves' parts of one request: a carried one (start -1), and what each wave begins
+  int open = -1, open_last = 0;
+  const int heads_max = min(g.G, HT);
+  for (int start = -1; start < NW; ++start) {
+    const int w0 = max(start, 0), place = start < 0 ? 0 : 1;
+    if (!(s_has[w0] & (start < 0 ? HAS_CARRIED : HAS_OPEN))) continue;
+    int count = 1;  // parts, of waves w0 .. w0 + count - 1
+    bool ended = start < 0 && (s_has[0] & CARRIED_ENDS);
+    while (!ended && w0 + count < NW && (s_has[w0 + count] & HAS_CARRIED))
+      ended = s_has[w0 + count++] & CARRIED_ENDS;
+    const bool whole = start >= 0 && ended;
+    const int b = s_req[w0][place];
+    if (start >= 0 && !ended) {
       open = b;
-      open_last = run_of(total, runs, first + n - 1);
+      open_last = s_last[w0];
     }
-    float* part = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + (t0 == 0)) *
-                               part_floats(min(g.G, HT), D);
+    float* to = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * slot;
     for (int e = threadIdx.x; e < nh * (D / 4); e += NT) {
       const int h = e / (D / 4), d = e % (D / 4) * 4;
+      const float* from = reinterpret_cast<const float*>(s_res) + (w0 * 2 + place) * slot;
+      auto part = [&](int i) {  // the first one in its place, the others carried
+        return i ? from + (2 * i - place) * slot : from;
+      };
       float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) m = fmaxf(m, s_m[i][h]);
+      for (int i = 0; i < count; ++i) m = fmaxf(m, part(i)[nh * D + h]);
       const float ref = m == -INFINITY ? 0.f : m;
       f32x4 sum = {};
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        const float wt = exp2_fast(s_m[i][h] - ref);
-        l += wt * s_l[i][h];
-        sum += wt * *reinterpret_cast<const f32x4*>(&s_o[i][h][d]);
+      for (int i = 0; i < count; ++i) {
+        const float* p = part(i);
+        const float wt = exp2_fast(p[nh * D + h] - ref);
+        l += wt * p[nh * D + nh + h];
+        sum += wt * *reinterpret_cast<const f32x4*>(p + h * D + d);
       }
       if (whole) {
         const float inv = 1.f / l;
@@ -347,25 +460,21 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
             u32x2{f2bf2(sum[0] * inv, sum[1] * inv), f2bf2(sum[2] * inv, sum[3] * inv)};
         if (d == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
       } else {
+        *reinterpret_cast<f32x4*>(to + h * D + d) = sum;
         if (d == 0) {
-          part[nh * D + h] = m;
-          part[nh * D + nh + h] = l;
+          to[nh * D + h] = m;
+          to[nh * D + nh + h] = l;
         }
-        *reinterpret_cast<f32x4*>(part + h * D + d) = sum;
       }
     }
-    first += n;
-    if (first >= r1) break;
-    __syncthreads();  // the waves' results have been read
   }
-  }
-  if (hk == 0 && ht == 0 && threadIdx.x == 0) g.shared[w] = make_int2(open, open_last);
+  if (hk == 0 && ht == 0 && threadIdx.x == 0) g.open[w] = make_int2(open, open_last);
 
-  // requests without tiles, spread over the runs
+  // requests without tiles, spread over the workgroups that have work
   int empty = 0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) empty |= s_empty[i];
-  const int every = max(runs, 1);
+  const int every = max((runs.runs + NW - 1) / NW, 1);
   if (empty && w < every)
     for (int b = w + every * wave; b < g.B; b += every * NW) {
       const int len = g.lens[b];
@@ -378,30 +487,34 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     }
 }
 
-// A workgroup a (run, query head): the parts of the request that the run begins and does not finish
-// (`shared`), in the order of their runs.
+// A workgroup a (workgroup of the first kernel, query head): the parts of the request that the former
+// begins and does not finish, in their order.
 constexpr int JT = 256;
 template <int D>
 __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   constexpr int SETS = JT / (D / 4);  // threads a value: every SETS-th part each
-  __shared__ float s_w[PARTS], s_l[PARTS], s_max[JT / 64];
+  __shared__ float s_w[PARTS], s_max[JT / 64], s_sum[JT / 64];
   __shared__ f32x4 s_o[SETS][D / 4];
   const int w0 = blockIdx.x, h = blockIdx.y;
-  const int2 open = g.shared[w0];
+  const int2 open = g.open[w0];
   const int b = open.x, count = open.y - w0 + 1;
   if (b < 0) return;
   const int hk = h / g.G, ht = (h - hk * g.G) / HT, hh = (h - hk * g.G) % HT;
-  const int nh = min(g.G - ht * HT, HT);
-  const int64_t size = part_floats(min(g.G, HT), D);
-  const float* base = g.part + ((int64_t)(hk * g.tiles_h + ht) * g.parts + w0) * 2 * size;
-  auto part = [&](int i) { return base + (2 * (int64_t)i + (i == 0)) * size; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < count; i += JT) {
-    const float* p = part(i) + nh * D + hh;
-    const float x = p[0];
-    s_w[i] = x;
-    s_l[i] = p[nh];
-    m = fmaxf(m, x);
+  const int nh = min(g.G - ht * HT, HT), slot = part_floats(min(g.G, HT), D);
+  const float* base = g.part + ((int64_t)(hk * g.tiles_h + ht) * g.parts + w0) * 2 * slot;
+  auto part = [&](int i) { return base + (int64_t)(2 * i + (i == 0)) * slot; };
+  constexpr int EACH = (PARTS + JT - 1) / JT;
+  float mi[EACH], li[EACH], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int i = threadIdx.x + k * JT;
+    mi[k] = -INFINITY;
+    li[k] = 0.f;
+    if (i < count) {
+      mi[k] = part(i)[nh * D + hh];
+      li[k] = part(i)[nh * D + nh + hh];
+    }
+    m = fmaxf(m, mi[k]);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
@@ -410,16 +523,28 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
 #pragma unroll
   for (int i = 0; i < JT / 64; ++i) m = fmaxf(m, s_max[i]);
   const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int i = threadIdx.x + k * JT;
+    const float wt = exp2_fast(mi[k] - ref);
+    if (i < count) s_w[i] = wt;
+    l += wt * li[k];
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = l;
+  __syncthreads();
   const int set = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
   f32x4 sum = {};
 #pragma unroll 4
   for (int i = set; i < count; i += SETS)
-    sum += exp2_fast(s_w[i] - ref) * *reinterpret_cast<const f32x4*>(part(i) + hh * D + 4 * c);
+    sum += s_w[i] * *reinterpret_cast<const f32x4*>(part(i) + hh * D + 4 * c);
   s_o[set][c] = sum;
   __syncthreads();
   if (set != 0) return;
-  float l = 0.f;
-  for (int i = 0; i < count; ++i) l += exp2_fast(s_w[i] - ref) * s_l[i];
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < JT / 64; ++i) l += s_sum[i];
 #pragma unroll
   for (int i = 1; i < SETS; ++i) sum += s_o[i][c];
   const float inv = 1.f / l;
@@ -433,6 +558,25 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
 static int parts_of(int kv_heads, int head_tiles) {
   const int n = PARTS / (kv_heads * head_tiles);
   return n > 1 ? n : 1;
+}
+template <int D>
+static int launch_paged_attn(const AttnArgs& g, hipStream_t stream, const char* what) {
+  // LDS: two places a wave; past 64 KB (16 heads of 128 values) the kernel asks for the most it can use
+  const size_t lds = (size_t)NW * 2 * part_floats(g.G < HT ? g.G : HT, D) * sizeof(float);
+  static uint64_t lds_done = 0;
+  if (lds > 48 * 1024) {
+    const int rc = reserve_lds((const void*)paged_attn_kernel<D>,
+                               (size_t)NW * 2 * part_floats(HT, D) * sizeof(float), lds_done, what);
+    if (rc != PLZ_OK) return rc;
+  }
+  const int pairs = (g.parts * g.Hkv + 7) / 8 * 8;
+  hipLaunchKernelGGL(paged_attn_kernel<D>, dim3((unsigned)(pairs * g.tiles_h)), dim3(NT), lds, stream,
+                     g);
+  const int rc = check_launch(what);
+  if (rc != PLZ_OK || g.parts == 1) return rc;
+  hipLaunchKernelGGL(paged_join_kernel<D>, dim3((unsigned)g.parts, (unsigned)g.Hq), dim3(JT), 0, stream,
+                     g);
+  return check_launch(what);
 }
 
 }  // namespace paged
@@ -491,22 +635,12 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
              scale * kLog2e};
   g.tiles_h = (g.G + HT - 1) / HT;
   g.parts = parts_of(kv_heads, g.tiles_h);
-  g.shared = reinterpret_cast<int2*>(g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 *
-                                                  part_floats(g.G < HT ? g.G : HT, head_dim));
+  g.open = reinterpret_cast<int2*>(g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 *
+                                                part_floats(g.G < HT ? g.G : HT, head_dim));
   while ((1 << g.shift) < page_size) ++g.shift;
-  const int pairs = (g.parts * kv_heads + 7) / 8 * 8;
-  const dim3 grid((unsigned)(pairs * g.tiles_h)), join((unsigned)g.parts, (unsigned)heads);
-  auto launch = [&](auto kernel, dim3 blocks, int threads) {
-    hipLaunchKernelGGL(kernel, blocks, dim3(threads), 0, (hipStream_t)stream, g);
-    return check_launch(what);
-  };
-  int rc = head_dim == 64    ? launch(paged_attn_kernel<64>, grid, NT)
-           : head_dim == 128 ? launch(paged_attn_kernel<128>, grid, NT)
-                             : launch(paged_attn_kernel<256>, grid, NT);
-  if (rc != PLZ_OK || g.parts == 1) return rc;
-  return head_dim == 64    ? launch(paged_join_kernel<64>, join, JT)
-         : head_dim == 128 ? launch(paged_join_kernel<128>, join, JT)
-                           : launch(paged_join_kernel<256>, join, JT);
+  return head_dim == 64    ? launch_paged_attn<64>(g, (hipStream_t)stream, what)
+         : head_dim == 128 ? launch_paged_attn<128>(g, (hipStream_t)stream, what)
+                           : launch_paged_attn<256>(g, (hipStream_t)stream, what);
 }
 
 }  // extern "C"

@@ -41,39 +41,38 @@ struct AttnArgs {
   const int32_t *table, *lens;
   uint16_t* o;
   float *lse, *part;
-  int2* open;  // [parts] of workgroup w: {the request that it begins and does not finish or -1, the
-               // workgroup that does}
+  float2* part_ml;  // [Hq][place][parts]: a part's maximum (log2 units) and sum
+  // What the second kernel joins: of workgroup w, {the request that it begins and does not finish or
+  // -1, the workgroup that does}; or, where there are fewer requests than that (by_request), of request
+  // b {the workgroup that begins it or -1, the one that ends it}.
+  int2* open;
+  int by_request;
   int64_t ldq;
   int B, W, Hq, Hkv, G, tiles_h, parts, num_pages, shift;  // tiles_h = head tiles a kv head
   float scale_log2;
 };
 
-// A partial result: heads x D values, then the heads' maxima (log2 units) and sums
+// A wave's partial result: heads x D values, then the heads' maxima (log2 units) and sums
 __host__ __device__ __forceinline__ int part_floats(int heads, int D) {
   return (heads * (D + 2) + 3) / 4 * 4;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Exclusive sum of v over the workgroup's threads, and the total
-__device__ __forceinline__ int scan_tiles(int v, int* part, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(s, off);
-    if (lane >= off) s += u;
-  }
-  if (lane == 63) part[wave] = s;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    before += w < wave ? part[w] : 0;
-    total += part[w];
-  }
-  return before + s - v;
+// Inclusive sum of v over the wave's lanes, in DPP moves (rows of 16, then rows 0 and 2 into 1 and 3,
+// then the lower half's sum into the upper): no LDS, where shuffles go through it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_0(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_or_0<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_or_0<0x112, 0xF>(v);
+  v += dpp_or_0<0x114, 0xF>(v);
+  v += dpp_or_0<0x118, 0xF>(v);
+  v += dpp_or_0<0x142, 0xA>(v);  // row_bcast 15 and 31
+  v += dpp_or_0<0x143, 0xC>(v);
+  return v;
 }
 
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -87,62 +86,56 @@ template <int D>
 __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnArgs g) {
   constexpr int KS = D / 32, VEC = D / 16, VDW = VEC / 2;
   extern __shared__ f32x4 s_res[];  // partial results, [wave][place]
-  __shared__ int s_part[NW], s_empty[NW], s_b[NW], s_first[NW], s_has[NW], s_req[NW][2], s_last[NW];
+  __shared__ int s_has[NW], s_req[NW][2], s_last[NW];
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int P = 1 << g.shift, cap = g.W << g.shift;
 
   // the head tiles of one workgroup number (the same K and V) sit side by side on one XCD (id % 8)
-  int w, hk, ht;
-  {
-    const int id = (int)blockIdx.x, per = 8 * g.tiles_h, pair = id / per * 8 + id % 8;
-    ht = id % per / 8;
-    w = pair / g.Hkv;
-    hk = pair - w * g.Hkv;
-  }
+  const int ht = (int)blockIdx.x >> 3, pair = (int)blockIdx.y * 8 + ((int)blockIdx.x & 7);
+  const int w = pair / g.Hkv, hk = pair - w * g.Hkv;
   if (w >= g.parts) return;  // the last eighth's padding
   const int h0 = ht * HT, nh = min(g.G - h0, HT);  // heads hk G + h0 .. + nh - 1
   const int slot = part_floats(min(g.G, HT), D);
   float* const res = reinterpret_cast<float*>(s_res) + wave * 2 * slot;
+  if (lane == 0) s_has[wave] = 0;
 
-  // every request's tiles, and where the workgroup's runs begin among them
-  const int per_thread = (g.B + NT - 1) / NT, b0 = threadIdx.x * per_thread;
+  // every request's tiles (a lane takes `each` consecutive requests) and their sums
+  const int each = (g.B + 63) >> 6;
+  int win_at = 0, win = 0;  // lane l: the length of request win_at + l
   int mine = 0;
-  bool none = false;
-  for (int b = b0; b < min(b0 + per_thread, g.B); ++b) {
-    const int n = tiles_of(g.lens[b], cap);
+  bool none = false;  // some request has no tiles
+  for (int i = 0; i < each; ++i) {
+    const int b = lane * each + i;
+    win = b < g.B ? g.lens[b] : 0;
+    const int n = tiles_of(win, cap);
     mine += n;
-    none |= n == 0;
+    none |= n == 0 && b < g.B;
   }
   none = __builtin_amdgcn_ballot_w64(none) != 0;
-  if (lane == 0) {
-    s_empty[wave] = none;
-    s_has[wave] = 0;
-  }
-  int total;
-  const int pre = scan_tiles(mine, s_part, total);
+  int sum = wave_scan(mine);
+  const int total = __builtin_amdgcn_readlane(sum, 63);
   const Deal runs = deal(total, g.parts * NW);
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int at = run_begin(runs, w * NW + i);
-    if (pre <= at && at < pre + mine) {
-      int b = b0, before = pre;
-      for (; b < g.B - 1; ++b) {  // the bound: lens may change under a caller's race, not past it
-        const int n = tiles_of(g.lens[b], cap);
-        if (at < before + n) break;
-        before += n;
-      }
-      s_b[i] = b;
-      s_first[i] = before;
-    }
-  }
-  __syncthreads();
 
   if (w * NW + wave < runs.runs) {
     const int r0 = run_begin(runs, w * NW + wave), r1 = run_begin(runs, w * NW + wave + 1);
-    int b = __builtin_amdgcn_readfirstlane(s_b[wave]);
-    int first = __builtin_amdgcn_readfirstlane(s_first[wave]);  // its first tile among all
-    int len = g.lens[b], n = tiles_of(len, cap);
+    // the request that holds tile r0, and its first tile among all: the lane, then its requests
+    auto holder = [&]() { return __builtin_ctzll(__builtin_amdgcn_ballot_w64(r0 < sum)); };
+    int at = holder();
+    int first = __builtin_amdgcn_readlane(sum - mine, at);
+    if (each > 1) {
+      for (win_at = at * each;; win_at += 64) {
+        win = win_at + lane < g.B ? g.lens[win_at + lane] : 0;
+        mine = tiles_of(win, cap);
+        sum = first + wave_scan(mine);
+        const int end = __builtin_amdgcn_readlane(sum, 63);
+        if (r0 < end || win_at + 64 >= g.B) break;
+        first = end;
+      }
+      at = __builtin_amdgcn_ballot_w64(r0 < sum) ? holder() : 63;
+      first = __builtin_amdgcn_readlane(sum - mine, at);
+    }
+    int b = win_at + at, len = __builtin_amdgcn_readlane(win, at), n = tiles_of(len, cap);
     const uint32_t koff = (uint32_t)(grp * P + col) * 16;
     const uint32_t voff = (uint32_t)(4 * grp * D + col * VEC) * 2;
     const int64_t page_bytes = (int64_t)D * 2 << g.shift;  // of one kv head
@@ -264,7 +257,11 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     auto look_ahead = [&]() {  // the next request with tokens, if the run goes on to it
       if (first + n >= r1) return;
       for (b_next = min(b + 1, g.B - 1);; ++b_next) {
-        len_next = g.lens[b_next];
+        if (b_next >= win_at + 64) {
+          win_at = b_next;
+          win = win_at + lane < g.B ? g.lens[win_at + lane] : 0;
+        }
+        len_next = __builtin_amdgcn_readlane(win, b_next - win_at);
         n_next = tiles_of(len_next, cap);
         if (n_next > 0 || b_next == g.B - 1) break;
       }
@@ -392,6 +389,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
                         f2bf2(acc[i + 2][r] * inv, acc[i + 3][r] * inv)};
           if (grp == 0) g.lse[at] = ((mrun == -INFINITY ? 0.f : mrun) + log2f(lrun)) * kLn2;
         }
+        if (g.by_request && lane == 0 && hk + ht == 0) g.open[b] = make_int2(-1, 0);
       } else {
         put(to);
         if (grp == 0 && col < nh) {
@@ -436,7 +434,10 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       open = b;
       open_last = s_last[w0];
     }
-    float* to = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * slot;
+    if (g.by_request && threadIdx.x == 0 && hk + ht == 0 && start >= 0)
+      g.open[b] = ended ? make_int2(-1, 0) : make_int2(w, s_last[w0]);
+    // [kv head][head tile][workgroup][place][heads][D]
+    float* to = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * (heads_max * D);
     for (int e = threadIdx.x; e < nh * (D / 4); e += NT) {
       const int h = e / (D / 4), d = e % (D / 4) * 4;
       const float* from = reinterpret_cast<const float*>(s_res) + (w0 * 2 + place) * slot;
@@ -461,21 +462,16 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         if (d == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
       } else {
         *reinterpret_cast<f32x4*>(to + h * D + d) = sum;
-        if (d == 0) {
-          to[nh * D + h] = m;
-          to[nh * D + nh + h] = l;
-        }
+        if (d == 0)
+          g.part_ml[((int64_t)(hk * g.G + h0 + h) * 2 + place) * g.parts + w] = make_float2(m, l);
       }
     }
   }
-  if (hk == 0 && ht == 0 && threadIdx.x == 0) g.open[w] = make_int2(open, open_last);
+  if (!g.by_request && threadIdx.x == 0 && hk + ht == 0) g.open[w] = make_int2(open, open_last);
 
   // requests without tiles, spread over the workgroups that have work
-  int empty = 0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) empty |= s_empty[i];
   const int every = max((runs.runs + NW - 1) / NW, 1);
-  if (empty && w < every)
+  if (none && w < every)
     for (int b = w + every * wave; b < g.B; b += every * NW) {
       const int len = g.lens[b];
       if (tiles_of(len, cap) != 0) continue;
@@ -484,69 +480,80 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       for (int e = lane; e < nh * (D / 4); e += 64)
         *reinterpret_cast<u32x2*>(g.o + at * D + 4 * e) = u32x2{f2bf2(x, x), f2bf2(x, x)};
       if (lane < nh) g.lse[at + lane] = len <= 0 ? -INFINITY : x;
+      if (g.by_request && lane == 0 && hk + ht == 0) g.open[b] = make_int2(-1, 0);
     }
 }
 
-// A workgroup a (workgroup of the first kernel, query head): the parts of the request that the former
-// begins and does not finish, in their order.
+// A workgroup an entry of `open` and a query head: the parts of a request in the order of their runs.
 constexpr int JT = 256;
 template <int D>
 __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   constexpr int SETS = JT / (D / 4);  // threads a value: every SETS-th part each
-  __shared__ float s_w[PARTS], s_max[JT / 64], s_sum[JT / 64];
+  constexpr int EACH = (PARTS + JT - 1) / JT, AHEAD = 8;
+  __shared__ float2 s_ml[EACH * JT];
+  __shared__ float s_max[JT / 64], s_l[SETS];
   __shared__ f32x4 s_o[SETS][D / 4];
-  const int w0 = blockIdx.x, h = blockIdx.y;
-  const int2 open = g.open[w0];
-  const int b = open.x, count = open.y - w0 + 1;
-  if (b < 0) return;
+  const int h = blockIdx.y;
+  const int2 open = g.open[blockIdx.x];
+  const int b = g.by_request ? blockIdx.x : open.x, w0 = g.by_request ? open.x : blockIdx.x;
+  if (open.x < 0) return;
+  const int count = open.y - w0 + 1;
+  const float2* ml = g.part_ml + (int64_t)h * 2 * g.parts;
+  float2 x[EACH];
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int w = min(w0 + (int)threadIdx.x + k * JT, g.parts - 1);
+    x[k] = ml[w == w0 ? g.parts + w : w];
+  }
   const int hk = h / g.G, ht = (h - hk * g.G) / HT, hh = (h - hk * g.G) % HT;
-  const int nh = min(g.G - ht * HT, HT), slot = part_floats(min(g.G, HT), D);
-  const float* base = g.part + ((int64_t)(hk * g.tiles_h + ht) * g.parts + w0) * 2 * slot;
-  auto part = [&](int i) { return base + (int64_t)(2 * i + (i == 0)) * slot; };
-  constexpr int EACH = (PARTS + JT - 1) / JT;
-  float mi[EACH], li[EACH], m = -INFINITY, l = 0.f;
+  const int size = min(g.G, HT) * D, set = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
+  const float* base =
+      g.part + ((int64_t)(hk * g.tiles_h + ht) * g.parts + w0) * 2 * size + hh * D + 4 * c;
+  float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
     const int i = threadIdx.x + k * JT;
-    mi[k] = -INFINITY;
-    li[k] = 0.f;
-    if (i < count) {
-      mi[k] = part(i)[nh * D + hh];
-      li[k] = part(i)[nh * D + nh + hh];
-    }
-    m = fmaxf(m, mi[k]);
+    s_ml[i] = x[k];
+    if (i < count) m = fmaxf(m, x[k].x);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < JT / 64; ++i) m = fmaxf(m, s_max[i]);
-  const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    const int i = threadIdx.x + k * JT;
-    const float wt = exp2_fast(mi[k] - ref);
-    if (i < count) s_w[i] = wt;
-    l += wt * li[k];
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
-  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = l;
-  __syncthreads();
-  const int set = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
   f32x4 sum = {};
-#pragma unroll 4
-  for (int i = set; i < count; i += SETS)
-    sum += s_w[i] * *reinterpret_cast<const f32x4*>(part(i) + hh * D + 4 * c);
+  float l = 0.f, ref = 0.f;
+  for (int i0 = 0; i0 < count; i0 += SETS * AHEAD) {
+    f32x4 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = min(i0 + k * SETS + set, count - 1);
+      v[k] = *reinterpret_cast<const f32x4*>(base + (int64_t)(2 * i + (i == 0)) * size);
+    }
+    if (i0 == 0) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < JT / 64; ++k) m = fmaxf(m, s_max[k]);
+      ref = m == -INFINITY ? 0.f : m;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * SETS + set;
+      if (i < count) {
+        const float2 p = s_ml[i];
+        const float wt = exp2_fast(p.x - ref);
+        l += wt * p.y;
+        sum += wt * v[k];
+      }
+    }
+  }
   s_o[set][c] = sum;
+  if (c == 0) s_l[set] = l;
   __syncthreads();
   if (set != 0) return;
-  l = 0.f;
 #pragma unroll
-  for (int i = 0; i < JT / 64; ++i) l += s_sum[i];
-#pragma unroll
-  for (int i = 1; i < SETS; ++i) sum += s_o[i][c];
+  for (int i = 1; i < SETS; ++i) {
+    sum += s_o[i][c];
+    l += s_l[i];
+  }
   const float inv = 1.f / l;
   const int64_t at = (int64_t)b * g.Hq + h;
   *reinterpret_cast<u32x2*>(g.o + at * D + 4 * c) =
@@ -569,12 +576,13 @@ static int launch_paged_attn(const AttnArgs& g, hipStream_t stream, const char* 
                                (size_t)NW * 2 * part_floats(HT, D) * sizeof(float), lds_done, what);
     if (rc != PLZ_OK) return rc;
   }
-  const int pairs = (g.parts * g.Hkv + 7) / 8 * 8;
-  hipLaunchKernelGGL(paged_attn_kernel<D>, dim3((unsigned)(pairs * g.tiles_h)), dim3(NT), lds, stream,
-                     g);
+  hipLaunchKernelGGL(paged_attn_kernel<D>,
+                     dim3((unsigned)(8 * g.tiles_h), (unsigned)((g.parts * g.Hkv + 7) / 8)), dim3(NT),
+                     lds, stream, g);
   const int rc = check_launch(what);
   if (rc != PLZ_OK || g.parts == 1) return rc;
-  hipLaunchKernelGGL(paged_join_kernel<D>, dim3((unsigned)g.parts, (unsigned)g.Hq), dim3(JT), 0, stream,
+  hipLaunchKernelGGL(paged_join_kernel<D>,
+                     dim3((unsigned)(g.by_request ? g.B : g.parts), (unsigned)g.Hq), dim3(JT), 0, stream,
                      g);
   return check_launch(what);
 }
@@ -591,8 +599,8 @@ size_t plz_paged_attn_workspace(int64_t batch, int heads, int kv_heads, int head
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads) return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
   const size_t parts = (size_t)parts_of(kv_heads, ht);
-  return parts * kv_heads * ht * 2 * part_floats(G < HT ? G : HT, head_dim) * sizeof(float) +
-         parts * sizeof(int2);
+  return parts * kv_heads * ht * 2 * (G < HT ? G : HT) * head_dim * sizeof(float) +
+         parts * heads * 2 * sizeof(float2) + parts * sizeof(int2);
 }
 
 int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
@@ -630,13 +638,15 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
     set_error("%s: workspace of %zu bytes (16-byte aligned) required", what, need);
     return PLZ_EWORKSPACE;
   }
-  AttnArgs g{q, k_cache, v_cache, block_table, lens, o, lse, (float*)workspace, nullptr, ld_q,
+  AttnArgs g{q, k_cache, v_cache, block_table, lens, o, lse, (float*)workspace, nullptr, nullptr, 0, ld_q,
              (int)batch, (int)width, heads, kv_heads, heads / kv_heads, 0, 0, (int)num_pages, 0,
              scale * kLog2e};
   g.tiles_h = (g.G + HT - 1) / HT;
   g.parts = parts_of(kv_heads, g.tiles_h);
-  g.open = reinterpret_cast<int2*>(g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 *
-                                                part_floats(g.G < HT ? g.G : HT, head_dim));
+  g.part_ml = reinterpret_cast<float2*>(
+      g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 * (g.G < HT ? g.G : HT) * head_dim);
+  g.open = reinterpret_cast<int2*>(g.part_ml + (int64_t)g.parts * heads * 2);
+  g.by_request = batch < g.parts;
   while ((1 << g.shift) < page_size) ++g.shift;
   return head_dim == 64    ? launch_paged_attn<64>(g, (hipStream_t)stream, what)
          : head_dim == 128 ? launch_paged_attn<128>(g, (hipStream_t)stream, what)

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
                            (int64_t)((tile * TILE + 16 * half) & (P - 1)) * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
-          kr[half][s] = *reinterpret_cast<const u32x4*>(base + (int64_t)s * 64 * P + koff);
+          kr[half][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + (int64_t)s * 64 * P + koff));
       }
     };
     auto load_v = [&](int page0, int page1, int tile) {
@@ -185,12 +185,12 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         for (int t = 0; t < 4; ++t) {
           uint32_t(&d)[VDW] = vr[4 * half + t];
           if constexpr (VDW == 2) {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(base + t * D * 2 + voff);
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(base + t * D * 2 + voff));
             d[0] = x[0], d[1] = x[1];
           } else {
 #pragma unroll
             for (int c = 0; c < VDW / 4; ++c) {
-              const u32x4 x = *reinterpret_cast<const u32x4*>(base + t * D * 2 + voff + 16 * c);
+              const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + t * D * 2 + voff + 16 * c));
 #pragma unroll
               for (int i = 0; i < 4; ++i) d[4 * c + i] = x[i];
             }
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
 }
 
 // A workgroup an entry of `open` and a query head: the parts of a request in the order of their runs.
-constexpr int JT = 256;
+constexpr int JT = 128;
 template <int D>
 __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   constexpr int SETS = JT / (D / 4);  // threads a value: every SETS-th part each

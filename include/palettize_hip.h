@@ -745,8 +745,10 @@ int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v
  * [batch, heads] = log-sum-exp of the scaled scores; heads % kv_heads == 0, head_dim 64, 128 or
  * 256. lens[b] <= 0: o = 0, lse = -inf. A request whose length passes width * page_size, or that
  * needs a page outside [0, num_pages), gives NaN in both; nothing is read past the cache. Values in
- * the cache behind a request's last token do not matter. Deterministic. */
-size_t plz_paged_attn_workspace(int64_t batch, int heads, int kv_heads, int head_dim);
+ * the cache behind a request's last token do not matter. Deterministic. The workspace (0 bytes where
+ * the table is so small that no request is shared) belongs to one call at a time. */
+size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
+                                int head_dim);
 int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
                    const uint16_t* v_cache, const int32_t* block_table, const int32_t* lens,
                    uint16_t* o, float* lse, void* workspace, size_t workspace_bytes, int64_t batch,

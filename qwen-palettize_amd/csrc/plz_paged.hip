@@ -11,7 +11,7 @@
 //                     positions of the step's token rows, all from the requests' lengths
 //   paged_rope_write  per-head RMSNorm and rotation of the rows' q and k, q written out, k and v
 //                     written into their slots
-#include "plz_common.h"
+#include "plz_paged.h"
 #include "palettize_hip.h"
 
 namespace plz {
@@ -24,11 +24,13 @@ namespace paged {
 //   given_b = clamp(pool - sum_{b' < b} want_b', 0, want_b)
 //   lens_out[b] = min(k + a, (pages(k) + given_b) P): what has room; token i of b, row starts[b] + i,
 //   has position k + i and the slot of that position, -1 where there is no room.
-// Everything is a prefix sum over the requests, then independent work a page and a token, which
-// find their request by binary search in the sums. One workgroup walks the requests in chunks of
-// its threads, twice: the pages handed back have to be on the stack before any is taken.
-constexpr int ST = 1024;  // threads, and requests a chunk
-
+// Everything is a prefix sum over the requests, then independent work a page and a token, which find
+// their request by binary search in the sums. One workgroup does it, a thread a request (in chunks of
+// its threads, twice, for larger batches: the pages handed back have to be on the stack before any is
+// taken): a step of 8 requests takes 3.0 us (5.1 with two passes for every batch, 1024 threads and sums
+// by shuffles), of which 1 is the launch and the rest dependent memory accesses. More than 4096 token
+// rows go to a second launch over the whole card: 27800 rows in 1700 new pages 5.1 + 2.4 us, in the one
+// workgroup 25.7; 5000 rows 7.5 in two, 10.7 in one.
 struct StepArgs {
   const int32_t *lens, *keep, *add;
   int32_t *table, *stack;
@@ -36,22 +38,6 @@ struct StepArgs {
   int32_t *slots, *pos, *starts, *lens_out, *count_out;
   int B, W, F, rows, shift;  // shift = log2 P
 };
-
-// Inclusive sum over the workgroup's threads (no overflow by the entry point's limits); part: one
-// word a wave.
-__device__ __forceinline__ int block_scan(int v, int* part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(v, off);
-    if (lane >= off) v += u;
-  }
-  __syncthreads();  // part's last readers are done
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) v += part[w];
-  return v;
-}
 
 // The last i in [0, n) with start[i] <= j (start ascending, start[0] <= j)
 __device__ __forceinline__ int find_row(const int* start, int n, int j) {
@@ -70,40 +56,52 @@ __device__ __forceinline__ int find_row(const int* start, int n, int j) {
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// a + b, at most cap, for 0 <= a, b <= cap <= 2^30
-__device__ __forceinline__ int add_cap(int a, int b, int cap) { return min(a + b, cap); }
-
-__device__ __forceinline__ int block_scan_cap(int v, int cap, int* part) {
+// Inclusive sums over the workgroup's threads of v and of u, u's at most cap (0 <= u <= cap <= 2^30, so
+// that no sum overflows; v's do not by the entry point's limits). part: two words a wave.
+template <int ST>
+__device__ __forceinline__ void block_scan(int& v, int& u, int cap, int2* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_scan(v);
+  u = wave_scan(u, cap);
+  __syncthreads();  // part's last readers are done
+  if (lane == 63) part[wave] = make_int2(v, u);
+  __syncthreads();
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(v, off);
-    if (lane >= off) v = add_cap(v, u, cap);
-  }
-  __syncthreads();
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) v = add_cap(v, part[w], cap);
-  return v;
+  for (int w = 0; w < ST / 64; ++w)
+    if (w < wave) {
+      v += part[w].x;
+      u = min(u + part[w].y, cap);
+    }
 }
 
+// TOKENS: the token rows too; else only the position of each request's first one (rows_kernel)
+template <int ST, bool TOKENS>
 __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
-  __shared__ int part[ST / 64];
+  __shared__ int2 part[ST / 64];
   __shared__ int s_tok[ST], s_page[ST], s_keep[ST], s_hold[ST], s_len[ST], s_last[2];
   const int tid = threadIdx.x, P1 = (1 << g.shift) - 1, cap = g.W << g.shift;
   const int count = clampi(*g.count, 0, g.F);
+  const bool one = g.B <= ST;  // all requests at once
+  int L = 0, k = 0, a = 0;
+  auto load = [&](int b) {
+    L = k = a = 0;
+    if (b < g.B) {
+      L = clampi(g.lens[b], 0, cap);
+      k = g.keep ? clampi(g.keep[b], 0, L) : L;
+      a = clampi(g.add[b], 0, g.rows);
+    }
+  };
   // pages handed back
   int back = 0;  // by the chunks before
+  int ends = 0;  // of a single chunk: the token rows up to this request's last
   for (int b0 = 0; b0 < g.B; b0 += ST) {
-    const int b = b0 + tid, nb = min(ST, g.B - b0);
-    int n = 0;
-    if (b < g.B) {
-      const int L = clampi(g.lens[b], 0, cap), k = g.keep ? clampi(g.keep[b], 0, L) : L;
-      const int hold = (k + P1) >> g.shift;
-      n = ((L + P1) >> g.shift) - hold;
-      s_hold[tid] = hold;
-    }
-    const int end = block_scan(n, part);
+    const int nb = min(ST, g.B - b0);
+    load(b0 + tid);
+    const int hold = (k + P1) >> g.shift, n = ((L + P1) >> g.shift) - hold;
+    int end = n;
+    ends = a;
+    block_scan<ST>(end, ends, g.rows, part);
+    s_hold[tid] = hold;
     s_page[tid] = end - n;
     if (tid == ST - 1) s_last[0] = end;
     __syncthreads();
@@ -113,45 +111,48 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
       if (at < g.F) g.stack[at] = g.table[(int64_t)(b0 + r) * g.W + s_hold[r] + j - s_page[r]];
     }
     back += total;
-    __syncthreads();
+    if (total > 0 || !one) __syncthreads();
   }
   const int pool = min(count + back, g.F);
   // pages taken, lengths, rows
   int tok0 = 0, want0 = 0;  // rows used and pages asked for by the chunks before
   for (int b0 = 0; b0 < g.B; b0 += ST) {
     const int b = b0 + tid, nb = min(ST, g.B - b0);
-    int L = 0, k = 0, a = 0;
-    if (b < g.B) {
-      L = clampi(g.lens[b], 0, cap);
-      k = g.keep ? clampi(g.keep[b], 0, L) : L;
-      a = clampi(g.add[b], 0, g.rows);
+    int none = 0;
+    if (!one) {
+      load(b);
+      ends = a;
+      block_scan<ST>(none, ends, g.rows, part);
+      ends = min(tok0 + ends, g.rows);
     }
-    const int tok_end = add_cap(tok0, block_scan_cap(a, g.rows, part), g.rows);
     // the row before: the previous thread's end
-    s_tok[tid] = tok_end;
+    s_tok[tid] = ends;
     __syncthreads();
     const int tok = tid ? s_tok[tid - 1] : tok0;
-    a = tok_end - tok;
+    a = ends - tok;
     const int hold = (k + P1) >> g.shift;
     const int full = (int)min((int64_t)k + a, (int64_t)cap);
     const int want = ((full + P1) >> g.shift) - hold;
-    const int want_end = want0 + block_scan(want, part);
+    int want_end = want;
+    none = 0;
+    block_scan<ST>(want_end, none, 0, part);
+    want_end += want0;
     const int before = want_end - want;
     const int given = clampi(pool - before, 0, want);
     const int len = min(full, (hold + given) << g.shift);
-    __syncthreads();  // s_tok has been read
-    s_tok[tid] = tok;
+    s_tok[tid] = tok;  // block_scan's barriers: the ends have been read
     s_page[tid] = before;
     s_keep[tid] = k;
     s_hold[tid] = hold;
     s_len[tid] = len;
     if (tid == ST - 1) {
-      s_last[0] = tok_end;
+      s_last[0] = ends;
       s_last[1] = want_end;
     }
     if (b < g.B) {
       g.lens_out[b] = len;
-      g.starts[b + 1] = tok_end;
+      g.starts[b + 1] = ends;
+      if (!TOKENS && a > 0) g.pos[tok] = k;
     }
     __syncthreads();
     const int tok1 = s_last[0], want1 = s_last[1];
@@ -159,29 +160,63 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
       const int r = find_row(s_page, nb, j);
       g.table[(int64_t)(b0 + r) * g.W + s_hold[r] + j - s_page[r]] = g.stack[pool - 1 - j];
     }
-    for (int t = tok0 + tid; t < tok1; t += ST) {
-      const int r = find_row(s_tok, nb, t), pos = s_keep[r] + t - s_tok[r];
-      int slot = -1;
-      if (pos < s_len[r]) {
-        const int w = pos >> g.shift;
-        const int page = w < s_hold[r] ? g.table[(int64_t)(b0 + r) * g.W + w]
-                                       : g.stack[pool - 1 - (s_page[r] + w - s_hold[r])];
-        if (page >= 0 && page < g.F) slot = (page << g.shift) + (pos & P1);
+    if constexpr (TOKENS)
+      for (int t = tok0 + tid; t < tok1; t += ST) {
+        const int r = find_row(s_tok, nb, t), pos = s_keep[r] + t - s_tok[r];
+        int slot = -1;
+        if (pos < s_len[r]) {
+          const int w = pos >> g.shift;
+          const int page = w < s_hold[r] ? g.table[(int64_t)(b0 + r) * g.W + w]
+                                         : g.stack[pool - 1 - (s_page[r] + w - s_hold[r])];
+          if (page >= 0 && page < g.F) slot = (page << g.shift) + (pos & P1);
+        }
+        g.slots[t] = slot;
+        g.pos[t] = pos;
       }
-      g.slots[t] = slot;
-      g.pos[t] = pos;
-    }
     tok0 = tok1;
     want0 = want1;
-    __syncthreads();
+    if (!one) __syncthreads();
   }
-  for (int t = tok0 + tid; t < g.rows; t += ST) {
-    g.slots[t] = -1;
-    g.pos[t] = 0;
-  }
+  if constexpr (TOKENS)
+    for (int t = tok0 + tid; t < g.rows; t += ST) {
+      g.slots[t] = -1;
+      g.pos[t] = 0;
+    }
   if (tid == 0) {
     g.starts[0] = 0;
     *g.count_out = pool - min(pool, want0);
+  }
+}
+
+// The token rows of a step whose table, lengths and starts step_kernel<TOKENS = false> has left, with
+// the position of each request's first token in its row of pos.
+constexpr int RT = 256, STAGED = 4096;
+constexpr int64_t ONE_LAUNCH_ROWS = 4096;
+__global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
+  __shared__ int s_starts[STAGED];
+  const int P1 = (1 << g.shift) - 1, total = g.starts[g.B];
+  const int* starts = g.starts;
+  if (g.B <= STAGED) {
+    for (int i = threadIdx.x; i < g.B; i += RT) s_starts[i] = g.starts[i];
+    starts = s_starts;
+  }
+  __syncthreads();
+  for (int t = blockIdx.x * RT + threadIdx.x; t < g.rows; t += gridDim.x * RT) {
+    int slot = -1, pos = 0;
+    if (t < total) {
+      const int b = find_row(starts, g.B, t), i = t - starts[b];
+      pos = g.pos[t - i] + i;
+      if (pos < g.lens_out[b]) {
+        const int page = g.table[(int64_t)b * g.W + (pos >> g.shift)];
+        if (page >= 0 && page < g.F) slot = (page << g.shift) + (pos & P1);
+      }
+      if (i == 0) {
+        g.slots[t] = slot;
+        continue;
+      }
+    }
+    g.slots[t] = slot;
+    g.pos[t] = pos;
   }
 }
 
@@ -201,59 +236,91 @@ struct WriteArgs {
   int H, Hkv, max_pos, shift;
   int64_t slots_end;  // num_pages * P
   float eps;
+  int each;  // heads a workgroup
 };
 
-template <int LPR>
+template <int LPR, int U>  // U rows of a lane in flight
 __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
   constexpr int D = 8 * LPR, RPW = 64 / LPR, TB = 4 * RPW;  // tokens a workgroup
   const int lane = threadIdx.x & 63, l = lane % LPR;
   const int64_t t = (int64_t)blockIdx.x * TB + (threadIdx.x >> 6) * RPW + lane / LPR;
-  const int head = blockIdx.y;  // 0..H-1 q, then Hkv k, then Hkv v
   const bool valid = t < g.T;
   const int64_t tt = valid ? t : 0;
   const int slot = g.slots[tt], p = g.pos[tt];
   const bool placed = p >= 0 && p < g.max_pos;  // else nothing is stored, and q is NaN
   const bool stored = valid && placed && slot >= 0 && slot < g.slots_end;
-  const int kind = head < g.H ? 0 : head < g.H + g.Hkv ? 1 : 2;
-  const int h = kind == 0 ? head : kind == 1 ? head - g.H : head - g.H - g.Hkv;
-  const uint16_t* src = kind == 0 ? g.q + tt * g.ldq : kind == 1 ? g.k + tt * g.ldk : g.v + tt * g.ldv;
-  const uint4 xv = reinterpret_cast<const uint4*>(src + (int64_t)h * D)[l];
   const int64_t page = stored ? slot >> g.shift : 0;
   const int64_t at = stored ? slot & ((1 << g.shift) - 1) : 0;
-  const int64_t block = page * g.Hkv + h;  // of D * P values
-  if (kind == 2) {
-    if (stored) reinterpret_cast<uint4*>(g.vc)[((block << g.shift) + at) * LPR + l] = xv;
-    return;
+  const int all = g.H + 2 * g.Hkv;  // heads: q's, k's, v's
+  const int head0 = blockIdx.y * g.each, head1 = min(head0 + g.each, all);
+  // the heads' sources and the row's sines are on their way together
+  float c[8], s[8], w[8];
+  const bool turns = head0 < g.H + g.Hkv;
+  if (turns) {
+    const int64_t row = (int64_t)(placed ? p : 0) * D + 8 * l;
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(g.cosv + row + j);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(g.sinv + row + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[j + e] = a[e];
+        s[j + e] = l < LPR / 2 ? -b[e] : b[e];
+      }
+    }
   }
-  float f[8];
-  unpack8(xv, f);
-  const uint16_t* wt = kind == 0 ? g.qw : g.kw;
-  if (wt) {
-    float ss = 0.f;
+  const uint16_t* weight = head0 < g.H ? g.qw : g.kw;  // the one that w holds
+  if (turns && weight) unpack8(reinterpret_cast<const uint4*>(weight)[l], w);
+  for (int first = head0; first < head1; first += U) {
+    uint4 xv[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+    for (int i = 0; i < U; ++i) {
+      const int head = min(first + i, head1 - 1);
+      const uint16_t* src = head < g.H           ? g.q + tt * g.ldq + (int64_t)head * D
+                            : head < g.H + g.Hkv ? g.k + tt * g.ldk + (int64_t)(head - g.H) * D
+                                                 : g.v + tt * g.ldv + (int64_t)(head - g.H - g.Hkv) * D;
+      xv[i] = reinterpret_cast<const uint4*>(src)[l];
+    }
 #pragma unroll
-    for (int off = LPR / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
-    const float r = rsqrtf(ss * (1.f / D) + g.eps);
-    float w[8];
-    unpack8(reinterpret_cast<const uint4*>(wt)[l], w);
+    for (int i = 0; i < U; ++i) {
+      const int head = first + i;
+      if (head >= head1) break;
+      const int kind = head < g.H ? 0 : head < g.H + g.Hkv ? 1 : 2;
+      const int h = kind == 0 ? head : kind == 1 ? head - g.H : head - g.H - g.Hkv;
+      const int64_t block = page * g.Hkv + h;  // of D * P values
+      if (kind == 2) {
+        if (stored) reinterpret_cast<uint4*>(g.vc)[((block << g.shift) + at) * LPR + l] = xv[i];
+        continue;
+      }
+      float f[8], o[8];
+      unpack8(xv[i], f);
+      const uint16_t* wt = kind == 0 ? g.qw : g.kw;
+      if (wt) {
+        if (wt != weight) {
+          unpack8(reinterpret_cast<const uint4*>(wt)[l], w);
+          weight = wt;
+        }
+        float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
-  }
-  const int64_t row = (int64_t)(placed ? p : 0) * D + 8 * l;
-  float o[8];
+        for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float other = __shfl_xor(f[j], LPR / 2);
-    const float c = g.cosv[row + j], s = g.sinv[row + j];
-    o[j] = l < LPR / 2 ? f[j] * c - other * s : f[j] * c + other * s;
-    if (!placed) o[j] = __builtin_nanf("");
-  }
-  const uint4 out = pack8(o);
-  if (kind == 0) {
-    if (valid) reinterpret_cast<uint4*>(g.q_out + (tt * g.H + h) * D)[l] = out;
-  } else if (stored) {
-    reinterpret_cast<uint4*>(g.kc)[((block * LPR + l) << g.shift) + at] = out;
+        for (int off = LPR / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off);
+        const float r = rsqrtf(ss * (1.f / D) + g.eps);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        o[j] = f[j] * c[j] + __shfl_xor(f[j], LPR / 2) * s[j];
+        if (!placed) o[j] = __builtin_nanf("");
+      }
+      const uint4 out = pack8(o);
+      if (kind == 0) {
+        if (valid) reinterpret_cast<uint4*>(g.q_out + (tt * g.H + h) * D)[l] = out;
+      } else if (stored) {
+        reinterpret_cast<uint4*>(g.kc)[((block * LPR + l) << g.shift) + at] = out;
+      }
+    }
   }
 }
 
@@ -291,8 +358,17 @@ int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_
   const StepArgs g{lens,  keep,   new_tokens, block_table,    free_pages, free_count, slots,
                    positions, starts, lens_out,   free_count_out, (int)batch, (int)width,
                    (int)num_pages, (int)rows, shift};
-  hipLaunchKernelGGL(step_kernel, dim3(1), dim3(ST), 0, (hipStream_t)stream, g);
-  return check_launch("plz_paged_step");
+  auto launch = [&](auto kernel, int blocks, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, (hipStream_t)stream,
+                       g);
+    return check_launch("plz_paged_step");
+  };
+  if (rows <= ONE_LAUNCH_ROWS)
+    return batch <= 256 && rows <= 256 ? launch(step_kernel<256, true>, 1, 256)
+                                       : launch(step_kernel<1024, true>, 1, 1024);
+  const int rc = launch(step_kernel<1024, false>, 1, 1024);
+  const int64_t blocks = (rows + RT - 1) / RT;
+  return rc != PLZ_OK ? rc : launch(rows_kernel, (int)(blocks < 2048 ? blocks : 2048), RT);
 }
 
 int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t ld_q,
@@ -330,17 +406,26 @@ int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v
               "%s: operands must be 16-byte aligned", what);
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
+  // Heads a workgroup: as many as leave it 1024 workgroups, up to 8 (its tokens' sines are read once)
+  const int lpr = head_dim / 8, tb = 4 * (64 / lpr), all = heads + 2 * kv_heads;
+  const int64_t blocks = (tokens + tb - 1) / tb;
+  int each = 1;
+  while (each < 8 && blocks * all >= 2048 * (int64_t)each) each *= 2;
   const WriteArgs g{q,     k,      v,   q_weight, k_weight, cos_table, sin_table, positions,
                     slots, q_out, k_cache, v_cache, tokens, ld_q, ld_k, ld_v,
-                    heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps};
-  const int lpr = head_dim / 8, tb = 4 * (64 / lpr);
-  const dim3 grid((unsigned)((tokens + tb - 1) / tb), (unsigned)(heads + 2 * kv_heads));
-  if (lpr == 8)
-    hipLaunchKernelGGL((rope_write_kernel<8>), grid, dim3(256), 0, (hipStream_t)stream, g);
-  else if (lpr == 16)
-    hipLaunchKernelGGL((rope_write_kernel<16>), grid, dim3(256), 0, (hipStream_t)stream, g);
+                    heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps, each};
+  const dim3 grid((unsigned)blocks, (unsigned)((all + each - 1) / each));
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
+  };
+  if (each < 4)
+    lpr == 8    ? launch(rope_write_kernel<8, 1>)
+    : lpr == 16 ? launch(rope_write_kernel<16, 1>)
+                : launch(rope_write_kernel<32, 1>);
   else
-    hipLaunchKernelGGL((rope_write_kernel<32>), grid, dim3(256), 0, (hipStream_t)stream, g);
+    lpr == 8    ? launch(rope_write_kernel<8, 4>)
+    : lpr == 16 ? launch(rope_write_kernel<16, 4>)
+                : launch(rope_write_kernel<32, 4>);
   return check_launch(what);
 }
 

@@ -59,22 +59,6 @@ __host__ __device__ __forceinline__ int part_floats(int heads, int D) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Inclusive sum of v over the wave's lanes, in DPP moves (rows of 16, then rows 0 and 2 into 1 and 3,
-// then the lower half's sum into the upper): no LDS, where shuffles go through it.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_or_0(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-  v += dpp_or_0<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
-  v += dpp_or_0<0x112, 0xF>(v);
-  v += dpp_or_0<0x114, 0xF>(v);
-  v += dpp_or_0<0x118, 0xF>(v);
-  v += dpp_or_0<0x142, 0xA>(v);  // row_bcast 15 and 31
-  v += dpp_or_0<0x143, 0xC>(v);
-  return v;
-}
-
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -467,7 +451,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       }
     }
   }
-  if (!g.by_request && threadIdx.x == 0 && hk + ht == 0) g.open[w] = make_int2(open, open_last);
+  if (g.open && !g.by_request && threadIdx.x == 0 && hk + ht == 0) g.open[w] = make_int2(open, open_last);
 
   // requests without tiles, spread over the workgroups that have work
   const int every = max((runs.runs + NW - 1) / NW, 1);
@@ -561,6 +545,11 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   if (c == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
 }
 
+// True where all requests together have a tile a wave of one workgroup at most, whatever their lengths:
+// then that workgroup joins whatever is shared, and there is no second kernel.
+static bool never_shared(int64_t batch, int64_t width, int64_t page_size) {
+  return batch <= NW && width <= NW * TILE && batch * ((width * page_size + TILE - 1) / TILE) <= NW;
+}
 // workgroups a (kv head, head tile)
 static int parts_of(int kv_heads, int head_tiles) {
   const int n = PARTS / (kv_heads * head_tiles);
@@ -595,8 +584,11 @@ using namespace plz::paged;
 
 extern "C" {
 
-size_t plz_paged_attn_workspace(int64_t batch, int heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads) return 0;
+size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
+                                int head_dim) {
+  if (batch <= 0 || width <= 0 || page_size <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
+      heads % kv_heads || never_shared(batch, width, page_size))
+    return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
   const size_t parts = (size_t)parts_of(kv_heads, ht);
   return parts * kv_heads * ht * 2 * (G < HT ? G : HT) * head_dim * sizeof(float) +
@@ -633,8 +625,10 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
               "%s: null pointer", what);
   for (const void* p : {(const void*)q, (const void*)k_cache, (const void*)v_cache, (const void*)o})
     PLZ_REQUIRE(((uintptr_t)p & 15) == 0, "%s: q, the caches and o must be 16-byte aligned", what);
-  const size_t need = plz_paged_attn_workspace(batch, heads, kv_heads, head_dim);
-  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+  const size_t need =
+      plz_paged_attn_workspace(batch, width, page_size, heads, kv_heads, head_dim);
+  if (need == 0) workspace = nullptr;
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("%s: workspace of %zu bytes (16-byte aligned) required", what, need);
     return PLZ_EWORKSPACE;
   }
@@ -643,10 +637,14 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
              scale * kLog2e};
   g.tiles_h = (g.G + HT - 1) / HT;
   g.parts = parts_of(kv_heads, g.tiles_h);
-  g.part_ml = reinterpret_cast<float2*>(
-      g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 * (g.G < HT ? g.G : HT) * head_dim);
-  g.open = reinterpret_cast<int2*>(g.part_ml + (int64_t)g.parts * heads * 2);
-  g.by_request = batch < g.parts;
+  if (need == 0) {
+    g.parts = 1;  // the one workgroup (a kv head and head tile) that gets any tiles
+  } else {
+    g.part_ml = reinterpret_cast<float2*>(
+        g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 * (g.G < HT ? g.G : HT) * head_dim);
+    g.open = reinterpret_cast<int2*>(g.part_ml + (int64_t)g.parts * heads * 2);
+    g.by_request = batch < g.parts;
+  }
   while ((1 << g.shift) < page_size) ++g.shift;
   return head_dim == 64    ? launch_paged_attn<64>(g, (hipStream_t)stream, what)
          : head_dim == 128 ? launch_paged_attn<128>(g, (hipStream_t)stream, what)

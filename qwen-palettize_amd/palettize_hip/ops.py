@@ -1167,12 +1167,8 @@ def attn_bwd(q, k, v, o, lse, grad_o, scale=None):
 
 
 # ---- decoding over a paged key-value cache -----------------------------------------------------
-def _on(t, others, name, *args):
-    """call() on the device of t, with its current stream last; every tensor of others is on it."""
-    dev = t.get_device()
-    for x in others:
-        if x is not None and x.get_device() != dev:
-            raise ValueError(f"{name}: the tensors are on different devices")
+def _on(dev, name, *args):
+    """call() on device `dev`, with its current stream as the last argument."""
     if torch._C._cuda_getDevice() == dev:
         call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -1180,10 +1176,30 @@ def _on(t, others, name, *args):
             call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
+def _one_device(name, *tensors):
+    """The device of the first tensor, which all others (or None) are on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: the tensors are on different devices")
+    return dev
+
+
+def _dense_int32(tensors):
+    """The device that dense int32 GPU tensors share; -1 where they are not that (the checks that say
+    what is wrong come after)."""
+    dev = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
+    for t in tensors:
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == dev
+                and t.is_contiguous()):
+            return -1
+    return dev
+
+
 def _ints(t, name, *shape):
     """An int32 GPU tensor of that shape."""
     _need(t, name, torch.int32, len(shape))
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     return t
 
@@ -1200,12 +1216,21 @@ def paged_cache(num_pages, page_size, kv_heads, head_dim, device):
             torch.zeros(num_pages, kv_heads, page_size, head_dim, **kw))
 
 
+_BF16 = torch.bfloat16
+
+
 def _paged_caches(k_cache, v_cache):
     """(num_pages, kv_heads, page_size, head_dim) of a layer's cache."""
+    if (isinstance(v_cache, torch.Tensor) and isinstance(k_cache, torch.Tensor) and v_cache.dim() == 4
+            and v_cache.is_cuda and v_cache.dtype is _BF16 and k_cache.dtype is _BF16
+            and v_cache.is_contiguous() and k_cache.is_contiguous() and k_cache.is_cuda):
+        n, hkv, P, D = shape = v_cache.shape
+        if k_cache.shape == (n, hkv, D >> 3, P, 8) and D & 7 == 0:
+            return shape
     _need(k_cache, "k_cache", torch.bfloat16, 5)
     _need(v_cache, "v_cache", torch.bfloat16, 4)
     n, hkv, P, D = v_cache.shape
-    if tuple(k_cache.shape) != (n, hkv, D // 8, P, 8) or D % 8:
+    if k_cache.shape != (n, hkv, D // 8, P, 8) or D % 8:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must be "
                          "[pages, kv_heads, head_dim / 8, page_size, 8] and "
                          "[pages, kv_heads, page_size, head_dim]")
@@ -1215,14 +1240,15 @@ def _paged_caches(k_cache, v_cache):
 def _token_rows(t, name, heads=None, dim=None):
     """The pitch of bf16 rows [tokens, heads, head_dim] whose heads are dense (a slice of a
     projection's output is fine)."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor")
-    if not _on_gpu(t):
-        raise RuntimeError(f"{name} must be a GPU tensor (palettize_hip has no CPU path)")
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be 3-D, got shape {tuple(t.shape)}")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.bfloat16 and t.dim() == 3):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if not _on_gpu(t):
+            raise RuntimeError(f"{name} must be a GPU tensor (palettize_hip has no CPU path)")
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be 3-D, got shape {tuple(t.shape)}")
     T, H, D = t.shape
     if (heads is not None and H != heads) or (dim is not None and D != dim):
         raise ValueError(f"{name} {tuple(t.shape)} does not match {heads or H} heads of {dim or D}")
@@ -1244,30 +1270,44 @@ def paged_step(lens, new_tokens, block_table, free_pages, free_count, page_size,
     Returns (slots [rows], positions [rows], starts [B + 1], lens [B], free_count [1]); lens_out and
     free_count_out receive the last two (lens and free_count themselves may be given). A request
     that finds no page keeps the tokens that have room, and the others get slot -1."""
-    _need(lens, "lens", torch.int32, 1)
-    B = lens.shape[0]
-    _ints(new_tokens, "new_tokens", B)
-    if keep is not None:
-        _ints(keep, "keep", B)
-    _need(block_table, "block_table", torch.int32, 2)
-    if block_table.shape[0] != B:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
-    _need(free_pages, "free_pages", torch.int32, 1)
-    _ints(free_count, "free_count", 1)
+    ints = (lens, new_tokens, block_table, free_pages, free_count)
+    if keep is not None or lens_out is not None or free_count_out is not None:
+        ints += tuple(t for t in (keep, lens_out, free_count_out) if t is not None)
+    dev = _dense_int32(ints)
+    B = lens.shape[0] if dev >= 0 else -1
+    if not (dev >= 0 and lens.dim() == 1 and new_tokens.shape == lens.shape and block_table.dim() == 2
+            and block_table.shape[0] == B and free_pages.dim() == 1 and free_count.shape == (1,)
+            and (keep is None or keep.shape == lens.shape)
+            and (lens_out is None or lens_out.shape == lens.shape)
+            and (free_count_out is None or free_count_out.shape == (1,))):
+        _need(lens, "lens", torch.int32, 1)
+        B = lens.shape[0]
+        _ints(new_tokens, "new_tokens", B)
+        _need(block_table, "block_table", torch.int32, 2)
+        if block_table.shape[0] != B:
+            raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
+        _need(free_pages, "free_pages", torch.int32, 1)
+        _ints(free_count, "free_count", 1)
+        for t, nm, n in ((keep, "keep", B), (lens_out, "lens_out", B),
+                         (free_count_out, "free_count_out", 1)):
+            if t is not None:
+                _ints(t, nm, n)
+        dev = _one_device("plz_paged_step", *ints)
     rows = B if rows is None else int(rows)
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
-    dev = lens.device
-    out = torch.empty(2 * rows + 2 * B + 2, dtype=torch.int32, device=dev)
-    slots, positions, starts, own_lens, own_count = out.split((rows, rows, B + 1, B, 1))
-    lens_out = own_lens if lens_out is None else _ints(lens_out, "lens_out", B)
-    free_count_out = (own_count if free_count_out is None
-                      else _ints(free_count_out, "free_count_out", 1))
-    _on(lens, (new_tokens, keep, block_table, free_pages, free_count, lens_out, free_count_out),
-        "plz_paged_step", _ptr(lens), _ptr(keep), _ptr(new_tokens), _ptr(block_table),
-        _ptr(free_pages), _ptr(free_count), _ptr(slots), _ptr(positions), _ptr(starts),
-        _ptr(lens_out), _ptr(free_count_out), B, block_table.shape[1], free_pages.shape[0], rows,
-        int(page_size))
+    # the five outputs in one allocation
+    buf = lens.new_empty(2 * (rows + B + 1))
+    slots, positions, starts, own_lens, own_count = buf.split_with_sizes((rows, rows, B + 1, B, 1))
+    if lens_out is None:
+        lens_out = own_lens
+    if free_count_out is None:
+        free_count_out = own_count
+    at = buf.data_ptr()
+    _on(dev, "plz_paged_step", lens.data_ptr(), _ptr(keep), new_tokens.data_ptr(),
+        block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), at, at + 4 * rows,
+        at + 8 * rows, lens_out.data_ptr(), free_count_out.data_ptr(), B, block_table.shape[1],
+        free_pages.shape[0], rows, int(page_size))
     return slots, positions, starts, lens_out, free_count_out
 
 
@@ -1281,24 +1321,33 @@ def paged_rope_write(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_we
     ldq = _token_rows(q, "q", None, D)
     T, H = q.shape[0], q.shape[1]
     ldk, ldv = _token_rows(k, "k", hkv, D), _token_rows(v, "v", hkv, D)
-    if k.shape[0] != T or v.shape[0] != T:
-        raise ValueError("q / k / v have different numbers of tokens")
-    for t, nm in ((cos, "cos"), (sin, "sin")):
-        _need(t, nm, torch.float32, 2)
-    if cos.shape != sin.shape or cos.shape[1] != D:
-        raise ValueError(f"cos and sin must be [positions, {D}]")
-    _ints(positions, "positions", T)
-    _ints(slots, "slots", T)
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight must be given together")
-    if q_weight is not None:
+    normed = q_weight is not None and k_weight is not None
+    if not (k.shape[0] == T and v.shape[0] == T and isinstance(cos, torch.Tensor)
+            and isinstance(sin, torch.Tensor) and cos.dim() == 2 and cos.shape[1] == D
+            and sin.shape == cos.shape and cos.dtype is torch.float32 and sin.dtype is torch.float32
+            and cos.is_cuda and sin.is_cuda and cos.is_contiguous() and sin.is_contiguous()
+            and _dense_int32((positions, slots)) >= 0 and positions.shape == (T,) == slots.shape
+            and (normed or (q_weight is None and k_weight is None))):
+        if k.shape[0] != T or v.shape[0] != T:
+            raise ValueError("q / k / v have different numbers of tokens")
+        for t, nm in ((cos, "cos"), (sin, "sin")):
+            _need(t, nm, torch.float32, 2)
+        if cos.shape != sin.shape or cos.shape[1] != D:
+            raise ValueError(f"cos and sin must be [positions, {D}]")
+        _ints(positions, "positions", T)
+        _ints(slots, "slots", T)
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("q_weight and k_weight must be given together")
+    if normed:
         _norm_weight(q_weight, D)
         _norm_weight(k_weight, D)
-    out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-    _on(q, (k, v, cos, sin, positions, slots, k_cache, v_cache, q_weight, k_weight),
-        "plz_paged_rope_write", _ptr(q), _ptr(k), _ptr(v), ldq, ldk, ldv, _ptr(q_weight),
-        _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots), _ptr(out),
-        _ptr(k_cache), _ptr(v_cache), T, H, hkv, D, cos.shape[0], n, P, float(eps))
+    dev = _one_device("plz_paged_rope_write", q, k, v, cos, sin, positions, slots, k_cache, v_cache,
+                      q_weight, k_weight)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D))
+    _on(dev, "plz_paged_rope_write", q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
+        _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), T, H, hkv, D,
+        cos.shape[0], n, P, float(eps))
     return out
 
 
@@ -1309,15 +1358,19 @@ def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
     n, hkv, P, D = _paged_caches(k_cache, v_cache)
     ldq = _token_rows(q, "q", None, D)
     B, H = q.shape[0], q.shape[1]
-    _need(block_table, "block_table", torch.int32, 2)
-    if block_table.shape[0] != B:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
-    _ints(lens, "lens", B)
+    if not (_dense_int32((block_table, lens)) >= 0 and block_table.dim() == 2
+            and block_table.shape[0] == B and lens.shape == (B,)):
+        _need(block_table, "block_table", torch.int32, 2)
+        if block_table.shape[0] != B:
+            raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
+        _ints(lens, "lens", B)
     scale = D ** -0.5 if scale is None else float(scale)
-    o = torch.empty((B, H, D), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((B, H), dtype=torch.float32, device=q.device)
-    ws = _opt_workspace(query("plz_paged_attn_workspace", B, H, hkv, D), q.device)
-    _on(q, (k_cache, v_cache, block_table, lens), "plz_paged_attn", _ptr(q), ldq, _ptr(k_cache),
-        _ptr(v_cache), _ptr(block_table), _ptr(lens), _ptr(o), _ptr(lse), _ptr(ws), _numel(ws), B,
-        block_table.shape[1], H, hkv, D, n, P, scale)
+    dev = _one_device("plz_paged_attn", q, k_cache, v_cache, block_table, lens)
+    o = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
+    lse = q.new_empty((B, H), dtype=torch.float32)
+    W = block_table.shape[1]
+    ws = _opt_workspace(query("plz_paged_attn_workspace", B, W, P, H, hkv, D), q.device)
+    _on(dev, "plz_paged_attn", q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
+        block_table.data_ptr(), lens.data_ptr(), o.data_ptr(), lse.data_ptr(), _ptr(ws), _numel(ws), B,
+        W, H, hkv, D, n, P, scale)
     return o, lse

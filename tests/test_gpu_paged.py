@@ -304,6 +304,19 @@ def test_attn_many_ragged_requests(dev):
                 + rng.sample(range(1500), 30))
 
 
+@pytest.mark.parametrize("lens,P", [([37], 64), ([128], 128), ([0, 16, 7, 1], 16), ([200], 128)])
+def test_attn_small_tables_without_a_workspace(dev, lens, P):
+    """Tables of a few tiles: one workgroup a kv head, no second launch; one length past its table."""
+    W = -(-128 // P) if len(lens) == 1 else 1
+    c = _attn_case([min(n, W * P) for n in lens], 8, 2, 128, P, 14, dev, width=W)
+    assert ops.query("plz_paged_attn_workspace", len(lens), W, P, 8, 2, 128) == 0
+    if max(lens) > W * P:
+        o, lse = ops.paged_attn(*c[:4], _ints(lens, dev))
+        assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
+    else:
+        _check_attn(*c)
+
+
 @pytest.mark.parametrize("std", [0.05, 12.0])
 def test_attn_flat_and_peaked(dev, std):
     _check_attn(*_attn_case([700, 90, 1, 2100], 8, 2, 128, 64, 5, dev, std=std))

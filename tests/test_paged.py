@@ -194,23 +194,18 @@ def test_cache_refusals(ops):
             ops.paged_cache(4, page, 2, dim, "cpu")
 
 
-def test_tensors_of_two_devices_are_refused(monkeypatch):
+def test_tensors_of_two_devices_are_refused():
     from types import SimpleNamespace
     from palettize_hip import ops as o
-
-    def stop(*args):
-        raise AssertionError("a refused call went through")
-
-    monkeypatch.setattr(o, "call", stop)
     a, b = SimpleNamespace(get_device=lambda: 0), SimpleNamespace(get_device=lambda: 1)
     with pytest.raises(ValueError, match="different devices"):
-        o._on(a, (a, None, b), "plz_paged_step")
+        o._one_device("plz_paged_step", a, None, b)
+    assert o._one_device("plz_paged_step", b, None, b) == 1
 
 
 def test_calls_run_on_their_tensors_device(monkeypatch):
     """The device of the tensors is current during the call, whatever was before, and so is its
     stream."""
-    from types import SimpleNamespace
     from palettize_hip import ops as o
     log, current = [], [0]
 
@@ -229,20 +224,27 @@ def test_calls_run_on_their_tensors_device(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
     for dev in (0, 1):
-        t = SimpleNamespace(get_device=lambda dev=dev: dev)
-        o._on(t, (t, None), "plz_paged_attn", 7)
+        o._on(dev, "plz_paged_attn", 7)
     assert log == [(("plz_paged_attn", 7, 100), 0), (("plz_paged_attn", 7, 101), 1)]
     assert current == [0]
 
 
 def test_attn_needs_its_workspace(lib):
-    need = lib.plz_paged_attn_workspace(3, 8, 2, 128)
+    need = lib.plz_paged_attn_workspace(3, 4, 16, 8, 2, 128)
     assert need > 0
     for kw in (dict(ws=None), dict(nws=need - 1), dict(ws=FAKE + 8)):
         assert lib.plz_paged_attn(*_attn_args(lib, **kw)) == 4
         assert b"workspace" in lib.plz_last_error()
-    for args in ((0, 8, 2, 128), (3, 0, 2, 128), (3, 8, 0, 128), (3, 9, 2, 128), (3, 8, 2, 0)):
+    for args in ((0, 4, 16, 8, 2, 128), (3, 0, 16, 8, 2, 128), (3, 4, 0, 8, 2, 128),
+                 (3, 4, 16, 0, 2, 128), (3, 4, 16, 8, 0, 128), (3, 4, 16, 9, 2, 128),
+                 (3, 4, 16, 8, 2, 0), (-1, 4, 16, 8, 2, 128), (3, -4, 16, 8, 2, 128)):
         assert lib.plz_paged_attn_workspace(*args) == 0
+    # no request is shared where all of them have a tile of 32 for each of four waves at most
+    assert lib.plz_paged_attn_workspace(1, 2, 64, 8, 2, 128) == 0
+    assert lib.plz_paged_attn_workspace(4, 1, 32, 8, 2, 128) == 0
+    assert lib.plz_paged_attn_workspace(1, 9, 16, 8, 2, 128) > 0
+    assert lib.plz_paged_attn_workspace(5, 1, 16, 8, 2, 128) > 0
+    assert lib.plz_paged_attn_workspace(1 << 40, 1 << 40, 1024, 8, 2, 128) > 0
 
 
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not available")

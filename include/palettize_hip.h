@@ -718,13 +718,16 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
  * then, keep + new unless pages ran out. The step's token rows follow each other in order of b:
  * request b has the rows starts[b] .. starts[b + 1] - 1 (starts [batch + 1]; rows past the given
  * `rows` are cut off), with their positions [rows] and slots [rows] (-1: no room). Rows behind the
- * last request's get slot -1 and position 0. free_count_out[0]: the pages left. lens_out and
- * free_count_out may be lens and free_count themselves. */
+ * last request's get slot -1 and position 0. With rows_each > 0 (rows = batch rows_each) every
+ * request owns rows_each rows instead, starts[b] = b rows_each, has at most that many new tokens, and
+ * the rows past them get slot -1 and position 0: a decoding batch whose row b is request b.
+ * free_count_out[0]: the pages left. lens_out and free_count_out may be lens and free_count themselves;
+ * lens_out is neither new_tokens nor keep. */
 int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_tokens,
                    int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
                    int32_t* slots, int32_t* positions, int32_t* starts, int32_t* lens_out,
                    int32_t* free_count_out, int64_t batch, int64_t width, int64_t num_pages,
-                   int64_t rows, int page_size, void* stream);
+                   int64_t rows, int64_t rows_each, int page_size, void* stream);
 /* The rows of a step on their way into the cache: q bf16 [tokens, heads, head_dim], k, v bf16
  * [tokens, kv_heads, head_dim], consecutive tokens ld_q, ld_k, ld_v elements apart (multiples of 8:
  * the three may lie side by side in one projection's output), head_dim 64, 128 or 256.

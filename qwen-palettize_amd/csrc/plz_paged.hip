@@ -24,6 +24,7 @@ namespace paged {
 //   given_b = clamp(pool - sum_{b' < b} want_b', 0, want_b)
 //   lens_out[b] = min(k + a, (pages(k) + given_b) P): what has room; token i of b, row starts[b] + i,
 //   has position k + i and the slot of that position, -1 where there is no room.
+// starts is the running sum of a, or b `each` where every request owns `each` rows (a at most that).
 // Everything is a prefix sum over the requests, then independent work a page and a token, which find
 // their request by binary search in the sums. One workgroup does it, a thread a request (in chunks of
 // its threads, twice, for larger batches: the pages handed back have to be on the stack before any is
@@ -37,6 +38,7 @@ struct StepArgs {
   const int32_t* count;
   int32_t *slots, *pos, *starts, *lens_out, *count_out;
   int B, W, F, rows, shift;  // shift = log2 P
+  int each;                  // rows a request owns, 0: as many as it has tokens
 };
 
 // The last i in [0, n) with start[i] <= j (start ascending, start[0] <= j)
@@ -78,7 +80,7 @@ __device__ __forceinline__ void block_scan(int& v, int& u, int cap, int2* part) 
 template <int ST, bool TOKENS>
 __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
   __shared__ int2 part[ST / 64];
-  __shared__ int s_tok[ST], s_page[ST], s_keep[ST], s_hold[ST], s_len[ST], s_last[2];
+  __shared__ int s_tok[ST], s_page[ST], s_keep[ST], s_hold[ST], s_len[ST], s_new[ST], s_last[2];
   const int tid = threadIdx.x, P1 = (1 << g.shift) - 1, cap = g.W << g.shift;
   const int count = clampi(*g.count, 0, g.F);
   const bool one = g.B <= ST;  // all requests at once
@@ -88,9 +90,11 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     if (b < g.B) {
       L = clampi(g.lens[b], 0, cap);
       k = g.keep ? clampi(g.keep[b], 0, L) : L;
-      a = clampi(g.add[b], 0, g.rows);
+      a = clampi(g.add[b], 0, g.each ? g.each : g.rows);
     }
   };
+  // a request's rows: as many as its tokens, or those that it owns (rows = B each then)
+  auto owned = [&](int b) { return g.each ? (b < g.B ? g.each : 0) : a; };
   // pages handed back
   int back = 0;  // by the chunks before
   int ends = 0;  // of a single chunk: the token rows up to this request's last
@@ -99,7 +103,7 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     load(b0 + tid);
     const int hold = (k + P1) >> g.shift, n = ((L + P1) >> g.shift) - hold;
     int end = n;
-    ends = a;
+    ends = owned(b0 + tid);
     block_scan<ST>(end, ends, g.rows, part);
     s_hold[tid] = hold;
     s_page[tid] = end - n;
@@ -121,7 +125,7 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     int none = 0;
     if (!one) {
       load(b);
-      ends = a;
+      ends = owned(b);
       block_scan<ST>(none, ends, g.rows, part);
       ends = min(tok0 + ends, g.rows);
     }
@@ -129,7 +133,7 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     s_tok[tid] = ends;
     __syncthreads();
     const int tok = tid ? s_tok[tid - 1] : tok0;
-    a = ends - tok;
+    a = min(a, ends - tok);
     const int hold = (k + P1) >> g.shift;
     const int full = (int)min((int64_t)k + a, (int64_t)cap);
     const int want = ((full + P1) >> g.shift) - hold;
@@ -145,6 +149,7 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     s_keep[tid] = k;
     s_hold[tid] = hold;
     s_len[tid] = len;
+    s_new[tid] = a;
     if (tid == ST - 1) {
       s_last[0] = ends;
       s_last[1] = want_end;
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     if (b < g.B) {
       g.lens_out[b] = len;
       g.starts[b + 1] = ends;
-      if (!TOKENS && a > 0) g.pos[tok] = k;
+      if (!TOKENS && ends > tok) g.pos[tok] = a > 0 ? k : -1;
     }
     __syncthreads();
     const int tok1 = s_last[0], want1 = s_last[1];
@@ -162,9 +167,10 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
     }
     if constexpr (TOKENS)
       for (int t = tok0 + tid; t < tok1; t += ST) {
-        const int r = find_row(s_tok, nb, t), pos = s_keep[r] + t - s_tok[r];
+        const int r = find_row(s_tok, nb, t), i = t - s_tok[r];
+        const int pos = i < s_new[r] ? s_keep[r] + i : 0;
         int slot = -1;
-        if (pos < s_len[r]) {
+        if (i < s_new[r] && pos < s_len[r]) {
           const int w = pos >> g.shift;
           const int page = w < s_hold[r] ? g.table[(int64_t)(b0 + r) * g.W + w]
                                          : g.stack[pool - 1 - (s_page[r] + w - s_hold[r])];
@@ -205,12 +211,14 @@ __global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
     int slot = -1, pos = 0;
     if (t < total) {
       const int b = find_row(starts, g.B, t), i = t - starts[b];
-      pos = g.pos[t - i] + i;
-      if (pos < g.lens_out[b]) {
+      const int k = g.pos[t - i];  // -1: the request owns rows and has no token
+      const bool live = k >= 0 && (!g.each || i < g.add[b]);
+      pos = live ? k + i : 0;
+      if (live && pos < g.lens_out[b]) {
         const int page = g.table[(int64_t)b * g.W + (pos >> g.shift)];
         if (page >= 0 && page < g.F) slot = (page << g.shift) + (pos & P1);
       }
-      if (i == 0) {
+      if (i == 0 && k >= 0) {
         g.slots[t] = slot;
         continue;
       }
@@ -338,7 +346,7 @@ int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_
                    int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
                    int32_t* slots, int32_t* positions, int32_t* starts, int32_t* lens_out,
                    int32_t* free_count_out, int64_t batch, int64_t width, int64_t num_pages,
-                   int64_t rows, int page_size, void* stream) {
+                   int64_t rows, int64_t rows_each, int page_size, void* stream) {
   PLZ_REQUIRE(batch >= 0 && width >= 0 && num_pages >= 0 && rows >= 0,
               "plz_paged_step: negative shape");
   PLZ_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
@@ -349,15 +357,20 @@ int plz_paged_step(const int32_t* lens, const int32_t* keep, const int32_t* new_
                   num_pages * page_size <= lim,
               "plz_paged_step: batch x width, width x page_size, num_pages x page_size and rows "
               "go up to 2^30");
+  PLZ_REQUIRE(rows_each >= 0 && rows_each <= lim && (rows_each == 0 || rows == batch * rows_each),
+              "plz_paged_step: with rows_each (%lld) there are batch x rows_each rows, got %lld",
+              (long long)rows_each, (long long)rows);
   PLZ_REQUIRE(free_count && free_count_out && starts && (num_pages == 0 || free_pages) &&
                   (batch == 0 || (lens && new_tokens && lens_out)) &&
                   (batch * width == 0 || block_table) && (rows == 0 || (slots && positions)),
               "plz_paged_step: null pointer");
+  PLZ_REQUIRE(batch == 0 || (lens_out != new_tokens && lens_out != keep),
+              "plz_paged_step: lens_out may be lens, not new_tokens or keep");
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
   const StepArgs g{lens,  keep,   new_tokens, block_table,    free_pages, free_count, slots,
                    positions, starts, lens_out,   free_count_out, (int)batch, (int)width,
-                   (int)num_pages, (int)rows, shift};
+                   (int)num_pages, (int)rows, shift, (int)rows_each};
   auto launch = [&](auto kernel, int blocks, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, (hipStream_t)stream,
                        g);

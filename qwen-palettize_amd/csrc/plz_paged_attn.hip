@@ -32,7 +32,7 @@ namespace plz {
 namespace paged {
 
 constexpr int NW = 4, NT = 64 * NW;  // waves, threads
-constexpr int PARTS = 512;           // workgroups: two for each of 256 CUs
+constexpr int PARTS = 512;           // most workgroups: two for each of 256 CUs (parts_of)
 constexpr int HT = 16;               // heads a workgroup (columns of the matrix instruction)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
@@ -550,9 +550,13 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
 static bool never_shared(int64_t batch, int64_t width, int64_t page_size) {
   return batch <= NW && width <= NW * TILE && batch * ((width * page_size + TILE - 1) / TILE) <= NW;
 }
-// workgroups a (kv head, head tile)
-static int parts_of(int kv_heads, int head_tiles) {
-  const int n = PARTS / (kv_heads * head_tiles);
+// Workgroups a (kv head, head tile): two a CU in all, one where a part is large (more than 1024 values:
+// writing and joining them costs more than the second workgroup's loads bring) or a workgroup takes the
+// whole CU's registers (heads of 256). Two and one: 16 x 4096 tokens, 4 kv heads of 128 with 20 heads
+// each 38.5 and 34.8 us, 32 ragged up to 4096 with 8 heads 16.4 and 16.6; 8 kv heads of 256 with 4, 32 x 2048 93.4 and 88.1.
+static int parts_of(int kv_heads, int G, int D) {
+  const int heads = G < HT ? G : HT, tiles = (G + HT - 1) / HT;
+  const int n = (D == 256 || heads * D > 1024 ? PARTS / 2 : PARTS) / (kv_heads * tiles);
   return n > 1 ? n : 1;
 }
 template <int D>
@@ -590,7 +594,7 @@ size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int
       heads % kv_heads || never_shared(batch, width, page_size))
     return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
-  const size_t parts = (size_t)parts_of(kv_heads, ht);
+  const size_t parts = (size_t)parts_of(kv_heads, G, head_dim);
   return parts * kv_heads * ht * 2 * (G < HT ? G : HT) * head_dim * sizeof(float) +
          parts * heads * 2 * sizeof(float2) + parts * sizeof(int2);
 }
@@ -636,7 +640,7 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
              (int)batch, (int)width, heads, kv_heads, heads / kv_heads, 0, 0, (int)num_pages, 0,
              scale * kLog2e};
   g.tiles_h = (g.G + HT - 1) / HT;
-  g.parts = parts_of(kv_heads, g.tiles_h);
+  g.parts = parts_of(kv_heads, g.G, head_dim);
   if (need == 0) {
     g.parts = 1;  // the one workgroup (a kv head and head tile) that gets any tiles
   } else {

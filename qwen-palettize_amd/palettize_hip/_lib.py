@@ -153,7 +153,7 @@ SIGNATURES: dict[str, tuple] = {
     "plz_swiglu_bwd": (i32, [p, p, p, p, p, i64, p]),
     "plz_swiglu_fwd_rows": (i32, [p, p, i64, p, i64, i64, i64, p]),
     "plz_swiglu_bwd_rows": (i32, [p, p, i64, p, i64, p, p, i64, i64, i64, p]),
-    "plz_paged_step": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i32, p]),
+    "plz_paged_step": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i64, i32, p]),
     "plz_paged_rope_write": (i32, [p, p, p, i64, i64, i64, p, p, p, p, p, p, p, p, p, i64, i32, i32,
                                    i32, i64, i64, i32, f32, p]),
     "plz_paged_attn_workspace": (sz, [i64, i64, i32, i32, i32, i32]),

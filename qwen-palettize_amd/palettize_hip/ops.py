@@ -1259,14 +1259,16 @@ def _token_rows(t, name, heads=None, dim=None):
 
 
 def paged_step(lens, new_tokens, block_table, free_pages, free_count, page_size, keep=None,
-               rows=None, lens_out=None, free_count_out=None):
+               rows=None, rows_each=0, lens_out=None, free_count_out=None):
     """One scheduler step of a paged cache: pages handed back and taken, and where the step's
     tokens go (plz_paged_step).
 
     lens, new_tokens, keep (optional) int32 [B]: the tokens each request has, adds and keeps of what
     it has (None: all; 0 ends a request and frees its row). block_table int32 [B, W] and free_pages
     int32 [num_pages], the stack of the pages that nobody holds, are updated in place; free_count
-    int32 [1] of them are valid. rows: the size of the token buffer (default B: one token each).
+    int32 [1] of them are valid. rows: the size of the token buffer (default B: one token each), in
+    which the requests' tokens follow each other; with rows_each every request owns that many rows of
+    it and adds at most that many tokens (rows is B rows_each: 1 for a batch whose row b is request b).
     Returns (slots [rows], positions [rows], starts [B + 1], lens [B], free_count [1]); lens_out and
     free_count_out receive the last two (lens and free_count themselves may be given). A request
     that finds no page keeps the tokens that have room, and the others get slot -1."""
@@ -1293,9 +1295,10 @@ def paged_step(lens, new_tokens, block_table, free_pages, free_count, page_size,
             if t is not None:
                 _ints(t, nm, n)
         dev = _one_device("plz_paged_step", *ints)
-    rows = B if rows is None else int(rows)
-    if rows < 0:
-        raise ValueError(f"rows must not be negative, got {rows}")
+    rows = B * (rows_each or 1) if rows is None else int(rows)
+    if rows < 0 or rows_each < 0 or (rows_each and rows != B * rows_each):
+        raise ValueError(f"rows ({rows}) must be at least 0, and B rows_each with rows_each "
+                         f"({rows_each})")
     # the five outputs in one allocation
     buf = lens.new_empty(2 * (rows + B + 1))
     slots, positions, starts, own_lens, own_count = buf.split_with_sizes((rows, rows, B + 1, B, 1))
@@ -1307,7 +1310,7 @@ def paged_step(lens, new_tokens, block_table, free_pages, free_count, page_size,
     _on(dev, "plz_paged_step", lens.data_ptr(), _ptr(keep), new_tokens.data_ptr(),
         block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), at, at + 4 * rows,
         at + 8 * rows, lens_out.data_ptr(), free_count_out.data_ptr(), B, block_table.shape[1],
-        free_pages.shape[0], rows, int(page_size))
+        free_pages.shape[0], rows, rows_each, int(page_size))
     return slots, positions, starts, lens_out, free_count_out
 
 
@@ -1369,8 +1372,9 @@ def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
     o = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
     lse = q.new_empty((B, H), dtype=torch.float32)
     W = block_table.shape[1]
-    ws = _opt_workspace(query("plz_paged_attn_workspace", B, W, P, H, hkv, D), q.device)
+    nbytes = query("plz_paged_attn_workspace", B, W, P, H, hkv, D)
+    ws = lens.new_empty((nbytes + 3) // 4) if nbytes else None
     _on(dev, "plz_paged_attn", q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
-        block_table.data_ptr(), lens.data_ptr(), o.data_ptr(), lse.data_ptr(), _ptr(ws), _numel(ws), B,
+        block_table.data_ptr(), lens.data_ptr(), o.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, B,
         W, H, hkv, D, n, P, scale)
     return o, lse

@@ -9,7 +9,7 @@ def pages(n, P):
     return -(-n // P)
 
 
-def step(lens, keep, new, table, free, count, P, rows):
+def step(lens, keep, new, table, free, count, P, rows, each=0):
     """paged_step on lists, literally: (slots, positions, starts, lens, count, table, free)."""
     table, free = [list(r) for r in table], list(free)
     W, F = len(table[0]) if table else 0, len(free)
@@ -25,7 +25,7 @@ def step(lens, keep, new, table, free, count, P, rows):
                 count += 1
     slots, positions, starts, out = [-1] * rows, [0] * rows, [0], []
     for b, k in enumerate(kept):
-        a = min(max(new[b], 0), rows - starts[-1])
+        a = min(max(new[b], 0), each or rows - starts[-1])
         have = pages(k, P)
         while have < pages(min(k + a, W * P), P) and count > 0:
             count -= 1
@@ -37,7 +37,7 @@ def step(lens, keep, new, table, free, count, P, rows):
             positions[starts[-1] + i] = pos
             if pos < out[b] and 0 <= table[b][pos // P] < F:
                 slots[starts[-1] + i] = table[b][pos // P] * P + pos % P
-        starts.append(starts[-1] + a)
+        starts.append(starts[-1] + (each or a))
     return slots, positions, starts, out, count, table, free
 
 

@@ -19,10 +19,10 @@ def _ints(v, dev):
 
 # ---- scheduler step ---------------------------------------------------------------------------
 def _run_step(c, dev, keep=True, **kw):
-    t = {k: _ints(v, dev) for k, v in c.items() if k not in ("P", "rows")}
+    t = {k: _ints(v, dev) for k, v in c.items() if k not in ("P", "rows", "each")}
     out = ops.paged_step(t["lens"], t["new"], t["table"].reshape(len(c["lens"]), -1), t["free"],
                          t["count"].reshape(1), c["P"], keep=t["keep"] if keep else None,
-                         rows=c["rows"], **kw)
+                         rows=c["rows"], rows_each=c.get("each", 0), **kw)
     return (*out, t["table"], t["free"])
 
 
@@ -58,6 +58,23 @@ def test_step_of_many_requests(dev, B):
     c = dict(lens=lens, keep=keep, new=new, table=table, count=len(ids), free=ids + [0] * (F - len(ids)),
              P=P, rows=sum(new) + 5)
     _same_step(_run_step(c, dev), paged_ref.step(**c), B)
+
+
+@pytest.mark.parametrize("each", [1, 4, 200])
+def test_step_with_rows_of_their_own(dev, each):
+    """Every request owns `each` rows, in one launch and in two: row b each is request b's first token,
+    also where others have none, more than they own, or no room."""
+    rng = random.Random(30 + each)
+    for i in range(12):
+        c = random_step(rng, short=i % 3 == 0)
+        _same_step(_run_step(dict(c, rows=len(c["lens"]) * each, each=each), dev),
+                   paged_ref.step(**dict(c, rows=len(c["lens"]) * each, each=each)), c)
+    B, P, W = 3000, 16, 20
+    new = [rng.choice((0, 0, 1, each, each + 3, -2)) for _ in range(B)]
+    c = dict(lens=[rng.randint(0, 30) for _ in range(B)], keep=[0] * B, new=new,
+             table=[[7] * W for _ in range(B)], free=list(range(4000)) + [0] * 6000, count=4000, P=P,
+             rows=B * each, each=each)
+    _same_step(_run_step(c, dev), paged_ref.step(**c), each)
 
 
 @pytest.mark.parametrize("rows_more", [0, 3])

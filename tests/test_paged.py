@@ -26,8 +26,8 @@ def lib():
 
 def _step_args(**kw):
     a = dict(lens=FAKE, keep=FAKE, new=FAKE, table=FAKE, free=FAKE, count=FAKE, slots=FAKE, pos=FAKE,
-             starts=FAKE, lens_out=FAKE, count_out=FAKE, batch=4, width=8, pages=32, rows=4, page=16,
-             stream=None)
+             starts=FAKE, lens_out=2 * FAKE, count_out=FAKE, batch=4, width=8, pages=32, rows=4, each=0,
+             page=16, stream=None)
     assert set(kw) <= set(a)
     return list({**a, **kw}.values())
 
@@ -40,7 +40,10 @@ def _step_args(**kw):
     (dict(pages=1 << 27), b"2^30"), (dict(lens=None), b"null"), (dict(new=None), b"null"),
     (dict(table=None), b"null"), (dict(free=None), b"null"), (dict(count=None), b"null"),
     (dict(slots=None), b"null"), (dict(pos=None), b"null"), (dict(starts=None), b"null"),
-    (dict(lens_out=None), b"null"), (dict(count_out=None), b"null")])
+    (dict(lens_out=None), b"null"), (dict(count_out=None), b"null"), (dict(each=2), b"rows_each"),
+    (dict(each=-1), b"rows_each"), (dict(each=1, rows=3), b"rows_each"),
+    (dict(new=FAKE + 64, lens_out=FAKE + 64, keep=None), b"new_tokens or keep"),
+    (dict(lens_out=FAKE), b"new_tokens or keep")])
 def test_step_refusals(lib, kw, word):
     assert lib.plz_paged_step(*_step_args(**kw)) == 1
     assert word in lib.plz_last_error()
@@ -146,6 +149,7 @@ def test_step_wrapper_refusals(ops):
                      (dict(block_table=_i32(4, 2).t()), ValueError),
                      (dict(free_pages=_i32(2, 4)), ValueError), (dict(free_count=_i32(2)), ValueError),
                      (dict(keep=_i32(3)), ValueError), (dict(rows=-1), ValueError),
+                     (dict(rows_each=-1), ValueError), (dict(rows_each=2, rows=3), ValueError),
                      (dict(lens_out=_i32(3)), ValueError), (dict(free_count_out=_i32(2)), ValueError),
                      (dict(lens=[1, 2]), TypeError)):
         with pytest.raises(err):

@@ -1,0 +1,166 @@
+"""GPU: palettized layers that answer token by token over a paged cache (palettize_hip.decode) against
+the same layers in 64 bits over whole sequences."""
+import math
+
+import pytest
+import torch
+
+from helpers import assert_close, f32
+
+pytestmark = pytest.mark.gpu
+decode = pytest.importorskip("palettize_hip.decode")
+layer = pytest.importorskip("palettize_hip.layer")
+
+CFGS = {"d128": dict(hidden=256, heads=4, kv_heads=2, head_dim=128, intermediate=512),
+        "d64": dict(hidden=256, heads=8, kv_heads=2, head_dim=64, intermediate=512)}
+
+
+def _layers(dev, kw, n=2):
+    cfg = layer.LayerConfig(**kw)
+    soft = [layer.PalettizedDecoderLayer(cfg, seed=i, device=dev, lora_b_std=0.02) for i in range(n)]
+    for i, s in enumerate(soft):  # the logits away from their one-hot start, norms away from one
+        g = torch.Generator().manual_seed(50 + i)
+        for lin in s.linears():
+            lin.index_logits.data.copy_(torch.randn(lin.index_logits.shape, generator=g))
+        for nm in decode.HardDecoderLayer.NORMS:
+            w = getattr(s, nm).weight
+            w.data.copy_(1 + 0.2 * torch.randn(w.shape, generator=g))
+    return cfg, [decode.HardDecoderLayer.from_soft(s) for s in soft], soft
+
+
+def _norm(x, w, eps):
+    return x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+
+
+def _reference(cfg, soft, hs, cos, sin):
+    """The layers on one sequence [S, hidden] in 64 bits, weights dequantised as bf16."""
+    S, D, G = hs.shape[0], cfg.head_dim, cfg.heads // cfg.kv_heads
+    c, s = cos[:S, None].double(), sin[:S, None].double()
+    mask = torch.triu(torch.ones(S, S, dtype=torch.bool, device=hs.device), 1)
+    for l in soft:
+        def lin(name, x):
+            p = getattr(l, name)
+            idx = p.index_logits.argmax(-1)
+            pal = p.palette.to(torch.bfloat16).repeat_interleave(256, 1)
+            w = torch.gather(pal, 2, idx[..., None])[..., 0].double()
+            return x @ w.T + p.lora_scale * (x @ p.lora_a.double().T) @ p.lora_b.double().T
+
+        def rope(x):
+            a, b = x.chunk(2, -1)
+            return x * c + torch.cat([-b, a], -1) * s
+
+        x = _norm(hs, l.input_layernorm.weight, cfg.eps)
+        q = rope(_norm(lin("q_proj", x).view(S, -1, D), l.q_norm.weight, cfg.eps))
+        k = rope(_norm(lin("k_proj", x).view(S, -1, D), l.k_norm.weight, cfg.eps))
+        v = lin("v_proj", x).view(S, -1, D)
+        k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+        score = torch.stack([q[:, h] @ k[:, h].T for h in range(cfg.heads)]) / math.sqrt(D)
+        p = torch.softmax(score.masked_fill(mask, -math.inf), -1)
+        o = torch.stack([p[h] @ v[:, h] for h in range(cfg.heads)], 1).reshape(S, -1)
+        hs = hs + lin("o_proj", o)
+        x = _norm(hs, l.post_attention_layernorm.weight, cfg.eps)
+        g = lin("gate_proj", x)
+        hs = hs + lin("down_proj", g * torch.sigmoid(g) * lin("up_proj", x))
+    return hs
+
+
+@pytest.mark.parametrize("kw", CFGS.values(), ids=CFGS.keys())
+def test_prompts_then_tokens(dev, kw):
+    """Prompts of 5, 130 and 64 tokens, then eleven steps in which a request ends, its row takes a new
+    prompt, and one row pauses: every row of every step against the whole sequence so far."""
+    cfg, hard, soft = _layers(dev, kw)
+    cos, sin = layer.rope_tables(256, cfg.head_dim, cfg.rope_theta, dev)
+    cache = decode.PagedKVCache(2, 3, 256, cfg.kv_heads, cfg.head_dim, page_size=16, device=dev)
+    g = torch.Generator().manual_seed(1)
+    seqs = [torch.zeros(0, cfg.hidden, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+
+    def tokens(n):
+        return torch.randn(n, cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+
+    def prefill(lens, keep=None):
+        step = cache.step(lens, keep)
+        parts = [tokens(n) for n in lens]
+        for b, n in enumerate(lens):
+            if n:
+                seqs[b] = parts[b]
+        hs = torch.cat(parts)
+        for i, l in enumerate(hard):
+            hs = l.prefill(hs, cache, i, step, lens, cos, sin)
+        row = 0
+        for b, n in enumerate(lens):
+            if n:
+                assert_close(f32(hs[row:row + n]), f32(_reference(cfg, soft, seqs[b].double(), cos, sin)),
+                             what=f"prompt of {n}")
+            row += n
+
+    prefill([5, 130, 64])
+    for t in range(11):
+        if t == 6:  # request 0 ends; its row starts again
+            prefill([33, 0, 0], keep=[0] + cache.lens.tolist()[1:])
+        new = [1, 1, 0 if t % 4 == 2 else 1]
+        step = cache.step(new, rows_each=1)
+        hs = tokens(3)
+        for b in range(3):
+            if new[b]:
+                seqs[b] = torch.cat([seqs[b], hs[b:b + 1]])
+        for i, l in enumerate(hard):
+            hs = l.decode(hs, cache, i, step, cos, sin)
+        assert cache.lens.tolist() == [len(s) for s in seqs]
+        for b in range(3):
+            if new[b]:
+                want = _reference(cfg, soft, seqs[b].double(), cos, sin)[-1:]
+                assert_close(f32(hs[b:b + 1]), f32(want), what=f"step {t} request {b}")
+    held = sum(-(-len(s) // 16) for s in seqs)
+    assert int(cache.free_count) == cache.num_pages - held
+
+
+def test_captured_step(dev):
+    """A step of two layers captured once and replayed with other tokens and counts, eager steps of
+    another batch and synchronisations in between, against the same steps run eagerly, bit for bit."""
+    cfg, hard, _ = _layers(dev, CFGS["d128"])
+    cos, sin = layer.rope_tables(128, cfg.head_dim, cfg.rope_theta, dev)
+    caches = [decode.PagedKVCache(2, 4, 128, cfg.kv_heads, cfg.head_dim, page_size=16, device=dev)
+              for _ in range(3)]
+    new = torch.ones(4, dtype=torch.int32, device=dev)
+    hs = torch.zeros(4, cfg.hidden, dtype=torch.bfloat16, device=dev)
+
+    def one(cache, x, n):
+        step = cache.step(n, rows_each=1)
+        for i, l in enumerate(hard):
+            x = l.decode(x, cache, i, step, cos, sin)
+        return x
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(caches[2], hs, new)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one(caches[0], hs, new)
+    g = torch.Generator().manual_seed(4)
+    for t in range(30):
+        x = torch.randn(4, cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+        n = torch.tensor([1, t % 2, 1, 1 if t > 9 else 0], dtype=torch.int32, device=dev)
+        want = one(caches[1], x, n)
+        hs.copy_(x)
+        new.copy_(n)
+        graph.replay()
+        if t % 3 == 0:
+            one(caches[2], x, n)
+        if t % 5 == 0:
+            torch.cuda.synchronize()
+        live = n.bool()
+        assert torch.equal(out[live], want[live]), t
+        assert torch.equal(caches[0].lens, caches[1].lens)
+
+
+def test_pages_run_out_and_come_back(dev):
+    """A pool smaller than its requests: what found no page is not in lens, and a request that ends
+    makes room."""
+    cache = decode.PagedKVCache(1, 3, 64, 2, 64, page_size=16, num_pages=4, device=dev)
+    cache.step([40, 20, 5])
+    assert cache.lens.tolist() == [40, 16, 0] and int(cache.free_count) == 0
+    step = cache.step([0, 4, 5], keep=[0, 16, 0])
+    assert cache.lens.tolist() == [0, 20, 5] and int(cache.free_count) == 1
+    assert int((step.slots >= 0).sum()) == 9

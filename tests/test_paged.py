@@ -322,3 +322,19 @@ def test_step_reference_conserves_pages():
         _, _, _, lens, count, table, free = paged_ref.step(**c)
         held = [p for b, n in enumerate(lens) for p in table[b][:paged_ref.pages(n, c["P"])]]
         assert sorted(held + free[:count]) == list(range(F))
+
+
+def test_cache_and_layer_refusals():
+    from palettize_hip import decode
+    for kw in (dict(batch=0), dict(layers=0), dict(max_tokens=0), dict(num_pages=0), dict(page_size=24),
+               dict(head_dim=100)):
+        with pytest.raises(ValueError):
+            decode.PagedKVCache(**{**dict(layers=1, batch=2, max_tokens=64, kv_heads=2, head_dim=64,
+                                          device="cpu"), **kw})
+    c = decode.PagedKVCache(2, 3, 100, 2, 64, page_size=16, device="cpu")
+    assert c.num_pages == 3 * 7 and c.block_table.shape == (3, 7) and len(c.k) == len(c.v) == 2
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        c.step([1, 1, 1])
+    with pytest.raises(ValueError, match="rows"):
+        decode.HardDecoderLayer.prefill.__wrapped__(
+            type("L", (), {"cfg": None})(), torch.zeros(5, 8), c, 0, None, [2, 2], None, None)

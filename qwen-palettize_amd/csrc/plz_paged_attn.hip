@@ -22,7 +22,7 @@
 // moves only when a tile exceeds it by more than 2^8.
 //
 // Each wave has a run of tiles (plz_paged.h) and goes through its requests without a word to the
-// others; the next request's length, pages and queries are on their way while it is at this one. Only
+// others; the next requests' lengths, pages and queries are on their way while it is at this one. Only
 // what a run has of a request that it does not have whole is joined: through LDS among the waves of a
 // workgroup, through the workspace among workgroups, by a second kernel, both in the order of the runs.
 #include "plz_paged.h"
@@ -236,22 +236,34 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     int t = r0 - first, t0 = t, pos = r0;  // tile of the request, its first one here; tile among all
     int page_t = t, pages = fetch_pages(b, t, len, n);
     load_q(b, qf);
-    bool bad = check_pages(pages), bad_next = false;
-    int b_next = 0, len_next = 0, n_next = 0, pages_next = 0;
-    auto look_ahead = [&]() {  // the next request with tokens, if the run goes on to it
-      if (first + n >= r1) return;
-      for (b_next = min(b + 1, g.B - 1);; ++b_next) {
-        if (b_next >= win_at + 64) {
-          win_at = b_next;
+    bool bad_next = false;
+    // The requests that the run goes on to: the next one, whose queries are loaded while this one is
+    // worked on, and the one after it, whose pages are: loads come back in order, so pages asked for
+    // behind a tile's K and V would hold up the tile that needs them until those are here.
+    int b1 = 0, len1 = 0, n1 = 0, pages1 = 0, b2 = 0, len2 = 0, n2 = 0, pages2 = 0;
+    auto find_after = [&](int req, int& at_req, int& tokens, int& tiles) {
+      for (at_req = min(req + 1, g.B - 1);; ++at_req) {
+        if (at_req >= win_at + 64) {
+          win_at = at_req;
           win = win_at + lane < g.B ? g.lens[win_at + lane] : 0;
         }
-        len_next = __builtin_amdgcn_readlane(win, b_next - win_at);
-        n_next = tiles_of(len_next, cap);
-        if (n_next > 0 || b_next == g.B - 1) break;
+        tokens = __builtin_amdgcn_readlane(win, at_req - win_at);
+        tiles = tiles_of(tokens, cap);
+        if (tiles > 0 || at_req == g.B - 1) break;
       }
-      pages_next = fetch_pages(b_next, 0, len_next, n_next);
-      load_q(b_next, qn);
     };
+    auto look_ahead = [&]() {
+      if (first + n >= r1) return;
+      load_q(b1, qn);
+      if (first + n + n1 >= r1) return;
+      find_after(b1, b2, len2, n2);
+      pages2 = fetch_pages(b2, 0, len2, n2);
+    };
+    if (first + n < r1) {
+      find_after(b, b1, len1, n1);
+      pages1 = fetch_pages(b1, 0, len1, n1);
+    }
+    bool bad = check_pages(pages);
     {
       const int page0 = __builtin_amdgcn_readlane(pages, 0), page1 = __builtin_amdgcn_readlane(pages, 1);
       load_k(page0, page1, t);
@@ -279,9 +291,9 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
           page0 = __builtin_amdgcn_readlane(pages, 2 * (t_next - page_t));
           page1 = __builtin_amdgcn_readlane(pages, 2 * (t_next - page_t) + 1);
         } else {
-          bad_next = check_pages(pages_next);
-          page0 = __builtin_amdgcn_readlane(pages_next, 0);
-          page1 = __builtin_amdgcn_readlane(pages_next, 1);
+          bad_next = check_pages(pages1);
+          page0 = __builtin_amdgcn_readlane(pages1, 0);
+          page1 = __builtin_amdgcn_readlane(pages1, 1);
         }
         load_k(page0, page1, t_next);
       }
@@ -388,8 +400,8 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       }
       if (!more) break;
       first += n;
-      b = b_next, len = len_next, n = n_next;
-      pages = pages_next, bad = bad_next;
+      b = b1, len = len1, n = n1, pages = pages1, bad = bad_next;
+      b1 = b2, len1 = len2, n1 = n2, pages1 = pages2;
       page_t = t = t0 = 0;
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[s] = qn[s];

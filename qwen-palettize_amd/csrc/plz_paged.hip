@@ -234,7 +234,10 @@ __global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
 // at the token's position p, all in fp32 and rounded once to bf16 (the training layers' norm and
 // rotation round the normalised and the weighted value too, as the modules that they stand for do:
 // here there is no such module to match). D / 8 lanes a row, 8 values a lane; the partner of value
-// j is in lane l ^ (D / 16).
+// j is in lane l ^ (D / 16). Bound by its bytes: 16384 tokens of 32/8 heads of 128 (407 MB read and
+// written) take 86 us, 4.7 TB/s where a plain copy reaches 5.1; up to 8 heads a workgroup share their
+// tokens' sines (109 us with one, 91 with 16), 4 rows of a lane in flight. K in its 8-value pieces is
+// stored as fast as in rows would be (86.1 and 85.7). One token takes the 3 us of its memory latencies.
 struct WriteArgs {
   const uint16_t *q, *k, *v, *qw, *kw;
   const float *cosv, *sinv;

@@ -6,6 +6,7 @@ Host-side mirror of the reference's Python interface over the C ABI of libpalett
   fused_lut_linear_cuda   drop-in for the reference module of the same name
   qwen_model              PalettizedLinear / QwenLoRA with the reference's constructor API
   layer                   one palettized Qwen-4B-shaped decoder layer training step
+  decode                  palettized layers that answer token by token over a paged key-value cache
 """
 from . import _lib, ops  # noqa: F401
 from ._lib import (PLZ_W_HARD_NOISY, PLZ_W_HARD_PLAIN, PLZ_W_SOFT,  # noqa: F401

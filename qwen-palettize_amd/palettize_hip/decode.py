@@ -28,6 +28,11 @@ from .layer import LayerConfig, PalettizedDecoderLayer, attention
 Step = namedtuple("Step", "slots positions starts")
 
 
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("decoding has no backward: call it under torch.no_grad()")
+
+
 class PagedKVCache:
     """Keys and values of `layers` layers for up to `batch` requests of up to `max_tokens` tokens, in
     `num_pages` pages of `page_size` tokens that the requests share (default: enough for all at their
@@ -71,19 +76,27 @@ class PagedKVCache:
     def write(self, layer, q, k, v, cos, sin, step, q_weight=None, k_weight=None, eps=1e-6):
         """The step's q, k, v rows [rows, heads, head_dim] through norm and rotation, k and v into layer
         `layer`'s pages; returns q (ops.paged_rope_write)."""
+        _no_grad(q, k, v)
         return ops.paged_rope_write(q, k, v, cos, sin, step.positions, step.slots, self.k[layer],
                                     self.v[layer], q_weight, k_weight, eps)
 
     def attend(self, layer, q, scale=None):
         """Attention of one new token a request, q [batch, heads, head_dim], over layer `layer`'s cached
         tokens (ops.paged_attn); zeros for requests without tokens."""
+        _no_grad(q)
         return ops.paged_attn(q, self.k[layer], self.v[layer], self.block_table, self.lens, scale)[0]
 
     def tokens(self, layer, request, n):
-        """Keys and values [n, kv_heads, head_dim] of the first n tokens of a request, copied out."""
+        """Keys and values [n, kv_heads, head_dim] of the first n tokens of a request, copied out (as
+        many as it has: lens is on the device and not looked at)."""
+        batch, width = self.block_table.shape
+        if not (0 <= request < batch and 0 <= n <= width * self.page_size):
+            raise ValueError(f"no {n} tokens of request {request} in a cache of {batch} requests of "
+                             f"{width * self.page_size}")
         k, v = self.k[layer], self.v[layer]
         t = torch.arange(n, device=v.device)
-        page, at = self.block_table[request, t // self.page_size].long(), t % self.page_size
+        page = self.block_table[request, t // self.page_size].long().clamp(0, self.num_pages - 1)
+        at = t % self.page_size
         return k[page, :, :, at].reshape(n, v.shape[1], v.shape[3]), v[page, :, at]
 
 

@@ -1319,7 +1319,8 @@ def paged_rope_write(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_we
     """q [T, H, D], k, v [T, Hkv, D] (bf16, dense heads, any row pitch that is a multiple of 8)
     through per-head RMSNorm (q_weight, k_weight bf16 [D], or neither) and the rotation at each
     token's position (cos, sin fp32 [max_positions, D]): returns q [T, H, D]; k and v go into
-    slots [T] of the cache in place (plz_paged_rope_write). Tokens with slot -1 are stored nowhere."""
+    slots [T] of the cache in place (plz_paged_rope_write). Tokens with slot -1 are stored nowhere; two
+    tokens must not share a slot. There is no backward."""
     n, hkv, P, D = _paged_caches(k_cache, v_cache)
     ldq = _token_rows(q, "q", None, D)
     T, H = q.shape[0], q.shape[1]
@@ -1357,7 +1358,7 @@ def paged_rope_write(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_we
 def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
     """Attention of one new token a request over its cached tokens: q [B, H, D] (bf16, dense heads),
     block_table int32 [B, W], lens int32 [B] (the new token's own included) -> (o [B, H, D] bf16,
-    lse [B, H] fp32) (plz_paged_attn). Requests without tokens give 0 and -inf."""
+    lse [B, H] fp32) (plz_paged_attn). Requests without tokens give 0 and -inf. There is no backward."""
     n, hkv, P, D = _paged_caches(k_cache, v_cache)
     ldq = _token_rows(q, "q", None, D)
     B, H = q.shape[0], q.shape[1]

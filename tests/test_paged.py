@@ -335,6 +335,15 @@ def test_cache_and_layer_refusals():
     assert c.num_pages == 3 * 7 and c.block_table.shape == (3, 7) and len(c.k) == len(c.v) == 2
     with pytest.raises(RuntimeError, match="GPU tensor"):
         c.step([1, 1, 1])
+    for request, n in ((3, 1), (-1, 1), (0, 113), (0, -1)):
+        with pytest.raises(ValueError, match="tokens of request"):
+            c.tokens(0, request, n)
+    assert c.tokens(1, 2, 112)[0].shape == (112, 2, 64) == c.tokens(1, 2, 112)[1].shape
+    q = _bf(3, 4, 64).requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        c.attend(0, q)
+    with pytest.raises(RuntimeError, match="no backward"):
+        c.write(0, q, _bf(3, 2, 64), _bf(3, 2, 64), None, None, None)
     with pytest.raises(ValueError, match="rows"):
         decode.HardDecoderLayer.prefill.__wrapped__(
             type("L", (), {"cfg": None})(), torch.zeros(5, 8), c, 0, None, [2, 2], None, None)

@@ -235,9 +235,10 @@ __global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
 // rotation round the normalised and the weighted value too, as the modules that they stand for do:
 // here there is no such module to match). D / 8 lanes a row, 8 values a lane; the partner of value
 // j is in lane l ^ (D / 16). Bound by its bytes: 16384 tokens of 32/8 heads of 128 (407 MB read and
-// written) take 86 us, 4.7 TB/s where a plain copy reaches 5.1; up to 8 heads a workgroup share their
-// tokens' sines (109 us with one, 91 with 16), 4 rows of a lane in flight. K in its 8-value pieces is
-// stored as fast as in rows would be (86.1 and 85.7). One token takes the 3 us of its memory latencies.
+// written) take 79.5 us, 5.1 TB/s, as a plain copy does. Up to 8 heads a workgroup share their tokens'
+// sines (109 us with one), and the workgroups of one block of tokens run side by side on one XCD (86 with
+// the blocks side by side: 58 MB of sines fetched again). 4 rows of a lane are in flight. K in its 8-value
+// pieces is stored as fast as in rows would be. One token takes the 3 us of its memory latencies.
 struct WriteArgs {
   const uint16_t *q, *k, *v, *qw, *kw;
   const float *cosv, *sinv;
@@ -247,14 +248,19 @@ struct WriteArgs {
   int H, Hkv, max_pos, shift;
   int64_t slots_end;  // num_pages * P
   float eps;
-  int each;  // heads a workgroup
+  int each, groups;  // heads a workgroup, workgroups a block of tokens
 };
 
 template <int LPR, int U>  // U rows of a lane in flight
 __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
   constexpr int D = 8 * LPR, RPW = 64 / LPR, TB = 4 * RPW;  // tokens a workgroup
   const int lane = threadIdx.x & 63, l = lane % LPR;
-  const int64_t t = (int64_t)blockIdx.x * TB + (threadIdx.x >> 6) * RPW + lane / LPR;
+  // the groups of heads of one block of tokens side by side on one XCD (id % 8), whose L2 then has the
+  // tokens' sines and cosines for all of them
+  const int seq = (int)(blockIdx.x >> 3), group = seq % g.groups;
+  const int64_t t = ((int64_t)(seq / g.groups) * 8 + (blockIdx.x & 7)) * TB +
+                    (threadIdx.x >> 6) * RPW + lane / LPR;
+  if (t - (threadIdx.x >> 6) * RPW - lane / LPR >= g.T) return;  // the last eight blocks' padding
   const bool valid = t < g.T;
   const int64_t tt = valid ? t : 0;
   const int slot = g.slots[tt], p = g.pos[tt];
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
   const int64_t page = stored ? slot >> g.shift : 0;
   const int64_t at = stored ? slot & ((1 << g.shift) - 1) : 0;
   const int all = g.H + 2 * g.Hkv;  // heads: q's, k's, v's
-  const int head0 = blockIdx.y * g.each, head1 = min(head0 + g.each, all);
+  const int head0 = group * g.each, head1 = min(head0 + g.each, all);
   // the heads' sources and the row's sines are on their way together
   float c[8], s[8], w[8];
   const bool turns = head0 < g.H + g.Hkv;
@@ -427,10 +433,12 @@ int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v
   const int64_t blocks = (tokens + tb - 1) / tb;
   int each = 1;
   while (each < 8 && blocks * all >= 2048 * (int64_t)each) each *= 2;
+  const int groups = (all + each - 1) / each;
   const WriteArgs g{q,     k,      v,   q_weight, k_weight, cos_table, sin_table, positions,
                     slots, q_out, k_cache, v_cache, tokens, ld_q, ld_k, ld_v,
-                    heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps, each};
-  const dim3 grid((unsigned)blocks, (unsigned)((all + each - 1) / each));
+                    heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps, each, groups};
+  PLZ_REQUIRE((blocks + 7) / 8 * 8 * groups < ((int64_t)1 << 31), "%s: too many tokens x heads", what);
+  const dim3 grid((unsigned)((blocks + 7) / 8 * 8 * groups));
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
   };

@@ -66,7 +66,8 @@ def _write_args(**kw):
     (dict(qw=None), 1, b"together"), (dict(kw=None), 1, b"together"), (dict(q=None), 1, b"null"),
     (dict(pos=None), 1, b"null"), (dict(slots=None), 1, b"null"), (dict(vc=None), 1, b"null"),
     (dict(k=FAKE + 8), 1, b"aligned"), (dict(kc=FAKE + 2), 1, b"aligned"),
-    (dict(cos=FAKE + 4), 1, b"aligned")])
+    (dict(cos=FAKE + 4), 1, b"aligned"),
+    (dict(tokens=1 << 30, heads=16384, ldq=1 << 21), 1, b"too many")])
 def test_write_refusals(lib, kw, code, word):
     if word == b"together":
         word = b"go together"

@@ -235,7 +235,7 @@ __global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
 // rotation round the normalised and the weighted value too, as the modules that they stand for do:
 // here there is no such module to match). D / 8 lanes a row, 8 values a lane; the partner of value
 // j is in lane l ^ (D / 16). Bound by its bytes: 16384 tokens of 32/8 heads of 128 (407 MB read and
-// written) take 79.5 us, 5.1 TB/s, as a plain copy does. Up to 8 heads a workgroup share their tokens'
+// written) take 77.2 us, 5.3 TB/s; a plain copy reaches 5.1. Up to 8 heads a workgroup share their tokens'
 // sines (109 us with one), and the workgroups of one block of tokens run side by side on one XCD (86 with
 // the blocks side by side: 58 MB of sines fetched again). 4 rows of a lane are in flight. K in its 8-value
 // pieces is stored as fast as in rows would be. One token takes the 3 us of its memory latencies.
@@ -250,6 +250,12 @@ struct WriteArgs {
   float eps;
   int each, groups;  // heads a workgroup, workgroups a block of tokens
 };
+
+// 16 bytes at base + 16 at, past the L2s' replacement order: whole rows that this kernel is done with
+// (16384 tokens 80.1 -> 77.2 us; the 64-byte pieces of K are left to the L2 to put together)
+__device__ __forceinline__ void store_nt(uint16_t* base, int64_t at, uint4 v) {
+  __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(base) + at);
+}
 
 template <int LPR, int U>  // U rows of a lane in flight
 __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
@@ -306,7 +312,7 @@ __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
       const int h = kind == 0 ? head : kind == 1 ? head - g.H : head - g.H - g.Hkv;
       const int64_t block = page * g.Hkv + h;  // of D * P values
       if (kind == 2) {
-        if (stored) reinterpret_cast<uint4*>(g.vc)[((block << g.shift) + at) * LPR + l] = xv[i];
+        if (stored) store_nt(g.vc, ((block << g.shift) + at) * LPR + l, xv[i]);
         continue;
       }
       float f[8], o[8];
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(256) void rope_write_kernel(WriteArgs g) {
       }
       const uint4 out = pack8(o);
       if (kind == 0) {
-        if (valid) reinterpret_cast<uint4*>(g.q_out + (tt * g.H + h) * D)[l] = out;
+        if (valid) store_nt(g.q_out, (tt * g.H + h) * LPR + l, out);
       } else if (stored) {
         reinterpret_cast<uint4*>(g.kc)[((block * LPR + l) << g.shift) + at] = out;
       }

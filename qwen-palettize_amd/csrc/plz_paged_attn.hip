@@ -41,6 +41,7 @@ namespace paged {
 constexpr int NW = 4, NT = 64 * NW;  // waves, threads
 constexpr int PARTS = 512;           // most workgroups: two for each of 256 CUs (parts_of)
 constexpr int HT = 16;               // heads a workgroup (columns of the matrix instruction)
+constexpr int ALONE = 512;           // tokens up to which a table's requests get a workgroup each
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct AttnArgs {
@@ -54,6 +55,7 @@ struct AttnArgs {
   // b {the workgroup that begins it or -1, the one that ends it}.
   int2* open;
   int by_request;
+  int alone;  // workgroup w has request w alone, and all of it: no workspace, no second kernel
   int64_t ldq;
   int B, W, Hq, Hkv, G, tiles_h, parts, num_pages, shift;  // tiles_h = head tiles a kv head
   float scale_log2;
@@ -83,7 +85,12 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   const int P = 1 << g.shift, cap = g.W << g.shift;
 
   // the head tiles of one workgroup number (the same K and V) sit side by side on one XCD (id % 8)
-  const int ht = (int)blockIdx.x >> 3, pair = (int)blockIdx.y * 8 + ((int)blockIdx.x & 7);
+  int pair = (int)blockIdx.x, ht = 0;
+  if (g.tiles_h > 1) {
+    const int per = 8 * g.tiles_h, r = pair % per;
+    ht = r >> 3;
+    pair = pair / per * 8 + (r & 7);
+  }
   const int w = pair / g.Hkv, hk = pair - w * g.Hkv;
   if (w >= g.parts) return;  // the last eighth's padding
   const int h0 = ht * HT, nh = min(g.G - h0, HT);  // heads hk G + h0 .. + nh - 1
@@ -91,36 +98,39 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   float* const res = reinterpret_cast<float*>(s_res) + wave * 2 * slot;
   if (lane == 0) s_has[wave] = 0;
 
-  // every request's tiles (a lane takes `each` consecutive requests) and their sums
-  const int each = (g.B + 63) >> 6;
-  int win_at = 0, win = 0;  // lane l: the length of request win_at + l
+  // The requests that this workgroup shares with others, all of them or its own one, and its number
+  // among these others: every one's tiles (a lane takes `each` consecutive requests) and their sums
+  const int from = g.alone ? w : 0, to = g.alone ? w + 1 : g.B;
+  const int me = g.alone ? 0 : w, others = g.alone ? 1 : g.parts;
+  const int each = (to - from + 63) >> 6;
+  int win_at = from, win = 0;  // lane l: the length of request win_at + l
   int mine = 0;
   bool none = false;  // some request has no tiles
   for (int i = 0; i < each; ++i) {
-    const int b = lane * each + i;
-    win = b < g.B ? g.lens[b] : 0;
+    const int b = from + lane * each + i;
+    win = b < to ? g.lens[b] : 0;
     const int n = tiles_of(win, cap);
     mine += n;
-    none |= n == 0 && b < g.B;
+    none |= n == 0 && b < to;
   }
   none = __builtin_amdgcn_ballot_w64(none) != 0;
   int sum = wave_scan(mine);
   const int total = __builtin_amdgcn_readlane(sum, 63);
-  const Deal runs = deal(total, g.parts * NW);
+  const Deal runs = deal(total, others * NW);
 
-  if (w * NW + wave < runs.runs) {
-    const int r0 = run_begin(runs, w * NW + wave), r1 = run_begin(runs, w * NW + wave + 1);
+  if (me * NW + wave < runs.runs) {
+    const int r0 = run_begin(runs, me * NW + wave), r1 = run_begin(runs, me * NW + wave + 1);
     // the request that holds tile r0, and its first tile among all: the lane, then its requests
     auto holder = [&]() { return __builtin_ctzll(__builtin_amdgcn_ballot_w64(r0 < sum)); };
     int at = holder();
     int first = __builtin_amdgcn_readlane(sum - mine, at);
     if (each > 1) {
       for (win_at = at * each;; win_at += 64) {
-        win = win_at + lane < g.B ? g.lens[win_at + lane] : 0;
+        win = win_at + lane < to ? g.lens[win_at + lane] : 0;
         mine = tiles_of(win, cap);
         sum = first + wave_scan(mine);
         const int end = __builtin_amdgcn_readlane(sum, 63);
-        if (r0 < end || win_at + 64 >= g.B) break;
+        if (r0 < end || win_at + 64 >= to) break;
         first = end;
       }
       at = __builtin_amdgcn_ballot_w64(r0 < sum) ? holder() : 63;
@@ -249,14 +259,14 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     // behind a tile's K and V would hold up the tile that needs them until those are here.
     int b1 = 0, len1 = 0, n1 = 0, pages1 = 0, b2 = 0, len2 = 0, n2 = 0, pages2 = 0;
     auto find_after = [&](int req, int& at_req, int& tokens, int& tiles) {
-      for (at_req = min(req + 1, g.B - 1);; ++at_req) {
+      for (at_req = min(req + 1, to - 1);; ++at_req) {
         if (at_req >= win_at + 64) {
           win_at = at_req;
-          win = win_at + lane < g.B ? g.lens[win_at + lane] : 0;
+          win = win_at + lane < to ? g.lens[win_at + lane] : 0;
         }
         tokens = __builtin_amdgcn_readlane(win, at_req - win_at);
         tiles = tiles_of(tokens, cap);
-        if (tiles > 0 || at_req == g.B - 1) break;
+        if (tiles > 0 || at_req == to - 1) break;
       }
     };
     auto look_ahead = [&]() {
@@ -344,11 +354,11 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       float any = 0.f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) any += acc[i][0] + acc[i][1] + acc[i][2] + acc[i][3];
-      float* const to = res + place_of(carried) * slot;
+      float* const left = res + place_of(carried) * slot;
       if (__builtin_amdgcn_ballot_w64(any != any && col < nh) != 0) {
         // An infinite value times the two pieces of its weight is NaN where the second is 0 or of the
         // other sign. For the outputs that are NaN, once more with the first pieces alone.
-        put(to);
+        put(left);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = f32x4{};
         for (int tt = t0; tt <= t; ++tt) {
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-              const float fine = to[col * D + (4 * grp + r) * VEC + i];
+              const float fine = left[col * D + (4 * grp + r) * VEC + i];
               if (fine == fine) acc[i][r] = fine;
             }
         }
@@ -394,10 +404,10 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         }
         if (g.by_request && lane == 0 && hk + ht == 0) g.open[b] = make_int2(-1, 0);
       } else {
-        put(to);
+        put(left);
         if (grp == 0 && col < nh) {
-          to[nh * D + col] = mrun;
-          to[nh * D + nh + col] = lrun;
+          left[nh * D + col] = mrun;
+          left[nh * D + nh + col] = lrun;
         }
         if (lane == 0) {
           s_has[wave] |= carried ? HAS_CARRIED | (same ? 0 : CARRIED_ENDS) : HAS_OPEN;
@@ -440,7 +450,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     if (g.by_request && threadIdx.x == 0 && hk + ht == 0 && start >= 0)
       g.open[b] = ended ? make_int2(-1, 0) : make_int2(w, s_last[w0]);
     // [kv head][head tile][workgroup][place][heads][D]
-    float* to = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * (heads_max * D);
+    float* part_out = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * (heads_max * D);
     for (int e = threadIdx.x; e < nh * (D / 4); e += NT) {
       const int h = e / (D / 4), d = e % (D / 4) * 4;
       const float* from = reinterpret_cast<const float*>(s_res) + (w0 * 2 + place) * slot;
@@ -464,7 +474,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
             u32x2{f2bf2(sum[0] * inv, sum[1] * inv), f2bf2(sum[2] * inv, sum[3] * inv)};
         if (d == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
       } else {
-        *reinterpret_cast<f32x4*>(to + h * D + d) = sum;
+        *reinterpret_cast<f32x4*>(part_out + h * D + d) = sum;
         if (d == 0)
           g.part_ml[((int64_t)(hk * g.G + h0 + h) * 2 + place) * g.parts + w] = make_float2(m, l);
       }
@@ -474,8 +484,8 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
 
   // requests without tiles, spread over the workgroups that have work
   const int every = max((runs.runs + NW - 1) / NW, 1);
-  if (none && w < every)
-    for (int b = w + every * wave; b < g.B; b += every * NW) {
+  if (none && me < every)
+    for (int b = from + me + every * wave; b < to; b += every * NW) {
       const int len = g.lens[b];
       if (tiles_of(len, cap) != 0) continue;
       const float x = len <= 0 ? 0.f : __builtin_nanf("");
@@ -564,11 +574,11 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   if (c == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
 }
 
-// True where all requests together have a tile a wave of one workgroup at most, whatever their lengths:
-// then that workgroup joins whatever is shared, and there is no second kernel.
-static bool never_shared(int64_t batch, int64_t width, int64_t page_size) {
-  return batch <= NW && width <= NW * TILE && batch * ((width * page_size + TILE - 1) / TILE) <= NW;
-}
+// A workgroup a request instead of equal runs, by the most tokens that the table can hold: one launch
+// and no workspace, at up to four tiles a wave no slower. Equal runs and one each, 32/8 heads of 128, in
+// us: 200 tokens B 1 8.3 and 6.0, B 16 9.8 and 7.1, B 256 41.2 and 42.0 (ragged 21.0 and 22.4); 500 tokens
+// B 1 8.5 and 8.5, B 4 8.9 and 9.4, B 16 12.5 and 10.5, B 256 85.6 and 85.4; 1000 tokens B 1 8.7 and 13.3.
+static bool one_each(int64_t width, int64_t page_size) { return width * page_size <= ALONE; }
 // Workgroups a (kv head, head tile): two a CU in all, one where a part is large (more than 1024 values:
 // writing and joining them costs more than the second workgroup's loads bring) or a workgroup takes the
 // whole CU's registers (heads of 256). Two and one: 16 x 4096 tokens, 4 kv heads of 128 with 20 heads
@@ -589,10 +599,10 @@ static int launch_paged_attn(const AttnArgs& g, hipStream_t stream, const char* 
     if (rc != PLZ_OK) return rc;
   }
   hipLaunchKernelGGL(paged_attn_kernel<D>,
-                     dim3((unsigned)(8 * g.tiles_h), (unsigned)((g.parts * g.Hkv + 7) / 8)), dim3(NT),
-                     lds, stream, g);
+                     dim3((unsigned)(((int64_t)g.parts * g.Hkv + 7) / 8 * 8 * g.tiles_h)), dim3(NT), lds,
+                     stream, g);
   const int rc = check_launch(what);
-  if (rc != PLZ_OK || g.parts == 1) return rc;
+  if (rc != PLZ_OK || g.alone || g.parts == 1) return rc;
   hipLaunchKernelGGL(paged_join_kernel<D>,
                      dim3((unsigned)(g.by_request ? g.B : g.parts), (unsigned)g.Hq), dim3(JT), 0, stream,
                      g);
@@ -610,7 +620,7 @@ extern "C" {
 size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
                                 int head_dim) {
   if (batch <= 0 || width <= 0 || page_size <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
-      heads % kv_heads || never_shared(batch, width, page_size))
+      heads % kv_heads || one_each(width, page_size))
     return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
   const size_t parts = (size_t)parts_of(kv_heads, G, head_dim);
@@ -655,13 +665,14 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
     set_error("%s: workspace of %zu bytes (16-byte aligned) required", what, need);
     return PLZ_EWORKSPACE;
   }
-  AttnArgs g{q, k_cache, v_cache, block_table, lens, o, lse, (float*)workspace, nullptr, nullptr, 0, ld_q,
+  AttnArgs g{q, k_cache, v_cache, block_table, lens, o, lse, (float*)workspace, nullptr, nullptr, 0, 0, ld_q,
              (int)batch, (int)width, heads, kv_heads, heads / kv_heads, 0, 0, (int)num_pages, 0,
              scale * kLog2e};
   g.tiles_h = (g.G + HT - 1) / HT;
   g.parts = parts_of(kv_heads, g.G, head_dim);
   if (need == 0) {
-    g.parts = 1;  // the one workgroup (a kv head and head tile) that gets any tiles
+    g.parts = g.B;
+    g.alone = 1;
   } else {
     g.part_ml = reinterpret_cast<float2*>(
         g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 * (g.G < HT ? g.G : HT) * head_dim);

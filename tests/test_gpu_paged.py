@@ -321,17 +321,35 @@ def test_attn_many_ragged_requests(dev):
                 + rng.sample(range(1500), 30))
 
 
-@pytest.mark.parametrize("lens,P", [([37], 64), ([128], 128), ([0, 16, 7, 1], 16), ([200], 128)])
-def test_attn_small_tables_without_a_workspace(dev, lens, P):
-    """Tables of a few tiles: one workgroup a kv head, no second launch; one length past its table."""
-    W = -(-128 // P) if len(lens) == 1 else 1
-    c = _attn_case([min(n, W * P) for n in lens], 8, 2, 128, P, 14, dev, width=W)
-    assert ops.query("plz_paged_attn_workspace", len(lens), W, P, 8, 2, 128) == 0
-    if max(lens) > W * P:
-        o, lse = ops.paged_attn(*c[:4], _ints(lens, dev))
-        assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
-    else:
-        _check_attn(*c)
+@pytest.mark.parametrize("H,Hkv,D,P", [(8, 2, 128, 64), (20, 1, 64, 16), (3, 3, 256, 512)])
+def test_attn_small_tables_without_a_workspace(dev, H, Hkv, D, P):
+    """Tables of up to 512 tokens: a workgroup a request, no second launch; empty rows, every number of
+    tiles a wave, one length past its table; and the same rows through a wider table's equal runs."""
+    lens = [37, 0, 512, 1, 128, 129, 300, 511, 0, 480, 33, 200, 0]
+    q, kc, vc, table, n = _attn_case(lens, H, Hkv, D, P, 14, dev, width=512 // P)
+    assert ops.query("plz_paged_attn_workspace", len(lens), 512 // P, P, H, Hkv, D) == 0
+    o, lse = _check_attn(q, kc, vc, table, n)
+    long = n.clone()
+    long[3] = 513
+    o2, lse2 = ops.paged_attn(q, kc, vc, table, long)
+    assert bool(torch.isnan(o2[3]).all()) and bool(torch.isnan(lse2[3]).all())
+    rest = [b for b in range(len(lens)) if b != 3]
+    assert torch.equal(o2[rest], o[rest]) and torch.equal(lse2[rest], lse[rest])
+    wide = torch.cat([table, table], 1).contiguous()
+    assert ops.query("plz_paged_attn_workspace", len(lens), wide.shape[1], P, H, Hkv, D) > 0
+    _check_attn(q, kc, vc, wide, n)
+
+
+def test_attn_many_requests_of_small_tables(dev):
+    """More (request, kv head) pairs than a grid's second dimension takes."""
+    B = 9000
+    g = torch.Generator(device=dev).manual_seed(2)
+    kc = torch.randn(64, 8, 8, 16, 8, generator=g, device=dev).to(torch.bfloat16)
+    vc = torch.randn(64, 8, 16, 64, generator=g, device=dev).to(torch.bfloat16)
+    q = torch.randn(B, 8, 64, generator=g, device=dev).to(torch.bfloat16)
+    table = torch.randint(0, 64, (B, 3), generator=g, device=dev, dtype=torch.int32)
+    lens = torch.randint(0, 49, (B,), generator=g, device=dev, dtype=torch.int32)
+    _check_attn(q, kc, vc, table, lens, rows=[0, 1, 8191, 8192, 8999] + list(range(5, B, 700)))
 
 
 @pytest.mark.parametrize("std", [0.05, 12.0])

@@ -77,7 +77,7 @@ def test_write_refusals(lib, kw, code, word):
 
 def _attn_args(lib, **kw):
     a = dict(q=FAKE, ldq=1024, kc=FAKE, vc=FAKE, table=FAKE, lens=FAKE, o=FAKE, lse=FAKE, ws=FAKE,
-             nws=1 << 40, batch=3, width=4, heads=8, kv=2, dim=128, pages=16, page=16, scale=0.1,
+             nws=1 << 40, batch=3, width=40, heads=8, kv=2, dim=128, pages=16, page=16, scale=0.1,
              stream=None)
     assert set(kw) <= set(a)
     return list({**a, **kw}.values())
@@ -235,21 +235,21 @@ def test_calls_run_on_their_tensors_device(monkeypatch):
 
 
 def test_attn_needs_its_workspace(lib):
-    need = lib.plz_paged_attn_workspace(3, 4, 16, 8, 2, 128)
+    need = lib.plz_paged_attn_workspace(3, 40, 16, 8, 2, 128)
     assert need > 0
     for kw in (dict(ws=None), dict(nws=need - 1), dict(ws=FAKE + 8)):
         assert lib.plz_paged_attn(*_attn_args(lib, **kw)) == 4
         assert b"workspace" in lib.plz_last_error()
-    for args in ((0, 4, 16, 8, 2, 128), (3, 0, 16, 8, 2, 128), (3, 4, 0, 8, 2, 128),
-                 (3, 4, 16, 0, 2, 128), (3, 4, 16, 8, 0, 128), (3, 4, 16, 9, 2, 128),
-                 (3, 4, 16, 8, 2, 0), (-1, 4, 16, 8, 2, 128), (3, -4, 16, 8, 2, 128)):
+    for args in ((0, 40, 16, 8, 2, 128), (3, 0, 16, 8, 2, 128), (3, 40, 0, 8, 2, 128),
+                 (3, 40, 16, 0, 2, 128), (3, 40, 16, 8, 0, 128), (3, 40, 16, 9, 2, 128),
+                 (3, 40, 16, 8, 2, 0), (-1, 40, 16, 8, 2, 128), (3, -40, 16, 8, 2, 128)):
         assert lib.plz_paged_attn_workspace(*args) == 0
-    # no request is shared where all of them have a tile of 32 for each of four waves at most
-    assert lib.plz_paged_attn_workspace(1, 2, 64, 8, 2, 128) == 0
-    assert lib.plz_paged_attn_workspace(4, 1, 32, 8, 2, 128) == 0
-    assert lib.plz_paged_attn_workspace(1, 9, 16, 8, 2, 128) > 0
-    assert lib.plz_paged_attn_workspace(5, 1, 16, 8, 2, 128) > 0
-    assert lib.plz_paged_attn_workspace(1 << 40, 1 << 40, 1024, 8, 2, 128) > 0
+    # tables of up to 512 tokens: a workgroup a request, nothing is shared
+    assert lib.plz_paged_attn_workspace(1, 8, 64, 8, 2, 128) == 0
+    assert lib.plz_paged_attn_workspace(65536, 32, 16, 8, 2, 128) == 0
+    assert lib.plz_paged_attn_workspace(1, 9, 64, 8, 2, 128) > 0
+    assert lib.plz_paged_attn_workspace(5, 33, 16, 8, 2, 128) > 0
+    assert lib.plz_paged_attn_workspace(1 << 40, 1 << 20, 1024, 8, 2, 128) > 0
 
 
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not available")

@@ -30,8 +30,7 @@ namespace paged {
 // its threads, twice, for larger batches: the pages handed back have to be on the stack before any is
 // taken): a step of 8 requests takes 3.0 us (5.1 with two passes for every batch, 1024 threads and sums
 // by shuffles), of which 1 is the launch and the rest dependent memory accesses. More than 4096 token
-// rows go to a second launch over the whole card: 27800 rows in 1700 new pages 5.1 + 2.4 us, in the one
-// workgroup 25.7; 5000 rows 7.5 in two, 10.7 in one.
+// rows go to a second launch over the whole card (ONE_LAUNCH_ROWS).
 struct StepArgs {
   const int32_t *lens, *keep, *add;
   int32_t *table, *stack;
@@ -197,6 +196,8 @@ __global__ __launch_bounds__(ST) void step_kernel(StepArgs g) {
 // The token rows of a step whose table, lengths and starts step_kernel<TOKENS = false> has left, with
 // the position of each request's first token in its row of pos.
 constexpr int RT = 256, STAGED = 4096;
+// 3300 rows 7.1 us in one launch and 7.6 in two, 5500 10.4 and 8.8, 7300 9.7 and 7.6, 27000 27 and 8.6: the
+// one workgroup is bound by the instructions of its searches (four rows a thread side by side: no gain)
 constexpr int64_t ONE_LAUNCH_ROWS = 4096;
 __global__ __launch_bounds__(RT) void rows_kernel(StepArgs g) {
   __shared__ int s_starts[STAGED];

@@ -68,6 +68,11 @@ __host__ __device__ __forceinline__ int part_floats(int heads, int D) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+template <class T>
+__device__ __forceinline__ T load_nt(const char* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+}
+
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -98,8 +103,8 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   float* const res = reinterpret_cast<float*>(s_res) + wave * 2 * slot;
   if (lane == 0) s_has[wave] = 0;
 
-  // The requests that this workgroup shares with others, all of them or its own one, and its number
-  // among these others: every one's tiles (a lane takes `each` consecutive requests) and their sums
+  // The requests that this workgroup shares with others (all of them, or its own one with none), and its
+  // number among these: every one's tiles (a lane takes `each` consecutive requests) and their sums
   const int from = g.alone ? w : 0, to = g.alone ? w + 1 : g.B;
   const int me = g.alone ? 0 : w, others = g.alone ? 1 : g.parts;
   const int each = (to - from + 63) >> 6;
@@ -125,7 +130,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     int at = holder();
     int first = __builtin_amdgcn_readlane(sum - mine, at);
     if (each > 1) {
-      for (win_at = at * each;; win_at += 64) {
+      for (win_at = from + at * each;; win_at += 64) {
         win = win_at + lane < to ? g.lens[win_at + lane] : 0;
         mine = tiles_of(win, cap);
         sum = first + wave_scan(mine);
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
                            (int64_t)((tile * TILE + 16 * half) & (P - 1)) * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
-          kr[half][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + (int64_t)s * 64 * P + koff));
+          kr[half][s] = load_nt<u32x4>(base + (int64_t)s * 64 * P + koff);
       }
     };
     auto load_v = [&](int page0, int page1, int tile) {
@@ -186,12 +191,12 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
         for (int t = 0; t < 4; ++t) {
           uint32_t(&d)[VDW] = vr[4 * half + t];
           if constexpr (VDW == 2) {
-            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(base + t * D * 2 + voff));
+            const u32x2 x = load_nt<u32x2>(base + t * D * 2 + voff);
             d[0] = x[0], d[1] = x[1];
           } else {
 #pragma unroll
             for (int c = 0; c < VDW / 4; ++c) {
-              const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + t * D * 2 + voff + 16 * c));
+              const u32x4 x = load_nt<u32x4>(base + t * D * 2 + voff + 16 * c);
 #pragma unroll
               for (int i = 0; i < 4; ++i) d[4 * c + i] = x[i];
             }
@@ -450,7 +455,8 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     if (g.by_request && threadIdx.x == 0 && hk + ht == 0 && start >= 0)
       g.open[b] = ended ? make_int2(-1, 0) : make_int2(w, s_last[w0]);
     // [kv head][head tile][workgroup][place][heads][D]
-    float* part_out = g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * (heads_max * D);
+    float* part_out =
+        g.part + (((int64_t)(hk * g.tiles_h + ht) * g.parts + w) * 2 + place) * (heads_max * D);
     for (int e = threadIdx.x; e < nh * (D / 4); e += NT) {
       const int h = e / (D / 4), d = e % (D / 4) * 4;
       const float* from = reinterpret_cast<const float*>(s_res) + (w0 * 2 + place) * slot;
@@ -480,7 +486,8 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
       }
     }
   }
-  if (g.open && !g.by_request && threadIdx.x == 0 && hk + ht == 0) g.open[w] = make_int2(open, open_last);
+  if (g.open && !g.by_request && threadIdx.x == 0 && hk + ht == 0)
+    g.open[w] = make_int2(open, open_last);
 
   // requests without tiles, spread over the workgroups that have work
   const int every = max((runs.runs + NW - 1) / NW, 1);
@@ -582,7 +589,8 @@ static bool one_each(int64_t width, int64_t page_size) { return width * page_siz
 // Workgroups a (kv head, head tile): two a CU in all, one where a part is large (more than 1024 values:
 // writing and joining them costs more than the second workgroup's loads bring) or a workgroup takes the
 // whole CU's registers (heads of 256). Two and one: 16 x 4096 tokens, 4 kv heads of 128 with 20 heads
-// each 38.5 and 34.8 us, 32 ragged up to 4096 with 8 heads 16.4 and 16.6; 8 kv heads of 256 with 4, 32 x 2048 93.4 and 88.1.
+// each 38.5 and 34.8 us, 32 ragged up to 4096 with 8 heads 16.4 and 16.6; 8 kv heads of 256 with 4 heads
+// each, 32 x 2048, 93.4 and 88.1.
 static int parts_of(int kv_heads, int G, int D) {
   const int heads = G < HT ? G : HT, tiles = (G + HT - 1) / HT;
   const int n = (D == 256 || heads * D > 1024 ? PARTS / 2 : PARTS) / (kv_heads * tiles);

@@ -155,6 +155,30 @@ def test_captured_step(dev):
         assert torch.equal(caches[0].lens, caches[1].lens)
 
 
+def test_layer_without_lora(dev):
+    """A layer whose linears have no LoRA equals one whose LoRA is zero, bit for bit."""
+    cfg, hard, _ = _layers(dev, CFGS["d128"], 1)
+    cos, sin = layer.rope_tables(64, cfg.head_dim, cfg.rope_theta, dev)
+    names, norms = decode.HardDecoderLayer.NAMES, decode.HardDecoderLayer.NORMS
+    parts = {n: [getattr(hard[0], f"{n}_{p}") for p in ("packed", "palette", "lora_a", "lora_b")]
+             for n in names}
+    norms = {n: getattr(hard[0], n) for n in norms}
+    outs = []
+    for lora in (False, True):
+        l = decode.HardDecoderLayer(cfg, {n: (*p[:2], p[2] if lora else None,
+                                              torch.zeros_like(p[3]) if lora else None)
+                                          for n, p in parts.items()}, norms)
+        cache = decode.PagedKVCache(1, 2, 64, cfg.kv_heads, cfg.head_dim, device=dev)
+        g = torch.Generator().manual_seed(9)
+        out = []
+        for _ in range(3):
+            step = cache.step([1, 1], rows_each=1)
+            hs = torch.randn(2, cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+            out.append(l.decode(hs, cache, 0, step, cos, sin))
+        outs.append(torch.cat(out))
+    assert torch.equal(*outs)
+
+
 def test_pages_run_out_and_come_back(dev):
     """A pool smaller than its requests: what found no page is not in lens, and a request that ends
     makes room."""

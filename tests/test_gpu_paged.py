@@ -563,6 +563,23 @@ def test_decoding_in_a_graph(dev):
         assert torch.equal(a.table, b.table) and torch.equal(a.lens, b.lens)
 
 
+def test_two_calls_at_once(dev):
+    """Eager attentions of two batches on two streams without a wait between them, again and again."""
+    cases = [_attn_case([2500, 5, 700, 1200], 8, 2, 128, 64, 40 + i, dev) for i in range(2)]
+    want = [ops.paged_attn(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.paged_attn(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, y) for g in got[i] for x, y in zip(g, want[i]))
+
+
 def test_two_graphs_of_attention_side_by_side(dev):
     """Two captured attentions replayed on two streams at once, each against its eager result."""
     cases = [_attn_case([3000, 5, 700], 8, 2, 128, 64, 30 + i, dev) for i in range(2)]

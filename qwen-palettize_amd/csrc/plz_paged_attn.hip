@@ -77,6 +77,19 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 constexpr int kNt = 2;  // buffer loads: nontemporal
 
+// op over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48), by swaps of rows and halves between two
+// registers: no LDS, where shuffles go through it
+template <class Op>
+__device__ __forceinline__ float across(float v, Op op) {
+  const auto pair = [&](auto both) {
+    const uint32_t a = both[0], c = both[1];
+    return op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, c));
+  };
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const uint32_t y = __builtin_bit_cast(uint32_t, pair(__builtin_amdgcn_permlane16_swap(x, x, false, false)));
+  return pair(__builtin_amdgcn_permlane32_swap(y, y, false, false));
+}
+
 enum { HAS_CARRIED = 1, CARRIED_ENDS = 2, HAS_OPEN = 4 };  // a wave's parts
 
 template <int D>
@@ -160,13 +173,12 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
     };
     u32x4 kr[2][KS], qf[KS], qn[KS];
     uint32_t vr[8][VDW];
-    auto load_q = [&](int req, u32x4(&to)[KS]) {  // columns past nh: zeros
+    auto load_q = [&](int req, u32x4(&to)[KS]) {  // columns past nh: the last head again
       const uint16_t* qp =
           g.q + req * g.ldq + (int64_t)(hk * g.G + h0 + min(col, nh - 1)) * D + 8 * grp;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         to[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
-        if (col >= nh) to[s] = u32x4{};
       }
     };
     // Buffer loads: a lane whose token does not exist (`tokens` in the request) gets an offset out of
@@ -330,15 +342,16 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
       if (__builtin_amdgcn_ballot_w64(mx > mrun + 8.f) != 0) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        mx = across(mx, [](float a, float b) { return fmaxf(a, b); });
         const float mnew = mx > mrun + 8.f ? mx : mrun;
         const float alpha = mnew == mrun ? 1.f : exp2_fast(mrun - mnew);
         mrun = mnew;
         neg = mnew == -INFINITY ? 0.f : -mnew;
         lrun *= alpha;
+        if (t != t0) {  // nothing is in acc before the first tile
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] *= alpha;
+          for (int i = 0; i < VEC; ++i) acc[i] *= alpha;
+        }
       }
       u32x4 hi, lo;
 #pragma unroll
@@ -360,8 +373,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
 
       // the request ends, here or for this run
       const bool carried = t0 > 0, whole = !carried && !same;
-      lrun += __shfl_xor(lrun, 16);
-      lrun += __shfl_xor(lrun, 32);
+      lrun = across(lrun, [](float a, float b) { return a + b; });
       float any = 0.f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) any += acc[i][0] + acc[i][1] + acc[i][2] + acc[i][3];
@@ -405,12 +417,19 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
           const float inv = 1.f / lrun;
           const int64_t at = (int64_t)b * g.Hq + hk * g.G + h0 + col;
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 4; ++r) {
+            uint32_t out[VDW];
 #pragma unroll
-            for (int i = 0; i < VEC; i += 4)
-              *reinterpret_cast<u32x2*>(g.o + at * D + (4 * grp + r) * VEC + i) =
-                  u32x2{f2bf2(acc[i][r] * inv, acc[i + 1][r] * inv),
-                        f2bf2(acc[i + 2][r] * inv, acc[i + 3][r] * inv)};
+            for (int i = 0; i < VDW; ++i) out[i] = f2bf2(acc[2 * i][r] * inv, acc[2 * i + 1][r] * inv);
+            uint16_t* const to = g.o + at * D + (4 * grp + r) * VEC;
+            if constexpr (VDW == 2) {
+              *reinterpret_cast<u32x2*>(to) = u32x2{out[0], out[1]};
+            } else {
+#pragma unroll
+              for (int i = 0; i < VDW; i += 4)
+                *reinterpret_cast<u32x4*>(to + 2 * i) = u32x4{out[i], out[i + 1], out[i + 2], out[i + 3]};
+            }
+          }
           if (grp == 0) g.lse[at] = ((mrun == -INFINITY ? 0.f : mrun) + log2f(lrun)) * kLn2;
         }
         if (g.by_request && lane == 0 && hk + ht == 0) g.open[b] = make_int2(-1, 0);

@@ -12,6 +12,7 @@ Native layout (the one the kernels use):
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -1169,11 +1170,12 @@ def attn_bwd(q, k, v, o, lse, grad_o, scale=None):
 # ---- decoding over a paged key-value cache -----------------------------------------------------
 def _on(dev, name, *args):
     """call() on device `dev`, with its current stream as the last argument."""
+    args += (torch._C._cuda_getCurrentRawStream(dev),)
     if torch._C._cuda_getDevice() == dev:
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        call(name, *args)
     else:
         with torch.cuda.device(dev):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+            call(name, *args)
 
 
 def _one_device(name, *tensors):
@@ -1342,17 +1344,31 @@ def paged_rope_write(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_we
         _ints(slots, "slots", T)
         if (q_weight is None) != (k_weight is None):
             raise ValueError("q_weight and k_weight must be given together")
+    dev = q.get_device()
     if normed:
-        _norm_weight(q_weight, D)
-        _norm_weight(k_weight, D)
-    dev = _one_device("plz_paged_rope_write", q, k, v, cos, sin, positions, slots, k_cache, v_cache,
-                      q_weight, k_weight)
+        if not (isinstance(q_weight, torch.Tensor) and isinstance(k_weight, torch.Tensor)
+                and q_weight.dtype is _BF16 and k_weight.dtype is _BF16
+                and q_weight.shape == (D,) == k_weight.shape
+                and q_weight.is_contiguous() and k_weight.is_contiguous()
+                and q_weight.get_device() == dev == k_weight.get_device()):
+            _norm_weight(q_weight, D)
+            _norm_weight(k_weight, D)
+            _one_device("plz_paged_rope_write", q, q_weight, k_weight)
+    if not (k.get_device() == dev == v.get_device() and cos.get_device() == dev == sin.get_device()
+            and positions.get_device() == dev == slots.get_device()
+            and k_cache.get_device() == dev == v_cache.get_device()):
+        _one_device("plz_paged_rope_write", q, k, v, cos, sin, positions, slots, k_cache, v_cache)
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D))
     _on(dev, "plz_paged_rope_write", q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
         _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
         slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), T, H, hkv, D,
         cos.shape[0], n, P, float(eps))
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_attn_workspace(*sizes):
+    return query("plz_paged_attn_workspace", *sizes)
 
 
 def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
@@ -1369,11 +1385,14 @@ def paged_attn(q, k_cache, v_cache, block_table, lens, scale=None):
             raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} requests")
         _ints(lens, "lens", B)
     scale = D ** -0.5 if scale is None else float(scale)
-    dev = _one_device("plz_paged_attn", q, k_cache, v_cache, block_table, lens)
+    dev = q.get_device()
+    if not (k_cache.get_device() == dev == v_cache.get_device()
+            and block_table.get_device() == dev == lens.get_device()):
+        _one_device("plz_paged_attn", q, k_cache, v_cache, block_table, lens)
     o = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
     lse = q.new_empty((B, H), dtype=torch.float32)
     W = block_table.shape[1]
-    nbytes = query("plz_paged_attn_workspace", B, W, P, H, hkv, D)
+    nbytes = _paged_attn_workspace(B, W, P, H, hkv, D)
     ws = lens.new_empty((nbytes + 3) // 4) if nbytes else None
     _on(dev, "plz_paged_attn", q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
         block_table.data_ptr(), lens.data_ptr(), o.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, B,

@@ -748,8 +748,10 @@ int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v
  * [batch, heads] = log-sum-exp of the scaled scores; heads % kv_heads == 0, head_dim 64, 128 or
  * 256. lens[b] <= 0: o = 0, lse = -inf. A request whose length passes width * page_size, or that
  * needs a page outside [0, num_pages), gives NaN in both; nothing is read past the cache. Values in
- * the cache behind a request's last token do not matter. Deterministic. The workspace (0 bytes where
- * the table is so small that no request is shared) belongs to one call at a time. */
+ * the cache behind a request's last token do not matter. Deterministic. batch goes up to 65536, heads
+ * to 16384, width * page_size and num_pages * page_size to 2^30, batch * width * page_size to 2^35. The
+ * workspace (0 bytes where tables and batch are so small that no request is shared) belongs to one call
+ * at a time. */
 size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
                                 int head_dim);
 int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,

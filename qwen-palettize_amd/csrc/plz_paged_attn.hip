@@ -31,7 +31,7 @@
 // what a run has of a request that it does not have whole is joined: through LDS among the waves of a
 // workgroup, through the workspace among workgroups, by a second kernel, both in the order of the runs.
 // (256 ragged requests up to 1024 tokens: 59 us with one run a workgroup and a join after each request,
-// 36 so.) The runs are dealt from the lengths by every wave for itself, a lane a request, in DPP sums.
+// 33 so.) The runs are dealt from the lengths by every wave for itself, a lane a request, in DPP sums.
 #include "plz_paged.h"
 #include "palettize_hip.h"
 
@@ -41,7 +41,7 @@ namespace paged {
 constexpr int NW = 4, NT = 64 * NW;  // waves, threads
 constexpr int PARTS = 512;           // most workgroups: two for each of 256 CUs (parts_of)
 constexpr int HT = 16;               // heads a workgroup (columns of the matrix instruction)
-constexpr int ALONE = 512;           // tokens up to which a table's requests get a workgroup each
+constexpr int ALONE = 512;           // tokens up to which a table's requests get a workgroup each (one_each)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct AttnArgs {
@@ -606,16 +606,22 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   if (c == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
 }
 
-// A workgroup a request instead of equal runs, by the most tokens that the table can hold: one launch
-// and no workspace, at up to four tiles a wave no slower. Equal runs and one each, 32/8 heads of 128, in
-// us: 200 tokens B 1 8.3 and 6.0, B 16 9.8 and 7.1, B 256 41.2 and 42.0 (ragged 21.0 and 22.4); 500 tokens
-// B 1 8.5 and 8.5, B 4 8.9 and 9.4, B 16 12.5 and 10.5, B 256 85.6 and 85.4; 1000 tokens B 1 8.7 and 13.3.
-static bool one_each(int64_t width, int64_t page_size) { return width * page_size <= ALONE; }
+// A workgroup a request (and kv head) instead of equal runs: one launch and no workspace. It pays where
+// the table holds so few tokens that a wave has four tiles at most, and where the workgroups are few, so
+// that each has its place at once or nearly: more of them start late, which the equal runs never do.
+// Equal runs and one each, 32/8 heads of 128, in us (a call that the host bounds saves another 4 by the
+// launch): tables of 200 tokens, B 1 8.3 and 6.2, B 16 9.4 and 7.1, B 64 17.7 and 12.5, B 128 25.9 and
+// 22.8 (ragged 12.8 and 12.6), B 192 35.6 and 31.3 (ragged 15.7 and 16.5), B 256 38.3 and 40.2 (ragged
+// 18.0 and 21.1); 500 tokens, B 1 8.4 and 9.0, B 16 12.5 and 11.5, B 128 45.6 and 43.9, B 256 83.7 and
+// 84.0 (ragged 25.9 and 28.4); 1000 tokens, B 1 8.7 and 14.4.
+static bool one_each(int64_t batch, int64_t width, int64_t page_size, int64_t kv_heads, int64_t tiles) {
+  return width * page_size <= ALONE && batch <= 3 * PARTS && batch * kv_heads * tiles <= 3 * PARTS;
+}
 // Workgroups a (kv head, head tile): two a CU in all, one where a part is large (more than 1024 values:
 // writing and joining them costs more than the second workgroup's loads bring) or a workgroup takes the
 // whole CU's registers (heads of 256). Two and one: 16 x 4096 tokens, 4 kv heads of 128 with 20 heads
-// each 38.5 and 34.8 us, 32 ragged up to 4096 with 8 heads 16.4 and 16.6; 8 kv heads of 256 with 4 heads
-// each, 32 x 2048, 93.4 and 88.1.
+// each 37.0 and 36.1 us (ragged, 32 up to 4096 and 8 heads each, so parts of 1024: 15.7 and 15.4); 8 kv
+// heads of 256 with 4 heads each, 32 x 2048, 92.4 and 85.6; small parts, 32 ragged up to 4096 20.1 and 21.6.
 static int parts_of(int kv_heads, int G, int D) {
   const int heads = G < HT ? G : HT, tiles = (G + HT - 1) / HT;
   const int n = (D == 256 || heads * D > 1024 ? PARTS / 2 : PARTS) / (kv_heads * tiles);
@@ -653,9 +659,10 @@ extern "C" {
 size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
                                 int head_dim) {
   if (batch <= 0 || width <= 0 || page_size <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
-      heads % kv_heads || one_each(width, page_size))
+      heads % kv_heads)
     return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
+  if (one_each(batch, width, page_size, kv_heads, ht)) return 0;
   const size_t parts = (size_t)parts_of(kv_heads, G, head_dim);
   return parts * kv_heads * ht * 2 * (G < HT ? G : HT) * head_dim * sizeof(float) +
          parts * heads * 2 * sizeof(float2) + parts * sizeof(int2);

@@ -341,7 +341,7 @@ def test_attn_small_tables_without_a_workspace(dev, H, Hkv, D, P):
 
 
 def test_attn_many_requests_of_small_tables(dev):
-    """More (request, kv head) pairs than a grid's second dimension takes."""
+    """More (request, kv head) pairs than a grid's second dimension takes, by equal runs."""
     B = 9000
     g = torch.Generator(device=dev).manual_seed(2)
     kc = torch.randn(64, 8, 8, 16, 8, generator=g, device=dev).to(torch.bfloat16)

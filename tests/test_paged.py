@@ -246,7 +246,11 @@ def test_attn_needs_its_workspace(lib):
         assert lib.plz_paged_attn_workspace(*args) == 0
     # tables of up to 512 tokens: a workgroup a request, nothing is shared
     assert lib.plz_paged_attn_workspace(1, 8, 64, 8, 2, 128) == 0
-    assert lib.plz_paged_attn_workspace(65536, 32, 16, 8, 2, 128) == 0
+    # ... while the workgroups are 1536 at most, batch x kv heads x tiles of 16 heads
+    for batch, heads, hkv in ((768, 8, 2), (384, 40, 2), (96, 16, 16)):
+        assert lib.plz_paged_attn_workspace(batch, 32, 16, heads, hkv, 128) == 0
+        assert lib.plz_paged_attn_workspace(batch + 1, 32, 16, heads, hkv, 128) > 0
+    assert lib.plz_paged_attn_workspace(65536, 32, 16, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(1, 9, 64, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(5, 33, 16, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(1 << 40, 1 << 20, 1024, 8, 2, 128) > 0

@@ -444,7 +444,8 @@ int plz_paged_rope_write(const uint16_t* q, const uint16_t* k, const uint16_t* v
   const WriteArgs g{q,     k,      v,   q_weight, k_weight, cos_table, sin_table, positions,
                     slots, q_out, k_cache, v_cache, tokens, ld_q, ld_k, ld_v,
                     heads, kv_heads, (int)max_positions, shift, num_pages * page_size, eps, each, groups};
-  PLZ_REQUIRE((blocks + 7) / 8 * 8 * groups < ((int64_t)1 << 31), "%s: too many tokens x heads", what);
+  // a launch takes fewer than 2^32 threads
+  PLZ_REQUIRE((blocks + 7) / 8 * 8 * groups < ((int64_t)1 << 24), "%s: too many tokens x heads", what);
   const dim3 grid((unsigned)((blocks + 7) / 8 * 8 * groups));
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, g);

@@ -658,7 +658,7 @@ extern "C" {
 
 size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int heads, int kv_heads,
                                 int head_dim) {
-  if (batch <= 0 || width <= 0 || page_size <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
+  if (batch <= 0 || width < 0 || page_size <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
       heads % kv_heads)
     return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;

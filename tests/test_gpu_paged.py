@@ -352,6 +352,32 @@ def test_attn_many_requests_of_small_tables(dev):
     _check_attn(q, kc, vc, table, lens, rows=[0, 1, 8191, 8192, 8999] + list(range(5, B, 700)))
 
 
+def test_attn_largest_batch(dev):
+    """65536 requests, 1024 a lane of the waves that deal them out."""
+    B = 65536
+    g = torch.Generator(device=dev).manual_seed(3)
+    kc = torch.randn(32, 1, 8, 16, 8, generator=g, device=dev).to(torch.bfloat16)
+    vc = torch.randn(32, 1, 16, 64, generator=g, device=dev).to(torch.bfloat16)
+    q = torch.randn(B, 2, 64, generator=g, device=dev).to(torch.bfloat16)
+    table = torch.randint(0, 32, (B, 4), generator=g, device=dev, dtype=torch.int32)
+    lens = torch.randint(-8, 66, (B,), generator=g, device=dev, dtype=torch.int32).clamp_(0, 64)
+    lens[:3000] = 0
+    lens[-1] = 64
+    _check_attn(q, kc, vc, table, lens, rows=[0, 2999, 3000, 65535] + list(range(3001, B, 1500)))
+
+
+@pytest.mark.parametrize("B", [3, 3000])
+def test_attn_table_without_columns(dev, B):
+    kc, vc = ops.paged_cache(2, 16, 2, 128, dev)
+    q = torch.randn(B, 4, 128, device=dev, dtype=torch.bfloat16)
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+    lens[1] = 5  # more than the table holds
+    o, lse = ops.paged_attn(q, kc, vc, lens.new_empty(B, 0), lens)
+    rest = [0] + list(range(2, B))
+    assert bool((o[rest] == 0).all()) and bool((lse[rest] == float("-inf")).all())
+    assert bool(torch.isnan(o[1]).all()) and bool(torch.isnan(lse[1]).all())
+
+
 @pytest.mark.parametrize("std", [0.05, 12.0])
 def test_attn_flat_and_peaked(dev, std):
     _check_attn(*_attn_case([700, 90, 1, 2100], 8, 2, 128, 64, 5, dev, std=std))

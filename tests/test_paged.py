@@ -67,7 +67,8 @@ def _write_args(**kw):
     (dict(pos=None), 1, b"null"), (dict(slots=None), 1, b"null"), (dict(vc=None), 1, b"null"),
     (dict(k=FAKE + 8), 1, b"aligned"), (dict(kc=FAKE + 2), 1, b"aligned"),
     (dict(cos=FAKE + 4), 1, b"aligned"),
-    (dict(tokens=1 << 30, heads=16384, ldq=1 << 21), 1, b"too many")])
+    (dict(tokens=1 << 30, heads=16384, ldq=1 << 21), 1, b"too many"),
+    (dict(tokens=1 << 28, heads=1, kv=1), 1, b"too many")])
 def test_write_refusals(lib, kw, code, word):
     if word == b"together":
         word = b"go together"
@@ -250,7 +251,8 @@ def test_attn_needs_its_workspace(lib):
     for batch, heads, hkv in ((768, 8, 2), (384, 40, 2), (96, 16, 16)):
         assert lib.plz_paged_attn_workspace(batch, 32, 16, heads, hkv, 128) == 0
         assert lib.plz_paged_attn_workspace(batch + 1, 32, 16, heads, hkv, 128) > 0
-    assert lib.plz_paged_attn_workspace(65536, 32, 16, 8, 2, 128) > 0
+    for width in (0, 32):
+        assert lib.plz_paged_attn_workspace(65536, width, 16, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(1, 9, 64, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(5, 33, 16, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(1 << 40, 1 << 20, 1024, 8, 2, 128) > 0

@@ -41,7 +41,8 @@ namespace paged {
 constexpr int NW = 4, NT = 64 * NW;  // waves, threads
 constexpr int PARTS = 512;           // most workgroups: two for each of 256 CUs (parts_of)
 constexpr int HT = 16;               // heads a workgroup (columns of the matrix instruction)
-constexpr int ALONE = 512;           // tokens up to which a table's requests get a workgroup each (one_each)
+constexpr int ALONE = 512;           // tokens up to which a table's requests get waves of their own (own_waves)
+constexpr int64_t ALONE_MOST = (int64_t)1 << 22;  // and how many of these at most: a launch has 2^32 threads
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct AttnArgs {
@@ -55,7 +56,8 @@ struct AttnArgs {
   // b {the workgroup that begins it or -1, the one that ends it}.
   int2* open;
   int by_request;
-  int alone;  // workgroup w has request w alone, and all of it: no workspace, no second kernel
+  int alone;  // waves a request, when each has its own ones in one workgroup (no workspace, no second
+              // kernel); 0: equal runs
   int64_t ldq;
   int B, W, Hq, Hkv, G, tiles_h, parts, num_pages, shift;  // tiles_h = head tiles a kv head
   float scale_log2;
@@ -117,10 +119,11 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   float* const res = reinterpret_cast<float*>(s_res) + wave * 2 * slot;
   if (lane == 0) s_has[wave] = 0;
 
-  // The requests that this workgroup shares with others (all of them, or its own one with none), and its
-  // number among these: every one's tiles (a lane takes `each` consecutive requests) and their sums
-  const int from = g.alone ? w : 0, to = g.alone ? w + 1 : g.B;
-  const int me = g.alone ? 0 : w, others = g.alone ? 1 : g.parts;
+  // The requests that this wave shares with others (all of them, or its own one), its number among these
+  // and how many they are: every request's tiles (a lane takes `each` consecutive ones) and their sums
+  const int number = w * NW + wave, from = g.alone ? number / g.alone : 0;
+  const int to = g.alone ? min(from + 1, g.B) : g.B;
+  const int me = g.alone ? number % g.alone : number, waves = g.alone ? g.alone : g.parts * NW;
   const int each = (to - from + 63) >> 6;
   int win_at = from, win = 0;  // lane l: the length of request win_at + l
   int mine = 0;
@@ -135,10 +138,10 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   none = __builtin_amdgcn_ballot_w64(none) != 0;
   int sum = wave_scan(mine);
   const int total = __builtin_amdgcn_readlane(sum, 63);
-  const Deal runs = deal(total, others * NW);
+  const Deal runs = deal(total, waves);
 
-  if (me * NW + wave < runs.runs) {
-    const int r0 = run_begin(runs, me * NW + wave), r1 = run_begin(runs, me * NW + wave + 1);
+  if (me < runs.runs) {
+    const int r0 = run_begin(runs, me), r1 = run_begin(runs, me + 1);
     // the request that holds tile r0, and its first tile among all: the lane, then its requests
     auto holder = [&]() { return __builtin_ctzll(__builtin_amdgcn_ballot_w64(r0 < sum)); };
     int at = holder();
@@ -516,10 +519,9 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   if (g.open && !g.by_request && threadIdx.x == 0 && hk + ht == 0)
     g.open[w] = make_int2(open, open_last);
 
-  // requests without tiles, spread over the workgroups that have work
-  const int every = max((runs.runs + NW - 1) / NW, 1);
-  if (none && me < every)
-    for (int b = from + me + every * wave; b < to; b += every * NW) {
+  // requests without tiles, spread over all waves
+  if (none)
+    for (int b = from + me; b < to; b += waves) {
       const int len = g.lens[b];
       if (tiles_of(len, cap) != 0) continue;
       const float x = len <= 0 ? 0.f : __builtin_nanf("");
@@ -608,16 +610,26 @@ __global__ __launch_bounds__(JT) void paged_join_kernel(AttnArgs g) {
   if (c == 0) g.lse[at] = (ref + log2f(l)) * kLn2;
 }
 
-// A workgroup a request (and kv head) instead of equal runs: one launch and no workspace. It pays where
-// the table holds so few tokens that a wave has four tiles at most, and where the workgroups are few, so
-// that each has its place at once or nearly: more of them start late, which the equal runs never do.
-// Equal runs and one each, 32/8 heads of 128, in us (a call that the host bounds saves another 4 by the
-// launch): tables of 200 tokens, B 1 8.3 and 6.2, B 16 9.4 and 7.1, B 64 17.7 and 12.5, B 128 25.9 and
-// 22.8 (ragged 12.8 and 12.6), B 192 35.6 and 31.3 (ragged 15.7 and 16.5), B 256 38.3 and 40.2 (ragged
-// 18.0 and 21.1); 500 tokens, B 1 8.4 and 9.0, B 16 12.5 and 11.5, B 128 45.6 and 43.9, B 256 83.7 and
-// 84.0 (ragged 25.9 and 28.4); 1000 tokens, B 1 8.7 and 14.4.
-static bool one_each(int64_t batch, int64_t width, int64_t page_size, int64_t kv_heads, int64_t tiles) {
-  return width * page_size <= ALONE && batch <= 3 * PARTS && batch * kv_heads * tiles <= 3 * PARTS;
+// Waves of its own for every request (and kv head, head tile) instead of equal runs, by the most tokens
+// that its table can hold: one launch and no workspace, and a call that the host bounds saves another 4 us
+// by the launch. Four, two or one, so that all workgroups have their place at once if they can;
+// short ones get one wave rather than two, whose start and join cost more than their tiles; what takes
+// several rounds even so pays up to 320 tokens. 0: equal runs. 32/8 heads of 128, in us, equal runs / 1 / 2 / 4:
+//    50 tokens: B 16 7.1 5.2 5.7 5.1, B 96 9.8 6.7 8.0 9.8, B 256 14.4 12.3 16.4 21.0, ragged 13.4 7.9 11.4 16.6
+//   200 tokens: B 16 9.5 12.7 10.1 7.3, B 96 23.4 17.1 18.1 19.0, ragged 11.8 11.6 10.0 11.3,
+//               B 256 38 36 39 40, ragged 18.2 14.7 16.9 21.5
+//   500 tokens: B 16 12.5 25.3 16.4 10.8, B 64 26.0 29.4 25.1 24.3, B 192 ragged 21.3 26.2 22.0 22.6,
+//               B 256 ragged 26.0 27.1 27.1 28.2;   1000 tokens: B 1 8.7, 14.4 with four, B 256 168 and 165
+// 1024 of 20 to 200 tokens: one 3 to 14% faster than equal runs. Heads of 64 and 256 are alike, with more
+// and fewer workgroups in place: 128 requests of 200 tokens 18.0 13.3 12.9 15.4, 64 27.6 27.8 21.6 25.4.
+static int own_waves(int64_t batch, int64_t width, int64_t page_size, int64_t kv_heads, int64_t tiles,
+                     int D) {
+  const int64_t longest = width * page_size;
+  if (longest > ALONE || batch > ALONE_MOST || batch * kv_heads * tiles > ALONE_MOST) return 0;
+  const int64_t all = batch * kv_heads * tiles, resident = D == 64 ? 768 : D == 128 ? 512 : 256;
+  if (all <= resident) return 4;
+  if (all <= 2 * resident) return longest * D <= 128 * 128 ? 1 : 2;
+  return longest <= 320 ? 1 : 0;
 }
 // Workgroups a (kv head, head tile): two a CU in all, one where a part is large (more than 1024 values:
 // writing and joining them costs more than the second workgroup's loads bring) or a workgroup takes the
@@ -664,7 +676,7 @@ size_t plz_paged_attn_workspace(int64_t batch, int64_t width, int page_size, int
       heads % kv_heads)
     return 0;
   const int G = heads / kv_heads, ht = (G + HT - 1) / HT;
-  if (one_each(batch, width, page_size, kv_heads, ht)) return 0;
+  if (own_waves(batch, width, page_size, kv_heads, ht, head_dim)) return 0;
   const size_t parts = (size_t)parts_of(kv_heads, G, head_dim);
   return parts * kv_heads * ht * 2 * (G < HT ? G : HT) * head_dim * sizeof(float) +
          parts * heads * 2 * sizeof(float2) + parts * sizeof(int2);
@@ -713,8 +725,8 @@ int plz_paged_attn(const uint16_t* q, int64_t ld_q, const uint16_t* k_cache,
   g.tiles_h = (g.G + HT - 1) / HT;
   g.parts = parts_of(kv_heads, g.G, head_dim);
   if (need == 0) {
-    g.parts = g.B;
-    g.alone = 1;
+    g.alone = own_waves(batch, width, page_size, kv_heads, g.tiles_h, head_dim);
+    g.parts = (g.B * g.alone + NW - 1) / NW;
   } else {
     g.part_ml = reinterpret_cast<float2*>(
         g.part + (int64_t)g.parts * kv_heads * g.tiles_h * 2 * (g.G < HT ? g.G : HT) * head_dim);

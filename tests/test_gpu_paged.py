@@ -321,27 +321,34 @@ def test_attn_many_ragged_requests(dev):
                 + rng.sample(range(1500), 30))
 
 
-@pytest.mark.parametrize("H,Hkv,D,P", [(8, 2, 128, 64), (20, 1, 64, 16), (3, 3, 256, 512)])
-def test_attn_small_tables_without_a_workspace(dev, H, Hkv, D, P):
-    """Tables of up to 512 tokens: a workgroup a request, no second launch; empty rows, every number of
-    tiles a wave, one length past its table; and the same rows through a wider table's equal runs."""
-    lens = [37, 0, 512, 1, 128, 129, 300, 511, 0, 480, 33, 200, 0]
-    q, kc, vc, table, n = _attn_case(lens, H, Hkv, D, P, 14, dev, width=512 // P)
-    assert ops.query("plz_paged_attn_workspace", len(lens), 512 // P, P, H, Hkv, D) == 0
+# four waves a request, two, one, one over several rounds
+@pytest.mark.parametrize("H,Hkv,D,P,width,many", [(8, 2, 128, 64, 8, 1), (20, 1, 64, 16, 32, 1),
+                                                  (3, 3, 256, 512, 1, 1), (16, 8, 128, 16, 32, 7),
+                                                  (40, 8, 256, 64, 4, 4), (80, 4, 64, 32, 16, 9),
+                                                  (16, 8, 128, 16, 8, 9), (4, 2, 256, 16, 20, 30),
+                                                  (40, 8, 128, 32, 10, 13)])
+def test_attn_small_tables_without_a_workspace(dev, H, Hkv, D, P, width, many):
+    """Tables of up to 512 tokens: waves of their own for every request, no second launch; empty rows,
+    every number of tiles a wave, one length past its table; and the same rows through a wider table's
+    equal runs."""
+    most = width * P
+    lens = [min(n, most) for n in [37, 0, 512, 1, 128, 129, 300, 511, 0, 480, 33, 200, 0]] * many
+    q, kc, vc, table, n = _attn_case(lens, H, Hkv, D, P, 14, dev, width=width)
+    assert ops.query("plz_paged_attn_workspace", len(lens), width, P, H, Hkv, D) == 0
     o, lse = _check_attn(q, kc, vc, table, n)
     long = n.clone()
-    long[3] = 513
+    long[3] = most + 1
     o2, lse2 = ops.paged_attn(q, kc, vc, table, long)
     assert bool(torch.isnan(o2[3]).all()) and bool(torch.isnan(lse2[3]).all())
     rest = [b for b in range(len(lens)) if b != 3]
     assert torch.equal(o2[rest], o[rest]) and torch.equal(lse2[rest], lse[rest])
-    wide = torch.cat([table, table], 1).contiguous()
+    wide = torch.cat([table] * (512 // most + 1), 1).contiguous()
     assert ops.query("plz_paged_attn_workspace", len(lens), wide.shape[1], P, H, Hkv, D) > 0
     _check_attn(q, kc, vc, wide, n)
 
 
 def test_attn_many_requests_of_small_tables(dev):
-    """More (request, kv head) pairs than a grid's second dimension takes, by equal runs."""
+    """More (request, kv head) pairs than a grid's second dimension takes."""
     B = 9000
     g = torch.Generator(device=dev).manual_seed(2)
     kc = torch.randn(64, 8, 8, 16, 8, generator=g, device=dev).to(torch.bfloat16)
@@ -353,17 +360,18 @@ def test_attn_many_requests_of_small_tables(dev):
 
 
 def test_attn_largest_batch(dev):
-    """65536 requests, 1024 a lane of the waves that deal them out."""
+    """65536 requests, 1024 a lane of the waves that deal them out; and a wave each."""
     B = 65536
     g = torch.Generator(device=dev).manual_seed(3)
     kc = torch.randn(32, 1, 8, 16, 8, generator=g, device=dev).to(torch.bfloat16)
     vc = torch.randn(32, 1, 16, 64, generator=g, device=dev).to(torch.bfloat16)
     q = torch.randn(B, 2, 64, generator=g, device=dev).to(torch.bfloat16)
-    table = torch.randint(0, 32, (B, 4), generator=g, device=dev, dtype=torch.int32)
+    table = torch.randint(0, 32, (B, 33), generator=g, device=dev, dtype=torch.int32)
     lens = torch.randint(-8, 66, (B,), generator=g, device=dev, dtype=torch.int32).clamp_(0, 64)
     lens[:3000] = 0
     lens[-1] = 64
-    _check_attn(q, kc, vc, table, lens, rows=[0, 2999, 3000, 65535] + list(range(3001, B, 1500)))
+    for t in (table, table[:, :4].contiguous()):
+        _check_attn(q, kc, vc, t, lens, rows=[0, 2999, 3000, 65535] + list(range(3001, B, 1500)))
 
 
 @pytest.mark.parametrize("B", [3, 3000])

@@ -245,14 +245,20 @@ def test_attn_needs_its_workspace(lib):
                  (3, 40, 16, 0, 2, 128), (3, 40, 16, 8, 0, 128), (3, 40, 16, 9, 2, 128),
                  (3, 40, 16, 8, 2, 0), (-1, 40, 16, 8, 2, 128), (3, -40, 16, 8, 2, 128)):
         assert lib.plz_paged_attn_workspace(*args) == 0
-    # tables of up to 512 tokens: a workgroup a request, nothing is shared
+    # tables of up to 512 tokens whose requests have waves of their own share nothing: up to 1024 of them
+    # (batch x kv heads x tiles of 16 heads; 1536 and 512 for heads of 64 and 256), any number up to 320
+    # tokens, and 2^22 at most
     assert lib.plz_paged_attn_workspace(1, 8, 64, 8, 2, 128) == 0
-    # ... while the workgroups are 1536 at most, batch x kv heads x tiles of 16 heads
-    for batch, heads, hkv in ((768, 8, 2), (384, 40, 2), (96, 16, 16)):
-        assert lib.plz_paged_attn_workspace(batch, 32, 16, heads, hkv, 128) == 0
-        assert lib.plz_paged_attn_workspace(batch + 1, 32, 16, heads, hkv, 128) > 0
-    for width in (0, 32):
-        assert lib.plz_paged_attn_workspace(65536, width, 16, 8, 2, 128) > 0
+    for batch, heads, hkv, dim in ((512, 8, 2, 128), (256, 40, 2, 128), (64, 16, 16, 128),
+                                   (768, 8, 2, 64), (256, 8, 2, 256)):
+        for width in (21, 32):
+            assert lib.plz_paged_attn_workspace(batch, width, 16, heads, hkv, dim) == 0
+            assert lib.plz_paged_attn_workspace(batch + 1, width, 16, heads, hkv, dim) > 0
+        assert lib.plz_paged_attn_workspace(batch + 1, 20, 16, heads, hkv, dim) == 0
+    for width in (0, 20):
+        assert lib.plz_paged_attn_workspace(65536, width, 16, 128, 64, 128) == 0
+        assert lib.plz_paged_attn_workspace(65536, width, 16, 130, 65, 128) > 0
+        assert lib.plz_paged_attn_workspace(1 << 40, width, 16, 1 << 30, 1 << 30, 128) > 0
     assert lib.plz_paged_attn_workspace(1, 9, 64, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(5, 33, 16, 8, 2, 128) > 0
     assert lib.plz_paged_attn_workspace(1 << 40, 1 << 20, 1024, 8, 2, 128) > 0

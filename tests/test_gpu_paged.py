@@ -462,6 +462,33 @@ def test_attn_nonfinite_values(dev):
     assert ((o[0].double() - wo).abs() <= bo).all() and ((lse[0].double() - wl).abs() <= bl).all()
 
 
+# waves a request (many requests of 8 kv heads): four, two, one, one over several rounds, equal runs
+@pytest.mark.parametrize("many,width", [(1, 16), (17, 32), (20, 8), (60, 20), (60, 40)])
+def test_attn_bad_and_nonfinite_rows_among_many(dev, many, width):
+    """Rows with a page outside the cache, an infinite value and a NaN key, each among good ones, through
+    every way of dealing requests to waves: only what they reach differs."""
+    lens = [100, 90, 128, 1, 0, 77]
+    q, kc, vc, table, n = _attn_case(lens, 16, 8, 128, 16, 17, dev, width=width)
+    again = dict(k_cache=kc, v_cache=vc, block_table=table.repeat(many, 1), lens=n.repeat(many))
+    qs = q.repeat(many, 1, 1)
+    want, want_lse = ops.paged_attn(qs, **again)
+    # row 0 needs a page that is not there, in its last tile; the first value of row 1's token 40 and of
+    # row 2's token 70 in kv head 3 are infinite and NaN
+    again["block_table"][:, 6].masked_fill_(again["lens"] == 100, kc.shape[0])
+    vc[table[1, 2], 3, 8, 0] = math.inf
+    kc[table[2, 4], 3, 0, 6, 0] = math.nan
+    o, lse = ops.paged_attn(qs, **again)
+    kind = torch.arange(len(lens) * many, device=dev) % len(lens)
+    assert bool(torch.isnan(o[kind == 0]).all()) and bool(torch.isnan(lse[kind == 0]).all())
+    assert bool((o[kind == 1][:, 6:8, 0] == math.inf).all())
+    assert bool(torch.isnan(o[kind == 2][:, 6:8]).all()) and bool(torch.isnan(lse[kind == 2][:, 6:8]).all())
+    same = (kind != 0)[:, None, None].expand_as(o).clone()
+    same[kind == 1, 6:8, 0] = False
+    same[kind == 2, 6:8] = False
+    assert torch.equal(o[same], want[same])
+    assert torch.equal(lse[kind == 1], want_lse[kind == 1]) and torch.equal(lse[kind > 2], want_lse[kind > 2])
+
+
 def test_attn_twice_gives_the_same_bits(dev):
     c = _attn_case([3000, 1, 77, 0, 900], 32, 8, 128, 64, 13, dev)
     o, lse = ops.paged_attn(*c)

@@ -87,8 +87,9 @@ class PagedKVCache:
         return ops.paged_attn(q, self.k[layer], self.v[layer], self.block_table, self.lens, scale)[0]
 
     def tokens(self, layer, request, n):
-        """Keys and values [n, kv_heads, head_dim] of the first n tokens of a request, copied out (as
-        many as it has: lens is on the device and not looked at)."""
+        """Keys and values [n, kv_heads, head_dim] of the first n tokens of a request, copied out. Rows
+        past the tokens that it has are zeros: its table's entries there name nothing, or pages of
+        others."""
         batch, width = self.block_table.shape
         if not (0 <= request < batch and 0 <= n <= width * self.page_size):
             raise ValueError(f"no {n} tokens of request {request} in a cache of {batch} requests of "
@@ -96,8 +97,9 @@ class PagedKVCache:
         k, v = self.k[layer], self.v[layer]
         t = torch.arange(n, device=v.device)
         page = self.block_table[request, t // self.page_size].long().clamp(0, self.num_pages - 1)
-        at = t % self.page_size
-        return k[page, :, :, at].reshape(n, v.shape[1], v.shape[3]), v[page, :, at]
+        at, none = t % self.page_size, (t >= self.lens[request])[:, None, None]
+        return (k[page, :, :, at].reshape(n, v.shape[1], v.shape[3]).masked_fill_(none, 0),
+                v[page, :, at].masked_fill_(none, 0))
 
 
 class HardDecoderLayer(nn.Module):
@@ -164,7 +166,8 @@ class HardDecoderLayer(nn.Module):
     def prefill(self, hs, cache, index, step, lens, cos, sin):
         """Prompts: hs bf16 [sum(lens), hidden], the requests' rows one after another; lens, a list, is
         what cache.step was given as new_tokens for requests without cached tokens. Whole sequences go
-        through the training layers' causal attention on the keys that the cache holds."""
+        through the training layers' causal attention on the keys that the cache holds. Rows of tokens that
+        found no room (slot -1) are NaN: their keys are nowhere, and later tokens would lack them."""
         cfg = self.cfg
         if hs.shape[0] != sum(lens):
             raise ValueError(f"hs has {hs.shape[0]} rows, the prompts have {sum(lens)} tokens")
@@ -181,6 +184,6 @@ class HardDecoderLayer(nn.Module):
                 y = attention(*qkv, cfg.heads, cfg.kv_heads)
                 o[row:row + n] = y[0, :n].view(n, cfg.heads, cfg.head_dim)
                 row += n
-            return o
+            return o.masked_fill_((step.slots < 0)[:, None, None], float("nan"))
 
         return self._rows(hs, cache, index, step, cos, sin, attend)

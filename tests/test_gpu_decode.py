@@ -188,3 +188,33 @@ def test_pages_run_out_and_come_back(dev):
     step = cache.step([0, 4, 5], keep=[0, 16, 0])
     assert cache.lens.tolist() == [0, 20, 5] and int(cache.free_count) == 1
     assert int((step.slots >= 0).sum()) == 9
+
+
+@pytest.mark.parametrize("kw", CFGS.values(), ids=CFGS.keys())
+def test_prompts_without_room(dev, kw):
+    """Prompts of 40, 20 and 5 tokens on a pool of four pages of 16: the second has room for 16, the third
+    for none. Rows with room are the rows of a pool with room for all, bit for bit, and right in 64 bits;
+    the others are NaN, whatever other requests have in the pages that stale table entries name."""
+    cfg, hard, soft = _layers(dev, kw)
+    cos, sin = layer.rope_tables(64, cfg.head_dim, cfg.rope_theta, dev)
+    lens, have = [40, 20, 5], [40, 16, 0]
+    g = torch.Generator().manual_seed(3)
+    hs = torch.randn(sum(lens), cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+    outs = []
+    for pages in (None, 4):
+        cache = decode.PagedKVCache(2, 3, 64, cfg.kv_heads, cfg.head_dim, page_size=16, num_pages=pages,
+                                    device=dev)
+        step, x = cache.step(lens), hs
+        for i, l in enumerate(hard):
+            x = l.prefill(x, cache, i, step, lens, cos, sin)
+        assert cache.lens.tolist() == (have if pages else lens)
+        outs.append(x)
+    full, got = outs
+    row = 0
+    for n, m in zip(lens, have):
+        assert torch.equal(got[row:row + m], full[row:row + m])
+        assert bool(torch.isnan(got[row + m:row + n]).all())
+        if m:
+            want = _reference(cfg, soft, hs[row:row + m].double(), cos, sin)
+            assert_close(f32(got[row:row + m]), f32(want), what=f"prompt of {n}")
+        row += n

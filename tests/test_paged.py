@@ -360,3 +360,20 @@ def test_cache_and_layer_refusals():
     with pytest.raises(ValueError, match="rows"):
         decode.HardDecoderLayer.prefill.__wrapped__(
             type("L", (), {"cfg": None})(), torch.zeros(5, 8), c, 0, None, [2, 2], None, None)
+
+
+def test_cache_tokens_that_a_request_does_not_have():
+    """tokens() reads a request's own pages only: rows past its length are zeros, whatever its table's
+    unused entries name."""
+    from palettize_hip import decode
+    c = decode.PagedKVCache(1, 3, 64, 2, 64, page_size=16, num_pages=4, device="cpu")
+    for t in (c.k[0], c.v[0]):
+        t.copy_(torch.arange(1, 5).view(4, 1, 1, 1, *[1] * (t.dim() - 4)))  # a page's number + 1
+    c.v[0][0, :, 5:] = float("nan")
+    c.lens.copy_(torch.tensor([5, 16, 0]))
+    c.block_table[1, 0], c.block_table[1, 1], c.block_table[2, 0] = 3, 2 ** 31 - 1, -1
+    for request, has, page in ((0, 5, 1), (1, 16, 4), (2, 0, None)):
+        for x in c.tokens(0, request, 20):
+            assert x.shape == (20, 2, 64)
+            assert bool((x[has:] == 0).all())
+            assert page is None or bool((x[:has] == page).all())

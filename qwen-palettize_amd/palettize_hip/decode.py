@@ -167,13 +167,15 @@ class HardDecoderLayer(nn.Module):
         """Prompts: hs bf16 [sum(lens), hidden], the requests' rows one after another; lens, a list, is
         what cache.step was given as new_tokens for requests without cached tokens. Whole sequences go
         through the training layers' causal attention on the keys that the cache holds. Rows of tokens that
-        found no room (slot -1) are NaN: their keys are nowhere, and later tokens would lack them."""
+        found no room (slot -1) are NaN: their keys are nowhere, and later tokens would lack them. So are
+        the rows of a request that had cached tokens: its prompt's tokens are not its first ones."""
         cfg = self.cfg
         if hs.shape[0] != sum(lens):
             raise ValueError(f"hs has {hs.shape[0]} rows, the prompts have {sum(lens)} tokens")
 
         def attend(q):
-            o, row = torch.empty_like(q), 0
+            o, row, dead = torch.empty_like(q), 0, step.slots < 0
+            at = torch.arange(max(lens, default=0), dtype=torch.int32, device=q.device)
             for b, n in enumerate(lens):
                 if n == 0:
                     continue
@@ -183,7 +185,8 @@ class HardDecoderLayer(nn.Module):
                 qkv = [nn.functional.pad(t, (0, 0, 0, 0, 0, pad))[None] for t in (q[row:row + n], k, v)]
                 y = attention(*qkv, cfg.heads, cfg.kv_heads)
                 o[row:row + n] = y[0, :n].view(n, cfg.heads, cfg.head_dim)
+                dead[row:row + n] |= step.positions[row:row + n] != at[:n]
                 row += n
-            return o.masked_fill_((step.slots < 0)[:, None, None], float("nan"))
+            return o.masked_fill_(dead[:, None, None], float("nan"))
 
         return self._rows(hs, cache, index, step, cos, sin, attend)

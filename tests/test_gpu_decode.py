@@ -218,3 +218,23 @@ def test_prompts_without_room(dev, kw):
             want = _reference(cfg, soft, hs[row:row + m].double(), cos, sin)
             assert_close(f32(got[row:row + m]), f32(want), what=f"prompt of {n}")
         row += n
+
+
+@pytest.mark.parametrize("kw", CFGS.values(), ids=CFGS.keys())
+def test_prompts_over_cached_tokens_are_marked(dev, kw):
+    """prefill is for requests without cached tokens: the rows of one that has some are NaN, the others
+    as they are alone."""
+    cfg, hard, _ = _layers(dev, kw, 1)
+    cos, sin = layer.rope_tables(64, cfg.head_dim, cfg.rope_theta, dev)
+    g = torch.Generator().manual_seed(7)
+    hs = torch.randn(29, cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+    outs = []
+    for first in ([0, 0], [3, 0]):
+        cache = decode.PagedKVCache(1, 2, 64, cfg.kv_heads, cfg.head_dim, page_size=16, device=dev)
+        step = cache.step(first)
+        hard[0].prefill(hs[:sum(first)], cache, 0, step, first, cos, sin) if sum(first) else None
+        step = cache.step([12, 17])
+        outs.append(hard[0].prefill(hs, cache, 0, step, [12, 17], cos, sin))
+    assert bool(torch.isfinite(outs[0]).all())
+    assert bool(torch.isnan(outs[1][:12]).all())
+    assert torch.equal(outs[1][12:], outs[0][12:])

@@ -16,6 +16,7 @@ All of it runs on the device and in the same buffers every time, so a step can b
 """
 from __future__ import annotations
 
+import functools
 from collections import namedtuple
 
 import torch
@@ -28,9 +29,19 @@ from .layer import LayerConfig, PalettizedDecoderLayer, attention
 Step = namedtuple("Step", "slots positions starts")
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_grad(*args):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
         raise RuntimeError("decoding has no backward: call it under torch.no_grad()")
+
+
+def _inference(fn):
+    """The method under no_grad, after a refusal of arguments that need a gradient where they are on."""
+    @functools.wraps(fn)
+    def run(self, *args, **kw):
+        _no_grad(*args, *kw.values())
+        with torch.no_grad():
+            return fn(self, *args, **kw)
+    return run
 
 
 class PagedKVCache:
@@ -155,14 +166,14 @@ class HardDecoderLayer(nn.Module):
         h = ops.swiglu_fwd(self._linear("gate_proj", x), self._linear("up_proj", x))
         return self._linear("down_proj", h, hs)
 
-    @torch.no_grad()
+    @_inference
     def decode(self, hs, cache, index, step, cos, sin):
         """One new token a request: hs bf16 [batch, hidden], step from cache.step(..., rows_each=1),
         cos, sin fp32 [positions, head_dim] (layer.rope_tables). A request that got no token in this
         step has its row computed from its cached tokens alone; that row means nothing."""
         return self._rows(hs, cache, index, step, cos, sin, lambda q: cache.attend(index, q))
 
-    @torch.no_grad()
+    @_inference
     def prefill(self, hs, cache, index, step, lens, cos, sin):
         """Prompts: hs bf16 [sum(lens), hidden], the requests' rows one after another; lens, a list, is
         what cache.step was given as new_tokens for requests without cached tokens. Whole sequences go

@@ -238,3 +238,28 @@ def test_prompts_over_cached_tokens_are_marked(dev, kw):
     assert bool(torch.isfinite(outs[0]).all())
     assert bool(torch.isnan(outs[1][:12]).all())
     assert torch.equal(outs[1][12:], outs[0][12:])
+
+
+def test_layers_refuse_gradients(dev):
+    """decode and prefill have no backward: a hidden state, or a table, that needs a gradient is refused
+    where gradients are on, and taken under no_grad."""
+    cfg, hard, _ = _layers(dev, CFGS["d128"], 1)
+    cos, sin = layer.rope_tables(64, cfg.head_dim, cfg.rope_theta, dev)
+    cache = decode.PagedKVCache(1, 2, 64, cfg.kv_heads, cfg.head_dim, page_size=16, device=dev)
+    hs = torch.randn(5, cfg.hidden, device=dev).to(torch.bfloat16)
+    step = cache.step([3, 2])
+    first = hard[0].prefill(hs, cache, 0, step, [3, 2], cos, sin)
+    needs = hs.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        hard[0].prefill(needs, cache, 0, step, [3, 2], cos, sin)
+    with pytest.raises(RuntimeError, match="no backward"):
+        hard[0].prefill(hs, cache, 0, step, [3, 2], cos=cos.clone().requires_grad_(), sin=sin)
+    with torch.no_grad():
+        assert torch.equal(hard[0].prefill(needs, cache, 0, step, [3, 2], cos, sin), first)
+    step = cache.step([1, 1], rows_each=1)
+    with pytest.raises(RuntimeError, match="no backward"):
+        hard[0].decode(needs[:2], cache, 0, step, cos, sin)
+    with torch.no_grad():
+        got = hard[0].decode(needs[:2], cache, 0, step, cos, sin)
+    assert not got.requires_grad
+    assert torch.equal(got, hard[0].decode(hs[:2], cache, 0, step, cos, sin))

@@ -377,3 +377,22 @@ def test_cache_tokens_that_a_request_does_not_have():
             assert x.shape == (20, 2, 64)
             assert bool((x[has:] == 0).all())
             assert page is None or bool((x[:has] == page).all())
+
+
+def test_operators_refuse_gradients(ops):
+    """The operators have no backward: each tensor of values that needs a gradient is refused where
+    gradients are on, and taken under no_grad (here: up to the call itself)."""
+    kc, vc = ops.paged_cache(4, 16, 2, 64, "cpu")
+    write = dict(q=_bf(3, 4, 64), k=_bf(3, 2, 64), v=_bf(3, 2, 64), cos=torch.zeros(8, 64),
+                 sin=torch.zeros(8, 64), positions=_i32(3), slots=_i32(3), k_cache=kc, v_cache=vc,
+                 q_weight=_bf(64), k_weight=_bf(64))
+    attn = dict(q=_bf(3, 4, 64), k_cache=kc, v_cache=vc, block_table=_i32(3, 2), lens=_i32(3))
+    for fn, ok in ((ops.paged_rope_write, write), (ops.paged_attn, attn)):
+        for name, t in ok.items():
+            if t.is_floating_point():
+                needs = {**ok, name: t.clone().requires_grad_()}
+                with pytest.raises(RuntimeError, match="no backward"):
+                    fn(**needs)
+                with torch.no_grad(), pytest.raises(Exception) as e:
+                    fn(**needs)
+                assert "no backward" not in str(e.value)

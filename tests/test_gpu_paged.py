@@ -663,3 +663,136 @@ def test_two_graphs_of_attention_side_by_side(dev):
             assert all(torch.equal(x, y) for x, y in zip(got, ref))
             for x in got:
                 x.zero_()
+
+
+# ---- what the sizes above do not reach ------------------------------------------------------------------
+def _each(T, H, Hkv, D):
+    """Heads a workgroup of the cache write."""
+    tb, heads = 4 * (64 // (D // 8)), H + 2 * Hkv
+    each = 1
+    while each < 8 and -(-T // tb) * heads >= 2048 * each:
+        each *= 2
+    return each
+
+
+# groups of 4 and 8 heads: across q | k and k | v, the last one ragged, tokens that fill no block
+@pytest.mark.parametrize("T,H,Hkv,D,P,norm,fused,each", [
+    (4001, 14, 2, 128, 64, True, True, 4), (9403, 5, 1, 128, 16, False, False, 4),
+    (8191, 14, 2, 128, 32, True, False, 8), (18811, 5, 1, 128, 64, True, True, 8),
+    (8007, 14, 2, 64, 16, True, False, 4), (37501, 5, 1, 64, 64, True, True, 8),
+    (17503, 9, 3, 64, 128, False, True, 8), (2201, 14, 2, 256, 64, False, True, 4),
+    (4771, 5, 1, 256, 16, True, True, 4), (4409, 9, 3, 256, 32, True, False, 8)])
+def test_write_of_many_heads_a_workgroup(dev, T, H, Hkv, D, P, norm, fused, each):
+    assert _each(T, H, Hkv, D) == each
+    c = list(_write_case(T, H, Hkv, D, P, T + D, dev, norm, fused))
+    pos, slots = c[5], c[6]
+    dead = torch.randperm(T, generator=torch.Generator().manual_seed(T))[:200].to(dev)
+    slots[dead[:100]] = -1
+    pos[dead[100:120]] = 300
+    slots[-3:] = -1
+    _check_write(*c, P)
+
+
+def _waves(batch, width, P, H, Hkv, D):
+    """Waves a (kv head, 16 query heads) that the equal runs are dealt to, from the workspace's size."""
+    G = H // Hkv
+    tiles = -(-G // 16)
+    need = ops.query("plz_paged_attn_workspace", batch, width, P, H, Hkv, D)
+    part = Hkv * tiles * 2 * min(G, 16) * D * 4 + H * 16 + 8
+    assert need > 0 and need % part == 0
+    return 4 * need // part
+
+
+# What tile i (32 tokens) of a request adds to its scores, in log2 units
+RAMPS = {"rising": lambda i: 10.0 * i, "falling": lambda i: -10.0 * i, "slow": lambda i: 3.0 * i,
+         "sawtooth": lambda i: (0.0, 9.0, 20.0, 4.0, 31.0)[i % 5] + i, "flat": lambda i: 0.0 * i}
+
+
+def _ramped(lens, H, Hkv, D, P, seed, dev, width=None):
+    """_attn_case whose request b's scores follow ramp b % 5, tile by tile: value 0 of a key is what its
+    tile adds, value 0 of a query 16, the others are noise of standard deviation about 1 in log2 units."""
+    q, kc, vc, table, n = _attn_case(lens, H, Hkv, D, P, seed, dev, std=0.7, width=width)
+    scale = D ** -0.5
+    unit = 16 * scale / math.log(2)
+    q[:, :, 0] = 16
+    ramps = list(RAMPS.values())
+    for b, x in enumerate(lens):
+        t = torch.arange(x, device=dev)
+        add = torch.tensor([ramps[b % len(ramps)](i) for i in range(-(-x // 32))], device=dev) / unit
+        page, at = table[b].long()[t // P], t % P
+        kc[page, :, 0, at, 0] = add[t // 32].to(torch.bfloat16)[:, None]
+    return q, kc, vc, table, n
+
+
+def _check_heads(c, heads, got=None, rows=None):
+    """paged_attn on c, these query heads of it (of one kv head each) against 64 bits."""
+    q, kc, vc, table, lens = c
+    o, lse = ops.paged_attn(*c) if got is None else got
+    G = q.shape[1] // vc.shape[1]
+    for b in range(q.shape[0]) if rows is None else rows:
+        k, v = paged_ref.rows_of(kc, vc, table[b], int(lens[b]))
+        for h in heads:
+            wo, wl, bo, bl = paged_ref.attend(q[b, h:h + 1], k[:, h // G, None], v[:, h // G, None],
+                                              q.shape[2] ** -0.5)
+            assert ((o[b, h].double() - wo[0]).abs() <= bo[0]).all(), (b, h)
+            assert ((lse[b, h].double() - wl[0]).abs() <= bl[0]).all(), (b, h)
+    return o, lse
+
+
+@pytest.mark.parametrize("H,Hkv,D,P", [(32, 32, 128, 64), (96, 48, 64, 16), (30, 15, 256, 32)])
+def test_attn_ramps_in_one_wave(dev, H, Hkv, D, P):
+    """Tables of 320 tokens and more pairs of requests and kv heads than have a place at once: one wave for
+    all ten tiles of a request, whose maximum moves at every tile, at some, or never."""
+    width = 320 // P
+    lens = [320, 320, 320, 320, 320, 311, 289, 300, 320, 257, 33, 64] * 4
+    resident = {64: 768, 128: 512, 256: 256}[D]
+    assert len(lens) * Hkv > 2 * resident
+    assert ops.query("plz_paged_attn_workspace", len(lens), width, P, H, Hkv, D) == 0
+    _check_heads(_ramped(lens, H, Hkv, D, P, 18, dev, width=width), [0, H // 2, H - 1],
+                 rows=list(range(12)) + [47])
+
+
+# (heads, kv heads, head dim, page, lengths, tiles a wave at least): 8 workgroups a (kv head, 16 heads) in
+# the first four, 1 and 32
+LONG = [(1024, 1, 64, 16, [40000, 40001], 70), (1024, 4, 64, 64, [30000, 20, 50007], 70),
+        (1024, 2, 64, 1024, [45000, 36001], 70), (512, 1, 128, 64, [40000, 36003], 70),
+        (8192, 1, 64, 32, [5000, 0, 5003, 65], 70), (8, 8, 256, 16, [21000, 1, 21500, 9], 8)]
+
+
+@pytest.mark.parametrize("H,Hkv,D,P,lens,tiles", LONG)
+def test_attn_many_tiles_a_wave(dev, H, Hkv, D, P, lens, tiles):
+    """Runs of more tiles of one request than a wave looks up pages for at once (32), a page that is not
+    there behind the first 32 tiles of a run, which makes its request NaN and leaves the others as they are,
+    and requests of every ramp, of about as many tiles as a run."""
+    heads = [0, 1, H // 2 + 1, H - 1]
+    q, kc, vc, table, n = c = _attn_case(lens, H, Hkv, D, P, 19, dev)
+    waves = _waves(len(lens), table.shape[1], P, H, Hkv, D)
+    total = sum(-(-x // 32) for x in lens)
+    assert total // waves >= tiles
+    o, lse = _check_heads(c, heads, rows=[b for b, x in enumerate(lens) if x])
+    for b, x in enumerate(lens):
+        if x == 0:
+            assert bool((o[b] == 0).all()) and bool((lse[b] == -math.inf).all())
+    run = total // waves
+    bad = table.clone()
+    bad[0, (min(run, 50) - 5) * 32 // P] = kc.shape[0]
+    o2, lse2 = ops.paged_attn(q, kc, vc, bad, n)
+    assert bool(torch.isnan(o2[0]).all()) and bool(torch.isnan(lse2[0]).all())
+    assert torch.equal(o2[1:], o[1:]) and torch.equal(lse2[1:], lse[1:])
+    if run < 32:
+        return
+    lens = [32 * 70, 32 * 71 - 5, 32 * 68 + 1, 32 * 70, 32 * 64] * (2 * waves // 5 + 1)
+    c = _ramped(lens, H, Hkv, D, P, 20, dev)
+    assert sum(-(-x // 32) for x in lens) // _waves(len(lens), c[3].shape[1], P, H, Hkv, D) >= 70
+    _check_heads(c, heads[1:3], rows=list(range(5)) + [len(lens) - 1])
+
+
+def test_attn_of_one_workgroup_a_head(dev):
+    """As many (kv head, 16 heads) pairs as workgroups: each has one, which joins nothing with others, for
+    several requests, empty ones among them."""
+    for H, Hkv, D in ((8192, 1, 64), (512, 512, 64), (512, 256, 256)):
+        lens = [700, 0, 2000, 1, 0, 515]
+        c = _attn_case(lens, H, Hkv, D, 16, 21, dev)
+        assert _waves(len(lens), c[3].shape[1], 16, H, Hkv, D) == 4
+        o, lse = _check_heads(c, [0, H // 2, H - 1], rows=[0, 2, 3, 5])
+        assert bool((o[[1, 4]] == 0).all()) and bool((lse[[1, 4]] == -math.inf).all())

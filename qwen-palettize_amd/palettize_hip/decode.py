@@ -153,7 +153,7 @@ class HardDecoderLayer(nn.Module):
         return y if residual is None else y + residual
 
     def _rows(self, hs, cache, index, step, cos, sin, attend):
-        """The layer on token rows hs [rows, hidden]; attend(q) is the attention's part."""
+        """The layer on token rows hs [rows, hidden]; attend(q, v) is the attention's part."""
         cfg = self.cfg
         hs = hs.contiguous()
         x, _ = ops.rmsnorm_fwd(hs, self.input_layernorm, cfg.eps)
@@ -161,7 +161,7 @@ class HardDecoderLayer(nn.Module):
                    for n, h in (("q_proj", cfg.heads), ("k_proj", cfg.kv_heads),
                                 ("v_proj", cfg.kv_heads)))
         q = cache.write(index, q, k, v, cos, sin, step, self.q_norm, self.k_norm, cfg.eps)
-        o = self._linear("o_proj", attend(q).reshape(-1, cfg.heads * cfg.head_dim))
+        o = self._linear("o_proj", attend(q, v).reshape(-1, cfg.heads * cfg.head_dim))
         hs, x, _ = ops.add_rmsnorm_fwd(hs, o, self.post_attention_layernorm, cfg.eps)
         h = ops.swiglu_fwd(self._linear("gate_proj", x), self._linear("up_proj", x))
         return self._linear("down_proj", h, hs)
@@ -171,7 +171,7 @@ class HardDecoderLayer(nn.Module):
         """One new token a request: hs bf16 [batch, hidden], step from cache.step(..., rows_each=1),
         cos, sin fp32 [positions, head_dim] (layer.rope_tables). A request that got no token in this
         step has its row computed from its cached tokens alone; that row means nothing."""
-        return self._rows(hs, cache, index, step, cos, sin, lambda q: cache.attend(index, q))
+        return self._rows(hs, cache, index, step, cos, sin, lambda q, v: cache.attend(index, q))
 
     @_inference
     def prefill(self, hs, cache, index, step, lens, cos, sin):
@@ -184,20 +184,28 @@ class HardDecoderLayer(nn.Module):
         if hs.shape[0] != sum(lens):
             raise ValueError(f"hs has {hs.shape[0]} rows, the prompts have {sum(lens)} tokens")
 
-        def attend(q):
-            o, row, dead = torch.empty_like(q), 0, step.slots < 0
-            at = torch.arange(max(lens, default=0), dtype=torch.int32, device=q.device)
-            for b, n in enumerate(lens):
+        def attend(q, v):
+            # rows that are not their request's first tokens, or have no slot
+            at = torch.arange(q.shape[0], dtype=torch.int32, device=q.device)
+            if len([n for n in lens if n]) > 1:
+                at = at - step.starts[torch.searchsorted(step.starts, at, right=True) - 1]
+            slots = step.slots.long()
+            dead = (step.positions != at).logical_or_(slots < 0)[:, None, None]
+            # the other rows' keys back from their slots; what is 0 times a dead row's value has to be 0
+            k, P = cache.k[index], cache.page_size
+            slots.clamp_(0, cache.num_pages * P - 1)
+            k = k[slots // P, :, :, slots % P].view(v.shape).masked_fill_(dead, 0)
+            v.masked_fill_(dead, 0)
+            o, row = [q[:0]], 0
+            for n in lens:
                 if n == 0:
                     continue
-                k, v = cache.tokens(index, b, n)
                 # the kernel takes multiples of 128; rows behind a sequence's last do not reach it
                 pad = -n % 128 if cfg.head_dim == 128 else 0
-                qkv = [nn.functional.pad(t, (0, 0, 0, 0, 0, pad))[None] for t in (q[row:row + n], k, v)]
+                qkv = [nn.functional.pad(t[row:row + n], (0, 0, 0, 0, 0, pad))[None] for t in (q, k, v)]
                 y = attention(*qkv, cfg.heads, cfg.kv_heads)
-                o[row:row + n] = y[0, :n].view(n, cfg.heads, cfg.head_dim)
-                dead[row:row + n] |= step.positions[row:row + n] != at[:n]
+                o.append(y[0, :n].view(n, cfg.heads, cfg.head_dim))
                 row += n
-            return o.masked_fill_(dead[:, None, None], float("nan"))
+            return torch.cat(o).masked_fill_(dead, float("nan"))
 
         return self._rows(hs, cache, index, step, cos, sin, attend)

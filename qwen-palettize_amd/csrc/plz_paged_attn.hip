@@ -8,9 +8,10 @@
 //
 // Every cached value is needed once, for G heads: 2 G operations a byte, so the cache's bytes bound
 // it, and the work is to keep enough of them in flight: 64 requests of 8192 tokens (2.15 GB, 32/8 heads
-// of 128) take 320 us, 6.7 TB/s; shorter batches add the 3-4 us before the first bytes arrive (lengths,
-// block table, the first tiles of all waves at once) and the second launch. A wave takes a tile of 32 tokens of one kv
-// head straight from memory into the registers that feed the matrix instructions, no LDS between:
+// of 128) take 320 us, 6.7 TB/s (times here are of calls replayed from a graph, the second kernel among
+// them); shorter batches add the 3-4 us before the first bytes arrive (lengths, block table, the first
+// tiles of all waves at once) and the second launch. A wave takes a tile of 32 tokens of one kv head
+// straight from memory into the registers that feed the matrix instructions, no LDS between:
 //   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, A = 16 tokens x 32 values of K, B = 16 heads. The K cache
 //                 is stored in 8-value pieces, [D / 8][P][8], so that the 16 lanes of a piece read 256
 //                 consecutive bytes (row-major K would give each of them 16 bytes of its own row, which
@@ -22,16 +23,19 @@
 // The weights enter as two bf16 pieces (p = hi + lo, together 16 bits): one piece would be as large an
 // error as the output's own rounding, and the matrix pipe has the room (no difference in time). The
 // running maximum of a head moves only when a tile exceeds it by more than 2^8. K and V are loaded past
-// the L2s' replacement order, since nobody reads them again (359 -> 320 us; a batch of 74 MB that the
-// last-level cache could hold from call to call 21.6 -> 21.7). Two tiles of V in flight a wave: no gain
-// (28.0 -> 28.8 us for one request of 32768); three waves a SIMD instead of two: 361 -> 385.
+// the L2s' replacement order, since with up to 16 heads a kv head nobody reads them again (359 -> 320 us;
+// a batch of 74 MB that the last-level cache could hold from call to call 21.6 -> 21.7). With more heads
+// the head tiles beside a workgroup on its XCD read them too, and may fetch them once more: 16 x 4096
+// tokens, 4 kv heads with 20 heads each (134 MB), take 36 us, as many bytes of one request of 32768 with
+// one head tile 28. Two tiles of V in flight a wave: no gain (28.0 -> 28.8); three waves a SIMD instead of
+// two: 361 -> 385.
 //
 // Each wave has a run of tiles (plz_paged.h) and goes through its requests without a word to the
 // others; the next requests' lengths, pages and queries are on their way while it is at this one. Only
 // what a run has of a request that it does not have whole is joined: through LDS among the waves of a
 // workgroup, through the workspace among workgroups, by a second kernel, both in the order of the runs.
 // (256 ragged requests up to 1024 tokens: 59 us with one run a workgroup and a join after each request,
-// 32.6 so.) The runs are dealt from the lengths by every wave for itself, a lane a request, in DPP sums.
+// 33.4 so.) The runs are dealt from the lengths by every wave for itself, a lane a request, in DPP sums.
 #include "plz_paged.h"
 #include "palettize_hip.h"
 
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(NT, D == 256 ? 1 : 2) void paged_attn_kernel(AttnAr
   const int each = (to - from + 63) >> 6;
   // Loads of lengths and pages have no branch around them: where paths of a divergent one meet, the
   // compiler takes the uniform values that meet there for divergent too, and with them all loops and
-  // branches below (219 -> 203 registers, 256 ragged requests 33.3 -> 32.6 us).
+  // branches below (219 -> 203 registers, 256 ragged requests 34.1 -> 33.4 us).
   auto length = [&](int b) {
     const int n = g.lens[min(b, g.B - 1)];
     return b < to ? n : 0;

@@ -263,3 +263,45 @@ def test_layers_refuse_gradients(dev):
         got = hard[0].decode(needs[:2], cache, 0, step, cos, sin)
     assert not got.requires_grad
     assert torch.equal(got, hard[0].decode(hs[:2], cache, 0, step, cos, sin))
+
+
+def test_captured_prompts(dev):
+    """A step of prompts (of 20, 0 and 7 tokens, on rows that had others) and two layers over them, captured
+    once and replayed with other hidden states, eager work and synchronisations in between, against the same
+    run eagerly, bit for bit; with a pool that has room for all, and one in which the last finds none."""
+    cfg, hard, _ = _layers(dev, CFGS["d128"])
+    cos, sin = layer.rope_tables(64, cfg.head_dim, cfg.rope_theta, dev)
+    lens = [20, 0, 7]
+    new = torch.tensor(lens, dtype=torch.int32, device=dev)
+    keep = torch.zeros_like(new)
+    for pages in (8, 2):
+        caches = [decode.PagedKVCache(2, 3, 64, cfg.kv_heads, cfg.head_dim, page_size=16, num_pages=pages,
+                                      device=dev) for _ in range(2)]
+        hs = torch.zeros(27, cfg.hidden, dtype=torch.bfloat16, device=dev)
+
+        def one(cache, x):
+            step = cache.step(new, keep, rows=27)
+            for i, l in enumerate(hard):
+                x = l.prefill(x, cache, i, step, lens, cos, sin)
+            return x
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one(caches[1], hs)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = one(caches[0], hs)
+        g = torch.Generator().manual_seed(6)
+        for t in range(12):
+            x = torch.randn(27, cfg.hidden, generator=g).to(torch.bfloat16).to(dev)
+            want = one(caches[1], x)
+            hs.copy_(x)
+            graph.replay()
+            if t % 3 == 0:
+                torch.cuda.synchronize()
+            rows = 27 if pages == 8 else 20
+            assert torch.equal(out[:rows], want[:rows]), t
+            assert bool(torch.isfinite(out[:rows]).all()) and bool(torch.isnan(out[rows:]).all())
+            assert torch.equal(caches[0].lens, caches[1].lens)

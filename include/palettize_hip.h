@@ -42,6 +42,11 @@ extern "C" {
 #define PLZ_DT_FP16 1
 #define PLZ_DT_FP32 2
 
+/* reductions of a loss over rows */
+#define PLZ_REDUCE_NONE 0
+#define PLZ_REDUCE_SUM 1
+#define PLZ_REDUCE_MEAN 2
+
 /* soft forward weight modes (plz_soft_build_w) */
 #define PLZ_W_SOFT 0       /* W = sum_c P_c pal_c                                        */
 #define PLZ_W_HARD_NOISY 1 /* W = pal[argmax_c P_c], first max wins (fused_lut_kernel.cu:1998-2003) */
@@ -701,6 +706,43 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
                          const float* grad_loss, float w_cos, float w_mse, float eps,
                          uint16_t* grad_student, const void* workspace, size_t workspace_bytes,
                          int64_t rows, int64_t dim, void* stream);
+
+/* ---- losses over a large vocabulary ---------------------------------------------------- */
+/* Cross entropy and distillation from hidden states x bf16 [N, H] and head weights w bf16 [V, H]
+ * (H % 8 == 0, any V), without keeping the logits z = x w^T. The reference distils hidden states
+ * only (train_qwen.py:229-249); these act on what the head makes of them.
+ *   cross entropy  loss[n] = log sum_v exp z[n, v] - z[n, label n]; a row whose label is ignore_index
+ *                  takes no part, a label outside [0, V) gives NaN (loss and gradients). labels are
+ *                  int64 or int32 (label_bytes 8 or 4).
+ *   distillation   loss[n] = sum_v p_v (log p_v - log q_v), p = softmax(z_teacher / T),
+ *                  q = softmax(z / T), over teacher_x [N, H_teacher] and teacher_w [V, H_teacher];
+ *                  mask uint8 [N]: rows of 0 take no part (NULL: all do).
+ * Rows that take no part have loss and lse 0 and gradient 0, and nothing of them, a NaN neither,
+ * reaches another output. loss fp32 [N]; lse fp32 [N] (cross entropy) or [2][N] (distillation: the
+ * student's, then the teacher's, of z / T), which the backward takes; total (NULL: not wanted) fp32
+ * [3] = {sum, mean over the rows that take part (0 without one), their number}.
+ * The backward takes grad fp32: [N] of every row's loss (PLZ_REDUCE_NONE), or [1] of the sum
+ * (PLZ_REDUCE_SUM) or of the mean (PLZ_REDUCE_MEAN). grad_x bf16 [N, H] and grad_w bf16 [V, H]; NULL:
+ * not wanted. The gradient of the logits is rounded to bf16 before its products with x and w. The
+ * teacher has no gradient. H_teacher = 0 in the workspace queries: cross entropy. */
+size_t plz_vocab_loss_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher);
+size_t plz_vocab_loss_bwd_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x);
+int plz_linear_ce_fwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                      int64_t ignore_index, float* loss, float* lse, float* total, void* workspace,
+                      size_t workspace_bytes, int64_t N, int64_t V, int64_t H, void* stream);
+int plz_linear_ce_bwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                      int64_t ignore_index, const float* lse, const float* grad, int reduction,
+                      uint16_t* grad_x, uint16_t* grad_w, void* workspace, size_t workspace_bytes,
+                      int64_t N, int64_t V, int64_t H, void* stream);
+int plz_linear_kl_fwd(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                      const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                      float* loss, float* lse, float* total, void* workspace, size_t workspace_bytes,
+                      int64_t N, int64_t V, int64_t H, int64_t H_teacher, void* stream);
+int plz_linear_kl_bwd(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                      const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                      const float* lse, const float* grad, int reduction, uint16_t* grad_x,
+                      uint16_t* grad_w, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
+                      int64_t H, int64_t H_teacher, void* stream);
 
 /* ---- decoding over a paged key-value cache ------------------------------------------- */
 /* A cache is a pool of num_pages pages of page_size tokens (a power of two, 16..1024); one layer's

@@ -1,0 +1,967 @@
+// Losses over a large vocabulary from hidden states and head weights, without keeping the logits:
+//
+//   z = x W^T                               x bf16 [N, H], W bf16 [V, H], fp32 sums
+//   cross entropy   loss_n = log sum_v exp z_nv - z_n,label
+//                   dz_nv  = softmax(z_n)_v - [v = label_n]
+//   distillation    p = softmax(z_teacher / T), q = softmax(z / T)
+//                   loss_n = sum_v p_v (log p_v - log q_v),   dz_nv = (q_v - p_v) / T
+//   dx = dz W,  dW = dz^T x
+//
+// The rows that take part (a label other than ignore_index; a mask that is set) are packed first, so
+// the others cost nothing and nothing of them, a NaN neither, reaches a sum. Every tile of logits is
+// 256 words x 256 rows of the 256x256 core with the words along the accumulator registers: a lane
+// holds 64 words of a row, so a row's maximum and sum of exponentials are register work, one exchange
+// with the other half wave and one through LDS. The forward keeps those statistics of each tile
+// (8 bytes a row and 256 words) and joins them in a second kernel, in 64 bits. The backward computes
+// the logits of a piece of the vocabulary again, now with the rows' normalisers at hand, rounds dz to
+// bf16 into a workspace dz^T [words, rows] of at most kPieceBytes, and multiplies it with x (dW of the
+// piece) and with W (dx, its fp32 parts summed over pieces and splits in a fixed order). The scale of
+// a mean and of its gradient is applied to the fp32 sums, not to dz: it would be rounded with it.
+//
+// A distillation tile needs both sides' logits: a workgroup keeps the teacher's 256 x 256 in a slot of
+// its own in the workspace (256 KB, 64 MB for 256 CUs) while it computes the student's.
+#include <algorithm>
+
+#include "plz_gemm2_dense.cuh"
+#include "palettize_hip.h"
+
+namespace plz {
+namespace voc {
+
+using namespace g2;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr size_t kPieceBytes = (size_t)1 << 30;
+constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
+constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
+constexpr int kPackRows = 16;
+
+enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
+enum { CE_STATS = 0, CE_GRAD = 1, KL_STATS = 2, KL_GRAD = 3 };
+
+// ---- rows that take part --------------------------------------------------------------------------
+struct Meta {
+  int rows;     // how many take part
+  float alpha;  // backward: the scale of the gradients that every row shares
+};
+struct PackArgs {
+  const void* key;  // labels or mask
+  int kind;
+  int64_t ignore, V, N;
+  const uint16_t* x[2];  // student, teacher
+  uint16_t* xp[2];
+  int64_t H[2];
+  Meta* meta;
+  int32_t* pos;    // [N] the packed row of a row, -1: takes no part
+  int32_t* src;    // [Np] and back
+  int32_t* lab;    // [Np] labels, -1: no word
+  float* zero[3];  // forward: outputs that are 0 for rows that take no part (or NULL)
+  // backward
+  const float* lse_in[2];
+  float* lse[2];  // [Np]
+  const float* grad;
+  int reduction;  // PLZ_REDUCE_*
+  float* g;       // [Np], reduction none
+  float inv_t;
+};
+
+__device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
+  switch (a.kind) {
+    case KEY_INT64: return reinterpret_cast<const int64_t*>(a.key)[r] != a.ignore;
+    case KEY_INT32: return reinterpret_cast<const int32_t*>(a.key)[r] != a.ignore;
+    case KEY_MASK: return reinterpret_cast<const uint8_t*>(a.key)[r] != 0;
+    default: return true;
+  }
+}
+
+// A workgroup packs kPackRows rows behind all that take part before them, which it counts itself (the
+// keys of 16384 rows are 128 KB in the L2s). The last one also clears the rows up to the next whole
+// stage of the dW product, whose reduction runs over the packed rows.
+__global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
+  __shared__ int red[4];
+  __shared__ int at[kPackRows];
+  const int64_t r0 = (int64_t)blockIdx.x * kPackRows;
+  int before = 0;
+  if (a.kind == KEY_NONE) {
+    before = (int)r0;
+  } else {
+    int c = 0;
+    for (int64_t r = threadIdx.x; r < r0; r += 256) c += takes_part(a, r) ? 1 : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    before = red[0] + red[1] + red[2] + red[3];
+  }
+  const int n = (int)min((int64_t)kPackRows, a.N - r0);
+  if (threadIdx.x < 64) {
+    const int i = threadIdx.x;
+    const bool on = i < n && takes_part(a, r0 + i);
+    const uint64_t all = __ballot(on);
+    if (i < kPackRows) at[i] = on ? before + __popcll(all & ((1ull << i) - 1)) : -1;
+    if (i < n) {
+      const int64_t r = r0 + i;
+      const int p = at[i];
+      a.pos[r] = p;
+      if (on) {
+        a.src[p] = (int)r;
+        if (a.kind == KEY_INT64 || a.kind == KEY_INT32) {
+          const int64_t l = a.kind == KEY_INT64 ? reinterpret_cast<const int64_t*>(a.key)[r]
+                                                : reinterpret_cast<const int32_t*>(a.key)[r];
+          a.lab[p] = l >= 0 && l < a.V ? (int)l : -1;
+        }
+        for (int k = 0; k < 2; ++k)
+          if (a.lse_in[k]) a.lse[k][p] = a.lse_in[k][r];
+        if (a.g) a.g[p] = a.grad[r];
+      } else {
+        for (int k = 0; k < 3; ++k)
+          if (a.zero[k]) a.zero[k][r] = 0.f;
+      }
+    }
+    if (i == 0 && r0 + n == a.N) {
+      const int rows = before + __popcll(all);
+      a.meta->rows = rows;
+      float alpha = a.inv_t;
+      if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
+      if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
+      a.meta->alpha = alpha;
+      red[0] = rows;
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < 2; ++k) {
+    if (!a.x[k]) continue;
+    const int64_t H = a.H[k];
+    const int c8 = (int)(H / 8);
+    for (int i = 0; i < n; ++i) {
+      const int p = at[i];
+      if (p < 0) continue;
+      const uint4* s = reinterpret_cast<const uint4*>(a.x[k] + (r0 + i) * H);
+      uint4* d = reinterpret_cast<uint4*>(a.xp[k] + (int64_t)p * H);
+      for (int c = threadIdx.x; c < c8; c += 256) d[c] = s[c];
+    }
+    if (r0 + n == a.N) {
+      const int rows = red[0], end = (rows + BK - 1) / BK * BK;
+      uint4* d = reinterpret_cast<uint4*>(a.xp[k] + (int64_t)rows * H);
+      for (int64_t c = threadIdx.x; c < (int64_t)(end - rows) * c8; c += 256)
+        d[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// ---- tiles of logits ------------------------------------------------------------------------------
+struct LogitArgs {
+  const uint16_t* w[2];  // student, teacher
+  const uint16_t* x[2];  // packed rows [Np, H]
+  int64_t H[2];
+  int64_t v0, v1;  // the words of this launch
+  int64_t Np;
+  const Meta* meta;
+  const int32_t* lab;
+  const float* lse[2];  // [Np]
+  const float* g;       // [Np] or NULL
+  float inv_t;
+  float* stats;  // [tile of words][2 or 5][Np]
+  float* zlab;   // [Np]
+  uint16_t* dzt;  // [words of the piece in whole tiles][Np]
+  float* park;    // [workgroup][256 * 256]
+};
+
+// exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
+// distance from the maximum (or the normaliser), which is small wherever the exponential counts
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// The statistics of a set of words: the maximum, the sum of exponentials relative to it and, for the
+// teacher, the sum of exponentials times (teacher - student).
+struct Stat {
+  float m, s, c;
+};
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+  const float M = fmaxf(a.m, b.m);
+  // no word above -inf on either side: nothing to scale (inf - inf is not 0)
+  if (M == -INFINITY) return Stat{M, a.s + b.s, a.c + b.c};
+  const float fa = exp_of(a.m - M), fb = exp_of(b.m - M);
+  return Stat{M, a.s * fa + b.s * fb, a.c * fa + b.c * fb};
+}
+__device__ __forceinline__ Stat join_halves(const Stat& a) {
+  const auto m = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.m), __float_as_uint(a.m), false, false);
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.s), __float_as_uint(a.s), false, false);
+  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.c), __float_as_uint(a.c), false, false);
+  return join(Stat{__uint_as_float(m[0]), __uint_as_float(s[0]), __uint_as_float(c[0])},
+              Stat{__uint_as_float(m[1]), __uint_as_float(s[1]), __uint_as_float(c[1])});
+}
+
+typedef __attribute__((address_space(3))) float lds_f32;
+typedef __attribute__((address_space(3))) uint16_t lds_u16t;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
+// acc[word, row] of words i0 .. and rows j0 ..; words from v1 on repeat the last one
+__device__ __forceinline__ void logits_tile(lds_u8* lbase, const uint16_t* w, const uint16_t* x,
+                                            int64_t H, int64_t i0, int64_t v1, int64_t j0,
+                                            f32x16 (&acc)[WT_I][WT_J], int wi, int wj, int lane) {
+#pragma unroll
+  for (int i = 0; i < WT_I; ++i)
+#pragma unroll
+    for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
+  const int64_t nw = min((int64_t)TILE, v1 - i0);
+  const uint16_t* wt = w + i0 * H;
+  const uint16_t* xt = x + j0 * H;
+  const TileDma dA = row_tile_dma(wt, H, 0, nw), dB = row_tile_dma(xt, H, 0, TILE);
+  const int nfull = (int)(H / BK);
+  dense_stages<false, false>(lbase, nfull, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
+    tile_copy(As, dA, (uint32_t)(kt * BK * 2));
+    tile_copy(Bs, dB, (uint32_t)(kt * BK * 2));
+  });
+  if (H % BK) {
+    copy_row_tile_masked((uint4*)lbase, wt, H, 0, nw, (int64_t)nfull * BK, H);
+    copy_row_tile_masked((uint4*)(lbase + TILE_BYTES), xt, H, 0, TILE, (int64_t)nfull * BK, H);
+    __syncthreads();
+    mma_stage_sync<false, false>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane,
+                                 (int)((H % BK + 15) / 16));
+    __syncthreads();
+  }
+}
+
+template <int MODE>
+__global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
+  extern __shared__ uint4 smem[];
+  lds_u8* lbase = (lds_u8*)smem;
+  constexpr bool KL = MODE == KL_STATS || MODE == KL_GRAD;
+  constexpr bool STATS = MODE == CE_STATS || MODE == KL_STATS;
+  constexpr int PLANES = KL ? 5 : 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = wave / WAVES_J, wj = wave % WAVES_J;
+  const int rows = a.meta->rows;
+  const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE), tiles_j = (rows + TILE - 1) / TILE;
+  const int64_t total = (int64_t)tiles_i * tiles_j;
+  // every XCD walks a run of its own, four tiles of words at a time over the rows
+  const int xcd = blockIdx.x % 8, step = gridDim.x / 8;
+  const int64_t end = total * (xcd + 1) / 8;
+  for (int64_t item = total * xcd / 8 + blockIdx.x / 8; item < end; item += step) {
+    int tile_i, tile_j;
+    tile_coords(4, tiles_i, tiles_j, (int)item, tile_i, tile_j);
+    const int64_t i0 = a.v0 + (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
+    f32x16 acc[WT_I][WT_J];
+    float4* slot = KL ? reinterpret_cast<float4*>(a.park) + (int64_t)blockIdx.x * (TILE * TILE / 4) : nullptr;
+    if constexpr (KL) {
+      logits_tile(lbase, a.w[1], a.x[1], a.H[1], i0, a.v1, j0, acc, wi, wj, lane);
+#pragma unroll
+      for (int ti = 0; ti < WT_I; ++ti)
+#pragma unroll
+        for (int tj = 0; tj < WT_J; ++tj)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4)
+            slot[((ti * WT_J + tj) * 4 + e4) * NTHR + threadIdx.x] =
+                make_float4(acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
+                            acc[ti][tj][4 * e4 + 3]);
+    }
+    logits_tile(lbase, a.w[0], a.x[0], a.H[0], i0, a.v1, j0, acc, wi, wj, lane);
+
+    // This lane's word of block ti and register e is vl + 32 ti + 8 (e / 4) + e % 4, from the tile's
+    // first one; of the tile's words, nw exist.
+    const int vl = wi * (32 * WT_I) + 4 * (lane >> 5);
+    const int nw = (int)min((int64_t)TILE, a.v1 - i0);
+#pragma unroll
+    for (int tj = 0; tj < WT_J; ++tj) {
+      const int nl = wj * (32 * WT_J) + 32 * tj + (lane & 31);
+      const int64_t n = j0 + nl;
+      const bool live = n < rows;
+      // block ti of the teacher's logits, as this thread put it away
+      auto teacher = [&](int ti) {
+        f32x16 z;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const float4 v = slot[((ti * WT_J + tj) * 4 + e4) * NTHR + threadIdx.x];
+          z[4 * e4] = v.x; z[4 * e4 + 1] = v.y; z[4 * e4 + 2] = v.z; z[4 * e4 + 3] = v.w;
+        }
+        return z;
+      };
+      // the label's logit, in the one lane that holds it: false elsewhere. lv: the label from vl
+      float zl = 0.f;
+      auto holds = [&](int l) {
+        const int lv = l - vl;
+        // its registers are those of words 0..3 of every 8
+        const bool mine = lv >= 0 && lv < 32 * WT_I && (lv & 4) == 0;
+        if (__ballot(mine) == 0) return false;
+#pragma unroll
+        for (int ti = 0; ti < WT_I; ++ti) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            zl = lv == 32 * ti + 8 * (e >> 2) + (e & 3) ? acc[ti][tj][e] : zl;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        return mine;
+      };
+      if constexpr (STATS) {
+        Stat st[KL ? 2 : 1];
+#pragma unroll
+        for (int k = 0; k < (KL ? 2 : 1); ++k) st[k] = Stat{-INFINITY, 0.f, 0.f};
+        if constexpr (!KL) {
+          if (live && holds(a.lab[n] - (int)i0)) a.zlab[n] = zl;
+        }
+#pragma unroll
+        for (int ti = 0; ti < WT_I; ++ti) {
+          f32x16 z = acc[ti][tj], t = {};
+          if constexpr (KL) {
+            z *= a.inv_t;
+            t = teacher(ti) * a.inv_t;
+          }
+          if (nw < TILE) {
+            const int left = nw - vl - 32 * ti;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              z[e] = 8 * (e >> 2) + (e & 3) < left ? z[e] : -INFINITY;
+              if constexpr (KL) t[e] = 8 * (e >> 2) + (e & 3) < left ? t[e] : -INFINITY;
+            }
+          }
+          auto top = [](const f32x16& v) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, v[e]);
+            return m;
+          };
+          Stat b{top(z), 0.f, 0.f};
+          const float m0 = b.m == -INFINITY ? 0.f : b.m;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) b.s += exp_of(z[e] - m0);
+          st[0] = join(st[0], b);
+          if constexpr (KL) {
+            b = Stat{top(t), 0.f, 0.f};
+            const float m1 = b.m == -INFINITY ? 0.f : b.m;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float p = exp_of(t[e] - m1);
+              b.s += p;
+              // a word without weight counts for nothing, however far the two sides are
+              b.c += p == 0.f ? 0.f : p * (t[e] - z[e]);
+            }
+            st[1] = join(st[1], b);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int k = 0; k < (KL ? 2 : 1); ++k) st[k] = join_halves(st[k]);
+        // the two waves of a column of the tile meet in LDS, behind the stages' slots
+        lds_f32* ex = reinterpret_cast<lds_f32*>(lbase + 4 * TILE_BYTES) + wj * 256;
+        if (wi == 1 && lane < 32) {
+          ex[lane] = st[0].m;
+          ex[32 + lane] = st[0].s;
+          if constexpr (KL) {
+            ex[64 + lane] = st[1].m;
+            ex[96 + lane] = st[1].s;
+            ex[128 + lane] = st[1].c;
+          }
+        }
+        __syncthreads();
+        if (wi == 0 && lane < 32 && live) {
+          float* out = a.stats + (i0 / TILE) * PLANES * a.Np + n;
+          const Stat s0 = join(st[0], Stat{ex[lane], ex[32 + lane], 0.f});
+          out[0] = s0.m;
+          out[a.Np] = s0.s;
+          if constexpr (KL) {
+            const Stat s1 = join(st[1], Stat{ex[64 + lane], ex[96 + lane], ex[128 + lane]});
+            out[2 * a.Np] = s1.m;
+            out[3 * a.Np] = s1.s;
+            out[4 * a.Np] = s1.c;
+          }
+        }
+        __syncthreads();
+      } else {
+        // dz of this row's words, bf16, into the tile staged in LDS [word][row]
+        const float lse = live ? a.lse[0][n] : 0.f, lt = KL && live ? a.lse[1][n] : 0.f;
+        float g = live && a.g ? a.g[n] : 1.f;
+        int l = -1;
+        if constexpr (!KL) {
+          l = live ? a.lab[n] : 0;
+          if (l < 0) g = __builtin_nanf("");  // no such word: nothing to learn from
+          l -= (int)i0;
+        }
+#pragma unroll
+        for (int ti = 0; ti < WT_I; ++ti) {
+          f32x16 t = {};
+          if constexpr (KL) t = teacher(ti) * a.inv_t;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float d = exp_of((KL ? acc[ti][tj][e] * a.inv_t : acc[ti][tj][e]) - lse);
+            if constexpr (KL) d -= exp_of(t[e] - lt);
+            d = live ? d * g : 0.f;
+            *reinterpret_cast<lds_u16t*>(lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS +
+                                         nl * 2) = (uint16_t)f2bf(d);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!KL) {
+          if (live && holds(l))
+            *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) =
+                (uint16_t)f2bf((exp_of(zl - lse) - 1.f) * g);
+        }
+      }
+    }
+    if constexpr (!STATS) {
+      __syncthreads();
+      uint16_t* out = a.dzt + (i0 - a.v0) * a.Np + j0;
+#pragma unroll 4
+      for (int it = 0; it < TILE * TILE / 8 / NTHR; ++it) {
+        const int ch = it * NTHR + threadIdx.x;
+        const int row = ch >> 5, c8 = (ch & 31) * 8;
+        u32x4 v = *reinterpret_cast<const lds_u32x4*>(lbase + row * EPI_RS + c8 * 2);
+        if (row >= nw) v = u32x4{0, 0, 0, 0};
+        *reinterpret_cast<u32x4*>(out + row * a.Np + c8) = v;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- joining the tiles' statistics ------------------------------------------------------------------
+// 256 threads: 1 << rb_log rows, the rest of the threads along the tiles; each joins its tiles in order
+// and the row's first thread all of them, so the order is fixed.
+struct JoinArgs {
+  const float* stats;
+  const float* zlab;
+  const Meta* meta;
+  const int32_t* src;
+  const int32_t* lab;
+  int64_t Np;
+  int tiles, rb_log;
+  float* loss;    // [N]
+  float* lse[2];  // [N]
+};
+template <bool KL>
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+  __shared__ float sh[KL ? 5 : 2][256];
+  constexpr int PLANES = KL ? 5 : 2;
+  const int RB = 1 << a.rb_log, slices = 256 >> a.rb_log;
+  const int rl = threadIdx.x & (RB - 1), sl = threadIdx.x >> a.rb_log;
+  const int64_t p = (int64_t)blockIdx.x * RB + rl;
+  const bool live = p < a.meta->rows;
+  Stat s0{-INFINITY, 0.f, 0.f}, s1{-INFINITY, 0.f, 0.f};
+  if (live) {
+#pragma unroll 4
+    for (int t = sl; t < a.tiles; t += slices) {
+      const float* v = a.stats + (int64_t)t * PLANES * a.Np + p;
+      s0 = join(s0, Stat{v[0], v[a.Np], 0.f});
+      if constexpr (KL) s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], v[4 * a.Np]});
+    }
+  }
+  sh[0][threadIdx.x] = s0.m;
+  sh[1][threadIdx.x] = s0.s;
+  if constexpr (KL) {
+    sh[2][threadIdx.x] = s1.m;
+    sh[3][threadIdx.x] = s1.s;
+    sh[4][threadIdx.x] = s1.c;
+  }
+  __syncthreads();
+  if (!live || sl != 0) return;
+  for (int k = 1; k < slices; ++k) {
+    const int i = k * RB + rl;
+    s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
+    if constexpr (KL) s1 = join(s1, Stat{sh[2][i], sh[3][i], sh[4][i]});
+  }
+  const int64_t r = a.src[p];
+  a.lse[0][r] = (float)((double)s0.m + log((double)s0.s));
+  if constexpr (KL) {
+    a.lse[1][r] = (float)((double)s1.m + log((double)s1.s));
+    // sum p (z_t - z_s) - (lse_t - lse_s), the normalisers' difference from the maxima's and the
+    // sums' quotient: as a difference of two rounded normalisers it would lose their common part
+    a.loss[r] = (float)((double)s1.c / s1.s - ((double)s1.m - s0.m) - log((double)s1.s / s0.s));
+  } else {
+    a.loss[r] = a.lab[p] < 0 ? __builtin_nanf("")
+                             : (float)((double)s0.m - a.zlab[p] + log((double)s0.s));
+  }
+}
+
+// out = {sum, mean over the rows that take part (0 without one), their number}
+__global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ loss, int64_t N,
+                                                     const Meta* __restrict__ meta,
+                                                     float* __restrict__ out) {
+  __shared__ double red[16];
+  double s = 0;
+  for (int64_t r = threadIdx.x; r < N; r += 1024) s += loss[r];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0;
+    for (int w = 0; w < 16; ++w) s += red[w];
+    const int rows = N > 0 ? meta->rows : 0;
+    out[0] = (float)s;
+    out[1] = rows > 0 ? (float)(s / rows) : 0.f;
+    out[2] = (float)rows;
+  }
+}
+
+// ---- dW of a piece: dz^T [words, rows] x [rows, H] ----------------------------------------------------
+struct DwArgs {
+  const uint16_t* dzt;
+  const uint16_t* x;
+  int64_t Np, H, words;
+  const Meta* meta;
+  uint16_t* out;  // [words][H]
+};
+__global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
+  extern __shared__ uint4 smem[];
+  lds_u8* lbase = (lds_u8*)smem;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = wave / WAVES_J, wj = wave % WAVES_J;
+  const int tiles_i = (int)((a.words + TILE - 1) / TILE), tiles_j = (int)((a.H + TILE - 1) / TILE);
+  const Item item = map_item(tiles_i * tiles_j, false, 0, 1, (int)blockIdx.x, 0, 1);
+  int tile_i, tile_j;
+  tile_coords(4, tiles_i, tiles_j, item.bid, tile_i, tile_j);
+  const int64_t i0 = (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
+  f32x16 acc[WT_I][WT_J];
+#pragma unroll
+  for (int i = 0; i < WT_I; ++i)
+#pragma unroll
+    for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
+  // whole stages: the packed rows past the last one are cleared, and so is dz there
+  const int nst = (a.meta->rows + BK - 1) / BK;
+  const TileDma dA = row_tile_dma(a.dzt + i0 * a.Np, a.Np, 0, TILE);
+  const TileDma dB = col_tile_dma(a.x, a.H, j0, a.H, a.Np);
+  dense_stages<false, true>(lbase, nst, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
+    tile_copy(As, dA, (uint32_t)(kt * BK * 2));
+    tile_copy(Bs, dB, (uint32_t)((int64_t)kt * BK * a.H * 2));
+  });
+  const float alpha = a.meta->alpha;
+#pragma unroll
+  for (int ti = 0; ti < WT_I; ++ti)
+#pragma unroll
+    for (int tj = 0; tj < WT_J; ++tj)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = wi * (32 * WT_I) + 32 * ti + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        const int col = wj * (32 * WT_J) + 32 * tj + (lane & 31);
+        *reinterpret_cast<lds_u16t*>(lbase + row * EPI_RS + col * 2) =
+            (uint16_t)f2bf(alpha * acc[ti][tj][e]);
+      }
+  __syncthreads();
+#pragma unroll 4
+  for (int it = 0; it < TILE * TILE / 8 / NTHR; ++it) {
+    const int ch = it * NTHR + threadIdx.x;
+    const int row = ch >> 5, c8 = (ch & 31) * 8;
+    if (i0 + row < a.words && j0 + c8 < a.H)
+      __builtin_nontemporal_store(
+          *reinterpret_cast<const lds_u32x4*>(lbase + row * EPI_RS + c8 * 2),
+          reinterpret_cast<u32x4*>(a.out + (i0 + row) * a.H + j0 + c8));
+  }
+}
+
+// ---- dx of a piece: dz [rows, words] W [words, H], in splits of the words --------------------------------
+struct DxArgs {
+  const uint16_t* dzt;
+  const uint16_t* w;
+  int64_t Np, H, words, split;
+  const Meta* meta;
+  float* part;  // [z][Np][H]
+  int z, add;   // add: to what earlier pieces left
+};
+__global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
+  extern __shared__ uint4 smem[];
+  lds_u8* lbase = (lds_u8*)smem;
+  const int rows = a.meta->rows;
+  const int tiles_i = (rows + TILE - 1) / TILE, tiles_j = (int)((a.H + TILE - 1) / TILE);
+  const int T = tiles_i * tiles_j;
+  if ((int64_t)blockIdx.x >= (int64_t)T * a.z) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = wave / WAVES_J, wj = wave % WAVES_J;
+  const Item item = map_item(T, false, 0, 1, (int)blockIdx.x, 0, a.z);
+  int tile_i, tile_j;
+  tile_coords(4, tiles_i, tiles_j, item.bid, tile_i, tile_j);
+  const int64_t i0 = (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
+  const int64_t rbeg = (int64_t)item.zsl * a.split, rend = min(a.words, rbeg + a.split);
+  f32x16 acc[WT_I][WT_J];
+#pragma unroll
+  for (int i = 0; i < WT_I; ++i)
+#pragma unroll
+    for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
+  const int64_t len = rend > rbeg ? rend - rbeg : 0;
+  const int nfull = (int)(len / BK);
+  const TileDma dA = col_tile_dma(a.dzt, a.Np, i0, a.Np, a.words);
+  const TileDma dB = col_tile_dma(a.w, a.H, j0, a.H, a.words);
+  col_stages<true>(lbase, nfull, acc, wi, wj, lane, [&](bool is_a, int kt, lds_u8* dst) {
+    const int64_t r0 = rbeg + (int64_t)kt * BK;
+    if (is_a) tile_copy(dst, dA, (uint32_t)(r0 * a.Np * 2));
+    else tile_copy(dst, dB, (uint32_t)(r0 * a.H * 2));
+  });
+  __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
+  __syncthreads();
+  if (len % BK) {
+    const int64_t r0 = rbeg + (int64_t)nfull * BK;
+    copy_col_tile_masked((uint4*)lbase, a.dzt, a.Np, i0, a.Np, r0, rend);
+    copy_col_tile_masked((uint4*)(lbase + TILE_BYTES), a.w, a.H, j0, a.H, r0, rend);
+    __syncthreads();
+    mma_stage_sync<true, true>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane,
+                               (int)((len % BK + 15) / 16));
+  }
+  float* part = a.part + (int64_t)item.zsl * a.Np * a.H;
+#pragma unroll
+  for (int ti = 0; ti < WT_I; ++ti)
+#pragma unroll
+    for (int tj = 0; tj < WT_J; ++tj) {
+      const int64_t h = j0 + wj * (32 * WT_J) + 32 * tj + (lane & 31);
+      if (h >= a.H) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t n = i0 + wi * (32 * WT_I) + 32 * ti + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (n >= rows) continue;
+        float* d = part + n * a.H + h;
+        *d = a.add ? *d + acc[ti][tj][e] : acc[ti][tj][e];
+      }
+    }
+}
+
+// grad_x of every row: alpha times the sum of its parts, or nothing
+__global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ part, int z,
+                                                     const int32_t* __restrict__ pos,
+                                                     const Meta* __restrict__ meta, int64_t Np,
+                                                     int64_t N, int64_t H,
+                                                     uint16_t* __restrict__ out) {
+  const int64_t c8 = H / 8, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= N * c8) return;
+  const int64_t r = t / c8, c = t % c8;
+  const int p = pos[r];
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (p >= 0) {
+    for (int k = 0; k < z; ++k) {
+      const float4* v = reinterpret_cast<const float4*>(part + ((int64_t)k * Np + p) * H + c * 8);
+      const float4 v0 = v[0], v1 = v[1];
+      s[0] += v0.x; s[1] += v0.y; s[2] += v0.z; s[3] += v0.w;
+      s[4] += v1.x; s[5] += v1.y; s[6] += v1.z; s[7] += v1.w;
+    }
+    const float alpha = meta->alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] *= alpha;
+  }
+  *reinterpret_cast<uint4*>(out + r * H + c * 8) = pack8(s);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------
+static int cu_count() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cache[dev] == 0) {
+    int v = 0;
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
+      v = 256;
+    cache[dev] = v;
+  }
+  return cache[dev];
+}
+static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Words of a piece: dz^T of all rows in kPieceBytes, a whole number of tiles, and W's rows of it within
+// the 4 GiB that the copies of dx address.
+static int64_t piece_words(int64_t N, int64_t V, int64_t H) {
+  int64_t w = (int64_t)(kPieceBytes / 2) / up(N, TILE);
+  w = std::min(w, (((int64_t)1 << 31) - 1) / H);
+  return std::min(std::max(w / TILE, (int64_t)1) * TILE, up(V, TILE));
+}
+// Splits of dx's reduction over the words of a piece: whole waves of workgroups at 1.9 us a stage and
+// 4 stages of prologue and epilogue, 8 bytes an element and split written and read at 5 TB/s.
+static int dx_splits(int64_t N, int64_t words, int64_t H) {
+  const int64_t tiles = up(N, TILE) / TILE * (up(H, TILE) / TILE), C = cu_count();
+  int best = 1;
+  double best_t = 1e300;
+  for (int z = 1; z <= 64; ++z) {
+    const int64_t len = split_len(words, z);
+    if (z > 1 && (len < 8 * BK || (int64_t)(z - 1) * len >= words)) break;
+    const double t = (double)((tiles * z + C - 1) / C) * ((double)len / BK + 4.0) * 1.9 +
+                     z * 8.0 * (double)N * (double)H / 5.0e6;
+    if (t < best_t * 0.97) {
+      best_t = t;
+      best = z;
+    }
+  }
+  return best;
+}
+
+// The workspace, carved in order; p = NULL: sizes only.
+struct Carve {
+  char* p;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t n) {
+    T* r = p ? reinterpret_cast<T*>(p + used) : nullptr;
+    used += (n * sizeof(T) + 255) / 256 * 256;
+    return r;
+  }
+};
+struct Ws {
+  Meta* meta;
+  int32_t *pos, *src, *lab;
+  uint16_t* xp[2];
+  float* zlab;
+  float* stats;
+  float* park;
+  float* lse[2];
+  float* g;
+  uint16_t* dzt;
+  float* part;
+};
+static Ws carve(Carve& c, bool bwd, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
+  Ws w = {};
+  const int64_t Np = up(N, TILE);
+  w.meta = c.take<Meta>(1);
+  w.pos = c.take<int32_t>(N);
+  w.src = c.take<int32_t>(Np);
+  w.lab = c.take<int32_t>(Np);
+  w.xp[0] = c.take<uint16_t>(Np * H);
+  if (Ht) {
+    w.xp[1] = c.take<uint16_t>(Np * Ht);
+    w.park = c.take<float>((size_t)(cu_count() / 8 * 8) * TILE * TILE);
+  }
+  if (!bwd) {
+    w.zlab = c.take<float>(Np);
+    w.stats = c.take<float>((size_t)(up(V, TILE) / TILE) * (Ht ? 5 : 2) * Np);
+    return w;
+  }
+  const int64_t words = piece_words(N, V, H);
+  for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
+  w.g = c.take<float>(Np);
+  w.dzt = c.take<uint16_t>((size_t)words * Np);
+  if (grad_x) w.part = c.take<float>((size_t)dx_splits(N, words, H) * Np * H);
+  return w;
+}
+
+static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// What the two losses share: the sides of a call and its checks.
+struct Sides {
+  const uint16_t *x, *w, *tx, *tw;
+  const void* key;
+  int kind;
+  int64_t ignore;
+  float inv_t;
+  int64_t N, V, H, Ht;
+};
+static int check(const Sides& s, bool kl, const char* what) {
+  PLZ_REQUIRE(s.N >= 0 && s.V >= 1 && s.H >= 8 && (!kl || s.Ht >= 8), "%s: bad shape", what);
+  PLZ_REQUIRE(s.H % 8 == 0 && s.Ht % 8 == 0, "%s: hidden widths must be multiples of 8", what);
+  const int64_t lim = (int64_t)1 << 31;
+  if (up(s.N, TILE) * s.H >= lim || up(s.N, TILE) * s.Ht >= lim || s.V >= lim - TILE ||
+      s.N >= ((int64_t)1 << 22) || up(s.N, TILE) / TILE * (up(s.V, TILE) / TILE) >= lim) {
+    set_error("%s: 2^31 values of x, words or tiles, or 2^22 rows, or more", what);
+    return PLZ_EUNSUPPORTED;
+  }
+  PLZ_REQUIRE(s.w && (s.x || s.N == 0) && (!kl || (s.tw && (s.tx || s.N == 0))),
+              "%s: null pointer", what);
+  PLZ_REQUIRE(a16(s.x) && a16(s.w) && a16(s.tx) && a16(s.tw),
+              "%s: x and weights must be 16-byte aligned", what);
+  if (kl) PLZ_REQUIRE(s.inv_t > 0.f && s.inv_t < INFINITY, "%s: bad temperature", what);
+  return PLZ_OK;
+}
+static int check_ws(const void* ws, size_t have, size_t need, const char* what) {
+  if (!ws || have < need) {
+    set_error("%s: workspace of %zu bytes needed, %zu given", what, need, ws ? have : 0);
+    return PLZ_EWORKSPACE;
+  }
+  PLZ_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace must be 16-byte aligned", what);
+  return PLZ_OK;
+}
+
+static PackArgs pack_args(const Sides& s, const Ws& w) {
+  PackArgs a = {};
+  a.key = s.key; a.kind = s.kind; a.ignore = s.ignore; a.V = s.V; a.N = s.N;
+  a.x[0] = s.x; a.xp[0] = w.xp[0]; a.H[0] = s.H;
+  if (s.Ht) {
+    a.x[1] = s.tx; a.xp[1] = w.xp[1]; a.H[1] = s.Ht;
+  }
+  a.meta = w.meta; a.pos = w.pos; a.src = w.src; a.lab = w.lab;
+  a.inv_t = s.inv_t;
+  a.reduction = PLZ_REDUCE_NONE;
+  return a;
+}
+static int pack(const PackArgs& a, hipStream_t st, const char* what) {
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows)), dim3(256), 0, st, a);
+  return check_launch(what);
+}
+static LogitArgs logit_args(const Sides& s, const Ws& w) {
+  LogitArgs a = {};
+  a.w[0] = s.w; a.x[0] = w.xp[0]; a.H[0] = s.H;
+  a.w[1] = s.tw; a.x[1] = w.xp[1]; a.H[1] = s.Ht;
+  a.Np = up(s.N, TILE);
+  a.meta = w.meta; a.lab = w.lab; a.inv_t = s.inv_t; a.park = w.park;
+  a.stats = w.stats; a.zlab = w.zlab;
+  a.lse[0] = w.lse[0]; a.lse[1] = w.lse[1];
+  a.dzt = w.dzt;
+  return a;
+}
+template <int MODE>
+static int logits(const LogitArgs& a, hipStream_t st, const char* what) {
+  static uint64_t done = 0;
+  auto kern = logits_kernel<MODE>;
+  if (int rc = reserve_lds((const void*)kern, kLdsLogits, done, what)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(cu_count() / 8 * 8)), dim3(NTHR), kLdsLogits, st, a);
+  return check_launch(what);
+}
+
+template <bool KL>
+static int forward(const Sides& s, float* loss, float* lse, float* total, void* ws, size_t ws_bytes,
+                   hipStream_t st, const char* what) {
+  if (int rc = check(s, KL, what)) return rc;
+  PLZ_REQUIRE(s.N == 0 || (loss && lse), "%s: null pointer", what);
+  Carve need{nullptr};
+  carve(need, false, s.N, s.V, s.H, s.Ht, false);
+  if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
+  Carve c{reinterpret_cast<char*>(ws)};
+  const Ws w = carve(c, false, s.N, s.V, s.H, s.Ht, false);
+  if (s.N > 0) {
+    PackArgs p = pack_args(s, w);
+    p.zero[0] = loss;
+    p.zero[1] = lse;
+    if (KL) p.zero[2] = lse + s.N;
+    if (int rc = pack(p, st, what)) return rc;
+    LogitArgs l = logit_args(s, w);
+    l.v0 = 0;
+    l.v1 = s.V;
+    if (int rc = logits<KL ? KL_STATS : CE_STATS>(l, st, what)) return rc;
+    JoinArgs j = {};
+    j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
+    j.Np = up(s.N, TILE);
+    j.tiles = (int)(up(s.V, TILE) / TILE);
+    j.rb_log = s.N >= 4096 ? 4 : s.N >= 512 ? 2 : 0;
+    j.loss = loss;
+    j.lse[0] = lse;
+    j.lse[1] = lse + s.N;
+    hipLaunchKernelGGL(join_kernel<KL>, dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)),
+                       dim3(256), 0, st, j);
+    if (int rc = check_launch(what)) return rc;
+  }
+  if (total) {
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, s.N, w.meta, total);
+    return check_launch(what);
+  }
+  return PLZ_OK;
+}
+
+template <bool KL>
+static int backward(const Sides& s, const float* lse, const float* grad, int reduction,
+                    uint16_t* grad_x, uint16_t* grad_w, void* ws, size_t ws_bytes, hipStream_t st,
+                    const char* what) {
+  if (int rc = check(s, KL, what)) return rc;
+  PLZ_REQUIRE(reduction == PLZ_REDUCE_NONE || reduction == PLZ_REDUCE_SUM || reduction == PLZ_REDUCE_MEAN,
+              "%s: bad reduction %d", what, reduction);
+  PLZ_REQUIRE(s.N == 0 || (lse && grad), "%s: null pointer", what);
+  PLZ_REQUIRE(a16(grad_x) && a16(grad_w), "%s: gradients must be 16-byte aligned", what);
+  if (!grad_x && !grad_w) return PLZ_OK;
+  if (s.N == 0) {
+    if (grad_w) zero_async(grad_w, (size_t)s.V * s.H * 2, st);
+    return check_launch(what);
+  }
+  Carve need{nullptr};
+  carve(need, true, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
+  Carve c{reinterpret_cast<char*>(ws)};
+  const Ws w = carve(c, true, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  const int64_t Np = up(s.N, TILE), words = piece_words(s.N, s.V, s.H);
+  PackArgs p = pack_args(s, w);
+  p.grad = grad;
+  p.reduction = reduction;
+  if (reduction == PLZ_REDUCE_NONE) p.g = w.g;
+  for (int k = 0; k < (KL ? 2 : 1); ++k) {
+    p.lse_in[k] = lse + k * s.N;
+    p.lse[k] = w.lse[k];
+  }
+  if (int rc = pack(p, st, what)) return rc;
+  static uint64_t done_w = 0, done_x = 0;
+  if (int rc = reserve_lds((const void*)dw_kernel, kLdsLogits, done_w, what)) return rc;
+  if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
+  const int z = grad_x ? dx_splits(s.N, words, s.H) : 0;
+  const int64_t tiles_h = up(s.H, TILE) / TILE;
+  LogitArgs l = logit_args(s, w);
+  l.g = p.g;
+  for (int64_t v0 = 0; v0 < s.V; v0 += words) {
+    l.v0 = v0;
+    l.v1 = std::min(s.V, v0 + words);
+    const int64_t n = l.v1 - l.v0;
+    if (int rc = logits<KL ? KL_GRAD : CE_GRAD>(l, st, what)) return rc;
+    if (grad_w) {
+      const DwArgs d = {w.dzt, w.xp[0], Np, s.H, n, w.meta, grad_w + v0 * s.H};
+      hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
+                         kLdsLogits, st, d);
+      if (int rc = check_launch(what)) return rc;
+    }
+    if (grad_x) {
+      const DxArgs d = {w.dzt, s.w + v0 * s.H, Np, s.H, n, split_len(words, z), w.meta, w.part, z, v0 > 0};
+      hipLaunchKernelGGL(dx_kernel, dim3((unsigned)(Np / TILE * tiles_h * z)), dim3(NTHR), kLdsRing,
+                         st, d);
+      if (int rc = check_launch(what)) return rc;
+    }
+  }
+  if (grad_x) {
+    hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)((s.N * (s.H / 8) + 255) / 256)), dim3(256), 0,
+                       st, w.part, z, w.pos, w.meta, Np, s.N, s.H, grad_x);
+    return check_launch(what);
+  }
+  return PLZ_OK;
+}
+
+static Sides ce_sides(const uint16_t* x, const uint16_t* w, const void* labels, int bytes,
+                      int64_t ignore, int64_t N, int64_t V, int64_t H) {
+  return Sides{x, w, nullptr, nullptr, labels, bytes == 8 ? KEY_INT64 : KEY_INT32, ignore, 1.f, N, V, H, 0};
+}
+static Sides kl_sides(const uint16_t* x, const uint16_t* w, const uint16_t* tx, const uint16_t* tw,
+                      const uint8_t* mask, float inv_t, int64_t N, int64_t V, int64_t H, int64_t Ht) {
+  return Sides{x, w, tx, tw, mask, mask ? KEY_MASK : KEY_NONE, 0, inv_t, N, V, H, Ht};
+}
+
+}  // namespace voc
+}  // namespace plz
+
+using namespace plz;
+using namespace plz::voc;
+
+extern "C" {
+
+size_t plz_vocab_loss_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher) {
+  if (N < 0 || V < 1 || H < 8 || H_teacher < 0) return 0;
+  Carve c{nullptr};
+  carve(c, false, N, V, H, H_teacher, false);
+  return c.used;
+}
+size_t plz_vocab_loss_bwd_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x) {
+  if (N < 1 || V < 1 || H < 8 || H_teacher < 0) return 0;
+  Carve c{nullptr};
+  carve(c, true, N, V, H, H_teacher, grad_x != 0);
+  return c.used;
+}
+
+int plz_linear_ce_fwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                      int64_t ignore_index, float* loss, float* lse, float* total, void* workspace,
+                      size_t workspace_bytes, int64_t N, int64_t V, int64_t H, void* stream) {
+  PLZ_REQUIRE(label_bytes == 8 || label_bytes == 4, "plz_linear_ce_fwd: labels of 4 or 8 bytes expected");
+  PLZ_REQUIRE(labels || N == 0, "plz_linear_ce_fwd: null pointer");
+  return forward<false>(ce_sides(x, w, labels, label_bytes, ignore_index, N, V, H), loss, lse, total,
+                        workspace, workspace_bytes, (hipStream_t)stream, "plz_linear_ce_fwd");
+}
+int plz_linear_ce_bwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                      int64_t ignore_index, const float* lse, const float* grad, int reduction,
+                      uint16_t* grad_x, uint16_t* grad_w, void* workspace, size_t workspace_bytes,
+                      int64_t N, int64_t V, int64_t H, void* stream) {
+  PLZ_REQUIRE(label_bytes == 8 || label_bytes == 4, "plz_linear_ce_bwd: labels of 4 or 8 bytes expected");
+  PLZ_REQUIRE(labels || N == 0, "plz_linear_ce_bwd: null pointer");
+  return backward<false>(ce_sides(x, w, labels, label_bytes, ignore_index, N, V, H), lse, grad,
+                         reduction, grad_x, grad_w, workspace, workspace_bytes, (hipStream_t)stream,
+                         "plz_linear_ce_bwd");
+}
+int plz_linear_kl_fwd(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                      const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                      float* loss, float* lse, float* total, void* workspace, size_t workspace_bytes,
+                      int64_t N, int64_t V, int64_t H, int64_t H_teacher, void* stream) {
+  return forward<true>(kl_sides(x, w, teacher_x, teacher_w, mask, inv_temperature, N, V, H, H_teacher),
+                       loss, lse, total, workspace, workspace_bytes, (hipStream_t)stream,
+                       "plz_linear_kl_fwd");
+}
+int plz_linear_kl_bwd(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                      const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                      const float* lse, const float* grad, int reduction, uint16_t* grad_x,
+                      uint16_t* grad_w, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
+                      int64_t H, int64_t H_teacher, void* stream) {
+  return backward<true>(kl_sides(x, w, teacher_x, teacher_w, mask, inv_temperature, N, V, H, H_teacher),
+                        lse, grad, reduction, grad_x, grad_w, workspace, workspace_bytes,
+                        (hipStream_t)stream, "plz_linear_kl_bwd");
+}
+
+}  // extern "C"

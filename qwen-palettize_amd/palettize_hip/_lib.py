@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libpalettize_hip.so")
 PLZ_OK, PLZ_EINVAL, PLZ_EHIP, PLZ_EUNSUPPORTED, PLZ_EWORKSPACE = 0, 1, 2, 3, 4
 PLZ_DT_BF16, PLZ_DT_FP16, PLZ_DT_FP32 = 0, 1, 2
 PLZ_W_SOFT, PLZ_W_HARD_NOISY, PLZ_W_HARD_PLAIN = 0, 1, 2
+PLZ_REDUCE_NONE, PLZ_REDUCE_SUM, PLZ_REDUCE_MEAN = 0, 1, 2
 PLZ_GEMV_NATIVE, PLZ_GEMV_DECODE, PLZ_GEMV_PLANES = 0, 1, 2
 
 p = C.c_void_p
@@ -153,6 +154,12 @@ SIGNATURES: dict[str, tuple] = {
     "plz_swiglu_bwd": (i32, [p, p, p, p, p, i64, p]),
     "plz_swiglu_fwd_rows": (i32, [p, p, i64, p, i64, i64, i64, p]),
     "plz_swiglu_bwd_rows": (i32, [p, p, i64, p, i64, p, p, i64, i64, i64, p]),
+    "plz_vocab_loss_workspace": (sz, [i64, i64, i64, i64]),
+    "plz_vocab_loss_bwd_workspace": (sz, [i64, i64, i64, i64, i32]),
+    "plz_linear_ce_fwd": (i32, [p, p, p, i32, i64, p, p, p, p, sz, i64, i64, i64, p]),
+    "plz_linear_ce_bwd": (i32, [p, p, p, i32, i64, p, p, i32, p, p, p, sz, i64, i64, i64, p]),
+    "plz_linear_kl_fwd": (i32, [p, p, p, p, p, f32, p, p, p, p, sz, i64, i64, i64, i64, p]),
+    "plz_linear_kl_bwd": (i32, [p, p, p, p, p, f32, p, p, i32, p, p, p, sz, i64, i64, i64, i64, p]),
     "plz_paged_step": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i64, i32, p]),
     "plz_paged_rope_write": (i32, [p, p, p, i64, i64, i64, p, p, p, p, p, p, p, p, p, i64, i32, i32,
                                    i32, i64, i64, i32, f32, p]),

@@ -11,6 +11,9 @@
       forward uses W_hard (or W_soft for mode=PLZ_W_SOFT), backward differentiates
       W_soft = sum_c P_c pal_c without the 1/tau factor unless scale_by_inv_tau.
 
+  linear_cross_entropy(x, weight, labels), linear_distill(x, weight, teacher_x, teacher_weight)
+      losses over a large vocabulary from hidden states and head weights, the logits never kept.
+
 Inputs are 2-D ([M, K]); callers flatten leading dimensions.
 """
 from __future__ import annotations
@@ -197,3 +200,87 @@ def soft_lut_linear(x, palette, logits, noise, tau, bias=None, lora_a=None, lora
     y = SoftLUTLinearFunction.apply(x.reshape(-1, x.shape[-1]), palette, logits, noise, tau, bias,
                                     lora_a, lora_b, lora_scale, mode, scale_by_inv_tau)
     return y.reshape(*lead, y.shape[-1])
+
+
+# ---- losses over a large vocabulary --------------------------------------------------------------
+def _rows(t, width):
+    """[..., width] as contiguous rows on 16 bytes, as the kernels read them."""
+    t = t.reshape(-1, width).contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+class LinearCrossEntropyFunction(torch.autograd.Function):
+    """Keeps the rows' normalisers (fp32 [N]); the backward computes the logits again, a piece of the
+    vocabulary at a time."""
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, reduction):
+        loss, lse, total = ops.linear_ce_fwd(x, weight, labels, ignore_index,
+                                             total=reduction != "none")
+        ctx.save_for_backward(x, weight, labels, lse)
+        ctx.args = reduction, ignore_index
+        return loss if total is None else total[0 if reduction == "sum" else 1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, labels, lse = ctx.saved_tensors
+        gx, gw = ops.linear_ce_bwd(x, weight, labels, lse, grad.contiguous(), *ctx.args,
+                                   grad_x=ctx.needs_input_grad[0], grad_weight=ctx.needs_input_grad[1])
+        return gx, gw, None, None, None
+
+
+def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean"):
+    """Cross entropy of labels under softmax(x weight^T): torch's cross_entropy of those logits in fp32,
+    without them. x bf16 [..., H], weight bf16 [V, H] (H a multiple of 8), labels int64 or int32 [...].
+    Rows whose label is ignore_index take no part (whatever x holds there; their gradient is 0); other
+    labels outside [0, V) give NaN. Returns fp32: the mean over the rows that take part (0 without
+    one), the sum, or every row's loss in the labels' shape. Gradients of x and weight are bf16."""
+    ops._reduction(reduction)
+    if labels.shape != x.shape[:-1]:
+        raise ValueError(f"labels {tuple(labels.shape)} do not match x {tuple(x.shape)}")
+    H = x.shape[-1]
+    loss = LinearCrossEntropyFunction.apply(_rows(x, H), _rows(weight, weight.shape[-1]),
+                                            labels.reshape(-1).contiguous(), int(ignore_index),
+                                            reduction)
+    return loss.reshape(labels.shape) if reduction == "none" else loss
+
+
+class LinearDistillFunction(torch.autograd.Function):
+    """As LinearCrossEntropyFunction, with the normalisers of both sides."""
+
+    @staticmethod
+    def forward(ctx, x, weight, teacher_x, teacher_weight, mask, temperature, reduction):
+        loss, lse, total = ops.linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask, temperature,
+                                             total=reduction != "none")
+        ctx.save_for_backward(x, weight, teacher_x, teacher_weight, mask, lse)
+        ctx.args = reduction, temperature
+        return loss if total is None else total[0 if reduction == "sum" else 1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, teacher_x, teacher_weight, mask, lse = ctx.saved_tensors
+        reduction, temperature = ctx.args
+        gx, gw = ops.linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad.contiguous(),
+                                   reduction, mask, temperature, grad_x=ctx.needs_input_grad[0],
+                                   grad_weight=ctx.needs_input_grad[1])
+        return gx, gw, None, None, None, None, None
+
+
+def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, reduction="mean"):
+    """Distillation on the teacher's distribution over the vocabulary: KL(p, q) with
+    p = softmax(teacher_x teacher_weight^T / temperature), q = softmax(x weight^T / temperature), without
+    the logits. x bf16 [..., H], weight bf16 [V, H]; teacher_x bf16 [..., Ht], teacher_weight bf16
+    [V, Ht], which get no gradient (a frozen head that both sides share is given twice); mask bool
+    [...]: rows that it leaves out take no part (whatever they hold; their gradient is 0). Returns as
+    linear_cross_entropy does; the loss is not multiplied by temperature^2."""
+    ops._reduction(reduction)
+    if teacher_x.shape[:-1] != x.shape[:-1] or (mask is not None and mask.shape != x.shape[:-1]):
+        raise ValueError("x, teacher_x and mask differ in their leading dimensions")
+    H, Ht = x.shape[-1], teacher_x.shape[-1]
+    loss = LinearDistillFunction.apply(
+        _rows(x, H), _rows(weight, weight.shape[-1]), _rows(teacher_x.detach(), Ht),
+        _rows(teacher_weight.detach(), teacher_weight.shape[-1]),
+        None if mask is None else mask.reshape(-1).contiguous(), float(temperature), reduction)
+    return loss.reshape(x.shape[:-1]) if reduction == "none" else loss

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 
 import torch
 
@@ -1129,6 +1130,143 @@ def distill_loss_bwd(student, teacher, out4, ws, grad_loss, w_cos=0.5, w_mse=0.5
          float(w_cos), float(w_mse), float(eps), _ptr(gs), _ptr(ws), ws.numel(), rows, dim,
          _stream(student))
     return gs
+
+
+# ---- losses over a large vocabulary --------------------------------------------------------------
+def _head(x, weight, name="x", wname="weight"):
+    """(N, V, H) of hidden states bf16 [N, H] and head weights bf16 [V, H]."""
+    _need(x, name, torch.bfloat16, 2)
+    _need(weight, wname, torch.bfloat16, 2)
+    if x.shape[1] != weight.shape[1]:
+        raise ValueError(f"{name} {tuple(x.shape)} and {wname} {tuple(weight.shape)} differ in width")
+    if weight.shape[0] < 1 or x.shape[1] < 8 or x.shape[1] % 8:
+        raise ValueError(f"{wname} {tuple(weight.shape)}: at least one word and a width of a multiple of "
+                         "8 expected")
+    return x.shape[0], *weight.shape
+
+
+def _labels(labels, N):
+    """Bytes of a label: int64 or int32 [N]."""
+    _need(labels, "labels", None, 1)
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
+    if labels.numel() != N:
+        raise ValueError(f"{labels.numel()} labels for {N} rows")
+    return labels.element_size()
+
+
+def _mask(mask, N):
+    if mask is not None:
+        _need(mask, "mask", torch.bool, 1)
+        if mask.numel() != N:
+            raise ValueError(f"mask has {mask.numel()} values for {N} rows")
+    return mask
+
+
+def _inv_temperature(temperature):
+    t = float(temperature)
+    if not 0.0 < t < math.inf:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    return 1.0 / t
+
+
+def _reduction(reduction):
+    try:
+        return {"none": _lib.PLZ_REDUCE_NONE, "sum": _lib.PLZ_REDUCE_SUM,
+                "mean": _lib.PLZ_REDUCE_MEAN}[reduction]
+    except KeyError:
+        raise ValueError(f"reduction must be none, sum or mean, got {reduction!r}") from None
+
+
+def _upstream(grad, reduction, N):
+    """The gradient of the loss as the library takes it: fp32, [N] or one value."""
+    _need(grad, "grad", torch.float32)
+    if grad.numel() != (N if reduction == _lib.PLZ_REDUCE_NONE else 1):
+        raise ValueError(f"grad has {grad.numel()} values for {N} rows")
+    return grad
+
+
+def _kept(t, name, *shape):
+    """What the forward returned for the backward: fp32 of that shape."""
+    _need(t, name, torch.float32, len(shape))
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    return t
+
+
+def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
+    """Cross entropy of labels (int64 or int32 [N]) under softmax(x weight^T), x bf16 [N, H], weight
+    bf16 [V, H], without the logits: (loss fp32 [N], lse fp32 [N] for the backward, total fp32 [3] =
+    sum, mean over the rows that take part (0 without one) and their number, or None). Rows whose label
+    is ignore_index take no part: loss 0. Another label outside [0, V) gives NaN."""
+    N, V, H = _head(x, weight)
+    size = _labels(labels, N)
+    dev = _one_device("linear_ce_fwd", x, weight, labels)
+    loss, lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
+    ws = _workspace(query("plz_vocab_loss_workspace", N, V, H, 0), x.device)
+    _on(dev, "plz_linear_ce_fwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
+        _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H)
+    return loss, lse, out
+
+
+def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-100, grad_x=True,
+                  grad_weight=True):
+    """Gradients (x, weight) of linear_ce_fwd's loss, bf16 (None where not wanted), from the gradient
+    of its mean or sum (fp32, one value) or of every row's (fp32 [N], reduction "none")."""
+    N, V, H = _head(x, weight)
+    size, mode = _labels(labels, N), _reduction(reduction)
+    _kept(lse, "lse", N)
+    _upstream(grad, mode, N)
+    dev = _one_device("linear_ce_bwd", x, weight, labels, lse, grad)
+    gx = torch.empty_like(x) if grad_x else None
+    gw = torch.empty_like(weight) if grad_weight else None
+    ws = _workspace(query("plz_vocab_loss_bwd_workspace", N, V, H, 0, int(grad_x)), x.device)
+    _on(dev, "plz_linear_ce_bwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
+        _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
+    return gx, gw
+
+
+def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, total=True):
+    """Distillation over the vocabulary, sum_v p_v (log p_v - log q_v) with p the teacher's
+    softmax(teacher_x teacher_weight^T / temperature) and q the student's, without the logits: (loss
+    fp32 [N], lse fp32 [2, N] for the backward, total as linear_ce_fwd's). mask bool [N]: rows that it
+    leaves out take no part."""
+    N, V, H = _head(x, weight)
+    M, Vt, Ht = _head(teacher_x, teacher_weight, "teacher_x", "teacher_weight")
+    if (M, Vt) != (N, V):
+        raise ValueError(f"the teacher has {M} rows and {Vt} words, the student {N} and {V}")
+    _mask(mask, N)
+    inv = _inv_temperature(temperature)
+    dev = _one_device("linear_kl_fwd", x, weight, teacher_x, teacher_weight, mask)
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
+    ws = _workspace(query("plz_vocab_loss_workspace", N, V, H, Ht), x.device)
+    _on(dev, "plz_linear_kl_fwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
+        _ptr(mask), inv, _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H, Ht)
+    return loss, lse, out
+
+
+def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="mean", mask=None,
+                  temperature=1.0, grad_x=True, grad_weight=True):
+    """Gradients (x, weight) of linear_kl_fwd's loss, as linear_ce_bwd's; the teacher has none."""
+    N, V, H = _head(x, weight)
+    M, Vt, Ht = _head(teacher_x, teacher_weight, "teacher_x", "teacher_weight")
+    if (M, Vt) != (N, V):
+        raise ValueError(f"the teacher has {M} rows and {Vt} words, the student {N} and {V}")
+    _mask(mask, N)
+    mode, inv = _reduction(reduction), _inv_temperature(temperature)
+    _kept(lse, "lse", 2, N)
+    _upstream(grad, mode, N)
+    dev = _one_device("linear_kl_bwd", x, weight, teacher_x, teacher_weight, mask, lse, grad)
+    gx = torch.empty_like(x) if grad_x else None
+    gw = torch.empty_like(weight) if grad_weight else None
+    ws = _workspace(query("plz_vocab_loss_bwd_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    _on(dev, "plz_linear_kl_bwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
+        _ptr(mask), inv, _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V,
+        H, Ht)
+    return gx, gw
 
 
 # ---- attention ---------------------------------------------------------------------------------

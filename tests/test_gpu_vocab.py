@@ -1,0 +1,368 @@
+"""Losses over a large vocabulary against their definitions in 64 bits (GPU)."""
+import pytest
+import torch
+
+from vocab_ref import close, inputs, reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu(dev):
+    pass
+
+
+@pytest.fixture(scope="module")
+def F():
+    from palettize_hip import functional
+    return functional
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from palettize_hip import ops
+    return ops
+
+
+SIZES = [(1, 1, 8), (1, 5, 8), (2, 256, 64), (3, 257, 72), (17, 1000, 128), (64, 1003, 200),
+         (255, 511, 64), (256, 512, 256), (257, 2049, 136), (300, 4099, 1000), (777, 3001, 512)]
+
+
+def run_ce(F, x, w, labels, reduction="mean", upstream=None, **kw):
+    x, w = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    loss = F.linear_cross_entropy(x, w, labels, reduction=reduction, **kw)
+    g = None if upstream is None and reduction != "none" else (
+        torch.ones_like(loss) if upstream is None else
+        torch.as_tensor(upstream, dtype=torch.float32, device=loss.device).reshape(loss.shape))
+    return (loss.detach(), *torch.autograd.grad(loss, (x, w), g))
+
+
+def check(got, ref):
+    loss, gx, gw = got
+    assert loss.dtype == torch.float32 and gx.dtype == gw.dtype == torch.bfloat16
+    close(loss, ref["loss"], ref["loss_tol"], "loss")
+    close(gx, ref["gx"], ref["gx_tol"], "grad_x")
+    close(gw, ref["gw"], ref["gw_tol"], "grad_weight")
+    assert not gx[~ref["keep"]].any()
+
+
+@pytest.mark.parametrize("N,V,H", SIZES)
+@pytest.mark.parametrize("ignored", [0.0, 0.5])
+def test_ce_mean(F, N, V, H, ignored):
+    x, w, labels = inputs(N, V, H, seed=N + V, ignored=ignored)
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+
+
+@pytest.mark.parametrize("N,V,H", [(17, 1000, 128), (300, 777, 72)])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("reduction,upstream", [("sum", None), ("sum", 0.37), ("mean", -3.0), ("none", None)])
+def test_ce_reductions(F, N, V, H, dtype, reduction, upstream):
+    x, w, labels = inputs(N, V, H, seed=1, ignored=0.3, dtype=dtype)
+    check(run_ce(F, x, w, labels, reduction, upstream),
+          reference(x, w, labels, reduction=reduction, upstream=upstream))
+
+
+def test_ce_upstream_of_every_row(F):
+    x, w, labels = inputs(130, 900, 96, seed=2, ignored=0.2)
+    up = torch.randn(130, device="cuda")
+    up[5] = 0
+    check(run_ce(F, x, w, labels, "none", up), reference(x, w, labels, reduction="none", upstream=up))
+
+
+def run_kl(F, x, w, tx, tw, reduction="mean", upstream=None, **kw):
+    x, w = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    loss = F.linear_distill(x, w, tx, tw, reduction=reduction, **kw)
+    g = None if reduction != "none" else torch.ones_like(loss) if upstream is None else upstream
+    return (loss.detach(), *torch.autograd.grad(loss, (x, w), g))
+
+
+def kl_inputs(N, V, H, Ht, seed, ignored):
+    x, w, labels = inputs(N, V, H, seed=seed, ignored=ignored)
+    if Ht:
+        tx, tw, _ = inputs(N, V, Ht, seed=seed + 1)
+    else:
+        tx, tw = (x.float() + 0.3 * torch.randn(N, H, device="cuda")).bfloat16(), w
+    return x, w, tx, tw, (labels != -100) if ignored else None
+
+
+@pytest.mark.parametrize("N,V,H", SIZES)
+@pytest.mark.parametrize("Ht,ignored,T", [(0, 0.0, 1.0), (72, 0.4, 2.0), (640, 0.0, 0.7)])
+def test_kl_mean(F, N, V, H, Ht, ignored, T):
+    x, w, tx, tw, mask = kl_inputs(N, V, H, Ht, N + V, ignored)
+    check(run_kl(F, x, w, tx, tw, mask=mask, temperature=T),
+          reference(x, w, tx=tx, tw=tw, mask=mask, T=T))
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_kl_reductions(F, reduction):
+    x, w, tx, tw, mask = kl_inputs(150, 1030, 128, 0, 7, 0.3)
+    up = torch.randn(150, device="cuda") if reduction == "none" else None
+    check(run_kl(F, x, w, tx, tw, reduction, up, mask=mask),
+          reference(x, w, tx=tx, tw=tw, mask=mask, reduction=reduction, upstream=up))
+
+
+def test_kl_of_itself_is_zero(F):
+    x, w, _ = inputs(70, 3000, 256, seed=3)
+    loss, gx, gw = run_kl(F, x, w, x, w, "none")
+    # both sides' sums are the same instructions on the same values
+    assert float(loss.abs().max()) == 0 and not gx.any() and not gw.any()
+
+
+# ---- what takes no part -------------------------------------------------------------------------------
+@pytest.mark.parametrize("N", [1, 40, 300])
+def test_ce_no_row_takes_part(F, N):
+    x, w, labels = inputs(N, 700, 64)
+    labels[:] = -100
+    for reduction in ("mean", "sum", "none"):
+        loss, gx, gw = run_ce(F, x, w, labels, reduction)
+        assert not loss.any() and not gx.any() and not gw.any()
+
+
+def test_no_rows(F):
+    x, w, labels = inputs(0, 700, 64)
+    for reduction in ("mean", "sum"):
+        loss, gx, gw = run_ce(F, x, w, labels, reduction)
+        assert float(loss) == 0 and gx.shape == (0, 64) and not gw.any()
+    loss, gx, gw = run_ce(F, x, w, labels, "none")
+    assert loss.shape == (0,) and not gw.any()
+    loss, gx, gw = run_kl(F, x, w, x, w)
+    assert float(loss) == 0 and not gw.any()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rows_without_part_may_hold_anything(F, value):
+    x, w, labels = inputs(333, 1500, 136, seed=5, ignored=0.4)
+    want = run_ce(F, x, w, labels)
+    bad = x.clone()
+    bad[labels == -100] = value
+    for a, b in zip(run_ce(F, bad, w, labels), want):
+        assert torch.equal(a, b)
+    mask = labels != -100
+    tx = (x.float() * 0.9).bfloat16()
+    want = run_kl(F, x, w, tx, w, mask=mask)
+    tbad = tx.clone()
+    tbad[~mask] = value
+    for a, b in zip(run_kl(F, bad, w, tbad, w, mask=mask), want):
+        assert torch.equal(a, b)
+
+
+def test_another_ignore_index(F):
+    x, w, labels = inputs(90, 300, 64, seed=6)
+    labels[::3] = 7
+    check(run_ce(F, x, w, labels, ignore_index=7), reference(x, w, labels, ignore_index=7))
+
+
+@pytest.mark.parametrize("bad", [-1, 300, 2 ** 31, 2 ** 40, -2 ** 33])
+def test_labels_outside_the_vocabulary_are_nan(F, bad):
+    x, w, labels = inputs(90, 300, 64, seed=6)
+    want = run_ce(F, x, w, labels, "none")
+    labels[17] = bad
+    loss, gx, gw = run_ce(F, x, w, labels, "none")
+    others = torch.arange(90, device="cuda") != 17
+    assert torch.isnan(loss[17]) and torch.equal(loss[others], want[0][others])
+    assert torch.isnan(gx[17]).all() and torch.equal(gx[others], want[1][others])
+    assert torch.isnan(gw).all()
+    assert torch.isnan(run_ce(F, x, w, labels)[0])
+
+
+# ---- extreme values -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shift", [60.0, -60.0, 3000.0])
+def test_far_logits(F, shift):
+    """All logits of a row moved by the same amount, far past what exp takes by itself."""
+    x, w, labels = inputs(64, 1000, 128, seed=8)
+    x[:, -8:] = 1.0
+    w[:, -8:] = shift / 8
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+
+
+def test_one_word_holds_all(F):
+    x, w, labels = inputs(64, 1000, 128, seed=9, lean=60.0)
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+
+
+def test_a_word_that_cannot_be(F):
+    """Logits of minus infinity: no weight, finite loss for the other words' rows."""
+    x, w, labels = inputs(40, 520, 64, seed=10)
+    x[:, 0] = 1.0
+    dead = torch.tensor([3, 300, 519], device="cuda")
+    w[dead] = 0
+    w[dead, 0] = -float("inf")
+    live = torch.ones(520, dtype=torch.bool, device="cuda")
+    live[dead] = False
+    labels = live.nonzero()[:, 0][labels % 517]
+    loss = F.linear_cross_entropy(x, w, labels, reduction="none")
+    index = torch.cumsum(live, 0) - 1
+    ref = reference(x, w[live], index[labels], reduction="none")
+    close(loss, ref["rows"], ref["rows_tol"], "loss")
+    labels[4] = 300
+    assert F.linear_cross_entropy(x, w, labels, reduction="none")[4] == float("inf")
+
+
+def test_nan_in_a_row_stays_in_its_row(F):
+    x, w, labels = inputs(50, 700, 64, seed=11)
+    want = F.linear_cross_entropy(x, w, labels, reduction="none")
+    x[9, 5] = float("nan")
+    got = F.linear_cross_entropy(x, w, labels, reduction="none")
+    others = torch.arange(50, device="cuda") != 9
+    assert torch.isnan(got[9]) and torch.equal(got[others], want[others])
+
+
+# ---- pieces, splits, shapes -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_pieces_of_the_vocabulary(F, kind):
+    """More words than a piece of the backward holds for so many rows (32768), and the last piece odd."""
+    x, w, labels = inputs(16384, 33333, 64, seed=12, ignored=0.1)
+    if kind == "ce":
+        check(run_ce(F, x, w, labels), reference(x, w, labels))
+    else:
+        tx = (x.float() * 0.8).bfloat16()
+        check(run_kl(F, x, w, tx, w, mask=labels != -100),
+              reference(x, w, tx=tx, tw=w, mask=labels != -100))
+
+
+def test_many_words_for_one_row(F):
+    """dx in many splits of the vocabulary."""
+    x, w, labels = inputs(1, 100003, 64, seed=13)
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+
+
+def test_leading_dimensions_and_strides(F):
+    x, w, labels = inputs(60, 500, 64, seed=14, ignored=0.2)
+    want = run_ce(F, x, w, labels, "none")
+    wide = torch.zeros(60, 2, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, 1] = x
+    got = run_ce(F, wide[:, 1].reshape(3, 20, 64), w, labels.reshape(3, 20), "none")
+    assert got[0].shape == (3, 20) and got[1].shape == (3, 20, 64)
+    assert torch.equal(got[0].flatten(), want[0]) and torch.equal(got[1].reshape(60, 64), want[1])
+    # weights that start off 16 bytes, rows in another order
+    off = torch.empty(500 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(500, 64)
+    off.copy_(w)
+    loss = F.linear_cross_entropy(x.t().contiguous().t(), off, labels, reduction="none")
+    assert torch.equal(loss, want[0])
+
+
+def test_only_the_gradients_that_are_wanted(ops):
+    x, w, labels = inputs(100, 900, 64, seed=15)
+    _, lse, _ = ops.linear_ce_fwd(x, w, labels)
+    one = torch.ones(1, device="cuda")
+    both = ops.linear_ce_bwd(x, w, labels, lse, one)
+    gx, none = ops.linear_ce_bwd(x, w, labels, lse, one, grad_weight=False)
+    assert none is None and torch.equal(gx, both[0])
+    none, gw = ops.linear_ce_bwd(x, w, labels, lse, one, grad_x=False)
+    assert none is None and torch.equal(gw, both[1])
+
+
+def test_same_bits_every_time(F):
+    x, w, labels = inputs(700, 3000, 256, seed=16, ignored=0.3)
+    first = run_ce(F, x, w, labels)
+    for _ in range(3):
+        for a, b in zip(run_ce(F, x, w, labels), first):
+            assert torch.equal(a, b)
+
+
+# ---- gradients against differences ------------------------------------------------------------------------
+def test_gradients_against_differences(F):
+    """Differences of the kernel's own sums of losses along the signs of its gradient, in steps of about
+    2^-6 of every value, between two bf16 points. Along a line on which a row's logits move by at most a,
+    the loss's second and third derivatives are at most a^2 and a^3, and the losses are fp32 sums off by
+    rows_tol each."""
+    x, w, labels = inputs(48, 700, 64, seed=17)
+    _, gx, gw = run_ce(F, x, w, labels, "sum")
+    ref = reference(x, w, labels, reduction="sum")
+    for t, grad, tol in ((x, gx, ref["gx_tol"]), (w, gw, ref["gw_tol"])):
+        step = grad.float().sign() * t.float().abs() * 2 ** -6
+        up, down = (t.float() + step).bfloat16(), (t.float() - step).bfloat16()
+        hi, lo = (F.linear_cross_entropy(*((v, w) if t is x else (x, v)), labels, reduction="none")
+                  for v in (up, down))
+        d = up.double() - down.double()
+        mid = ((up.double() + down.double()) / 2 - t.double()).abs()
+        moved, skew = ((v @ w.double().abs().T if t is x else x.double().abs() @ v.T).max(1).values
+                       for v in (d.abs(), mid))
+        bound = float((moved ** 3 / 24 + moved * skew).sum() + 3 * ref["rows_tol"].sum()
+                      + (tol * d.abs()).sum())
+        change = float((hi.double() - lo.double()).sum())
+        assert abs(change - float((grad.double() * d).sum())) <= bound < 0.2 * change
+
+
+# ---- streams, graphs, refusals ------------------------------------------------------------------------------
+def test_other_stream(F):
+    x, w, labels = inputs(200, 2000, 128, seed=18)
+    want = run_ce(F, x, w, labels)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run_ce(F, x, w, labels)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_captured_and_replayed(ops, kind):
+    """Forward and backward in a graph; replays on other inputs and other masks than the captured."""
+    N, V, H = 300, 3001, 136
+    x, w, labels = inputs(N, V, H, seed=19)
+    tx = torch.zeros_like(x)
+    mask = torch.ones(N, dtype=torch.bool, device="cuda")
+    one = torch.ones(1, device="cuda")
+
+    def step():
+        if kind == "ce":
+            loss, lse, total = ops.linear_ce_fwd(x, w, labels)
+            return (loss, total, *ops.linear_ce_bwd(x, w, labels, lse, one))
+        loss, lse, total = ops.linear_kl_fwd(x, w, tx, w, mask)
+        return (loss, total, *ops.linear_kl_bwd(x, w, tx, w, lse, one, mask=mask))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        nx, _, nl = inputs(N, V, H, seed=30 + seed, ignored=0.25 * seed)
+        x.copy_(nx)
+        labels.copy_(nl)
+        mask.copy_(nl != -100)
+        tx.copy_(nx.flip(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+def test_refusals(F, ops):
+    x, w, labels = inputs(10, 50, 64)
+    with pytest.raises(ValueError, match="reduction"):
+        F.linear_cross_entropy(x, w, labels, reduction="average")
+    with pytest.raises(ValueError, match="labels"):
+        F.linear_cross_entropy(x, w, labels[:9])
+    with pytest.raises(TypeError, match="bfloat16"):
+        F.linear_cross_entropy(x.float(), w, labels)
+    with pytest.raises(TypeError, match="bfloat16"):
+        F.linear_cross_entropy(x, w.half(), labels)
+    with pytest.raises(TypeError, match="labels"):
+        F.linear_cross_entropy(x, w, labels.float())
+    with pytest.raises(ValueError, match="width"):
+        F.linear_cross_entropy(x, w[:, :56], labels)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        F.linear_cross_entropy(x[:, :60].contiguous(), w[:, :60].contiguous(), labels)
+    with pytest.raises(ValueError, match="word"):
+        F.linear_cross_entropy(x, w[:0], labels)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        F.linear_cross_entropy(x.cpu(), w, labels)
+    with pytest.raises(ValueError, match="temperature"):
+        F.linear_distill(x, w, x, w, temperature=0.0)
+    with pytest.raises(TypeError, match="mask"):
+        F.linear_distill(x, w, x, w, mask=torch.ones(10, device="cuda"))
+    with pytest.raises(ValueError, match="leading"):
+        F.linear_distill(x, w, x[:9], w)
+    with pytest.raises(ValueError, match="words"):
+        F.linear_distill(x, w, x, w[:49])
+    with pytest.raises(ValueError, match="grad"):
+        ops.linear_ce_bwd(x, w, labels, torch.zeros(10, device="cuda"), torch.ones(2, device="cuda"))
+    with pytest.raises(ValueError, match="lse"):
+        ops.linear_ce_bwd(x, w, labels, torch.zeros(9, device="cuda"), torch.ones(1, device="cuda"))

@@ -1,0 +1,72 @@
+"""CPU checks of the losses over a vocabulary: what the C entry points refuse, and their workspaces."""
+import ctypes as C
+import os
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from palettize_hip import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__
+        __graft_entry__.build()
+    return _lib.lib()
+
+
+A = C.c_void_p(4096)  # an address on 16 bytes that no refused call reads
+
+
+def ce_fwd(lib, x=A, w=A, labels=A, size=8, loss=A, lse=A, ws=A, ws_bytes=1 << 40, N=4, V=100, H=64):
+    return lib.plz_linear_ce_fwd(x, w, labels, size, -100, loss, lse, None, ws, ws_bytes, N, V, H, None)
+
+
+def kl_fwd(lib, tx=A, tw=A, inv=1.0, N=4, V=100, H=64, Ht=64, ws=A, ws_bytes=1 << 40):
+    return lib.plz_linear_kl_fwd(A, A, tx, tw, None, inv, A, A, None, ws, ws_bytes, N, V, H, Ht, None)
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(size=2), 1, b"bytes"), (dict(x=None), 1, b"null"), (dict(w=None), 1, b"null"),
+    (dict(labels=None), 1, b"null"), (dict(loss=None), 1, b"null"), (dict(lse=None), 1, b"null"),
+    (dict(H=60), 1, b"multiples of 8"), (dict(H=0), 1, b"shape"), (dict(V=0), 1, b"shape"),
+    (dict(N=-1), 1, b"shape"), (dict(x=C.c_void_p(4098)), 1, b"aligned"),
+    (dict(ws=None), 4, b"workspace"), (dict(ws_bytes=1000), 4, b"workspace"),
+    (dict(ws=C.c_void_p(4098)), 1, b"aligned"),
+    (dict(N=1 << 22), 3, b"2^22"), (dict(N=1 << 20, H=4096), 3, b"2^31"),
+    (dict(V=(1 << 31) - 1), 3, b"2^31")])
+def test_ce_forward_refuses(lib, kw, status, word):
+    assert ce_fwd(lib, **kw) == status and word in lib.plz_last_error()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(tx=None), 1, b"null"), (dict(tw=None), 1, b"null"), (dict(inv=0.0), 1, b"temperature"),
+    (dict(inv=-1.0), 1, b"temperature"), (dict(inv=float("nan")), 1, b"temperature"),
+    (dict(inv=float("inf")), 1, b"temperature"), (dict(Ht=0), 1, b"shape"), (dict(Ht=12), 1, b"multiples"),
+    (dict(tw=C.c_void_p(4104)), 1, b"aligned"), (dict(ws_bytes=64), 4, b"workspace")])
+def test_kl_forward_refuses(lib, kw, status, word):
+    assert kl_fwd(lib, **kw) == status and word in lib.plz_last_error()
+
+
+def test_backward_refuses(lib):
+    def bwd(lse=A, grad=A, mode=2, gx=A, gw=A, ws=A, ws_bytes=1 << 40, size=8):
+        return lib.plz_linear_ce_bwd(A, A, A, size, -100, lse, grad, mode, gx, gw, ws, ws_bytes, 4, 100, 64,
+                                     None)
+    for kw, status, word in ((dict(lse=None), 1, b"null"), (dict(grad=None), 1, b"null"),
+                             (dict(mode=3), 1, b"reduction"), (dict(gx=C.c_void_p(8)), 1, b"aligned"),
+                             (dict(gw=C.c_void_p(8)), 1, b"aligned"), (dict(ws=None), 4, b"workspace"),
+                             (dict(ws_bytes=10), 4, b"workspace"), (dict(size=1), 1, b"bytes")):
+        assert bwd(**kw) == status and word in lib.plz_last_error(), kw
+    assert bwd(gx=None, gw=None) == 0  # nothing wanted, nothing done
+
+
+def test_workspaces(lib):
+    fwd, bwd = lib.plz_vocab_loss_workspace, lib.plz_vocab_loss_bwd_workspace
+    N, V, H = 4096, 151936, 2560
+    # the packed rows and the tiles' statistics: far less than the logits (2.5 GB)
+    assert N * H * 2 < fwd(N, V, H, 0) < 64 << 20
+    # at most a piece of bf16 gradients of logits (1 GiB), the packed rows and dx in fp32 parts
+    assert bwd(N, V, H, 0, 1) < (1 << 30) + (1 << 29)
+    assert bwd(N, V, H, 0, 0) < bwd(N, V, H, 0, 1) < bwd(N, V, H, 2560, 1)
+    assert bwd(1 << 17, V, 2560, 0, 0) < (1 << 30) + (1 << 30)
+    assert fwd(0, 1, 8, 0) > 0
+    assert fwd(-1, 100, 64, 0) == 0 and bwd(0, 100, 64, 0, 1) == 0

@@ -744,6 +744,21 @@ int plz_linear_kl_bwd(const uint16_t* x, const uint16_t* w, const uint16_t* teac
                       uint16_t* grad_w, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
                       int64_t H, int64_t H_teacher, void* stream);
 
+/* ---- gradient norm and clipping ---------------------------------------------------------- */
+/* norm = sqrt(sum of the squares of every value of every tensor), squared and summed in 64 bits, and
+ * out[i] = grads[i] min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_,
+ * train_qwen.py:1303-1319). grads, sizes (values of each), dtypes (PLZ_DT_*) and out are host arrays
+ * of `count`, read before the call returns; a tensor of no values is passed over. Tensors are
+ * contiguous, on the size of their values at least (on 16 bytes they are faster). out[i] has a type of
+ * its own and is grads[i] itself (of the same type) or overlaps no tensor of the call. norm_out fp32
+ * [1]. A norm of infinity gives 0, and NaN for the infinite values; a norm of NaN NaN. */
+size_t plz_grad_norm_workspace(const int64_t* sizes, int count);
+int plz_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count,
+                  float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+int plz_clip_grads(const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
+                   void* const* out, const int32_t* out_dtypes, int count, float max_norm,
+                   float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- decoding over a paged key-value cache ------------------------------------------- */
 /* A cache is a pool of num_pages pages of page_size tokens (a power of two, 16..1024); one layer's
  * pages are k_cache bf16 [num_pages, kv_heads, head_dim / 8, page_size, 8] (value d of a token at

@@ -160,6 +160,9 @@ SIGNATURES: dict[str, tuple] = {
     "plz_linear_ce_bwd": (i32, [p, p, p, i32, i64, p, p, i32, p, p, p, sz, i64, i64, i64, p]),
     "plz_linear_kl_fwd": (i32, [p, p, p, p, p, f32, p, p, p, p, sz, i64, i64, i64, i64, p]),
     "plz_linear_kl_bwd": (i32, [p, p, p, p, p, f32, p, p, i32, p, p, p, sz, i64, i64, i64, i64, p]),
+    "plz_grad_norm_workspace": (sz, [p, i32]),
+    "plz_grad_norm": (i32, [p, p, p, i32, p, p, sz, p]),
+    "plz_clip_grads": (i32, [p, p, p, p, p, i32, f32, p, p, sz, p]),
     "plz_paged_step": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i64, i32, p]),
     "plz_paged_rope_write": (i32, [p, p, p, i64, i64, i64, p, p, p, p, p, p, p, p, p, i64, i32, i32,
                                    i32, i64, i64, i32, f32, p]),

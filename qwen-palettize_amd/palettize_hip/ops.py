@@ -1269,6 +1269,83 @@ def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="me
     return gx, gw
 
 
+# ---- gradient norm and clipping --------------------------------------------------------------------
+_Tensor = torch.Tensor
+
+
+def _grad_table(name, tensors):
+    """(addresses, values, dtypes) of contiguous GPU tensors of one device, as arrays of the C ABI."""
+    n = len(tensors)
+    # one pass of C calls for each property: 0.2 us a tensor in all, a loop over checks 1.5
+    try:
+        devices = set(map(_Tensor.get_device, tensors))
+        dense = all(map(_Tensor.is_contiguous, tensors))
+        kinds = [_DT[t.dtype] for t in tensors]
+    except (TypeError, KeyError):
+        raise TypeError(f"{name}: bf16, fp16 or fp32 tensors expected") from None
+    if -1 in devices:
+        raise RuntimeError(f"{name}: GPU tensors expected (palettize_hip has no CPU path)")
+    if len(devices) > 1:
+        raise ValueError(f"{name}: the tensors are on different devices")
+    if not dense:
+        raise ValueError(f"{name}: the tensors must be contiguous")
+    return ((C.c_void_p * n)(*map(_Tensor.data_ptr, tensors)),
+            (C.c_int64 * n)(*map(_Tensor.numel, tensors)), (C.c_int32 * n)(*kinds), devices.pop())
+
+
+def grad_norm(grads):
+    """The 2-norm of all values of a sequence of tensors (bf16, fp16 or fp32, of one device, at least
+    one), squared and summed in 64 bits: fp32, no dimensions."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grad_norm: at least one tensor expected")
+    ptrs, sizes, kinds, dev = _grad_table("grad_norm", grads)
+    _no_backward("grad_norm", *grads)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = _workspace(query("plz_grad_norm_workspace", sizes, len(grads)), norm.device)
+    _on(dev, "plz_grad_norm", ptrs, sizes, kinds, len(grads), _ptr(norm), _ptr(ws), ws.numel())
+    return norm
+
+
+def clip_grads(grads, max_norm, out=None):
+    """out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) with the norm of all of them (grad_norm),
+    which it returns, unclipped. out: tensors of the same sizes and of types of their own (fp32
+    accumulators into bf16 gradients), each grads[i] itself or one that overlaps none of the call; None:
+    in place."""
+    grads, max_norm = list(grads), float(max_norm)
+    if not grads:
+        raise ValueError("clip_grads: at least one tensor expected")
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
+    ptrs, sizes, kinds, dev = _grad_table("clip_grads", grads)
+    to, to_kinds = ptrs, kinds
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"clip_grads: {len(out)} outputs for {len(grads)} tensors")
+        to, to_sizes, to_kinds, to_dev = _grad_table("clip_grads", out)
+        if to_dev != dev:
+            raise ValueError("clip_grads: the tensors are on different devices")
+        if any(a.shape != b.shape for a, b in zip(grads, out)):
+            raise ValueError("clip_grads: outputs and gradients differ in shape")
+    _no_backward("clip_grads", *grads, *(out or ()))
+    # a tensor that is written twice, or read as one gradient and written as another, would race
+    live = [i for i, n in enumerate(sizes) if n]
+    if len({to[i] for i in live}) != len(live):
+        raise ValueError("clip_grads: a tensor is written twice")
+    if out is not None:
+        where = {ptrs[i]: i for i in live}
+        for i in live:
+            j = where.get(to[i])
+            if j is not None and (ptrs[i] != to[i] or kinds[i] != to_kinds[i]):
+                raise ValueError("clip_grads: an output is another gradient, or of another type in place")
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = _workspace(query("plz_grad_norm_workspace", sizes, len(grads)), norm.device)
+    _on(dev, "plz_clip_grads", ptrs, sizes, kinds, to, to_kinds, len(grads), max_norm, _ptr(norm),
+        _ptr(ws), ws.numel())
+    return norm
+
+
 # ---- attention ---------------------------------------------------------------------------------
 def attn_fwd(q, k, v, scale=None):
     """Causal grouped-query attention. q [B, S, Hq, 128], k/v [B, S, Hkv, 128] bf16 ->

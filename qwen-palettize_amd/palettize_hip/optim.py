@@ -9,8 +9,25 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import PLZ_DT_BF16, PLZ_DT_FP32, PLZ_W_HARD_NOISY, call, query
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """torch.nn.utils.clip_grad_norm_ (the 2-norm) for parameters of one device whose gradients are bf16,
+    fp16 or fp32, as train_qwen.py:1303-1319 calls it for each of its tiers before an optimizer other
+    than FusedAdamW, which clips by itself: scales the gradients in place and returns their unclipped
+    norm, fp32 (0 where no parameter has a gradient). A parameter that is given twice counts once."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    live = list({id(p): p for p in parameters if p.grad is not None}.values())
+    if not live:
+        return torch.zeros((), dtype=torch.float32,
+                           device=parameters[0].device if parameters else None)
+    for p in live:
+        if not p.grad.is_contiguous():
+            p.grad = p.grad.contiguous()
+    return ops.clip_grads([p.grad for p in live], max_norm)
 
 
 class NextBuild:

@@ -43,6 +43,7 @@ enum { CE_STATS = 0, CE_GRAD = 1, KL_STATS = 2, KL_GRAD = 3 };
 struct Meta {
   int rows;     // how many take part
   float alpha;  // backward: the scale of the gradients that every row shares
+  int z;        // backward: splits of dx's reduction over the words of a piece
 };
 struct PackArgs {
   const void* key;  // labels or mask
@@ -63,7 +64,29 @@ struct PackArgs {
   int reduction;  // PLZ_REDUCE_*
   float* g;       // [Np], reduction none
   float inv_t;
+  int64_t words, z_floats;  // of a piece, and of dx's parts: 0 without dx
+  int cus;
 };
+
+// Splits of dx's reduction over the words of a piece for `rows` rows: whole waves of workgroups at 1.9
+// us a stage and 4 stages of prologue and epilogue, 8 bytes an element and split written and read at
+// 5 TB/s; at least 8 stages a split, and no more parts than `floats` hold.
+__host__ __device__ inline int dx_splits(int64_t rows, int64_t words, int64_t H, int64_t C, int64_t floats) {
+  const int64_t tiles = (rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE);
+  const float part = 8.f * (float)rows * (float)H / 5.0e6f;
+  int best = 1;
+  float best_t = INFINITY;
+  for (int z = 1; z <= 64; ++z) {
+    const int len = (int)(((words + z - 1) / z + BK - 1) / BK);
+    if (z > 1 && (len < 8 || z * rows * H > floats)) break;
+    const float t = (float)((tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
+    if (t < best_t * 0.97f) {
+      best_t = t;
+      best = z;
+    }
+  }
+  return best;
+}
 
 __device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
   switch (a.kind) {
@@ -125,6 +148,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
       if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
       if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
       a.meta->alpha = alpha;
+      if (a.z_floats) a.meta->z = dx_splits(rows, a.words, a.H[0], a.cus, a.z_floats);
       red[0] = rows;
     }
   }
@@ -133,12 +157,12 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
     if (!a.x[k]) continue;
     const int64_t H = a.H[k];
     const int c8 = (int)(H / 8);
-    for (int i = 0; i < n; ++i) {
-      const int p = at[i];
-      if (p < 0) continue;
-      const uint4* s = reinterpret_cast<const uint4*>(a.x[k] + (r0 + i) * H);
-      uint4* d = reinterpret_cast<uint4*>(a.xp[k] + (int64_t)p * H);
-      for (int c = threadIdx.x; c < c8; c += 256) d[c] = s[c];
+    const uint4* from = reinterpret_cast<const uint4*>(a.x[k] + r0 * H);
+    uint4* to = reinterpret_cast<uint4*>(a.xp[k]);
+#pragma unroll 4
+    for (int j = threadIdx.x; j < n * c8; j += 256) {
+      const int i = j / c8, p = at[i];
+      if (p >= 0) to[(int64_t)p * c8 + (j - i * c8)] = from[j];
     }
     if (r0 + n == a.N) {
       const int rows = red[0], end = (rows + BK - 1) / BK * BK;
@@ -242,20 +266,27 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
     tile_coords(4, tiles_i, tiles_j, (int)item, tile_i, tile_j);
     const int64_t i0 = a.v0 + (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
     f32x16 acc[WT_I][WT_J];
-    float4* slot = KL ? reinterpret_cast<float4*>(a.park) + (int64_t)blockIdx.x * (TILE * TILE / 4) : nullptr;
-    if constexpr (KL) {
-      logits_tile(lbase, a.w[1], a.x[1], a.H[1], i0, a.v1, j0, acc, wi, wj, lane);
+    // where the teacher's logits wait, in the accumulators' order: four of a thread 16 bytes apart from
+    // the next thread's, addressed by constants (one address register for all of them)
+    const BufRsrc slot = make_rsrc(KL ? a.park + (int64_t)blockIdx.x * (TILE * TILE) : nullptr,
+                                   TILE * TILE * 4);
+    // one body for both sides: two would keep both sides' copy offsets in registers
+#pragma unroll 1
+    for (int side = KL ? 1 : 0; side >= 0; --side) {
+      logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
+      if (side == 0) break;
 #pragma unroll
       for (int ti = 0; ti < WT_I; ++ti)
 #pragma unroll
         for (int tj = 0; tj < WT_J; ++tj)
 #pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4)
-            slot[((ti * WT_J + tj) * 4 + e4) * NTHR + threadIdx.x] =
-                make_float4(acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
-                            acc[ti][tj][4 * e4 + 3]);
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const f32x4 v = {acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
+                             acc[ti][tj][4 * e4 + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), slot, threadIdx.x * 16,
+                                                   ((ti * WT_J + tj) * 4 + e4) * NTHR * 16, 0);
+          }
     }
-    logits_tile(lbase, a.w[0], a.x[0], a.H[0], i0, a.v1, j0, acc, wi, wj, lane);
 
     // This lane's word of block ti and register e is vl + 32 ti + 8 (e / 4) + e % 4, from the tile's
     // first one; of the tile's words, nw exist.
@@ -271,7 +302,9 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         f32x16 z;
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
-          const float4 v = slot[((ti * WT_J + tj) * 4 + e4) * NTHR + threadIdx.x];
+          const f32x4 v = __builtin_bit_cast(
+              f32x4, __builtin_amdgcn_raw_buffer_load_b128(slot, threadIdx.x * 16,
+                                                           ((ti * WT_J + tj) * 4 + e4) * NTHR * 16, 0));
           z[4 * e4] = v.x; z[4 * e4 + 1] = v.y; z[4 * e4 + 2] = v.z; z[4 * e4 + 3] = v.w;
         }
         return z;
@@ -414,8 +447,8 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
 }
 
 // ---- joining the tiles' statistics ------------------------------------------------------------------
-// 256 threads: 1 << rb_log rows, the rest of the threads along the tiles; each joins its tiles in order
-// and the row's first thread all of them, so the order is fixed.
+// 256 threads: 1 << rb_log rows, the rest of the threads along the tiles; each joins its tiles in order,
+// then pairs of threads join theirs, so the order is fixed.
 struct JoinArgs {
   const float* stats;
   const float* zlab;
@@ -444,20 +477,25 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
       if constexpr (KL) s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], v[4 * a.Np]});
     }
   }
-  sh[0][threadIdx.x] = s0.m;
-  sh[1][threadIdx.x] = s0.s;
-  if constexpr (KL) {
-    sh[2][threadIdx.x] = s1.m;
-    sh[3][threadIdx.x] = s1.s;
-    sh[4][threadIdx.x] = s1.c;
+  for (int half = slices / 2; half >= 1; half >>= 1) {
+    if (sl >= half && sl < 2 * half) {
+      sh[0][threadIdx.x] = s0.m;
+      sh[1][threadIdx.x] = s0.s;
+      if constexpr (KL) {
+        sh[2][threadIdx.x] = s1.m;
+        sh[3][threadIdx.x] = s1.s;
+        sh[4][threadIdx.x] = s1.c;
+      }
+    }
+    __syncthreads();
+    if (sl < half) {
+      const int i = threadIdx.x + half * RB;
+      s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
+      if constexpr (KL) s1 = join(s1, Stat{sh[2][i], sh[3][i], sh[4][i]});
+    }
+    // (the next round writes the lower half of what this one read)
   }
-  __syncthreads();
   if (!live || sl != 0) return;
-  for (int k = 1; k < slices; ++k) {
-    const int i = k * RB + rl;
-    s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
-    if constexpr (KL) s1 = join(s1, Stat{sh[2][i], sh[3][i], sh[4][i]});
-  }
   const int64_t r = a.src[p];
   a.lse[0][r] = (float)((double)s0.m + log((double)s0.s));
   if constexpr (KL) {
@@ -551,25 +589,27 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
 struct DxArgs {
   const uint16_t* dzt;
   const uint16_t* w;
-  int64_t Np, H, words, split;
+  int64_t Np, H, words;
   const Meta* meta;
-  float* part;  // [z][Np][H]
-  int z, add;   // add: to what earlier pieces left
+  float* part;  // [z][rows][H]
+  int add;      // to what earlier pieces left
 };
 __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
-  const int rows = a.meta->rows;
-  const int tiles_i = (rows + TILE - 1) / TILE, tiles_j = (int)((a.H + TILE - 1) / TILE);
-  const int T = tiles_i * tiles_j;
-  if ((int64_t)blockIdx.x >= (int64_t)T * a.z) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave / WAVES_J, wj = wave % WAVES_J;
-  const Item item = map_item(T, false, 0, 1, (int)blockIdx.x, 0, a.z);
+  const int rows = a.meta->rows, z = a.meta->z;
+  const int tiles_i = (rows + TILE - 1) / TILE, tiles_j = (int)((a.H + TILE - 1) / TILE);
+  const int T = tiles_i * tiles_j;
+  if ((int64_t)blockIdx.x >= (int64_t)T * z) return;  // the launch is for as many as there may be
+  const int64_t split = ((a.words + z - 1) / z + BK - 1) / BK * BK;
+  const Item item = map_item(T, false, 0, 1, (int)blockIdx.x % T, (int)blockIdx.x / T, z);
+  const int zsl = item.zsl;
   int tile_i, tile_j;
   tile_coords(4, tiles_i, tiles_j, item.bid, tile_i, tile_j);
   const int64_t i0 = (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
-  const int64_t rbeg = (int64_t)item.zsl * a.split, rend = min(a.words, rbeg + a.split);
+  const int64_t rbeg = (int64_t)zsl * split, rend = min(a.words, rbeg + split);
   f32x16 acc[WT_I][WT_J];
 #pragma unroll
   for (int i = 0; i < WT_I; ++i)
@@ -593,38 +633,48 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
     __syncthreads();
     mma_stage_sync<true, true>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane,
                                (int)((len % BK + 15) / 16));
+    __syncthreads();
   }
-  float* part = a.part + (int64_t)item.zsl * a.Np * a.H;
+  // from the tile's first row: a lane's address and a uniform one of its register's row
+  const int nr = min(rows - (int)i0, TILE);
+  const BufRsrc part = make_rsrc(a.part + ((int64_t)zsl * rows + i0) * a.H, (uint32_t)(nr * a.H * 4));
+  const int r0 = wi * (32 * WT_I) + 4 * (lane >> 5);
 #pragma unroll
-  for (int ti = 0; ti < WT_I; ++ti)
+  for (int tj = 0; tj < WT_J; ++tj) {
+    const int64_t h = j0 + wj * (32 * WT_J) + 32 * tj + (lane & 31);
+    if (h >= a.H) continue;
+    const uint32_t off = (uint32_t)((r0 * a.H + h) * 4);
 #pragma unroll
-    for (int tj = 0; tj < WT_J; ++tj) {
-      const int64_t h = j0 + wj * (32 * WT_J) + 32 * tj + (lane & 31);
-      if (h >= a.H) continue;
+    for (int ti = 0; ti < WT_I; ++ti)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int64_t n = i0 + wi * (32 * WT_I) + 32 * ti + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        if (n >= rows) continue;
-        float* d = part + n * a.H + h;
-        *d = a.add ? *d + acc[ti][tj][e] : acc[ti][tj][e];
+        const int row = 32 * ti + 8 * (e >> 2) + (e & 3);
+        const uint32_t at = (uint32_t)(row * a.H * 4);
+        if (r0 + row >= nr) continue;
+        float v = acc[ti][tj][e];
+        if (a.add)
+          v += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part, off, at, 0));
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), part, off, at, 0);
       }
-    }
+  }
 }
 
 // grad_x of every row: alpha times the sum of its parts, or nothing
-__global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ part, int z,
+__global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ part,
                                                      const int32_t* __restrict__ pos,
-                                                     const Meta* __restrict__ meta, int64_t Np,
-                                                     int64_t N, int64_t H,
-                                                     uint16_t* __restrict__ out) {
+                                                     const Meta* __restrict__ meta, int64_t N,
+                                                     int64_t H, uint16_t* __restrict__ out) {
   const int64_t c8 = H / 8, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= N * c8) return;
   const int64_t r = t / c8, c = t % c8;
   const int p = pos[r];
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (p >= 0) {
+    const int z = meta->z;
+    const int64_t rows = meta->rows;
+#pragma unroll 4
     for (int k = 0; k < z; ++k) {
-      const float4* v = reinterpret_cast<const float4*>(part + ((int64_t)k * Np + p) * H + c * 8);
+      const float4* v = reinterpret_cast<const float4*>(part + (k * rows + p) * H + c * 8);
       const float4 v0 = v[0], v1 = v[1];
       s[0] += v0.x; s[1] += v0.y; s[2] += v0.z; s[3] += v0.w;
       s[4] += v1.x; s[5] += v1.y; s[6] += v1.z; s[7] += v1.w;
@@ -651,30 +701,18 @@ static int cu_count() {
 }
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Words of a piece: dz^T of all rows in kPieceBytes, a whole number of tiles, and W's rows of it within
-// the 4 GiB that the copies of dx address.
+// Words of a piece: dz^T of all rows in kPieceBytes and W's rows of it within the 4 GiB that the copies
+// of dx address, the pieces of one size but for the last tiles.
 static int64_t piece_words(int64_t N, int64_t V, int64_t H) {
-  int64_t w = (int64_t)(kPieceBytes / 2) / up(N, TILE);
-  w = std::min(w, (((int64_t)1 << 31) - 1) / H);
-  return std::min(std::max(w / TILE, (int64_t)1) * TILE, up(V, TILE));
+  const int64_t tiles = up(V, TILE) / TILE;
+  int64_t most = std::min((int64_t)(kPieceBytes / 2) / up(N, TILE), (((int64_t)1 << 31) - 1) / H) / TILE;
+  most = std::max(most, (int64_t)1);
+  const int64_t pieces = (tiles + most - 1) / most;
+  return (tiles + pieces - 1) / pieces * TILE;
 }
-// Splits of dx's reduction over the words of a piece: whole waves of workgroups at 1.9 us a stage and
-// 4 stages of prologue and epilogue, 8 bytes an element and split written and read at 5 TB/s.
-static int dx_splits(int64_t N, int64_t words, int64_t H) {
-  const int64_t tiles = up(N, TILE) / TILE * (up(H, TILE) / TILE), C = cu_count();
-  int best = 1;
-  double best_t = 1e300;
-  for (int z = 1; z <= 64; ++z) {
-    const int64_t len = split_len(words, z);
-    if (z > 1 && (len < 8 * BK || (int64_t)(z - 1) * len >= words)) break;
-    const double t = (double)((tiles * z + C - 1) / C) * ((double)len / BK + 4.0) * 1.9 +
-                     z * 8.0 * (double)N * (double)H / 5.0e6;
-    if (t < best_t * 0.97) {
-      best_t = t;
-      best = z;
-    }
-  }
-  return best;
+// Floats of dx's parts: the splits that all rows would take
+static int64_t part_floats(int64_t N, int64_t words, int64_t H) {
+  return (int64_t)dx_splits(N, words, H, cu_count(), INT64_MAX) * N * H;
 }
 
 // The workspace, carved in order; p = NULL: sizes only.
@@ -721,7 +759,7 @@ static Ws carve(Carve& c, bool bwd, int64_t N, int64_t V, int64_t H, int64_t Ht,
   for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
   w.g = c.take<float>(Np);
   w.dzt = c.take<uint16_t>((size_t)words * Np);
-  if (grad_x) w.part = c.take<float>((size_t)dx_splits(N, words, H) * Np * H);
+  if (grad_x) w.part = c.take<float>((size_t)part_floats(N, words, H));
   return w;
 }
 
@@ -860,6 +898,11 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   p.grad = grad;
   p.reduction = reduction;
   if (reduction == PLZ_REDUCE_NONE) p.g = w.g;
+  if (grad_x) {
+    p.words = words;
+    p.z_floats = part_floats(s.N, words, s.H);
+    p.cus = cu_count();
+  }
   for (int k = 0; k < (KL ? 2 : 1); ++k) {
     p.lse_in[k] = lse + k * s.N;
     p.lse[k] = w.lse[k];
@@ -868,7 +911,6 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   static uint64_t done_w = 0, done_x = 0;
   if (int rc = reserve_lds((const void*)dw_kernel, kLdsLogits, done_w, what)) return rc;
   if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
-  const int z = grad_x ? dx_splits(s.N, words, s.H) : 0;
   const int64_t tiles_h = up(s.H, TILE) / TILE;
   LogitArgs l = logit_args(s, w);
   l.g = p.g;
@@ -884,15 +926,16 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
       if (int rc = check_launch(what)) return rc;
     }
     if (grad_x) {
-      const DxArgs d = {w.dzt, s.w + v0 * s.H, Np, s.H, n, split_len(words, z), w.meta, w.part, z, v0 > 0};
-      hipLaunchKernelGGL(dx_kernel, dim3((unsigned)(Np / TILE * tiles_h * z)), dim3(NTHR), kLdsRing,
-                         st, d);
+      const DxArgs d = {w.dzt, s.w + v0 * s.H, Np, s.H, n, w.meta, w.part, v0 > 0};
+      // at most z tiles of rows: z rows H <= the parts' floats, and 64 splits of a tile that is not full
+      const int64_t items = (p.z_floats / s.H / TILE + 64) * tiles_h;
+      hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
       if (int rc = check_launch(what)) return rc;
     }
   }
   if (grad_x) {
     hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)((s.N * (s.H / 8) + 255) / 256)), dim3(256), 0,
-                       st, w.part, z, w.pos, w.meta, Np, s.N, s.H, grad_x);
+                       st, w.part, w.pos, w.meta, s.N, s.H, grad_x);
     return check_launch(what);
   }
   return PLZ_OK;

@@ -724,12 +724,26 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
  * The backward takes grad fp32: [N] of every row's loss (PLZ_REDUCE_NONE), or [1] of the sum
  * (PLZ_REDUCE_SUM) or of the mean (PLZ_REDUCE_MEAN). grad_x bf16 [N, H] and grad_w bf16 [V, H]; NULL:
  * not wanted. The gradient of the logits is rounded to bf16 before its products with x and w. The
- * teacher has no gradient. H_teacher = 0 in the workspace queries: cross entropy. */
+ * teacher has no gradient. H_teacher = 0 in the workspace queries: cross entropy.
+ * A step is the forward with the gradients of the sum or mean (reduction) for an upstream gradient of
+ * 1: it keeps what the gradients of the logits are made of for the length of the call (2 bytes a logit,
+ * a distillation 10) instead of computing the logits twice. Its workspace query returns 0 where N V
+ * logits are more than it keeps, or N = 0: forward and backward do those. */
 size_t plz_vocab_loss_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher);
 size_t plz_vocab_loss_bwd_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x);
 int plz_linear_ce_fwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
                       int64_t ignore_index, float* loss, float* lse, float* total, void* workspace,
                       size_t workspace_bytes, int64_t N, int64_t V, int64_t H, void* stream);
+size_t plz_vocab_loss_step_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x);
+int plz_linear_ce_step(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                       int64_t ignore_index, int reduction, float* loss, float* lse, float* total,
+                       uint16_t* grad_x, uint16_t* grad_w, void* workspace, size_t workspace_bytes,
+                       int64_t N, int64_t V, int64_t H, void* stream);
+int plz_linear_kl_step(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                       const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                       int reduction, float* loss, float* lse, float* total, uint16_t* grad_x,
+                       uint16_t* grad_w, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
+                       int64_t H, int64_t H_teacher, void* stream);
 int plz_linear_ce_bwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
                       int64_t ignore_index, const float* lse, const float* grad, int reduction,
                       uint16_t* grad_x, uint16_t* grad_w, void* workspace, size_t workspace_bytes,
@@ -758,6 +772,9 @@ int plz_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t*
 int plz_clip_grads(const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
                    void* const* out, const int32_t* out_dtypes, int count, float max_norm,
                    float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+/* grads[i] *= *factor in place (factor fp32 on the device; nothing is read or written where it is 1) */
+int plz_scale_grads(void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count,
+                    const float* factor, void* stream);
 
 /* ---- decoding over a paged key-value cache ------------------------------------------- */
 /* A cache is a pool of num_pages pages of page_size tokens (a power of two, 16..1024); one layer's

@@ -280,6 +280,28 @@ static int norm(const void* const* in, const int64_t* n, const int32_t* type, in
   return check_launch(what);
 }
 
+// out[i] = in[i] * *factor: launches from the last tensors to the first, as the workgroups within each
+static int scale_all(const void* const* in, void* const* out, const int64_t* sizes,
+                     const int32_t* in_type, const int32_t* out_type, int count, const float* factor,
+                     hipStream_t st, const char* what) {
+  Tensors t;
+  for (int hi = count; hi > 0;) {
+    int lo = hi, taken = 0;
+    int64_t blocks = 0;
+    while (lo > 0 && taken < kTensors && blocks + chunks(sizes[lo - 1]) <= kMaxBlocks) {
+      blocks += chunks(sizes[--lo]);
+      taken += sizes[lo] > 0;
+    }
+    fill(t, in, out, sizes, in_type, out_type, lo, hi);
+    hi = lo;
+    if (t.count == 0) continue;
+    hipLaunchKernelGGL(clip_kernel, dim3((unsigned)t.begin[t.count]), dim3(kThreads), 0,
+                       st, t, factor);
+    if (int rc = check_launch(what)) return rc;
+  }
+  return PLZ_OK;
+}
+
 }  // namespace gn
 }  // namespace plz
 
@@ -314,23 +336,17 @@ int plz_clip_grads(const void* const* grads, const int64_t* sizes, const int32_t
   if (int rc = norm(grads, sizes, dtypes, count, max_norm, norm_out, true, workspace, workspace_bytes,
                     (hipStream_t)stream, what))
     return rc;
-  // launches from the last tensors to the first, as the workgroups within each
-  Tensors t;
-  for (int hi = count; hi > 0;) {
-    int lo = hi, taken = 0;
-    int64_t blocks = 0;
-    while (lo > 0 && taken < kTensors && blocks + chunks(sizes[lo - 1]) <= kMaxBlocks) {
-      blocks += chunks(sizes[--lo]);
-      taken += sizes[lo] > 0;
-    }
-    fill(t, grads, out, sizes, dtypes, out_dtypes, lo, hi);
-    hi = lo;
-    if (t.count == 0) continue;
-    hipLaunchKernelGGL(clip_kernel, dim3((unsigned)t.begin[t.count]), dim3(kThreads), 0,
-                       (hipStream_t)stream, t, reinterpret_cast<const float*>(workspace));
-    if (int rc = check_launch(what)) return rc;
-  }
-  return PLZ_OK;
+  return scale_all(grads, out, sizes, dtypes, out_dtypes, count, reinterpret_cast<const float*>(workspace),
+                   (hipStream_t)stream, what);
+}
+
+int plz_scale_grads(void* const* grads, const int64_t* sizes, const int32_t* dtypes, int count,
+                    const float* factor, void* stream) {
+  const char* what = "plz_scale_grads";
+  const void* const* in = reinterpret_cast<const void* const*>(grads);
+  if (int rc = check(in, sizes, dtypes, count, what)) return rc;
+  PLZ_REQUIRE(factor, "%s: null pointer", what);
+  return scale_all(in, grads, sizes, dtypes, dtypes, count, factor, (hipStream_t)stream, what);
 }
 
 }  // extern "C"

@@ -32,12 +32,15 @@ using namespace g2;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kPieceBytes = (size_t)1 << 30;
+constexpr size_t kKeepBytes = (size_t)8 << 30;
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
 constexpr int kPackRows = 16;
 
 enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
-enum { CE_STATS = 0, CE_GRAD = 1, KL_STATS = 2, KL_GRAD = 3 };
+// What a launch over tiles of logits leaves: their statistics, the gradients of the logits, or the
+// statistics and what the gradients are made of once the normalisers are known
+enum { CE_STATS, CE_GRAD, KL_STATS, KL_GRAD, CE_KEEP, KL_KEEP };
 
 // ---- rows that take part --------------------------------------------------------------------------
 struct Meta {
@@ -187,8 +190,11 @@ struct LogitArgs {
   float inv_t;
   float* stats;  // [tile of words][2 or 5][Np]
   float* zlab;   // [Np]
-  uint16_t* dzt;  // [words of the piece in whole tiles][Np]
-  float* park;    // [workgroup][256 * 256]
+  // [tile of rows][word of the piece, whole tiles][256 rows]: dz, or the exponentials kept for it
+  uint16_t* dzt;
+  int64_t words;  // of a piece, whole tiles
+  float* park;    // the teacher's logits: [workgroup][256 * 256], kept: [tile][256 * 256]
+  float* kept;    // the student's, [tile][256 * 256]
 };
 
 // exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
@@ -213,6 +219,29 @@ __device__ __forceinline__ Stat join_halves(const Stat& a) {
   const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.c), __float_as_uint(a.c), false, false);
   return join(Stat{__uint_as_float(m[0]), __uint_as_float(s[0]), __uint_as_float(c[0])},
               Stat{__uint_as_float(m[1]), __uint_as_float(s[1]), __uint_as_float(c[1])});
+}
+
+// over lanes l and l ^ 32
+__device__ __forceinline__ float swap32_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap32_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 16 bytes to a uniform address and a lane's 32-bit offset. Not a buffer store: behind one whose scalar
+// offset is a register, gfx950 still reads the data while the next instruction may write it again, and
+// the compiler leaves no gap (values of the last lanes of every 16 were those of the next block). The
+// empty asm statement keeps the address in scalar registers: folded with the lanes' offsets, 32 stores
+// would take 32 pairs of vector registers.
+__device__ __forceinline__ void store16(void* base, uint32_t off, u32x4 v) {
+  typedef __attribute__((address_space(1))) char gchar;
+  typedef __attribute__((address_space(1))) u32x4 gu32x4;
+  uint64_t p = reinterpret_cast<uint64_t>(base);
+  asm volatile("" : "+s"(p));
+  *reinterpret_cast<gu32x4*>(reinterpret_cast<gchar*>(p) + off) = v;
 }
 
 typedef __attribute__((address_space(3))) float lds_f32;
@@ -250,8 +279,8 @@ template <int MODE>
 __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
-  constexpr bool KL = MODE == KL_STATS || MODE == KL_GRAD;
-  constexpr bool STATS = MODE == CE_STATS || MODE == KL_STATS;
+  constexpr bool KL = MODE == KL_STATS || MODE == KL_GRAD || MODE == KL_KEEP;
+  constexpr bool STATS = MODE != CE_GRAD && MODE != KL_GRAD;
   constexpr int PLANES = KL ? 5 : 2;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave / WAVES_J, wj = wave % WAVES_J;
@@ -268,8 +297,10 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
     f32x16 acc[WT_I][WT_J];
     // where the teacher's logits wait, in the accumulators' order: four of a thread 16 bytes apart from
     // the next thread's, addressed by constants (one address register for all of them)
-    const BufRsrc slot = make_rsrc(KL ? a.park + (int64_t)blockIdx.x * (TILE * TILE) : nullptr,
-                                   TILE * TILE * 4);
+    const int64_t tile = (int64_t)tile_j * tiles_i + tile_i;
+    float* const parked =
+        KL ? a.park + (MODE == KL_KEEP ? tile : (int64_t)blockIdx.x) * (TILE * TILE) : nullptr;
+    const BufRsrc slot = make_rsrc(parked, TILE * TILE * 4);
     // one body for both sides: two would keep both sides' copy offsets in registers
 #pragma unroll 1
     for (int side = KL ? 1 : 0; side >= 0; --side) {
@@ -283,8 +314,8 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
           for (int e4 = 0; e4 < 4; ++e4) {
             const f32x4 v = {acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
                              acc[ti][tj][4 * e4 + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), slot, threadIdx.x * 16,
-                                                   ((ti * WT_J + tj) * 4 + e4) * NTHR * 16, 0);
+            store16(parked + ((ti * WT_J + tj) * 4 + e4) * NTHR * 4, threadIdx.x * 16,
+                    __builtin_bit_cast(u32x4, v));
           }
     }
 
@@ -325,78 +356,122 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         }
         return mine;
       };
-      if constexpr (STATS) {
-        Stat st[KL ? 2 : 1];
+      // block ti of a row's words without those that do not exist
+      auto only = [&](f32x16& z, int ti) {
+        const int left = nw - vl - 32 * ti;
 #pragma unroll
-        for (int k = 0; k < (KL ? 2 : 1); ++k) st[k] = Stat{-INFINITY, 0.f, 0.f};
-        if constexpr (!KL) {
-          if (live && holds(a.lab[n] - (int)i0)) a.zlab[n] = zl;
-        }
+        for (int e = 0; e < 16; ++e) z[e] = 8 * (e >> 2) + (e & 3) < left ? z[e] : -INFINITY;
+      };
+      auto top = [](const f32x16& v, float m) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, v[e]);
+        return m;
+      };
+      if constexpr (STATS && KL) {
+        Stat st[2] = {Stat{-INFINITY, 0.f, 0.f}, Stat{-INFINITY, 0.f, 0.f}};
 #pragma unroll
         for (int ti = 0; ti < WT_I; ++ti) {
-          f32x16 z = acc[ti][tj], t = {};
-          if constexpr (KL) {
-            z *= a.inv_t;
-            t = teacher(ti) * a.inv_t;
-          }
-          if (nw < TILE) {
-            const int left = nw - vl - 32 * ti;
+          if constexpr (MODE == KL_KEEP) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              z[e] = 8 * (e >> 2) + (e & 3) < left ? z[e] : -INFINITY;
-              if constexpr (KL) t[e] = 8 * (e >> 2) + (e & 3) < left ? t[e] : -INFINITY;
+            for (int e4 = 0; e4 < 4; ++e4) {
+              const f32x4 v = {acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
+                               acc[ti][tj][4 * e4 + 3]};
+              store16(a.kept + tile * (TILE * TILE) + ((ti * WT_J + tj) * 4 + e4) * NTHR * 4,
+                      threadIdx.x * 16, __builtin_bit_cast(u32x4, v));
             }
           }
-          auto top = [](const f32x16& v) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m = fmaxf(m, v[e]);
-            return m;
-          };
-          Stat b{top(z), 0.f, 0.f};
+          f32x16 z = acc[ti][tj] * a.inv_t, t = teacher(ti) * a.inv_t;
+          if (nw < TILE) {
+            only(z, ti);
+            only(t, ti);
+          }
+          Stat b{top(z, -INFINITY), 0.f, 0.f};
           const float m0 = b.m == -INFINITY ? 0.f : b.m;
 #pragma unroll
           for (int e = 0; e < 16; ++e) b.s += exp_of(z[e] - m0);
           st[0] = join(st[0], b);
-          if constexpr (KL) {
-            b = Stat{top(t), 0.f, 0.f};
-            const float m1 = b.m == -INFINITY ? 0.f : b.m;
+          b = Stat{top(t, -INFINITY), 0.f, 0.f};
+          const float m1 = b.m == -INFINITY ? 0.f : b.m;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p = exp_of(t[e] - m1);
-              b.s += p;
-              // a word without weight counts for nothing, however far the two sides are
-              b.c += p == 0.f ? 0.f : p * (t[e] - z[e]);
-            }
-            st[1] = join(st[1], b);
+          for (int e = 0; e < 16; ++e) {
+            const float p = exp_of(t[e] - m1);
+            b.s += p;
+            // a word without weight counts for nothing, however far the two sides are
+            b.c += p == 0.f ? 0.f : p * (t[e] - z[e]);
           }
+          st[1] = join(st[1], b);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int k = 0; k < (KL ? 2 : 1); ++k) st[k] = join_halves(st[k]);
+        for (int k = 0; k < 2; ++k) st[k] = join_halves(st[k]);
         // the two waves of a column of the tile meet in LDS, behind the stages' slots
         lds_f32* ex = reinterpret_cast<lds_f32*>(lbase + 4 * TILE_BYTES) + wj * 256;
         if (wi == 1 && lane < 32) {
           ex[lane] = st[0].m;
           ex[32 + lane] = st[0].s;
-          if constexpr (KL) {
-            ex[64 + lane] = st[1].m;
-            ex[96 + lane] = st[1].s;
-            ex[128 + lane] = st[1].c;
-          }
+          ex[64 + lane] = st[1].m;
+          ex[96 + lane] = st[1].s;
+          ex[128 + lane] = st[1].c;
         }
         __syncthreads();
         if (wi == 0 && lane < 32 && live) {
           float* out = a.stats + (i0 / TILE) * PLANES * a.Np + n;
           const Stat s0 = join(st[0], Stat{ex[lane], ex[32 + lane], 0.f});
+          const Stat s1 = join(st[1], Stat{ex[64 + lane], ex[96 + lane], ex[128 + lane]});
           out[0] = s0.m;
           out[a.Np] = s0.s;
-          if constexpr (KL) {
-            const Stat s1 = join(st[1], Stat{ex[64 + lane], ex[96 + lane], ex[128 + lane]});
-            out[2 * a.Np] = s1.m;
-            out[3 * a.Np] = s1.s;
-            out[4 * a.Np] = s1.c;
+          out[2 * a.Np] = s1.m;
+          out[3 * a.Np] = s1.s;
+          out[4 * a.Np] = s1.c;
+        }
+        __syncthreads();
+      } else if constexpr (STATS) {
+        if (live && holds(a.lab[n] - (int)i0)) a.zlab[n] = zl;
+        if (nw < TILE) {
+#pragma unroll
+          for (int ti = 0; ti < WT_I; ++ti) only(acc[ti][tj], ti);
+        }
+        // the tile's maximum: of the lane, of both halves, of both waves of the column
+        float m = -INFINITY;
+#pragma unroll
+        for (int ti = 0; ti < WT_I; ++ti) m = top(acc[ti][tj], m);
+        m = swap32_max(m);
+        lds_f32* ex = reinterpret_cast<lds_f32*>(lbase + 4 * TILE_BYTES) + wj * 256;
+        ex[wi * 32 + (lane & 31)] = m;
+        __syncthreads();
+        m = fmaxf(ex[lane & 31], ex[32 + (lane & 31)]);
+        const float m0 = m == -INFINITY ? 0.f : m;
+        uint16_t* const kept =
+            MODE == CE_KEEP ? a.dzt + ((int64_t)tile_j * a.words + (i0 - a.v0)) * TILE : nullptr;
+        float sum = 0.f;
+#pragma unroll
+        for (int ti = 0; ti < WT_I; ++ti) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              p[e] = exp_of(acc[ti][tj][8 * h + e] - m0);
+              sum += p[e];
+            }
+            if constexpr (MODE == CE_KEEP) {
+              // relative to the tile's maximum, fp16: off by 2^-12, an eighth of a step of the bf16
+              // that dz is rounded to, or by 2^-25 of that maximum
+              u32x4 v;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);
+              store16(kept + ti * 8192 + tj * 1024 + h * 512, wi * 65536 + wj * 4096 + lane * 16, v);
+            }
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        sum = swap32_sum(sum);
+        if (wi == 1 && lane < 32) ex[64 + lane] = sum;
+        __syncthreads();
+        if (wi == 0 && lane < 32 && live) {
+          float* out = a.stats + (i0 / TILE) * PLANES * a.Np + n;
+          out[0] = m;
+          out[a.Np] = sum + ex[64 + lane];
         }
         __syncthreads();
       } else {
@@ -432,14 +507,14 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
     }
     if constexpr (!STATS) {
       __syncthreads();
-      uint16_t* out = a.dzt + (i0 - a.v0) * a.Np + j0;
+      uint16_t* out = a.dzt + ((int64_t)tile_j * a.words + (i0 - a.v0)) * TILE;
 #pragma unroll 4
       for (int it = 0; it < TILE * TILE / 8 / NTHR; ++it) {
         const int ch = it * NTHR + threadIdx.x;
         const int row = ch >> 5, c8 = (ch & 31) * 8;
         u32x4 v = *reinterpret_cast<const lds_u32x4*>(lbase + row * EPI_RS + c8 * 2);
         if (row >= nw) v = u32x4{0, 0, 0, 0};
-        *reinterpret_cast<u32x4*>(out + row * a.Np + c8) = v;
+        *reinterpret_cast<u32x4*>(out + row * TILE + c8) = v;
       }
       __syncthreads();
     }
@@ -459,6 +534,7 @@ struct JoinArgs {
   int tiles, rb_log;
   float* loss;    // [N]
   float* lse[2];  // [N]
+  float* lsep[2];  // [Np], of the packed rows (or NULL)
 };
 template <bool KL>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
@@ -497,9 +573,13 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   }
   if (!live || sl != 0) return;
   const int64_t r = a.src[p];
-  a.lse[0][r] = (float)((double)s0.m + log((double)s0.s));
+  const float lse = (float)((double)s0.m + log((double)s0.s));
+  a.lse[0][r] = lse;
+  if (a.lsep[0]) a.lsep[0][p] = lse;
   if constexpr (KL) {
-    a.lse[1][r] = (float)((double)s1.m + log((double)s1.s));
+    const float lt = (float)((double)s1.m + log((double)s1.s));
+    a.lse[1][r] = lt;
+    if (a.lsep[1]) a.lsep[1][p] = lt;
     // sum p (z_t - z_s) - (lse_t - lse_s), the normalisers' difference from the maxima's and the
     // sums' quotient: as a difference of two rounded normalisers it would lose their common part
     a.loss[r] = (float)((double)s1.c / s1.s - ((double)s1.m - s0.m) - log((double)s1.s / s0.s));
@@ -530,9 +610,103 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ l
   }
 }
 
+// ---- dz of tiles that were kept ----------------------------------------------------------------------
+// A workgroup takes 32 words x 256 rows (wave column wj the rows 64 wj ..): HBM-bound, 4 (cross entropy,
+// in place) or 10 bytes a logit. The cross entropy's block of exponentials lies where its dz goes, and
+// is in registers before any of that is written.
+struct FinishArgs {
+  uint16_t* dzt;
+  int64_t words, V, Np;
+  const Meta* meta;
+  const int32_t* lab;
+  const float* stats;
+  const float* zlab;
+  const float* lse[2];  // [Np]
+  float inv_t;
+  const float* park;
+  const float* kept;
+};
+template <bool KL>
+__global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
+  __shared__ __align__(16) uint8_t st[32 * EPI_RS];
+  const int lane = threadIdx.x & 63, wj = threadIdx.x >> 6;
+  const int tiles_i = (int)(a.words / TILE), block = (int)blockIdx.x % 8;
+  const int64_t tile = (int64_t)blockIdx.x / 8;
+  const int tile_j = (int)(tile / tiles_i), tile_i = (int)(tile % tiles_i);
+  const int rows = a.meta->rows;
+  if (tile_j * TILE >= rows) return;
+  const int wi = block >> 2, ti = block & 3;
+  uint8_t* at = reinterpret_cast<uint8_t*>(a.dzt + ((int64_t)tile_j * a.words + tile_i * TILE) * TILE) +
+                block * 16384;
+  const int v0 = tile_i * TILE + block * 32;  // the block's first word
+  uint4 raw[KL ? 1 : WT_J][2];
+  if constexpr (!KL) {
+#pragma unroll
+    for (int tj = 0; tj < WT_J; ++tj)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        raw[tj][h] = *reinterpret_cast<const uint4*>(at + wj * 4096 + tj * 2048 + h * 1024 + lane * 16);
+  }
+#pragma unroll
+  for (int tj = 0; tj < WT_J; ++tj) {
+    const int nl = wj * 64 + 32 * tj + (lane & 31), n = tile_j * TILE + nl;
+    const bool live = n < rows;
+    const float lse = live ? a.lse[0][n] : 0.f;
+    float d[16];
+    if constexpr (KL) {
+      const float lt = live ? a.lse[1][n] : 0.f;
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int64_t o = tile * (TILE * TILE / 4) + ((ti * WT_J + tj) * 4 + e4) * NTHR +
+                          (wi * WAVES_J + wj) * 64 + lane;
+        const float4 z = reinterpret_cast<const float4*>(a.kept)[o];
+        const float4 t = reinterpret_cast<const float4*>(a.park)[o];
+        d[4 * e4] = exp_of(z.x * a.inv_t - lse) - exp_of(t.x * a.inv_t - lt);
+        d[4 * e4 + 1] = exp_of(z.y * a.inv_t - lse) - exp_of(t.y * a.inv_t - lt);
+        d[4 * e4 + 2] = exp_of(z.z * a.inv_t - lse) - exp_of(t.z * a.inv_t - lt);
+        d[4 * e4 + 3] = exp_of(z.w * a.inv_t - lse) - exp_of(t.w * a.inv_t - lt);
+      }
+    } else {
+      const int l = live ? a.lab[n] : 0;
+      float f = live ? exp_of(a.stats[(int64_t)tile_i * 2 * a.Np + n] - lse) : 0.f;
+      if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w[4] = {raw[tj][h].x, raw[tj][h].y, raw[tj][h].z, raw[tj][h].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d[8 * h + 2 * e] = h2f(w[e] & 0xffffu) * f;
+          d[8 * h + 2 * e + 1] = h2f(w[e] >> 16) * f;
+        }
+      }
+      // the label's word from the logit itself
+      const int lv = l - v0 - 4 * (lane >> 5);
+      if (live && lv >= 0 && lv < 32 && (lv & 4) == 0) {
+        const float dl = exp_of(a.zlab[n] - lse) - 1.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = lv == 8 * (e >> 2) + (e & 3) ? dl : d[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+      *reinterpret_cast<uint16_t*>(st + row * EPI_RS + nl * 2) =
+          (uint16_t)f2bf(live && v0 + row < a.V ? d[e] : 0.f);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int c = it * 256 + threadIdx.x;
+    *reinterpret_cast<uint4*>(at + c * 16) =
+        *reinterpret_cast<const uint4*>(st + (c >> 5) * EPI_RS + (c & 31) * 16);
+  }
+}
+
 // ---- dW of a piece: dz^T [words, rows] x [rows, H] ----------------------------------------------------
 struct DwArgs {
   const uint16_t* dzt;
+  int64_t panel;  // words of dz's panels, whole tiles
   const uint16_t* x;
   int64_t Np, H, words;
   const Meta* meta;
@@ -555,10 +729,13 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
     for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
   // whole stages: the packed rows past the last one are cleared, and so is dz there
   const int nst = (a.meta->rows + BK - 1) / BK;
-  const TileDma dA = row_tile_dma(a.dzt + i0 * a.Np, a.Np, 0, TILE);
+  // (row_tile_dma bounds the copies by its rows: here by all panels)
+  TileDma dA = row_tile_dma(a.dzt + i0 * TILE, TILE, 0, TILE);
+  dA.r = make_rsrc(a.dzt + i0 * TILE, (uint32_t)((a.Np / TILE * a.panel - i0) * TILE * 2));
   const TileDma dB = col_tile_dma(a.x, a.H, j0, a.H, a.Np);
+  const uint32_t panel = (uint32_t)(a.panel * TILE * 2);
   dense_stages<false, true>(lbase, nst, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
-    tile_copy(As, dA, (uint32_t)(kt * BK * 2));
+    tile_copy(As, dA, (uint32_t)(kt / (TILE / BK)) * panel + (uint32_t)(kt % (TILE / BK)) * (BK * 2));
     tile_copy(Bs, dB, (uint32_t)((int64_t)kt * BK * a.H * 2));
   });
   const float alpha = a.meta->alpha;
@@ -588,8 +765,9 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
 // ---- dx of a piece: dz [rows, words] W [words, H], in splits of the words --------------------------------
 struct DxArgs {
   const uint16_t* dzt;
+  int64_t panel;  // words of dz's panels, whole tiles
   const uint16_t* w;
-  int64_t Np, H, words;
+  int64_t H, words;
   const Meta* meta;
   float* part;  // [z][rows][H]
   int add;      // to what earlier pieces left
@@ -617,18 +795,19 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
     for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
   const int64_t len = rend > rbeg ? rend - rbeg : 0;
   const int nfull = (int)(len / BK);
-  const TileDma dA = col_tile_dma(a.dzt, a.Np, i0, a.Np, a.words);
+  const uint16_t* dz = a.dzt + tile_i * a.panel * TILE;
+  const TileDma dA = col_tile_dma(dz, TILE, 0, TILE, a.words);
   const TileDma dB = col_tile_dma(a.w, a.H, j0, a.H, a.words);
   col_stages<true>(lbase, nfull, acc, wi, wj, lane, [&](bool is_a, int kt, lds_u8* dst) {
     const int64_t r0 = rbeg + (int64_t)kt * BK;
-    if (is_a) tile_copy(dst, dA, (uint32_t)(r0 * a.Np * 2));
+    if (is_a) tile_copy(dst, dA, (uint32_t)(r0 * TILE * 2));
     else tile_copy(dst, dB, (uint32_t)(r0 * a.H * 2));
   });
   __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
   __syncthreads();
   if (len % BK) {
     const int64_t r0 = rbeg + (int64_t)nfull * BK;
-    copy_col_tile_masked((uint4*)lbase, a.dzt, a.Np, i0, a.Np, r0, rend);
+    copy_col_tile_masked((uint4*)lbase, dz, TILE, 0, TILE, r0, rend);
     copy_col_tile_masked((uint4*)(lbase + TILE_BYTES), a.w, a.H, j0, a.H, r0, rend);
     __syncthreads();
     mma_stage_sync<true, true>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane,
@@ -733,14 +912,16 @@ struct Ws {
   float* zlab;
   float* stats;
   float* park;
+  float* kept;
   float* lse[2];
   float* g;
   uint16_t* dzt;
   float* part;
 };
-static Ws carve(Carve& c, bool bwd, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
+enum { WS_FWD, WS_BWD, WS_STEP };
+static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
   Ws w = {};
-  const int64_t Np = up(N, TILE);
+  const int64_t Np = up(N, TILE), Vp = up(V, TILE);
   w.meta = c.take<Meta>(1);
   w.pos = c.take<int32_t>(N);
   w.src = c.take<int32_t>(Np);
@@ -748,19 +929,27 @@ static Ws carve(Carve& c, bool bwd, int64_t N, int64_t V, int64_t H, int64_t Ht,
   w.xp[0] = c.take<uint16_t>(Np * H);
   if (Ht) {
     w.xp[1] = c.take<uint16_t>(Np * Ht);
-    w.park = c.take<float>((size_t)(cu_count() / 8 * 8) * TILE * TILE);
+    w.park = c.take<float>(use == WS_STEP ? (size_t)(Np * Vp)
+                                          : (size_t)(cu_count() / 8 * 8) * TILE * TILE);
+    if (use == WS_STEP) w.kept = c.take<float>((size_t)(Np * Vp));
   }
-  if (!bwd) {
+  if (use != WS_BWD) {
     w.zlab = c.take<float>(Np);
-    w.stats = c.take<float>((size_t)(up(V, TILE) / TILE) * (Ht ? 5 : 2) * Np);
-    return w;
+    w.stats = c.take<float>((size_t)(Vp / TILE) * (Ht ? 5 : 2) * Np);
   }
-  const int64_t words = piece_words(N, V, H);
+  if (use == WS_FWD) return w;
+  const int64_t words = use == WS_STEP ? Vp : piece_words(N, V, H);
   for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
-  w.g = c.take<float>(Np);
+  if (use == WS_BWD) w.g = c.take<float>(Np);
   w.dzt = c.take<uint16_t>((size_t)words * Np);
   if (grad_x) w.part = c.take<float>((size_t)part_floats(N, words, H));
   return w;
+}
+// Whether the forward of so many rows may keep what the gradients are made of
+static bool step_fits(int64_t N, int64_t V, int64_t H, int64_t Ht) {
+  const int64_t logits = up(N, TILE) * up(V, TILE);
+  return N > 0 && V < ((int64_t)1 << 31) - TILE && logits <= (int64_t)(kKeepBytes / (Ht ? 10 : 2)) &&
+         logits * 2 < ((int64_t)1 << 32) && V * H < ((int64_t)1 << 31);
 }
 
 static bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -811,6 +1000,11 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
   a.reduction = PLZ_REDUCE_NONE;
   return a;
 }
+static void set_splits(PackArgs& p, const Sides& s, int64_t words) {
+  p.words = words;
+  p.z_floats = part_floats(s.N, words, s.H);
+  p.cus = cu_count();
+}
 static int pack(const PackArgs& a, hipStream_t st, const char* what) {
   hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows)), dim3(256), 0, st, a);
   return check_launch(what);
@@ -823,7 +1017,7 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.meta = w.meta; a.lab = w.lab; a.inv_t = s.inv_t; a.park = w.park;
   a.stats = w.stats; a.zlab = w.zlab;
   a.lse[0] = w.lse[0]; a.lse[1] = w.lse[1];
-  a.dzt = w.dzt;
+  a.dzt = w.dzt; a.kept = w.kept;
   return a;
 }
 template <int MODE>
@@ -835,43 +1029,107 @@ static int logits(const LogitArgs& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
-template <bool KL>
-static int forward(const Sides& s, float* loss, float* lse, float* total, void* ws, size_t ws_bytes,
-                   hipStream_t st, const char* what) {
+// dW and dx of a piece of n words from its dz
+struct Products {
+  const Sides& s;
+  const Ws& w;
+  uint16_t *grad_x, *grad_w;
+  int64_t panel;  // words of dz's panels
+  hipStream_t st;
+  const char* what;
+  int piece(int64_t v0, int64_t n, bool add) const {
+    static uint64_t done_w = 0, done_x = 0;
+    if (int rc = reserve_lds((const void*)dw_kernel, kLdsLogits, done_w, what)) return rc;
+    if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
+    const int64_t tiles_h = up(s.H, TILE) / TILE;
+    if (grad_w) {
+      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H};
+      hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
+                         kLdsLogits, st, d);
+      if (int rc = check_launch(what)) return rc;
+    }
+    if (grad_x) {
+      const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add};
+      // at most z tiles of rows: z rows H <= the parts' floats, and 64 splits of a tile that is not full
+      const int64_t items = (part_floats(s.N, panel, s.H) / s.H / TILE + 64) * tiles_h;
+      hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
+      if (int rc = check_launch(what)) return rc;
+    }
+    return PLZ_OK;
+  }
+  int sum() const {
+    if (!grad_x) return PLZ_OK;
+    hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)((s.N * (s.H / 8) + 255) / 256)), dim3(256), 0,
+                       st, w.part, w.pos, w.meta, s.N, s.H, grad_x);
+    return check_launch(what);
+  }
+};
+
+// The forward, and with grad_x or grad_w the gradients of its sum or mean (step)
+template <bool KL, bool STEP>
+static int forward(const Sides& s, int reduction, float* loss, float* lse, float* total,
+                   uint16_t* grad_x, uint16_t* grad_w, void* ws, size_t ws_bytes, hipStream_t st,
+                   const char* what) {
   if (int rc = check(s, KL, what)) return rc;
   PLZ_REQUIRE(s.N == 0 || (loss && lse), "%s: null pointer", what);
+  const int use = STEP ? WS_STEP : WS_FWD;
+  if (STEP) {
+    PLZ_REQUIRE(reduction == PLZ_REDUCE_SUM || reduction == PLZ_REDUCE_MEAN, "%s: bad reduction %d",
+                what, reduction);
+    PLZ_REQUIRE(a16(grad_x) && a16(grad_w), "%s: gradients must be 16-byte aligned", what);
+    if (!step_fits(s.N, s.V, s.H, s.Ht)) {
+      set_error("%s: no rows, or more logits than a forward keeps", what);
+      return PLZ_EUNSUPPORTED;
+    }
+  }
   Carve need{nullptr};
-  carve(need, false, s.N, s.V, s.H, s.Ht, false);
+  carve(need, use, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
   if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
   Carve c{reinterpret_cast<char*>(ws)};
-  const Ws w = carve(c, false, s.N, s.V, s.H, s.Ht, false);
+  const Ws w = carve(c, use, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  const int64_t Np = up(s.N, TILE), Vp = up(s.V, TILE);
   if (s.N > 0) {
     PackArgs p = pack_args(s, w);
     p.zero[0] = loss;
     p.zero[1] = lse;
     if (KL) p.zero[2] = lse + s.N;
+    if (STEP) {
+      p.reduction = reduction;
+      if (grad_x) set_splits(p, s, Vp);
+    }
     if (int rc = pack(p, st, what)) return rc;
     LogitArgs l = logit_args(s, w);
     l.v0 = 0;
     l.v1 = s.V;
-    if (int rc = logits<KL ? KL_STATS : CE_STATS>(l, st, what)) return rc;
+    l.words = Vp;
+    constexpr int MODE = STEP ? (KL ? KL_KEEP : CE_KEEP) : (KL ? KL_STATS : CE_STATS);
+    if (int rc = logits<MODE>(l, st, what)) return rc;
     JoinArgs j = {};
     j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
-    j.Np = up(s.N, TILE);
-    j.tiles = (int)(up(s.V, TILE) / TILE);
+    j.Np = Np;
+    j.tiles = (int)(Vp / TILE);
     j.rb_log = s.N >= 4096 ? 4 : s.N >= 512 ? 2 : 0;
     j.loss = loss;
     j.lse[0] = lse;
     j.lse[1] = lse + s.N;
+    j.lsep[0] = w.lse[0];
+    j.lsep[1] = w.lse[1];
     hipLaunchKernelGGL(join_kernel<KL>, dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)),
                        dim3(256), 0, st, j);
     if (int rc = check_launch(what)) return rc;
   }
   if (total) {
     hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, s.N, w.meta, total);
-    return check_launch(what);
+    if (int rc = check_launch(what)) return rc;
   }
-  return PLZ_OK;
+  if (!STEP || (!grad_x && !grad_w)) return PLZ_OK;
+  const FinishArgs f = {w.dzt, Vp, s.V, Np, w.meta, w.lab, w.stats, w.zlab, {w.lse[0], w.lse[1]},
+                        s.inv_t, w.park, w.kept};
+  hipLaunchKernelGGL(finish_kernel<KL>, dim3((unsigned)(Np / TILE * (Vp / TILE) * 8)), dim3(256), 0, st, f);
+  if (int rc = check_launch(what)) return rc;
+  const Products prod = {s, w, grad_x, grad_w, Vp, st, what};
+  if (int rc = prod.piece(0, s.V, false)) return rc;
+  return prod.sum();
 }
 
 template <bool KL>
@@ -889,56 +1147,32 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
     return check_launch(what);
   }
   Carve need{nullptr};
-  carve(need, true, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  carve(need, WS_BWD, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
   if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
   Carve c{reinterpret_cast<char*>(ws)};
-  const Ws w = carve(c, true, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
-  const int64_t Np = up(s.N, TILE), words = piece_words(s.N, s.V, s.H);
+  const Ws w = carve(c, WS_BWD, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  const int64_t words = piece_words(s.N, s.V, s.H);
   PackArgs p = pack_args(s, w);
   p.grad = grad;
   p.reduction = reduction;
   if (reduction == PLZ_REDUCE_NONE) p.g = w.g;
-  if (grad_x) {
-    p.words = words;
-    p.z_floats = part_floats(s.N, words, s.H);
-    p.cus = cu_count();
-  }
+  if (grad_x) set_splits(p, s, words);
   for (int k = 0; k < (KL ? 2 : 1); ++k) {
     p.lse_in[k] = lse + k * s.N;
     p.lse[k] = w.lse[k];
   }
   if (int rc = pack(p, st, what)) return rc;
-  static uint64_t done_w = 0, done_x = 0;
-  if (int rc = reserve_lds((const void*)dw_kernel, kLdsLogits, done_w, what)) return rc;
-  if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
-  const int64_t tiles_h = up(s.H, TILE) / TILE;
   LogitArgs l = logit_args(s, w);
   l.g = p.g;
+  l.words = words;
+  const Products prod = {s, w, grad_x, grad_w, words, st, what};
   for (int64_t v0 = 0; v0 < s.V; v0 += words) {
     l.v0 = v0;
     l.v1 = std::min(s.V, v0 + words);
-    const int64_t n = l.v1 - l.v0;
     if (int rc = logits<KL ? KL_GRAD : CE_GRAD>(l, st, what)) return rc;
-    if (grad_w) {
-      const DwArgs d = {w.dzt, w.xp[0], Np, s.H, n, w.meta, grad_w + v0 * s.H};
-      hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
-                         kLdsLogits, st, d);
-      if (int rc = check_launch(what)) return rc;
-    }
-    if (grad_x) {
-      const DxArgs d = {w.dzt, s.w + v0 * s.H, Np, s.H, n, w.meta, w.part, v0 > 0};
-      // at most z tiles of rows: z rows H <= the parts' floats, and 64 splits of a tile that is not full
-      const int64_t items = (p.z_floats / s.H / TILE + 64) * tiles_h;
-      hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
-      if (int rc = check_launch(what)) return rc;
-    }
+    if (int rc = prod.piece(v0, l.v1 - v0, v0 > 0)) return rc;
   }
-  if (grad_x) {
-    hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)((s.N * (s.H / 8) + 255) / 256)), dim3(256), 0,
-                       st, w.part, w.pos, w.meta, s.N, s.H, grad_x);
-    return check_launch(what);
-  }
-  return PLZ_OK;
+  return prod.sum();
 }
 
 static Sides ce_sides(const uint16_t* x, const uint16_t* w, const void* labels, int bytes,
@@ -961,13 +1195,19 @@ extern "C" {
 size_t plz_vocab_loss_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher) {
   if (N < 0 || V < 1 || H < 8 || H_teacher < 0) return 0;
   Carve c{nullptr};
-  carve(c, false, N, V, H, H_teacher, false);
+  carve(c, WS_FWD, N, V, H, H_teacher, false);
   return c.used;
 }
 size_t plz_vocab_loss_bwd_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x) {
   if (N < 1 || V < 1 || H < 8 || H_teacher < 0) return 0;
   Carve c{nullptr};
-  carve(c, true, N, V, H, H_teacher, grad_x != 0);
+  carve(c, WS_BWD, N, V, H, H_teacher, grad_x != 0);
+  return c.used;
+}
+size_t plz_vocab_loss_step_workspace(int64_t N, int64_t V, int64_t H, int64_t H_teacher, int grad_x) {
+  if (N < 1 || V < 1 || H < 8 || H_teacher < 0 || !step_fits(N, V, H, H_teacher)) return 0;
+  Carve c{nullptr};
+  carve(c, WS_STEP, N, V, H, H_teacher, grad_x != 0);
   return c.used;
 }
 
@@ -976,8 +1216,19 @@ int plz_linear_ce_fwd(const uint16_t* x, const uint16_t* w, const void* labels, 
                       size_t workspace_bytes, int64_t N, int64_t V, int64_t H, void* stream) {
   PLZ_REQUIRE(label_bytes == 8 || label_bytes == 4, "plz_linear_ce_fwd: labels of 4 or 8 bytes expected");
   PLZ_REQUIRE(labels || N == 0, "plz_linear_ce_fwd: null pointer");
-  return forward<false>(ce_sides(x, w, labels, label_bytes, ignore_index, N, V, H), loss, lse, total,
-                        workspace, workspace_bytes, (hipStream_t)stream, "plz_linear_ce_fwd");
+  return forward<false, false>(ce_sides(x, w, labels, label_bytes, ignore_index, N, V, H),
+                               PLZ_REDUCE_NONE, loss, lse, total, nullptr, nullptr, workspace,
+                               workspace_bytes, (hipStream_t)stream, "plz_linear_ce_fwd");
+}
+int plz_linear_ce_step(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
+                       int64_t ignore_index, int reduction, float* loss, float* lse, float* total,
+                       uint16_t* grad_x, uint16_t* grad_w, void* workspace, size_t workspace_bytes,
+                       int64_t N, int64_t V, int64_t H, void* stream) {
+  PLZ_REQUIRE(label_bytes == 8 || label_bytes == 4, "plz_linear_ce_step: labels of 4 or 8 bytes expected");
+  PLZ_REQUIRE(labels || N == 0, "plz_linear_ce_step: null pointer");
+  return forward<false, true>(ce_sides(x, w, labels, label_bytes, ignore_index, N, V, H), reduction,
+                              loss, lse, total, grad_x, grad_w, workspace, workspace_bytes,
+                              (hipStream_t)stream, "plz_linear_ce_step");
 }
 int plz_linear_ce_bwd(const uint16_t* x, const uint16_t* w, const void* labels, int label_bytes,
                       int64_t ignore_index, const float* lse, const float* grad, int reduction,
@@ -993,9 +1244,19 @@ int plz_linear_kl_fwd(const uint16_t* x, const uint16_t* w, const uint16_t* teac
                       const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
                       float* loss, float* lse, float* total, void* workspace, size_t workspace_bytes,
                       int64_t N, int64_t V, int64_t H, int64_t H_teacher, void* stream) {
-  return forward<true>(kl_sides(x, w, teacher_x, teacher_w, mask, inv_temperature, N, V, H, H_teacher),
-                       loss, lse, total, workspace, workspace_bytes, (hipStream_t)stream,
-                       "plz_linear_kl_fwd");
+  return forward<true, false>(
+      kl_sides(x, w, teacher_x, teacher_w, mask, inv_temperature, N, V, H, H_teacher), PLZ_REDUCE_NONE,
+      loss, lse, total, nullptr, nullptr, workspace, workspace_bytes, (hipStream_t)stream,
+      "plz_linear_kl_fwd");
+}
+int plz_linear_kl_step(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
+                       const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,
+                       int reduction, float* loss, float* lse, float* total, uint16_t* grad_x,
+                       uint16_t* grad_w, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
+                       int64_t H, int64_t H_teacher, void* stream) {
+  return forward<true, true>(
+      kl_sides(x, w, teacher_x, teacher_w, mask, inv_temperature, N, V, H, H_teacher), reduction, loss,
+      lse, total, grad_x, grad_w, workspace, workspace_bytes, (hipStream_t)stream, "plz_linear_kl_step");
 }
 int plz_linear_kl_bwd(const uint16_t* x, const uint16_t* w, const uint16_t* teacher_x,
                       const uint16_t* teacher_w, const uint8_t* mask, float inv_temperature,

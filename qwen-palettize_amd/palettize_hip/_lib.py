@@ -157,12 +157,16 @@ SIGNATURES: dict[str, tuple] = {
     "plz_vocab_loss_workspace": (sz, [i64, i64, i64, i64]),
     "plz_vocab_loss_bwd_workspace": (sz, [i64, i64, i64, i64, i32]),
     "plz_linear_ce_fwd": (i32, [p, p, p, i32, i64, p, p, p, p, sz, i64, i64, i64, p]),
+    "plz_vocab_loss_step_workspace": (sz, [i64, i64, i64, i64, i32]),
+    "plz_linear_ce_step": (i32, [p, p, p, i32, i64, i32, p, p, p, p, p, p, sz, i64, i64, i64, p]),
+    "plz_linear_kl_step": (i32, [p, p, p, p, p, f32, i32, p, p, p, p, p, p, sz, i64, i64, i64, i64, p]),
     "plz_linear_ce_bwd": (i32, [p, p, p, i32, i64, p, p, i32, p, p, p, sz, i64, i64, i64, p]),
     "plz_linear_kl_fwd": (i32, [p, p, p, p, p, f32, p, p, p, p, sz, i64, i64, i64, i64, p]),
     "plz_linear_kl_bwd": (i32, [p, p, p, p, p, f32, p, p, i32, p, p, p, sz, i64, i64, i64, i64, p]),
     "plz_grad_norm_workspace": (sz, [p, i32]),
     "plz_grad_norm": (i32, [p, p, p, i32, p, p, sz, p]),
     "plz_clip_grads": (i32, [p, p, p, p, p, i32, f32, p, p, sz, p]),
+    "plz_scale_grads": (i32, [p, p, p, i32, p, p]),
     "plz_paged_step": (i32, [p, p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i64, i32, p]),
     "plz_paged_rope_write": (i32, [p, p, p, i64, i64, i64, p, p, p, p, p, p, p, p, p, i64, i32, i32,
                                    i32, i64, i64, i32, f32, p]),

@@ -209,25 +209,38 @@ def _rows(t, width):
     return t.clone() if t.data_ptr() % 16 else t
 
 
-class LinearCrossEntropyFunction(torch.autograd.Function):
-    """Keeps the rows' normalisers (fp32 [N]); the backward computes the logits again, a piece of the
-    vocabulary at a time."""
+class _VocabLossFunction(torch.autograd.Function):
+    """A loss over the vocabulary of x and weight. Of a sum or mean whose logits are few enough
+    (ops.vocab_step_fits), the forward computes the gradients too, for an upstream gradient of 1, and the
+    backward multiplies them by the one that it gets (where that is not 1 they are rounded again): the
+    logits are computed once instead of twice. Otherwise, and in a second backward of the same graph, the
+    backward computes the logits again, a piece of the vocabulary at a time.
+
+    fwd(*args), step(*args, reduction, grad_x, grad_weight) and bwd(*args, lse, grad, reduction, grad_x,
+    grad_weight) are a loss's calls of ops; args begin with x, weight. wanted: gradients are recorded."""
 
     @staticmethod
-    def forward(ctx, x, weight, labels, ignore_index, reduction):
-        loss, lse, total = ops.linear_ce_fwd(x, weight, labels, ignore_index,
-                                             total=reduction != "none")
-        ctx.save_for_backward(x, weight, labels, lse)
-        ctx.args = reduction, ignore_index
+    def forward(ctx, calls, wanted, reduction, *args):
+        fwd, step, _ = calls
+        grad_x, grad_w = (wanted and need for need in ctx.needs_input_grad[3:5])
+        ctx.grads, ctx.calls, ctx.reduction = None, calls, reduction
+        if step is not None and (grad_x or grad_w) and reduction != "none":
+            loss, lse, total, *ctx.grads = step(*args, reduction, grad_x, grad_w)
+        else:
+            loss, lse, total = fwd(*args, reduction != "none")
+        ctx.save_for_backward(lse, *args)
         return loss if total is None else total[0 if reduction == "sum" else 1]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, labels, lse = ctx.saved_tensors
-        gx, gw = ops.linear_ce_bwd(x, weight, labels, lse, grad.contiguous(), *ctx.args,
-                                   grad_x=ctx.needs_input_grad[0], grad_weight=ctx.needs_input_grad[1])
-        return gx, gw, None, None, None
+        lse, *args = ctx.saved_tensors
+        grads, ctx.grads = ctx.grads, None
+        if grads is not None:
+            ops.scale_grads([g for g in grads if g is not None], grad.contiguous())
+        else:
+            grads = ctx.calls[2](*args, lse, grad.contiguous(), ctx.reduction, *ctx.needs_input_grad[3:5])
+        return None, None, None, *grads, *[None] * (len(args) - 2)
 
 
 def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean"):
@@ -239,33 +252,17 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean")
     ops._reduction(reduction)
     if labels.shape != x.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not match x {tuple(x.shape)}")
-    H = x.shape[-1]
-    loss = LinearCrossEntropyFunction.apply(_rows(x, H), _rows(weight, weight.shape[-1]),
-                                            labels.reshape(-1).contiguous(), int(ignore_index),
-                                            reduction)
+    ignore, H = int(ignore_index), x.shape[-1]
+    calls = (
+        lambda x, w, labels, total: ops.linear_ce_fwd(x, w, labels, ignore, total),
+        lambda x, w, labels, reduction, gx, gw: ops.linear_ce_step(x, w, labels, reduction, ignore, gx, gw),
+        lambda x, w, labels, lse, grad, reduction, gx, gw: ops.linear_ce_bwd(
+            x, w, labels, lse, grad, reduction, ignore, gx, gw))
+    if not ops.vocab_step_fits(labels.numel(), weight.shape[0], H):
+        calls = calls[0], None, calls[2]
+    loss = _VocabLossFunction.apply(calls, torch.is_grad_enabled(), reduction, _rows(x, H),
+                                    _rows(weight, weight.shape[-1]), labels.reshape(-1).contiguous())
     return loss.reshape(labels.shape) if reduction == "none" else loss
-
-
-class LinearDistillFunction(torch.autograd.Function):
-    """As LinearCrossEntropyFunction, with the normalisers of both sides."""
-
-    @staticmethod
-    def forward(ctx, x, weight, teacher_x, teacher_weight, mask, temperature, reduction):
-        loss, lse, total = ops.linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask, temperature,
-                                             total=reduction != "none")
-        ctx.save_for_backward(x, weight, teacher_x, teacher_weight, mask, lse)
-        ctx.args = reduction, temperature
-        return loss if total is None else total[0 if reduction == "sum" else 1]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, teacher_x, teacher_weight, mask, lse = ctx.saved_tensors
-        reduction, temperature = ctx.args
-        gx, gw = ops.linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad.contiguous(),
-                                   reduction, mask, temperature, grad_x=ctx.needs_input_grad[0],
-                                   grad_weight=ctx.needs_input_grad[1])
-        return gx, gw, None, None, None, None, None
 
 
 def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, reduction="mean"):
@@ -278,9 +275,17 @@ def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=
     ops._reduction(reduction)
     if teacher_x.shape[:-1] != x.shape[:-1] or (mask is not None and mask.shape != x.shape[:-1]):
         raise ValueError("x, teacher_x and mask differ in their leading dimensions")
-    H, Ht = x.shape[-1], teacher_x.shape[-1]
-    loss = LinearDistillFunction.apply(
-        _rows(x, H), _rows(weight, weight.shape[-1]), _rows(teacher_x.detach(), Ht),
-        _rows(teacher_weight.detach(), teacher_weight.shape[-1]),
-        None if mask is None else mask.reshape(-1).contiguous(), float(temperature), reduction)
+    N, H, Ht, T = x.shape[:-1].numel(), x.shape[-1], teacher_x.shape[-1], float(temperature)
+    calls = (
+        lambda x, w, tx, tw, mask, total: ops.linear_kl_fwd(x, w, tx, tw, mask, T, total),
+        lambda x, w, tx, tw, mask, reduction, gx, gw: ops.linear_kl_step(
+            x, w, tx, tw, reduction, mask, T, gx, gw),
+        lambda x, w, tx, tw, mask, lse, grad, reduction, gx, gw: ops.linear_kl_bwd(
+            x, w, tx, tw, lse, grad, reduction, mask, T, gx, gw))
+    if not ops.vocab_step_fits(N, weight.shape[0], H, Ht):
+        calls = calls[0], None, calls[2]
+    loss = _VocabLossFunction.apply(
+        calls, torch.is_grad_enabled(), reduction, _rows(x, H), _rows(weight, weight.shape[-1]),
+        _rows(teacher_x.detach(), Ht), _rows(teacher_weight.detach(), teacher_weight.shape[-1]),
+        None if mask is None else mask.reshape(-1).contiguous())
     return loss.reshape(x.shape[:-1]) if reduction == "none" else loss

@@ -1145,6 +1145,15 @@ def _head(x, weight, name="x", wname="weight"):
     return x.shape[0], *weight.shape
 
 
+def _two_heads(x, weight, teacher_x, teacher_weight):
+    """(N, V, H, teacher's H) of both sides of a distillation."""
+    N, V, H = _head(x, weight)
+    M, Vt, Ht = _head(teacher_x, teacher_weight, "teacher_x", "teacher_weight")
+    if (M, Vt) != (N, V):
+        raise ValueError(f"the teacher has {M} rows and {Vt} words, the student {N} and {V}")
+    return N, V, H, Ht
+
+
 def _labels(labels, N):
     """Bytes of a label: int64 or int32 [N]."""
     _need(labels, "labels", None, 1)
@@ -1210,6 +1219,28 @@ def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     return loss, lse, out
 
 
+def vocab_step_fits(N, V, H, H_teacher=0) -> bool:
+    """Whether linear_ce_step (linear_kl_step with H_teacher) takes N rows: it keeps 2 (10) bytes a logit
+    for the length of the call, 4 (8) GiB at most."""
+    return query("plz_vocab_loss_step_workspace", N, V, H, H_teacher, 0) > 0
+
+
+def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_x=True, grad_weight=True):
+    """linear_ce_fwd and the gradients of its mean or sum in one call, which computes the logits once:
+    (loss, lse, total, gradient of x, of weight: bf16, None where not wanted). For vocab_step_fits."""
+    N, V, H = _head(x, weight)
+    size, mode = _labels(labels, N), _reduction(reduction)
+    dev = _one_device("linear_ce_step", x, weight, labels)
+    loss, lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    total = torch.empty(3, dtype=torch.float32, device=x.device)
+    gx = torch.empty_like(x) if grad_x else None
+    gw = torch.empty_like(weight) if grad_weight else None
+    ws = _workspace(query("plz_vocab_loss_step_workspace", N, V, H, 0, int(grad_x)), x.device)
+    _on(dev, "plz_linear_ce_step", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index), mode,
+        _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
+    return loss, lse, total, gx, gw
+
+
 def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-100, grad_x=True,
                   grad_weight=True):
     """Gradients (x, weight) of linear_ce_fwd's loss, bf16 (None where not wanted), from the gradient
@@ -1232,10 +1263,7 @@ def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1
     softmax(teacher_x teacher_weight^T / temperature) and q the student's, without the logits: (loss
     fp32 [N], lse fp32 [2, N] for the backward, total as linear_ce_fwd's). mask bool [N]: rows that it
     leaves out take no part."""
-    N, V, H = _head(x, weight)
-    M, Vt, Ht = _head(teacher_x, teacher_weight, "teacher_x", "teacher_weight")
-    if (M, Vt) != (N, V):
-        raise ValueError(f"the teacher has {M} rows and {Vt} words, the student {N} and {V}")
+    N, V, H, Ht = _two_heads(x, weight, teacher_x, teacher_weight)
     _mask(mask, N)
     inv = _inv_temperature(temperature)
     dev = _one_device("linear_kl_fwd", x, weight, teacher_x, teacher_weight, mask)
@@ -1248,13 +1276,29 @@ def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1
     return loss, lse, out
 
 
+def linear_kl_step(x, weight, teacher_x, teacher_weight, reduction="mean", mask=None, temperature=1.0,
+                   grad_x=True, grad_weight=True):
+    """linear_kl_fwd and the gradients of its mean or sum, as linear_ce_step."""
+    N, V, H, Ht = _two_heads(x, weight, teacher_x, teacher_weight)
+    _mask(mask, N)
+    mode, inv = _reduction(reduction), _inv_temperature(temperature)
+    dev = _one_device("linear_kl_step", x, weight, teacher_x, teacher_weight, mask)
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    total = torch.empty(3, dtype=torch.float32, device=x.device)
+    gx = torch.empty_like(x) if grad_x else None
+    gw = torch.empty_like(weight) if grad_weight else None
+    ws = _workspace(query("plz_vocab_loss_step_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    _on(dev, "plz_linear_kl_step", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
+        _ptr(mask), inv, mode, _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws),
+        ws.numel(), N, V, H, Ht)
+    return loss, lse, total, gx, gw
+
+
 def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="mean", mask=None,
                   temperature=1.0, grad_x=True, grad_weight=True):
     """Gradients (x, weight) of linear_kl_fwd's loss, as linear_ce_bwd's; the teacher has none."""
-    N, V, H = _head(x, weight)
-    M, Vt, Ht = _head(teacher_x, teacher_weight, "teacher_x", "teacher_weight")
-    if (M, Vt) != (N, V):
-        raise ValueError(f"the teacher has {M} rows and {Vt} words, the student {N} and {V}")
+    N, V, H, Ht = _two_heads(x, weight, teacher_x, teacher_weight)
     _mask(mask, N)
     mode, inv = _reduction(reduction), _inv_temperature(temperature)
     _kept(lse, "lse", 2, N)
@@ -1305,6 +1349,22 @@ def grad_norm(grads):
     ws = _workspace(query("plz_grad_norm_workspace", sizes, len(grads)), norm.device)
     _on(dev, "plz_grad_norm", ptrs, sizes, kinds, len(grads), _ptr(norm), _ptr(ws), ws.numel())
     return norm
+
+
+def scale_grads(grads, factor):
+    """grads[i] *= factor in place, factor fp32 of one value on the GPU; contiguous tensors (bf16, fp16
+    or fp32, of one device) that do not overlap. Nothing is read or written where the factor is 1."""
+    grads = list(grads)
+    if not grads:
+        return
+    ptrs, sizes, kinds, dev = _grad_table("scale_grads", grads)
+    _need(factor, "factor", torch.float32)
+    if factor.numel() != 1 or factor.get_device() != dev:
+        raise ValueError("scale_grads: factor must be one value on the gradients' device")
+    _no_backward("scale_grads", *grads, factor)
+    if len({a for a, n in zip(ptrs, sizes) if n}) != sum(n > 0 for n in sizes):
+        raise ValueError("scale_grads: a tensor is written twice")
+    _on(dev, "plz_scale_grads", ptrs, sizes, kinds, len(grads), _ptr(factor))
 
 
 def clip_grads(grads, max_norm, out=None):

@@ -184,6 +184,22 @@ def test_captured_and_replayed(ops):
         check_clipped(out, grads, 1.0)
 
 
+def test_scale(ops):
+    grads = grads_of([(5000,), (33,), (0,), (70001,)], TYPES)
+    keep = [g.clone() for g in grads]
+    ops.scale_grads(grads, torch.ones((), device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(grads, keep))
+    ops.scale_grads(grads, torch.tensor(-2.0, device="cuda"))
+    assert all(torch.equal(a, -2 * b) for a, b in zip(grads, keep))
+    ops.scale_grads([], torch.ones((), device="cuda"))
+    with pytest.raises(ValueError, match="written twice"):
+        ops.scale_grads([grads[0], grads[0]], torch.ones((), device="cuda"))
+    with pytest.raises(ValueError, match="one value"):
+        ops.scale_grads(grads, torch.ones(2, device="cuda"))
+    with pytest.raises(TypeError, match="factor"):
+        ops.scale_grads(grads, torch.ones((), device="cuda", dtype=torch.float64))
+
+
 def test_refusals(ops):
     a, b = (torch.ones(10, device="cuda") for _ in range(2))
     with pytest.raises(ValueError, match="at least one"):

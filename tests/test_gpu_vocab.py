@@ -108,6 +108,114 @@ def test_kl_of_itself_is_zero(F):
     assert float(loss.abs().max()) == 0 and not gx.any() and not gw.any()
 
 
+# ---- forward and backward as two calls, which compute the logits twice ----------------------------------
+def two_calls_ce(ops, x, w, labels, reduction="mean", upstream=1.0):
+    _, lse, total = ops.linear_ce_fwd(x, w, labels)
+    grad = torch.tensor([upstream], device="cuda")
+    return (total[0 if reduction == "sum" else 1], *ops.linear_ce_bwd(x, w, labels, lse, grad, reduction))
+
+
+def two_calls_kl(ops, x, w, tx, tw, mask=None, T=1.0, reduction="mean"):
+    _, lse, total = ops.linear_kl_fwd(x, w, tx, tw, mask, T)
+    grad = torch.ones(1, device="cuda")
+    return (total[0 if reduction == "sum" else 1],
+            *ops.linear_kl_bwd(x, w, tx, tw, lse, grad, reduction, mask, T))
+
+
+@pytest.mark.parametrize("N,V,H", SIZES)
+def test_two_calls(ops, N, V, H):
+    x, w, labels = inputs(N, V, H, seed=N + V, ignored=0.3)
+    check(two_calls_ce(ops, x, w, labels), reference(x, w, labels, kept=False))
+    check(two_calls_ce(ops, x, w, labels, "sum", -0.7),
+          reference(x, w, labels, reduction="sum", upstream=-0.7, kept=False))
+    x, w, tx, tw, mask = kl_inputs(N, V, H, 136, N + V, 0.3)
+    check(two_calls_kl(ops, x, w, tx, tw, mask, 1.5),
+          reference(x, w, tx=tx, tw=tw, mask=mask, T=1.5))
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_two_calls_over_pieces(ops, kind):
+    """More words than a piece of the backward holds for so many rows, and the last piece odd."""
+    x, w, labels = inputs(16384, 33333, 64, seed=12, ignored=0.1)
+    if kind == "ce":
+        check(two_calls_ce(ops, x, w, labels), reference(x, w, labels, kept=False))
+    else:
+        tx, mask = (x.float() * 0.8).bfloat16(), labels != -100
+        check(two_calls_kl(ops, x, w, tx, w, mask), reference(x, w, tx=tx, tw=w, mask=mask))
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_second_backward(F, kind):
+    """The first backward hands over what the forward computed; another one computes it again."""
+    x, w, labels = inputs(200, 1500, 128, seed=20, ignored=0.2)
+    tx, tw, _ = inputs(200, 1500, 72, seed=21)
+    x.requires_grad_(), w.requires_grad_()
+    if kind == "ce":
+        loss, ref = F.linear_cross_entropy(x, w, labels), dict(labels=labels)
+    else:
+        loss, ref = F.linear_distill(x, w, tx, tw), dict(tx=tx, tw=tw)
+    for g in (1.0, -0.6, 2.0):
+        got = torch.autograd.grad(loss, (x, w), torch.tensor(g, device="cuda"), retain_graph=True)
+        want = reference(x.detach(), w.detach(), upstream=g, **ref)
+        # a factor other than 1 rounds what the first one hands over again
+        for a, n in zip(got, ("gx", "gw")):
+            close(a, want[n], want[n + "_tol"] + 2.0 ** -8 * 1.01 * want[n].abs(), n)
+    loss.backward(retain_graph=True)
+    first = x.grad.clone()
+    loss.backward()
+    close(x.grad, 2 * first.double(), 2.0 ** -7 * first.double().abs() + 1e-30, "accumulated")
+
+
+def test_gradients_that_a_step_leaves_out(F):
+    x, w, labels = inputs(150, 700, 64, seed=22, ignored=0.2)
+    want = run_ce(F, x, w, labels)
+    for wants_x in (True, False):
+        xs, ws = x.detach().clone().requires_grad_(wants_x), w.detach().clone().requires_grad_(not wants_x)
+        loss = F.linear_cross_entropy(xs, ws, labels)
+        loss.backward()
+        assert torch.equal(loss, want[0])
+        assert (ws if wants_x else xs).grad is None
+        assert torch.equal((xs if wants_x else ws).grad, want[1 if wants_x else 2])
+    with torch.no_grad():
+        assert torch.equal(F.linear_cross_entropy(xs, ws, labels), want[0])
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_step_captured_and_replayed(ops, kind):
+    N, V, H = 300, 3001, 136
+    x, w, labels = inputs(N, V, H, seed=23)
+    tx = torch.zeros_like(x)
+    mask = torch.ones(N, dtype=torch.bool, device="cuda")
+    up = torch.ones(1, device="cuda")
+
+    def step():
+        out = (ops.linear_ce_step(x, w, labels) if kind == "ce" else
+               ops.linear_kl_step(x, w, tx, w, mask=mask))
+        ops.scale_grads(out[3:], up)
+        return out
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(4):
+        nx, _, nl = inputs(N, V, H, seed=30 + seed, ignored=0.25 * seed)
+        x.copy_(nx)
+        labels.copy_(nl)
+        mask.copy_(nl != -100)
+        tx.copy_(nx.flip(0))
+        up.fill_(1.0 + seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
 # ---- what takes no part -------------------------------------------------------------------------------
 @pytest.mark.parametrize("N", [1, 40, 300])
 def test_ce_no_row_takes_part(F, N):

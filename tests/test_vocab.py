@@ -70,3 +70,21 @@ def test_workspaces(lib):
     assert bwd(1 << 17, V, 2560, 0, 0) < (1 << 30) + (1 << 30)
     assert fwd(0, 1, 8, 0) > 0
     assert fwd(-1, 100, 64, 0) == 0 and bwd(0, 100, 64, 0, 1) == 0
+
+
+def test_steps_that_fit(lib):
+    step = lib.plz_vocab_loss_step_workspace
+    # 2 bytes a logit of whole tiles, under 4 GiB; 10 of a distillation, under 8 GiB
+    assert (1 << 30) < step(4096, 151936, 2560, 0, 1) < (2 << 30)
+    assert step(14080, 151936, 2560, 0, 1) > 0 and step(14337, 151936, 2560, 0, 1) == 0
+    assert step(5632, 151936, 2560, 2560, 1) > 0 and step(5889, 151936, 2560, 2560, 1) == 0
+    assert step(0, 1000, 64, 0, 1) == 0 and step(16, 1 << 20, 2048, 0, 1) == 0
+
+    def call(N, mode=2, gx=A, gw=A):
+        return lib.plz_linear_ce_step(A, A, A, 8, -100, mode, A, A, None, gx, gw, A, 1 << 44, N, 151936,
+                                      2560, None)
+    assert call(14337) == 3 and b"logits" in lib.plz_last_error()
+    assert call(0) == 3
+    for kw, word in ((dict(mode=0), b"reduction"), (dict(mode=7), b"reduction"),
+                     (dict(gx=C.c_void_p(8)), b"aligned"), (dict(gw=C.c_void_p(2)), b"aligned")):
+        assert call(64, **kw) == 1 and word in lib.plz_last_error()

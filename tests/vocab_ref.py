@@ -14,10 +14,12 @@ def logits(x, w, T=1.0):
 
 
 def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None, T=1.0,
-              reduction="mean", upstream=None):
+              reduction="mean", upstream=None, kept=None):
     """A dict of the loss and gradients of `reduction` in 64 bits and the bounds of their errors
     (loss_tol, gx_tol, gw_tol), and every row's loss (rows, rows_tol). upstream: the gradient of the
-    loss, a number or one of every row."""
+    loss, a number or one of every row. kept: the gradient is of a cross entropy that kept its
+    exponentials in fp16, relative to the greatest of 256 words (a sum or mean of linear_cross_entropy)."""
+    kept = labels is not None and reduction != "none" if kept is None else kept
     N, V = x.shape[0], w.shape[0]
     dev = x.device
     keep = (labels != ignore_index) if labels is not None else (
@@ -50,6 +52,8 @@ def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None,
             rows_tol[r] = off + dz[i, l] + 4 * U32 * (lse.abs() + z[i, l].abs())
             d = q.clone()
             d[i, l] -= 1
+            if kept:  # half a step of fp16, or of its subnormals
+                q_tol = q_tol + 2.0 ** -11 * q + 2.0 ** -25 * q.max(1, keepdim=True).values
         else:
             zt, dzt = logits(tx[r], tw, T)
             lt = torch.logsumexp(zt, 1)

@@ -18,8 +18,11 @@
 // piece) and with W (dx, its fp32 parts summed over pieces and splits in a fixed order). The scale of
 // a mean and of its gradient is applied to the fp32 sums, not to dz: it would be rounded with it.
 //
-// A distillation tile needs both sides' logits: a workgroup keeps the teacher's 256 x 256 in a slot of
-// its own in the workspace (256 KB, 64 MB for 256 CUs) while it computes the student's.
+// A sum or mean whose logits are few enough has its gradients with the forward (step): the tiles keep
+// what dz is made of and a memory-bound pass makes dz of it once the normalisers are known, instead of
+// computing the logits again. A cross entropy keeps its exponentials relative to the tile's maximum, in
+// fp16; a distillation keeps both sides' logits in fp32, since dz is the difference of probabilities
+// that may be close. Other distillations do the same with a piece of the vocabulary at a time.
 #include <algorithm>
 
 #include "plz_gemm2_dense.cuh"
@@ -31,16 +34,16 @@ namespace voc {
 using namespace g2;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr size_t kPieceBytes = (size_t)1 << 30;
-constexpr size_t kKeepBytes = (size_t)8 << 30;
+constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dz, and of the logits of a piece
+constexpr size_t kKeepBytes = (size_t)8 << 30;   // of what a step keeps
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
-constexpr int kPackRows = 16;
+constexpr int kPackRows = 4;
 
 enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
-// What a launch over tiles of logits leaves: their statistics, the gradients of the logits, or the
-// statistics and what the gradients are made of once the normalisers are known
-enum { CE_STATS, CE_GRAD, KL_STATS, KL_GRAD, CE_KEEP, KL_KEEP };
+// What a launch over tiles of logits leaves: their statistics, the gradients of the logits, the
+// statistics and the exponentials in fp16, or the statistics and the logits in fp32 (of both sides)
+enum { CE_STATS, CE_GRAD, CE_KEEP, Z_KEEP };
 
 // ---- rows that take part --------------------------------------------------------------------------
 struct Meta {
@@ -71,23 +74,21 @@ struct PackArgs {
   int cus;
 };
 
-// Splits of dx's reduction over the words of a piece for `rows` rows: whole waves of workgroups at 1.9
-// us a stage and 4 stages of prologue and epilogue, 8 bytes an element and split written and read at
-// 5 TB/s; at least 8 stages a split, and no more parts than `floats` hold.
-__host__ __device__ inline int dx_splits(int64_t rows, int64_t words, int64_t H, int64_t C, int64_t floats) {
-  const int64_t tiles = (rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE);
+// Modelled time of dx over the words of a piece for `rows` rows in z splits: whole waves of workgroups
+// at 1.9 us a stage and 4 stages of prologue and epilogue, 8 bytes an element and split written and read
+// at 5 TB/s; infinite for splits of less than 8 stages or parts of more than `floats`.
+__host__ __device__ inline float dx_us(int z, int64_t rows, int64_t words, int64_t H, int C, int64_t floats) {
+  const int tiles = (int)((rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE));
+  const int len = ((int)words + z * BK - 1) / (z * BK);
+  if (z > 1 && (len < 8 || z * rows * H > floats)) return INFINITY;
   const float part = 8.f * (float)rows * (float)H / 5.0e6f;
+  return (float)(((int64_t)tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
+}
+constexpr int kMaxSplits = 64;
+inline int dx_splits(int64_t rows, int64_t words, int64_t H, int C) {
   int best = 1;
-  float best_t = INFINITY;
-  for (int z = 1; z <= 64; ++z) {
-    const int len = (int)(((words + z - 1) / z + BK - 1) / BK);
-    if (z > 1 && (len < 8 || z * rows * H > floats)) break;
-    const float t = (float)((tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
-    if (t < best_t * 0.97f) {
-      best_t = t;
-      best = z;
-    }
-  }
+  for (int z = 2; z <= kMaxSplits; ++z)
+    if (dx_us(z, rows, words, H, C, INT64_MAX) < dx_us(best, rows, words, H, C, INT64_MAX)) best = z;
   return best;
 }
 
@@ -101,23 +102,54 @@ __device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
 }
 
 // A workgroup packs kPackRows rows behind all that take part before them, which it counts itself (the
-// keys of 16384 rows are 128 KB in the L2s). The last one also clears the rows up to the next whole
-// stage of the dW product, whose reduction runs over the packed rows.
+// keys of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come BK / kPackRows that clear
+// the packed rows up to the next whole stage of the dW product, whose reduction runs over them; the
+// first of them writes meta, a split of dx a lane.
 __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   __shared__ int red[4];
   __shared__ int at[kPackRows];
-  const int64_t r0 = (int64_t)blockIdx.x * kPackRows;
-  int before = 0;
-  if (a.kind == KEY_NONE) {
-    before = (int)r0;
-  } else {
+  const int64_t r0 = min((int64_t)blockIdx.x * kPackRows, a.N);
+  const int pad = (int)(blockIdx.x - (a.N + kPackRows - 1) / kPackRows);  // < 0: rows
+  int before = (int)r0;
+  if (a.kind != KEY_NONE) {
     int c = 0;
+#pragma unroll 4
     for (int64_t r = threadIdx.x; r < r0; r += 256) c += takes_part(a, r) ? 1 : 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
     __syncthreads();
     before = red[0] + red[1] + red[2] + red[3];
+  }
+  if (pad >= 0) {
+    const int rows = before, first = rows + pad * kPackRows;
+    const int end = min(first + kPackRows, (rows + BK - 1) / BK * BK);
+    for (int k = 0; k < 2; ++k) {
+      if (!a.x[k] || first >= end) continue;
+      const int64_t c8 = a.H[k] / 8;
+      uint4* d = reinterpret_cast<uint4*>(a.xp[k]) + first * c8;
+      for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) d[c] = make_uint4(0, 0, 0, 0);
+    }
+    if (pad == 0 && threadIdx.x < 64) {
+      int z = threadIdx.x + 1;
+      float us = a.z_floats ? dx_us(z, rows, a.words, a.H[0], a.cus, a.z_floats) : 0.f;
+#pragma unroll
+      for (int o = 1; o < kMaxSplits; o <<= 1) {
+        const float u = __shfl_xor(us, o);
+        const int v = __shfl_xor(z, o);
+        if (u < us || (u == us && v < z)) {
+          us = u;
+          z = v;
+        }
+      }
+      if (threadIdx.x == 0) {
+        float alpha = a.inv_t;
+        if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
+        if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
+        *a.meta = Meta{rows, alpha, z};
+      }
+    }
+    return;
   }
   const int n = (int)min((int64_t)kPackRows, a.N - r0);
   if (threadIdx.x < 64) {
@@ -144,16 +176,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
           if (a.zero[k]) a.zero[k][r] = 0.f;
       }
     }
-    if (i == 0 && r0 + n == a.N) {
-      const int rows = before + __popcll(all);
-      a.meta->rows = rows;
-      float alpha = a.inv_t;
-      if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
-      if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
-      a.meta->alpha = alpha;
-      if (a.z_floats) a.meta->z = dx_splits(rows, a.words, a.H[0], a.cus, a.z_floats);
-      red[0] = rows;
-    }
   }
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
@@ -167,12 +189,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
       const int i = j / c8, p = at[i];
       if (p >= 0) to[(int64_t)p * c8 + (j - i * c8)] = from[j];
     }
-    if (r0 + n == a.N) {
-      const int rows = red[0], end = (rows + BK - 1) / BK * BK;
-      uint4* d = reinterpret_cast<uint4*>(a.xp[k] + (int64_t)rows * H);
-      for (int64_t c = threadIdx.x; c < (int64_t)(end - rows) * c8; c += 256)
-        d[c] = make_uint4(0, 0, 0, 0);
-    }
   }
 }
 
@@ -181,20 +197,22 @@ struct LogitArgs {
   const uint16_t* w[2];  // student, teacher
   const uint16_t* x[2];  // packed rows [Np, H]
   int64_t H[2];
+  int sides;
   int64_t v0, v1;  // the words of this launch
   int64_t Np;
   const Meta* meta;
   const int32_t* lab;
-  const float* lse[2];  // [Np]
-  const float* g;       // [Np] or NULL
+  const float* lse;  // [Np]
+  const float* g;    // [Np] or NULL
   float inv_t;
-  float* stats;  // [tile of words][2 or 5][Np]
-  float* zlab;   // [Np]
+  float* stats;  // [tile of words][planes][Np]: maximum and sum of the student, of the teacher
+  int planes, tile0;  // tile0: the first of this launch
+  float* zlab;        // [Np]
   // [tile of rows][word of the piece, whole tiles][256 rows]: dz, or the exponentials kept for it
   uint16_t* dzt;
   int64_t words;  // of a piece, whole tiles
-  float* park;    // the teacher's logits: [workgroup][256 * 256], kept: [tile][256 * 256]
-  float* kept;    // the student's, [tile][256 * 256]
+  float* kept;    // logits over T, [side][tile of the launch][256 * 256] in the accumulators' order
+  int64_t kept_side;  // floats of a side
 };
 
 // exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
@@ -213,14 +231,6 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
   const float fa = exp_of(a.m - M), fb = exp_of(b.m - M);
   return Stat{M, a.s * fa + b.s * fb, a.c * fa + b.c * fb};
 }
-__device__ __forceinline__ Stat join_halves(const Stat& a) {
-  const auto m = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.m), __float_as_uint(a.m), false, false);
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.s), __float_as_uint(a.s), false, false);
-  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(a.c), __float_as_uint(a.c), false, false);
-  return join(Stat{__uint_as_float(m[0]), __uint_as_float(s[0]), __uint_as_float(c[0])},
-              Stat{__uint_as_float(m[1]), __uint_as_float(s[1]), __uint_as_float(c[1])});
-}
-
 // over lanes l and l ^ 32
 __device__ __forceinline__ float swap32_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -279,45 +289,22 @@ template <int MODE>
 __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
-  constexpr bool KL = MODE == KL_STATS || MODE == KL_GRAD || MODE == KL_KEEP;
-  constexpr bool STATS = MODE != CE_GRAD && MODE != KL_GRAD;
-  constexpr int PLANES = KL ? 5 : 2;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave / WAVES_J, wj = wave % WAVES_J;
   const int rows = a.meta->rows;
   const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE), tiles_j = (rows + TILE - 1) / TILE;
   const int64_t total = (int64_t)tiles_i * tiles_j;
-  // every XCD walks a run of its own, four tiles of words at a time over the rows
+  // every XCD walks a run of its own, four tiles of words at a time over the rows, of one side after
+  // the other
   const int xcd = blockIdx.x % 8, step = gridDim.x / 8;
-  const int64_t end = total * (xcd + 1) / 8;
-  for (int64_t item = total * xcd / 8 + blockIdx.x / 8; item < end; item += step) {
+  const int64_t begin = total * xcd / 8, run = total * (xcd + 1) / 8 - begin;
+  for (int64_t at = blockIdx.x / 8; at < run * a.sides; at += step) {
+    const int side = MODE == Z_KEEP && at >= run ? 1 : 0;
     int tile_i, tile_j;
-    tile_coords(4, tiles_i, tiles_j, (int)item, tile_i, tile_j);
+    tile_coords(4, tiles_i, tiles_j, (int)(begin + at - side * run), tile_i, tile_j);
     const int64_t i0 = a.v0 + (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
     f32x16 acc[WT_I][WT_J];
-    // where the teacher's logits wait, in the accumulators' order: four of a thread 16 bytes apart from
-    // the next thread's, addressed by constants (one address register for all of them)
-    const int64_t tile = (int64_t)tile_j * tiles_i + tile_i;
-    float* const parked =
-        KL ? a.park + (MODE == KL_KEEP ? tile : (int64_t)blockIdx.x) * (TILE * TILE) : nullptr;
-    const BufRsrc slot = make_rsrc(parked, TILE * TILE * 4);
-    // one body for both sides: two would keep both sides' copy offsets in registers
-#pragma unroll 1
-    for (int side = KL ? 1 : 0; side >= 0; --side) {
-      logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
-      if (side == 0) break;
-#pragma unroll
-      for (int ti = 0; ti < WT_I; ++ti)
-#pragma unroll
-        for (int tj = 0; tj < WT_J; ++tj)
-#pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4) {
-            const f32x4 v = {acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
-                             acc[ti][tj][4 * e4 + 3]};
-            store16(parked + ((ti * WT_J + tj) * 4 + e4) * NTHR * 4, threadIdx.x * 16,
-                    __builtin_bit_cast(u32x4, v));
-          }
-    }
+    logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
 
     // This lane's word of block ti and register e is vl + 32 ti + 8 (e / 4) + e % 4, from the tile's
     // first one; of the tile's words, nw exist.
@@ -328,18 +315,6 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
       const int nl = wj * (32 * WT_J) + 32 * tj + (lane & 31);
       const int64_t n = j0 + nl;
       const bool live = n < rows;
-      // block ti of the teacher's logits, as this thread put it away
-      auto teacher = [&](int ti) {
-        f32x16 z;
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const f32x4 v = __builtin_bit_cast(
-              f32x4, __builtin_amdgcn_raw_buffer_load_b128(slot, threadIdx.x * 16,
-                                                           ((ti * WT_J + tj) * 4 + e4) * NTHR * 16, 0));
-          z[4 * e4] = v.x; z[4 * e4 + 1] = v.y; z[4 * e4 + 2] = v.z; z[4 * e4 + 3] = v.w;
-        }
-        return z;
-      };
       // the label's logit, in the one lane that holds it: false elsewhere. lv: the label from vl
       float zl = 0.f;
       auto holds = [&](int l) {
@@ -356,92 +331,47 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         }
         return mine;
       };
-      // block ti of a row's words without those that do not exist
-      auto only = [&](f32x16& z, int ti) {
-        const int left = nw - vl - 32 * ti;
+      if constexpr (MODE != CE_GRAD) {
+        if constexpr (MODE == Z_KEEP) {
+          float* const kept = a.kept + side * a.kept_side +
+                              ((int64_t)tile_j * tiles_i + tile_i) * (TILE * TILE);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = 8 * (e >> 2) + (e & 3) < left ? z[e] : -INFINITY;
-      };
-      auto top = [](const f32x16& v, float m) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, v[e]);
-        return m;
-      };
-      if constexpr (STATS && KL) {
-        Stat st[2] = {Stat{-INFINITY, 0.f, 0.f}, Stat{-INFINITY, 0.f, 0.f}};
-#pragma unroll
-        for (int ti = 0; ti < WT_I; ++ti) {
-          if constexpr (MODE == KL_KEEP) {
+          for (int ti = 0; ti < WT_I; ++ti) {
+            acc[ti][tj] *= a.inv_t;
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
               const f32x4 v = {acc[ti][tj][4 * e4], acc[ti][tj][4 * e4 + 1], acc[ti][tj][4 * e4 + 2],
                                acc[ti][tj][4 * e4 + 3]};
-              store16(a.kept + tile * (TILE * TILE) + ((ti * WT_J + tj) * 4 + e4) * NTHR * 4,
-                      threadIdx.x * 16, __builtin_bit_cast(u32x4, v));
+              store16(kept + ((ti * WT_J + tj) * 4 + e4) * NTHR * 4, threadIdx.x * 16,
+                      __builtin_bit_cast(u32x4, v));
             }
           }
-          f32x16 z = acc[ti][tj] * a.inv_t, t = teacher(ti) * a.inv_t;
-          if (nw < TILE) {
-            only(z, ti);
-            only(t, ti);
+        } else {
+          if (live && holds(a.lab[n] - (int)i0)) a.zlab[n] = zl;
+        }
+        if (nw < TILE) {  // words that do not exist
+#pragma unroll
+          for (int ti = 0; ti < WT_I; ++ti) {
+            const int left = nw - vl - 32 * ti;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              acc[ti][tj][e] = 8 * (e >> 2) + (e & 3) < left ? acc[ti][tj][e] : -INFINITY;
           }
-          Stat b{top(z, -INFINITY), 0.f, 0.f};
-          const float m0 = b.m == -INFINITY ? 0.f : b.m;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) b.s += exp_of(z[e] - m0);
-          st[0] = join(st[0], b);
-          b = Stat{top(t, -INFINITY), 0.f, 0.f};
-          const float m1 = b.m == -INFINITY ? 0.f : b.m;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p = exp_of(t[e] - m1);
-            b.s += p;
-            // a word without weight counts for nothing, however far the two sides are
-            b.c += p == 0.f ? 0.f : p * (t[e] - z[e]);
-          }
-          st[1] = join(st[1], b);
-          __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) st[k] = join_halves(st[k]);
-        // the two waves of a column of the tile meet in LDS, behind the stages' slots
-        lds_f32* ex = reinterpret_cast<lds_f32*>(lbase + 4 * TILE_BYTES) + wj * 256;
-        if (wi == 1 && lane < 32) {
-          ex[lane] = st[0].m;
-          ex[32 + lane] = st[0].s;
-          ex[64 + lane] = st[1].m;
-          ex[96 + lane] = st[1].s;
-          ex[128 + lane] = st[1].c;
-        }
-        __syncthreads();
-        if (wi == 0 && lane < 32 && live) {
-          float* out = a.stats + (i0 / TILE) * PLANES * a.Np + n;
-          const Stat s0 = join(st[0], Stat{ex[lane], ex[32 + lane], 0.f});
-          const Stat s1 = join(st[1], Stat{ex[64 + lane], ex[96 + lane], ex[128 + lane]});
-          out[0] = s0.m;
-          out[a.Np] = s0.s;
-          out[2 * a.Np] = s1.m;
-          out[3 * a.Np] = s1.s;
-          out[4 * a.Np] = s1.c;
-        }
-        __syncthreads();
-      } else if constexpr (STATS) {
-        if (live && holds(a.lab[n] - (int)i0)) a.zlab[n] = zl;
-        if (nw < TILE) {
-#pragma unroll
-          for (int ti = 0; ti < WT_I; ++ti) only(acc[ti][tj], ti);
-        }
-        // the tile's maximum: of the lane, of both halves, of both waves of the column
+        // the tile's maximum: of the lane, of both halves, of both waves of the column, which meet in
+        // LDS behind the stages' slots
         float m = -INFINITY;
 #pragma unroll
-        for (int ti = 0; ti < WT_I; ++ti) m = top(acc[ti][tj], m);
+        for (int ti = 0; ti < WT_I; ++ti)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[ti][tj][e]);
         m = swap32_max(m);
         lds_f32* ex = reinterpret_cast<lds_f32*>(lbase + 4 * TILE_BYTES) + wj * 256;
         ex[wi * 32 + (lane & 31)] = m;
         __syncthreads();
         m = fmaxf(ex[lane & 31], ex[32 + (lane & 31)]);
         const float m0 = m == -INFINITY ? 0.f : m;
-        uint16_t* const kept =
+        uint16_t* const exps =
             MODE == CE_KEEP ? a.dzt + ((int64_t)tile_j * a.words + (i0 - a.v0)) * TILE : nullptr;
         float sum = 0.f;
 #pragma unroll
@@ -460,7 +390,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
               u32x4 v;
 #pragma unroll
               for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);
-              store16(kept + ti * 8192 + tj * 1024 + h * 512, wi * 65536 + wj * 4096 + lane * 16, v);
+              store16(exps + ti * 8192 + tj * 1024 + h * 512, wi * 65536 + wj * 4096 + lane * 16, v);
             }
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -469,43 +399,34 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         if (wi == 1 && lane < 32) ex[64 + lane] = sum;
         __syncthreads();
         if (wi == 0 && lane < 32 && live) {
-          float* out = a.stats + (i0 / TILE) * PLANES * a.Np + n;
+          float* out = a.stats + ((int64_t)(a.tile0 + tile_i) * a.planes + 2 * side) * a.Np + n;
           out[0] = m;
           out[a.Np] = sum + ex[64 + lane];
         }
         __syncthreads();
       } else {
         // dz of this row's words, bf16, into the tile staged in LDS [word][row]
-        const float lse = live ? a.lse[0][n] : 0.f, lt = KL && live ? a.lse[1][n] : 0.f;
+        const float lse = live ? a.lse[n] : 0.f;
         float g = live && a.g ? a.g[n] : 1.f;
-        int l = -1;
-        if constexpr (!KL) {
-          l = live ? a.lab[n] : 0;
-          if (l < 0) g = __builtin_nanf("");  // no such word: nothing to learn from
-          l -= (int)i0;
-        }
+        int l = live ? a.lab[n] : 0;
+        if (l < 0) g = __builtin_nanf("");  // no such word: nothing to learn from
+        l -= (int)i0;
 #pragma unroll
         for (int ti = 0; ti < WT_I; ++ti) {
-          f32x16 t = {};
-          if constexpr (KL) t = teacher(ti) * a.inv_t;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float d = exp_of((KL ? acc[ti][tj][e] * a.inv_t : acc[ti][tj][e]) - lse);
-            if constexpr (KL) d -= exp_of(t[e] - lt);
-            d = live ? d * g : 0.f;
+            const float d = live ? exp_of(acc[ti][tj][e] - lse) * g : 0.f;
             *reinterpret_cast<lds_u16t*>(lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS +
                                          nl * 2) = (uint16_t)f2bf(d);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!KL) {
-          if (live && holds(l))
-            *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) =
-                (uint16_t)f2bf((exp_of(zl - lse) - 1.f) * g);
-        }
+        if (live && holds(l))
+          *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) =
+              (uint16_t)f2bf((exp_of(zl - lse) - 1.f) * g);
       }
     }
-    if constexpr (!STATS) {
+    if constexpr (MODE == CE_GRAD) {
       __syncthreads();
       uint16_t* out = a.dzt + ((int64_t)tile_j * a.words + (i0 - a.v0)) * TILE;
 #pragma unroll 4
@@ -521,6 +442,61 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   }
 }
 
+// Sum of p (t - s) over the words of each tile of a launch that kept both sides' logits, with the
+// weights relative to the teacher's maximum of the tile: the fifth plane of the statistics. HBM-bound, 8
+// bytes a logit. A workgroup takes a tile's column of 64 rows, wave w its words 64 w .. 64 w + 63.
+struct CrossArgs {
+  const float* kept;
+  int64_t kept_side;
+  const Meta* meta;
+  float* stats;
+  int64_t Np, v0, v1;
+};
+__global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
+  __shared__ float sh[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wj = (int)blockIdx.x & 3;
+  const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE);
+  const int64_t tile = (int64_t)blockIdx.x >> 2;
+  const int tile_j = (int)(tile / tiles_i), tile_i = (int)(tile % tiles_i);
+  const int rows = a.meta->rows;
+  if (tile_j * TILE + wj * 64 >= rows) return;
+  const int nw = (int)min((int64_t)TILE, a.v1 - a.v0 - (int64_t)tile_i * TILE);
+  float* st = a.stats + ((a.v0 / TILE + tile_i) * 5) * a.Np + tile_j * TILE + wj * 64;
+  const int wi = w >> 1;
+#pragma unroll
+  for (int tj = 0; tj < WT_J; ++tj) {
+    const int n = 32 * tj + (lane & 31);
+    const float m = tile_j * TILE + wj * 64 + n < rows ? st[2 * a.Np + n] : 0.f;
+    const float m0 = m == -INFINITY ? 0.f : m;
+    float c = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int ti = 2 * (w & 1) + t;
+      const int left = nw - 128 * wi - 32 * ti - 4 * (lane >> 5);
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int64_t o = tile * (TILE * TILE / 4) + ((ti * WT_J + tj) * 4 + e4) * NTHR +
+                          (wi * WAVES_J + wj) * 64 + lane;
+        const float4 z = reinterpret_cast<const float4*>(a.kept)[o];
+        const float4 t = reinterpret_cast<const float4*>(a.kept + a.kept_side)[o];
+        const float zs[4] = {z.x, z.y, z.z, z.w}, zt[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = exp_of(zt[e] - m0);
+          // a word without weight counts for nothing, however far the two sides are
+          if (8 * e4 + e < left && p != 0.f) c += p * (zt[e] - zs[e]);
+        }
+      }
+    }
+    c = swap32_sum(c);
+    if (lane < 32) sh[w][n] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64 && tile_j * TILE + wj * 64 + threadIdx.x < rows)
+    st[4 * a.Np + threadIdx.x] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] +
+                                 sh[3][threadIdx.x];
+}
+
 // ---- joining the tiles' statistics ------------------------------------------------------------------
 // 256 threads: 1 << rb_log rows, the rest of the threads along the tiles; each joins its tiles in order,
 // then pairs of threads join theirs, so the order is fixed.
@@ -532,14 +508,16 @@ struct JoinArgs {
   const int32_t* lab;
   int64_t Np;
   int tiles, rb_log;
-  float* loss;    // [N]
-  float* lse[2];  // [N]
+  float* loss;     // [N]
+  float* lse[2];   // [N]
   float* lsep[2];  // [Np], of the packed rows (or NULL)
+  float* apart;    // [Np] the teacher's normaliser less the student's (or NULL)
 };
-template <bool KL>
+enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
+template <int WHAT>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
-  __shared__ float sh[KL ? 5 : 2][256];
-  constexpr int PLANES = KL ? 5 : 2;
+  constexpr int PLANES = WHAT == JOIN_CE ? 2 : WHAT == JOIN_KL ? 5 : 4;
+  __shared__ float sh[PLANES][256];
   const int RB = 1 << a.rb_log, slices = 256 >> a.rb_log;
   const int rl = threadIdx.x & (RB - 1), sl = threadIdx.x >> a.rb_log;
   const int64_t p = (int64_t)blockIdx.x * RB + rl;
@@ -550,24 +528,25 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
     for (int t = sl; t < a.tiles; t += slices) {
       const float* v = a.stats + (int64_t)t * PLANES * a.Np + p;
       s0 = join(s0, Stat{v[0], v[a.Np], 0.f});
-      if constexpr (KL) s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], v[4 * a.Np]});
+      if constexpr (PLANES > 2)
+        s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], PLANES > 4 ? v[4 * a.Np] : 0.f});
     }
   }
   for (int half = slices / 2; half >= 1; half >>= 1) {
     if (sl >= half && sl < 2 * half) {
       sh[0][threadIdx.x] = s0.m;
       sh[1][threadIdx.x] = s0.s;
-      if constexpr (KL) {
+      if constexpr (PLANES > 2) {
         sh[2][threadIdx.x] = s1.m;
         sh[3][threadIdx.x] = s1.s;
-        sh[4][threadIdx.x] = s1.c;
+        if constexpr (PLANES > 4) sh[4][threadIdx.x] = s1.c;
       }
     }
     __syncthreads();
     if (sl < half) {
       const int i = threadIdx.x + half * RB;
       s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
-      if constexpr (KL) s1 = join(s1, Stat{sh[2][i], sh[3][i], sh[4][i]});
+      if constexpr (PLANES > 2) s1 = join(s1, Stat{sh[2][i], sh[3][i], PLANES > 4 ? sh[4][i] : 0.f});
     }
     // (the next round writes the lower half of what this one read)
   }
@@ -576,17 +555,40 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   const float lse = (float)((double)s0.m + log((double)s0.s));
   a.lse[0][r] = lse;
   if (a.lsep[0]) a.lsep[0][p] = lse;
-  if constexpr (KL) {
+  if constexpr (PLANES > 2) {
     const float lt = (float)((double)s1.m + log((double)s1.s));
     a.lse[1][r] = lt;
     if (a.lsep[1]) a.lsep[1][p] = lt;
-    // sum p (z_t - z_s) - (lse_t - lse_s), the normalisers' difference from the maxima's and the
-    // sums' quotient: as a difference of two rounded normalisers it would lose their common part
-    a.loss[r] = (float)((double)s1.c / s1.s - ((double)s1.m - s0.m) - log((double)s1.s / s0.s));
+    // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
+    // would lose their common part
+    const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
+    if constexpr (PLANES > 4) a.loss[r] = (float)((double)s1.c / s1.s - apart);
+    else a.apart[p] = (float)apart;
   } else {
     a.loss[r] = a.lab[p] < 0 ? __builtin_nanf("")
                              : (float)((double)s0.m - a.zlab[p] + log((double)s0.s));
   }
+}
+
+// The loss of every row that takes part from its parts [parts][Np], in order
+__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ part, int parts,
+                                                   const Meta* __restrict__ meta,
+                                                   const int32_t* __restrict__ src, int64_t Np,
+                                                   float* __restrict__ loss) {
+  __shared__ double sh[256];
+  const int rl = threadIdx.x & 7, sl = threadIdx.x >> 3;  // 8 rows
+  const int64_t p = (int64_t)blockIdx.x * 8 + rl;
+  const bool live = p < meta->rows;
+  double s = 0;
+  if (live) {
+#pragma unroll 4
+    for (int k = sl; k < parts; k += 32) s += part[k * Np + p];
+  }
+  sh[threadIdx.x] = s;
+  __syncthreads();
+  if (!live || sl != 0) return;
+  for (int k = 1; k < 32; ++k) s += sh[k * 8 + rl];
+  loss[src[p]] = (float)s;
 }
 
 // out = {sum, mean over the rows that take part (0 without one), their number}
@@ -611,95 +613,119 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ l
 }
 
 // ---- dz of tiles that were kept ----------------------------------------------------------------------
-// A workgroup takes 32 words x 256 rows (wave column wj the rows 64 wj ..): HBM-bound, 4 (cross entropy,
-// in place) or 10 bytes a logit. The cross entropy's block of exponentials lies where its dz goes, and
-// is in registers before any of that is written.
+// A workgroup takes blocks of 32 words x 256 rows (wave column wj the rows 64 wj ..): HBM-bound, 4
+// (cross entropy, in place) or 10 bytes a logit. The cross entropy's block of exponentials lies where
+// its dz goes, and is in registers before any of that is written. A distillation's blocks also add up
+// their words' share of the loss.
 struct FinishArgs {
   uint16_t* dzt;
-  int64_t words, V, Np;
+  int64_t words, n, Np;  // of the panels, of the piece
+  int per;               // blocks of a workgroup: 1, 2, 4 or 8 of a tile
   const Meta* meta;
   const int32_t* lab;
   const float* stats;
   const float* zlab;
   const float* lse[2];  // [Np]
-  float inv_t;
-  const float* park;
+  const float* apart;   // [Np]
+  const float* g;       // [Np] or NULL
   const float* kept;
+  int64_t kept_side;
+  float* loss;  // [words / 32 / per][Np], or NULL
 };
 template <bool KL>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
   __shared__ __align__(16) uint8_t st[32 * EPI_RS];
   const int lane = threadIdx.x & 63, wj = threadIdx.x >> 6;
-  const int tiles_i = (int)(a.words / TILE), block = (int)blockIdx.x % 8;
-  const int64_t tile = (int64_t)blockIdx.x / 8;
+  const int tiles_i = (int)((a.n + TILE - 1) / TILE), of = 8 / a.per;
+  const int64_t tile = (int64_t)blockIdx.x / of;
   const int tile_j = (int)(tile / tiles_i), tile_i = (int)(tile % tiles_i);
   const int rows = a.meta->rows;
   if (tile_j * TILE >= rows) return;
-  const int wi = block >> 2, ti = block & 3;
-  uint8_t* at = reinterpret_cast<uint8_t*>(a.dzt + ((int64_t)tile_j * a.words + tile_i * TILE) * TILE) +
-                block * 16384;
-  const int v0 = tile_i * TILE + block * 32;  // the block's first word
-  uint4 raw[KL ? 1 : WT_J][2];
-  if constexpr (!KL) {
+  const int part = (int)blockIdx.x % of;
+  float kl[WT_J] = {0.f, 0.f};
+  for (int block = part * a.per; block < (part + 1) * a.per; ++block) {
+    const int wi = block >> 2, ti = block & 3;
+    uint8_t* at = reinterpret_cast<uint8_t*>(a.dzt + ((int64_t)tile_j * a.words + tile_i * TILE) * TILE) +
+                  block * 16384;
+    const int v0 = tile_i * TILE + block * 32;  // the block's first word
+    uint4 raw[KL ? 1 : WT_J][2];
+    if constexpr (!KL) {
 #pragma unroll
-    for (int tj = 0; tj < WT_J; ++tj)
+      for (int tj = 0; tj < WT_J; ++tj)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        raw[tj][h] = *reinterpret_cast<const uint4*>(at + wj * 4096 + tj * 2048 + h * 1024 + lane * 16);
-  }
+        for (int h = 0; h < 2; ++h)
+          raw[tj][h] = *reinterpret_cast<const uint4*>(at + wj * 4096 + tj * 2048 + h * 1024 + lane * 16);
+    }
 #pragma unroll
-  for (int tj = 0; tj < WT_J; ++tj) {
-    const int nl = wj * 64 + 32 * tj + (lane & 31), n = tile_j * TILE + nl;
-    const bool live = n < rows;
-    const float lse = live ? a.lse[0][n] : 0.f;
-    float d[16];
-    if constexpr (KL) {
-      const float lt = live ? a.lse[1][n] : 0.f;
+    for (int tj = 0; tj < WT_J; ++tj) {
+      const int nl = wj * 64 + 32 * tj + (lane & 31), n = tile_j * TILE + nl;
+      const bool live = n < rows;
+      const float lse = live ? a.lse[0][n] : 0.f;
+      const int left = (int)(a.n - v0) - 4 * (lane >> 5);  // words from the lane's first one
+      float d[16];
+      if constexpr (KL) {
+        const float lt = live ? a.lse[1][n] : 0.f, apart = live && a.loss ? a.apart[n] : 0.f;
+        const float g = live && a.g ? a.g[n] : 1.f;
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int64_t o = tile * (TILE * TILE / 4) + ((ti * WT_J + tj) * 4 + e4) * NTHR +
-                          (wi * WAVES_J + wj) * 64 + lane;
-        const float4 z = reinterpret_cast<const float4*>(a.kept)[o];
-        const float4 t = reinterpret_cast<const float4*>(a.park)[o];
-        d[4 * e4] = exp_of(z.x * a.inv_t - lse) - exp_of(t.x * a.inv_t - lt);
-        d[4 * e4 + 1] = exp_of(z.y * a.inv_t - lse) - exp_of(t.y * a.inv_t - lt);
-        d[4 * e4 + 2] = exp_of(z.z * a.inv_t - lse) - exp_of(t.z * a.inv_t - lt);
-        d[4 * e4 + 3] = exp_of(z.w * a.inv_t - lse) - exp_of(t.w * a.inv_t - lt);
-      }
-    } else {
-      const int l = live ? a.lab[n] : 0;
-      float f = live ? exp_of(a.stats[(int64_t)tile_i * 2 * a.Np + n] - lse) : 0.f;
-      if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int64_t o = tile * (TILE * TILE / 4) + ((ti * WT_J + tj) * 4 + e4) * NTHR +
+                            (wi * WAVES_J + wj) * 64 + lane;
+          const float4 z = reinterpret_cast<const float4*>(a.kept)[o];
+          const float4 t = reinterpret_cast<const float4*>(a.kept + a.kept_side)[o];
+          const float zs[4] = {z.x, z.y, z.z, z.w}, zt[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w[4] = {raw[tj][h].x, raw[tj][h].y, raw[tj][h].z, raw[tj][h].w};
+          for (int e = 0; e < 4; ++e) {
+            const float q = exp_of(zs[e] - lse), p = exp_of(zt[e] - lt);
+            d[4 * e4 + e] = (q - p) * g;
+            // a word without weight counts for nothing, however far the two sides are
+            if (8 * e4 + e < left && p != 0.f) kl[tj] += p * ((zt[e] - zs[e]) - apart);
+          }
+        }
+      } else {
+        const int l = live ? a.lab[n] : 0;
+        float f = live ? exp_of(a.stats[(int64_t)tile_i * 2 * a.Np + n] - lse) : 0.f;
+        if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[8 * h + 2 * e] = h2f(w[e] & 0xffffu) * f;
-          d[8 * h + 2 * e + 1] = h2f(w[e] >> 16) * f;
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w[4] = {raw[tj][h].x, raw[tj][h].y, raw[tj][h].z, raw[tj][h].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d[8 * h + 2 * e] = h2f(w[e] & 0xffffu) * f;
+            d[8 * h + 2 * e + 1] = h2f(w[e] >> 16) * f;
+          }
+        }
+        // the label's word from the logit itself
+        const int lv = l - v0 - 4 * (lane >> 5);
+        if (live && lv >= 0 && lv < 32 && (lv & 4) == 0) {
+          const float dl = exp_of(a.zlab[n] - lse) - 1.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) d[e] = lv == 8 * (e >> 2) + (e & 3) ? dl : d[e];
         }
       }
-      // the label's word from the logit itself
-      const int lv = l - v0 - 4 * (lane >> 5);
-      if (live && lv >= 0 && lv < 32 && (lv & 4) == 0) {
-        const float dl = exp_of(a.zlab[n] - lse) - 1.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] = lv == 8 * (e >> 2) + (e & 3) ? dl : d[e];
+      for (int e = 0; e < 16; ++e) {
+        const int row = 8 * (e >> 2) + (e & 3);
+        *reinterpret_cast<uint16_t*>(st + (row + 4 * (lane >> 5)) * EPI_RS + nl * 2) =
+            (uint16_t)f2bf(live && row < left ? d[e] : 0.f);
       }
     }
+    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int row = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-      *reinterpret_cast<uint16_t*>(st + row * EPI_RS + nl * 2) =
-          (uint16_t)f2bf(live && v0 + row < a.V ? d[e] : 0.f);
+    for (int it = 0; it < 4; ++it) {
+      const int c = it * 256 + threadIdx.x;
+      *reinterpret_cast<uint4*>(at + c * 16) =
+          *reinterpret_cast<const uint4*>(st + (c >> 5) * EPI_RS + (c & 31) * 16);
     }
+    __syncthreads();
   }
-  __syncthreads();
+  if constexpr (KL) {
+    if (!a.loss) return;
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int c = it * 256 + threadIdx.x;
-    *reinterpret_cast<uint4*>(at + c * 16) =
-        *reinterpret_cast<const uint4*>(st + (c >> 5) * EPI_RS + (c & 31) * 16);
+    for (int tj = 0; tj < WT_J; ++tj) {
+      const int n = tile_j * TILE + wj * 64 + 32 * tj + (lane & 31);
+      const float s = swap32_sum(kl[tj]);
+      if (lane < 32 && n < rows) a.loss[((int64_t)tile_i * of + part) * a.Np + n] = s;
+    }
   }
 }
 
@@ -880,18 +906,18 @@ static int cu_count() {
 }
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Words of a piece: dz^T of all rows in kPieceBytes and W's rows of it within the 4 GiB that the copies
-// of dx address, the pieces of one size but for the last tiles.
-static int64_t piece_words(int64_t N, int64_t V, int64_t H) {
+// Words of a piece: `bytes` a logit of all rows in kPieceBytes and W's rows of it within the 4 GiB that
+// the copies of dx address, the pieces of one size but for the last tiles.
+static int64_t piece_words(int64_t N, int64_t V, int64_t H, int bytes) {
   const int64_t tiles = up(V, TILE) / TILE;
-  int64_t most = std::min((int64_t)(kPieceBytes / 2) / up(N, TILE), (((int64_t)1 << 31) - 1) / H) / TILE;
+  int64_t most = std::min((int64_t)(kPieceBytes / bytes) / std::max(up(N, TILE), (int64_t)1), (((int64_t)1 << 31) - 1) / H) / TILE;
   most = std::max(most, (int64_t)1);
   const int64_t pieces = (tiles + most - 1) / most;
   return (tiles + pieces - 1) / pieces * TILE;
 }
 // Floats of dx's parts: the splits that all rows would take
 static int64_t part_floats(int64_t N, int64_t words, int64_t H) {
-  return (int64_t)dx_splits(N, words, H, cu_count(), INT64_MAX) * N * H;
+  return (int64_t)dx_splits(N, words, H, cu_count()) * N * H;
 }
 
 // The workspace, carved in order; p = NULL: sizes only.
@@ -911,17 +937,25 @@ struct Ws {
   uint16_t* xp[2];
   float* zlab;
   float* stats;
-  float* park;
   float* kept;
   float* lse[2];
+  float* apart;
+  float* kl;
   float* g;
   uint16_t* dzt;
   float* part;
+  int64_t words;  // of a piece
 };
 enum { WS_FWD, WS_BWD, WS_STEP };
+// Blocks of 32 words that a workgroup of the finishing pass takes: a tile where there are many
+static int finish_per(int64_t N, int64_t words) {
+  const int64_t tiles = up(N, TILE) / TILE * (words / TILE);
+  return tiles >= 4096 ? 8 : tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
+}
 static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
   Ws w = {};
   const int64_t Np = up(N, TILE), Vp = up(V, TILE);
+  w.words = use == WS_STEP ? Vp : piece_words(N, V, H, !Ht ? 2 : use == WS_FWD ? 8 : 10);
   w.meta = c.take<Meta>(1);
   w.pos = c.take<int32_t>(N);
   w.src = c.take<int32_t>(Np);
@@ -929,20 +963,21 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
   w.xp[0] = c.take<uint16_t>(Np * H);
   if (Ht) {
     w.xp[1] = c.take<uint16_t>(Np * Ht);
-    w.park = c.take<float>(use == WS_STEP ? (size_t)(Np * Vp)
-                                          : (size_t)(cu_count() / 8 * 8) * TILE * TILE);
-    if (use == WS_STEP) w.kept = c.take<float>((size_t)(Np * Vp));
-  }
-  if (use != WS_BWD) {
+    w.kept = c.take<float>((size_t)(2 * Np * w.words));
+  } else {
     w.zlab = c.take<float>(Np);
-    w.stats = c.take<float>((size_t)(Vp / TILE) * (Ht ? 5 : 2) * Np);
   }
+  if (Ht || use != WS_BWD)
+    w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / TILE) * (Ht ? 5 : 2) * Np);
   if (use == WS_FWD) return w;
-  const int64_t words = use == WS_STEP ? Vp : piece_words(N, V, H);
   for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
   if (use == WS_BWD) w.g = c.take<float>(Np);
-  w.dzt = c.take<uint16_t>((size_t)words * Np);
-  if (grad_x) w.part = c.take<float>((size_t)part_floats(N, words, H));
+  if (use == WS_STEP && Ht) {
+    w.apart = c.take<float>(Np);
+    w.kl = c.take<float>((size_t)(Vp / 32 / finish_per(N, Vp)) * Np);
+  }
+  w.dzt = c.take<uint16_t>((size_t)w.words * Np);
+  if (grad_x) w.part = c.take<float>((size_t)part_floats(N, w.words, H));
   return w;
 }
 // Whether the forward of so many rows may keep what the gradients are made of
@@ -1006,18 +1041,21 @@ static void set_splits(PackArgs& p, const Sides& s, int64_t words) {
   p.cus = cu_count();
 }
 static int pack(const PackArgs& a, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows + BK / kPackRows)),
+                     dim3(256), 0, st, a);
   return check_launch(what);
 }
 static LogitArgs logit_args(const Sides& s, const Ws& w) {
   LogitArgs a = {};
   a.w[0] = s.w; a.x[0] = w.xp[0]; a.H[0] = s.H;
   a.w[1] = s.tw; a.x[1] = w.xp[1]; a.H[1] = s.Ht;
+  a.sides = s.Ht ? 2 : 1;
   a.Np = up(s.N, TILE);
-  a.meta = w.meta; a.lab = w.lab; a.inv_t = s.inv_t; a.park = w.park;
+  a.meta = w.meta; a.lab = w.lab; a.inv_t = s.inv_t;
   a.stats = w.stats; a.zlab = w.zlab;
-  a.lse[0] = w.lse[0]; a.lse[1] = w.lse[1];
-  a.dzt = w.dzt; a.kept = w.kept;
+  a.lse = w.lse[0];
+  a.dzt = w.dzt; a.words = w.words;
+  a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
   return a;
 }
 template <int MODE>
@@ -1065,6 +1103,22 @@ struct Products {
   }
 };
 
+static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
+  FinishArgs f = {};
+  f.dzt = w.dzt; f.words = w.words; f.n = n; f.Np = up(s.N, TILE);
+  f.per = finish_per(s.N, w.words);
+  f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
+  f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
+  f.kept = w.kept; f.kept_side = f.Np * w.words;
+  return f;
+}
+template <bool KL>
+static int finish(const FinishArgs& f, hipStream_t st, const char* what) {
+  hipLaunchKernelGGL(finish_kernel<KL>, dim3((unsigned)(f.Np / TILE * (up(f.n, TILE) / TILE) * (8 / f.per))),
+                     dim3(256), 0, st, f);
+  return check_launch(what);
+}
+
 // The forward, and with grad_x or grad_w the gradients of its sum or mean (step)
 template <bool KL, bool STEP>
 static int forward(const Sides& s, int reduction, float* loss, float* lse, float* total,
@@ -1099,11 +1153,19 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     }
     if (int rc = pack(p, st, what)) return rc;
     LogitArgs l = logit_args(s, w);
-    l.v0 = 0;
-    l.v1 = s.V;
-    l.words = Vp;
-    constexpr int MODE = STEP ? (KL ? KL_KEEP : CE_KEEP) : (KL ? KL_STATS : CE_STATS);
-    if (int rc = logits<MODE>(l, st, what)) return rc;
+    l.planes = !KL ? 2 : STEP ? 4 : 5;
+    for (int64_t v0 = 0; v0 < s.V; v0 += KL ? w.words : s.V) {
+      l.v0 = v0;
+      l.v1 = KL ? std::min(s.V, v0 + w.words) : s.V;
+      l.tile0 = (int)(v0 / TILE);
+      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, st, what)) return rc;
+      if (KL && !STEP) {
+        const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1};
+        hipLaunchKernelGGL(cross_kernel, dim3((unsigned)(Np / TILE * (up(l.v1 - l.v0, TILE) / TILE) * 4)),
+                           dim3(256), 0, st, x);
+        if (int rc = check_launch(what)) return rc;
+      }
+    }
     JoinArgs j = {};
     j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
     j.Np = Np;
@@ -1114,19 +1176,26 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.lse[1] = lse + s.N;
     j.lsep[0] = w.lse[0];
     j.lsep[1] = w.lse[1];
-    hipLaunchKernelGGL(join_kernel<KL>, dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)),
-                       dim3(256), 0, st, j);
+    j.apart = w.apart;
+    hipLaunchKernelGGL(join_kernel<!KL ? JOIN_CE : STEP ? JOIN_LSE : JOIN_KL>,
+                       dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)), dim3(256), 0, st, j);
     if (int rc = check_launch(what)) return rc;
+  }
+  if (STEP && (KL || grad_x || grad_w)) {
+    FinishArgs f = finish_args(s, w, s.V);
+    f.loss = w.kl;
+    if (int rc = finish<KL>(f, st, what)) return rc;
+    if (KL) {
+      hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((s.N + 7) / 8)), dim3(256), 0, st, w.kl,
+                         (int)(Vp / 32 / f.per), w.meta, w.src, Np, loss);
+      if (int rc = check_launch(what)) return rc;
+    }
   }
   if (total) {
     hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, s.N, w.meta, total);
     if (int rc = check_launch(what)) return rc;
   }
   if (!STEP || (!grad_x && !grad_w)) return PLZ_OK;
-  const FinishArgs f = {w.dzt, Vp, s.V, Np, w.meta, w.lab, w.stats, w.zlab, {w.lse[0], w.lse[1]},
-                        s.inv_t, w.park, w.kept};
-  hipLaunchKernelGGL(finish_kernel<KL>, dim3((unsigned)(Np / TILE * (Vp / TILE) * 8)), dim3(256), 0, st, f);
-  if (int rc = check_launch(what)) return rc;
   const Products prod = {s, w, grad_x, grad_w, Vp, st, what};
   if (int rc = prod.piece(0, s.V, false)) return rc;
   return prod.sum();
@@ -1151,7 +1220,7 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
   Carve c{reinterpret_cast<char*>(ws)};
   const Ws w = carve(c, WS_BWD, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
-  const int64_t words = piece_words(s.N, s.V, s.H);
+  const int64_t words = w.words;
   PackArgs p = pack_args(s, w);
   p.grad = grad;
   p.reduction = reduction;
@@ -1164,12 +1233,17 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   if (int rc = pack(p, st, what)) return rc;
   LogitArgs l = logit_args(s, w);
   l.g = p.g;
-  l.words = words;
+  l.planes = KL ? 4 : 2;
   const Products prod = {s, w, grad_x, grad_w, words, st, what};
   for (int64_t v0 = 0; v0 < s.V; v0 += words) {
     l.v0 = v0;
     l.v1 = std::min(s.V, v0 + words);
-    if (int rc = logits<KL ? KL_GRAD : CE_GRAD>(l, st, what)) return rc;
+    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, st, what)) return rc;
+    if (KL) {
+      FinishArgs f = finish_args(s, w, l.v1 - l.v0);
+      f.g = p.g;
+      if (int rc = finish<true>(f, st, what)) return rc;
+    }
     if (int rc = prod.piece(v0, l.v1 - v0, v0 > 0)) return rc;
   }
   return prod.sum();

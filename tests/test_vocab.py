@@ -68,7 +68,7 @@ def test_workspaces(lib):
     assert bwd(N, V, H, 0, 1) < (1 << 30) + (1 << 29)
     assert bwd(N, V, H, 0, 0) < bwd(N, V, H, 0, 1) < bwd(N, V, H, 2560, 1)
     assert bwd(1 << 17, V, 2560, 0, 0) < (1 << 30) + (1 << 30)
-    assert fwd(0, 1, 8, 0) > 0
+    assert fwd(0, 1, 8, 0) > 0 and fwd(0, 1, 8, 8) > 0
     assert fwd(-1, 100, 64, 0) == 0 and bwd(0, 100, 64, 0, 1) == 0
 
 

@@ -442,6 +442,199 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   }
 }
 
+// ---- tiles of logits of few rows ------------------------------------------------------------------------
+// 128 words x 32 NB rows by four waves of 32 words each, reduction stages of 64 through a ring of
+// kFewSlots of the words' 16 KB and the rows' 4 NB KB: two workgroups a CU, each with several stages on
+// their way, where the 256x256 tiles would leave CUs without work or multiply rows that do not exist.
+// HBM-bound for up to 32 rows (W is read once, ~100 KB a CU in flight), by the LDS reads of five
+// fragments for four MFMAs at 128. The statistics are those of 128 words.
+constexpr int kFewWords = 128;
+constexpr int kFewThreads = 256;
+template <int NB>
+constexpr int few_slots() { return NB == 1 ? 4 : NB == 2 ? 3 : 2; }
+template <int NB>
+constexpr int few_stage() { return (kFewWords + 32 * NB) * BK * 2; }
+
+// acc[word, row] of the wave's 32 words and 32 NB rows; of the tile's 128 words, nw exist
+template <int MODE, int NB>
+__device__ __forceinline__ void few_tile(lds_u8* lbase, const uint16_t* w, const uint16_t* x, int64_t H,
+                                         int nw, f32x16 (&acc)[NB], int wave, int lane) {
+  constexpr int SLOTS = few_slots<NB>(), STAGE = few_stage<NB>(), COPIES = 4 + NB;
+  // copies: a lane's chunk of 16 bytes of every 32 rows, swizzled as the core's row tiles
+  const BufRsrc rw = make_rsrc(w, (uint32_t)(nw * H * 2)), rx = make_rsrc(x, (uint32_t)(32 * NB * H * 2));
+  uint32_t ow[4], ox[NB];
+  const int row = threadIdx.x >> 3, ch = (threadIdx.x & 7) ^ row_swz(row);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ow[i] = (uint32_t)((min(32 * i + row, nw - 1) * H + ch * 8) * 2);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) ox[i] = (uint32_t)(((32 * i + row) * H + ch * 8) * 2);
+  const int wbase = __builtin_amdgcn_readfirstlane(wave * 1024);
+  auto copy = [&](int kt, int slot) {
+    lds_u8* d = lbase + slot * STAGE + wbase;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, d + i * 4096, 16, ow[i], kt * (BK * 2), 0, 0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, d + (4 + i) * 4096, 16, ox[i], kt * (BK * 2), 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
+  auto stage = [&](const lds_u8* s, int nks) {
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      if (ks >= nks) break;
+      const bf16x8 fa = frag_row((const uint4*)s, 32 * wave, ks, lane);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            fa, frag_row((const uint4*)(s + 16384), 32 * i, ks, lane), acc[i], 0, 0, 0);
+    }
+  };
+  // Stage kt is waited for with the SLOTS - 2 stages behind it still on their way; the barrier also
+  // frees the slot of stage kt - 1, which stage kt + SLOTS - 1 goes to. Past the last stage the copies
+  // repeat it, so that every stage waits for as many.
+  const int nfull = (int)(H / BK);
+  if (nfull > 0) {
+#pragma unroll
+    for (int k = 0; k < SLOTS - 1; ++k) copy(min(k, nfull - 1), k);
+    int slot = 0;
+    for (int kt = 0; kt < nfull; ++kt) {
+      wait_vmcnt<(SLOTS - 2) * COPIES>();
+      stage_barrier();
+      copy(min(kt + SLOTS - 1, nfull - 1), slot == 0 ? SLOTS - 1 : slot - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      stage(lbase + slot * STAGE, BK / 16);
+      slot = slot == SLOTS - 1 ? 0 : slot + 1;
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
+  __syncthreads();
+  if (H % BK) {
+    const int64_t r0 = (int64_t)nfull * BK;
+    const int c = threadIdx.x & 7;
+#pragma unroll
+    for (int i = 0; i < 4 + NB; ++i) {
+      const int r = 32 * i + row;  // of the words, then of the rows
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r0 + 8 * c < H && (i >= 4 || r < nw))
+        v = *reinterpret_cast<const uint4*>((i < 4 ? w + r * H : x + (r - kFewWords) * H) + r0 + 8 * c);
+      reinterpret_cast<lds_u32x4*>(lbase)[row_chunk(r, c)] = u32x4{v.x, v.y, v.z, v.w};
+    }
+    __syncthreads();
+    stage(lbase, (int)((H % BK + 15) / 16));
+    __syncthreads();
+  }
+}
+
+template <int MODE, int NB>
+__global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a) {
+  extern __shared__ uint4 smem[];
+  lds_u8* lbase = (lds_u8*)smem;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rows = a.meta->rows;
+  const int tiles_i = (int)((a.v1 - a.v0 + kFewWords - 1) / kFewWords);
+  const int tiles_j = (rows + 32 * NB - 1) / (32 * NB);
+  const int total = tiles_i * tiles_j;
+  int at = (int)blockIdx.x, side = 0;
+  if (MODE == Z_KEEP && at >= total) {
+    at -= total;
+    side = 1;
+  }
+  if (at >= total || (side == 1 && a.sides < 2)) return;
+  // the rows' tiles of a tile of words on one XCD, after each other
+  const int xcd = at % 8, q8 = total / 8, r8 = total % 8;
+  const int item = xcd * q8 + (xcd < r8 ? xcd : r8) + at / 8;
+  const int tile_i = item / tiles_j, tile_j = item % tiles_j;
+  const int64_t i0 = a.v0 + (int64_t)tile_i * kFewWords, j0 = (int64_t)tile_j * (32 * NB), H = a.H[side];
+  const int nw = (int)min((int64_t)kFewWords, a.v1 - i0);
+  f32x16 acc[NB];
+  few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, acc, wave, lane);
+
+  // The wave's 32 words of the panel's block, 16 a lane: word vl + 8 (e / 4) + e % 4 of the tile.
+  const int vl = 32 * wave + 4 * (lane >> 5);
+  const int64_t rel = i0 - a.v0;  // within the launch
+  const int block = (int)(rel % TILE) / 32 + wave, wi = block >> 2, ti = block & 3;
+  lds_f32* ex = reinterpret_cast<lds_f32*>(lbase);
+  float m[NB], sum[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int64_t n = j0 + 32 * i + (lane & 31);
+    const int nb = (int)(n % TILE) / 32;
+    if constexpr (MODE == Z_KEEP) {
+      const int tiles256 = (int)((a.v1 - a.v0 + TILE - 1) / TILE);
+      float* const kept = a.kept + side * a.kept_side +
+                          ((j0 + 32 * i) / TILE * tiles256 + rel / TILE) * (TILE * TILE);
+      acc[i] *= a.inv_t;
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const f32x4 v = {acc[i][4 * e4], acc[i][4 * e4 + 1], acc[i][4 * e4 + 2], acc[i][4 * e4 + 3]};
+        *reinterpret_cast<f32x4*>(kept + ((ti * WT_J + (nb & 1)) * 4 + e4) * NTHR * 4 +
+                                  ((wi * WAVES_J + (nb >> 1)) * 64 + lane) * 4) = v;
+      }
+    } else if (n < rows) {
+      const int lv = a.lab[n] - (int)i0 - vl;
+      if (lv >= 0 && lv < 32 && (lv & 4) == 0) {
+        float zl = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zl = lv == 8 * (e >> 2) + (e & 3) ? acc[i][e] : zl;
+        a.zlab[n] = zl;
+      }
+    }
+    m[i] = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (8 * (e >> 2) + (e & 3) >= nw - vl) acc[i][e] = -INFINITY;
+      m[i] = fmaxf(m[i], acc[i][e]);
+    }
+    m[i] = swap32_max(m[i]);
+    if (lane < 32) ex[wave * (32 * NB) + 32 * i + lane] = m[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[i] = fmaxf(m[i], ex[k * (32 * NB) + 32 * i + (lane & 31)]);
+    const float m0 = m[i] == -INFINITY ? 0.f : m[i];
+    const int64_t n0 = j0 + 32 * i;
+    uint16_t* const exps =
+        MODE == CE_KEEP ? a.dzt + (n0 / TILE * a.words + rel / TILE * TILE) * TILE + block * 8192 +
+                              (n0 % TILE) / 32 * 1024
+                        : nullptr;
+    sum[i] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = exp_of(acc[i][8 * h + e] - m0);
+        sum[i] += p[e];
+      }
+      if constexpr (MODE == CE_KEEP) {
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);
+        *reinterpret_cast<u32x4*>(exps + h * 512 + lane * 8) = v;
+      }
+    }
+    sum[i] = swap32_sum(sum[i]);
+    if (lane < 32) ex[(4 + wave) * (32 * NB) + 32 * i + lane] = sum[i];
+  }
+  __syncthreads();
+  const int64_t n = j0 + threadIdx.x;
+  if (threadIdx.x < 32 * NB && n < rows) {
+    float t = -INFINITY, u = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      t = fmaxf(t, ex[k * (32 * NB) + threadIdx.x]);
+      u += ex[(4 + k) * (32 * NB) + threadIdx.x];
+    }
+    float* out = a.stats + ((int64_t)(a.tile0 + tile_i) * a.planes + 2 * side) * a.Np + n;
+    out[0] = t;
+    out[a.Np] = u;
+  }
+}
+
 // Sum of p (t - s) over the words of each tile of a launch that kept both sides' logits, with the
 // weights relative to the teacher's maximum of the tile: the fifth plane of the statistics. HBM-bound, 8
 // bytes a logit. A workgroup takes a tile's column of 64 rows, wave w its words 64 w .. 64 w + 63.
@@ -451,6 +644,7 @@ struct CrossArgs {
   const Meta* meta;
   float* stats;
   int64_t Np, v0, v1;
+  int halves;  // statistics of 128 words
 };
 __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
   __shared__ float sh[4][64];
@@ -461,12 +655,15 @@ __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
   const int rows = a.meta->rows;
   if (tile_j * TILE + wj * 64 >= rows) return;
   const int nw = (int)min((int64_t)TILE, a.v1 - a.v0 - (int64_t)tile_i * TILE);
-  float* st = a.stats + ((a.v0 / TILE + tile_i) * 5) * a.Np + tile_j * TILE + wj * 64;
+  // the statistics of this wave's words
   const int wi = w >> 1;
+  float* const st0 = a.stats + tile_j * TILE + wj * 64;
+  const int64_t tile_v = a.v0 / TILE + tile_i;
+  const float* st = st0 + (a.halves ? 2 * tile_v + wi : tile_v) * 5 * a.Np;
 #pragma unroll
   for (int tj = 0; tj < WT_J; ++tj) {
     const int n = 32 * tj + (lane & 31);
-    const float m = tile_j * TILE + wj * 64 + n < rows ? st[2 * a.Np + n] : 0.f;
+    const float m = (!a.halves || nw > 128 * wi) && tile_j * TILE + wj * 64 + n < rows ? st[2 * a.Np + n] : 0.f;
     const float m0 = m == -INFINITY ? 0.f : m;
     float c = 0.f;
 #pragma unroll
@@ -492,9 +689,9 @@ __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
     if (lane < 32) sh[w][n] = c;
   }
   __syncthreads();
-  if (threadIdx.x < 64 && tile_j * TILE + wj * 64 + threadIdx.x < rows)
-    st[4 * a.Np + threadIdx.x] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] +
-                                 sh[3][threadIdx.x];
+  if (lane + tile_j * TILE + wj * 64 >= rows || w > (a.halves && nw > 128 ? 1 : 0)) return;
+  if (a.halves) st0[((2 * tile_v + w) * 5 + 4) * a.Np + lane] = sh[2 * w][lane] + sh[2 * w + 1][lane];
+  else st0[(tile_v * 5 + 4) * a.Np + lane] = sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane];
 }
 
 // ---- joining the tiles' statistics ------------------------------------------------------------------
@@ -621,6 +818,7 @@ struct FinishArgs {
   uint16_t* dzt;
   int64_t words, n, Np;  // of the panels, of the piece
   int per;               // blocks of a workgroup: 1, 2, 4 or 8 of a tile
+  int stat_log;          // words of a statistic: 7 or 8
   const Meta* meta;
   const int32_t* lab;
   const float* stats;
@@ -683,7 +881,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         }
       } else {
         const int l = live ? a.lab[n] : 0;
-        float f = live ? exp_of(a.stats[(int64_t)tile_i * 2 * a.Np + n] - lse) : 0.f;
+        float f = live && v0 < a.n ? exp_of(a.stats[(int64_t)(v0 >> a.stat_log) * 2 * a.Np + n] - lse) : 0.f;
         if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -947,6 +1145,9 @@ struct Ws {
   int64_t words;  // of a piece
 };
 enum { WS_FWD, WS_BWD, WS_STEP };
+// Whether the tiles are those of few rows
+static bool few(int64_t N) { return N <= 128; }
+static int stat_words(int64_t N) { return few(N) ? kFewWords : TILE; }
 // Blocks of 32 words that a workgroup of the finishing pass takes: a tile where there are many
 static int finish_per(int64_t N, int64_t words) {
   const int64_t tiles = up(N, TILE) / TILE * (words / TILE);
@@ -968,7 +1169,7 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
     w.zlab = c.take<float>(Np);
   }
   if (Ht || use != WS_BWD)
-    w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / TILE) * (Ht ? 5 : 2) * Np);
+    w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / stat_words(N)) * (Ht ? 5 : 2) * Np);
   if (use == WS_FWD) return w;
   for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
   if (use == WS_BWD) w.g = c.take<float>(Np);
@@ -1058,8 +1259,23 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
   return a;
 }
+template <int MODE, int NB>
+static int few_logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* what) {
+  static uint64_t done = 0;
+  auto kern = few_kernel<MODE, NB>;
+  constexpr size_t lds = (size_t)few_slots<NB>() * few_stage<NB>();
+  if (int rc = reserve_lds((const void*)kern, lds, done, what)) return rc;
+  const int64_t items = up(a.v1 - a.v0, kFewWords) / kFewWords * (up(N, 32 * NB) / (32 * NB)) * a.sides;
+  hipLaunchKernelGGL(kern, dim3((unsigned)items), dim3(kFewThreads), lds, st, a);
+  return check_launch(what);
+}
 template <int MODE>
-static int logits(const LogitArgs& a, hipStream_t st, const char* what) {
+static int logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* what) {
+  if constexpr (MODE != CE_GRAD) {
+    if (few(N))
+      return N <= 32 ? few_logits<MODE, 1>(a, N, st, what)
+             : N <= 64 ? few_logits<MODE, 2>(a, N, st, what) : few_logits<MODE, 4>(a, N, st, what);
+  }
   static uint64_t done = 0;
   auto kern = logits_kernel<MODE>;
   if (int rc = reserve_lds((const void*)kern, kLdsLogits, done, what)) return rc;
@@ -1107,6 +1323,7 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   FinishArgs f = {};
   f.dzt = w.dzt; f.words = w.words; f.n = n; f.Np = up(s.N, TILE);
   f.per = finish_per(s.N, w.words);
+  f.stat_log = few(s.N) ? 7 : 8;
   f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
   f.kept = w.kept; f.kept_side = f.Np * w.words;
@@ -1157,10 +1374,10 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     for (int64_t v0 = 0; v0 < s.V; v0 += KL ? w.words : s.V) {
       l.v0 = v0;
       l.v1 = KL ? std::min(s.V, v0 + w.words) : s.V;
-      l.tile0 = (int)(v0 / TILE);
-      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, st, what)) return rc;
+      l.tile0 = (int)(v0 / stat_words(s.N));
+      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, s.N, st, what)) return rc;
       if (KL && !STEP) {
-        const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1};
+        const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1, few(s.N)};
         hipLaunchKernelGGL(cross_kernel, dim3((unsigned)(Np / TILE * (up(l.v1 - l.v0, TILE) / TILE) * 4)),
                            dim3(256), 0, st, x);
         if (int rc = check_launch(what)) return rc;
@@ -1169,7 +1386,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     JoinArgs j = {};
     j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
     j.Np = Np;
-    j.tiles = (int)(Vp / TILE);
+    j.tiles = (int)(up(s.V, stat_words(s.N)) / stat_words(s.N));
     j.rb_log = s.N >= 4096 ? 4 : s.N >= 512 ? 2 : 0;
     j.loss = loss;
     j.lse[0] = lse;
@@ -1238,7 +1455,7 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   for (int64_t v0 = 0; v0 < s.V; v0 += words) {
     l.v0 = v0;
     l.v1 = std::min(s.V, v0 + words);
-    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, st, what)) return rc;
+    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, s.N, st, what)) return rc;
     if (KL) {
       FinishArgs f = finish_args(s, w, l.v1 - l.v0);
       f.g = p.g;

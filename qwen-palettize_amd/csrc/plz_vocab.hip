@@ -48,6 +48,7 @@ enum { CE_STATS, CE_GRAD, CE_KEEP, Z_KEEP };
 // ---- rows that take part --------------------------------------------------------------------------
 struct Meta {
   int rows;     // how many take part
+  int done;     // workgroups that have written their rows' losses
   float alpha;  // backward: the scale of the gradients that every row shares
   int z;        // backward: splits of dx's reduction over the words of a piece
 };
@@ -76,11 +77,11 @@ struct PackArgs {
 
 // Modelled time of dx over the words of a piece for `rows` rows in z splits: whole waves of workgroups
 // at 1.9 us a stage and 4 stages of prologue and epilogue, 8 bytes an element and split written and read
-// at 5 TB/s; infinite for splits of less than 8 stages or parts of more than `floats`.
+// at 5 TB/s; infinite for splits of less than 3 stages or parts of more than `floats`.
 __host__ __device__ inline float dx_us(int z, int64_t rows, int64_t words, int64_t H, int C, int64_t floats) {
   const int tiles = (int)((rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE));
   const int len = ((int)words + z * BK - 1) / (z * BK);
-  if (z > 1 && (len < 8 || z * rows * H > floats)) return INFINITY;
+  if (z > 1 && (len < 3 || z * rows * H > floats)) return INFINITY;
   const float part = 8.f * (float)rows * (float)H / 5.0e6f;
   return (float)(((int64_t)tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
 }
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
         float alpha = a.inv_t;
         if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
         if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
-        *a.meta = Meta{rows, alpha, z};
+        *a.meta = Meta{rows, 0, alpha, z};
       }
     }
     return;
@@ -694,23 +695,85 @@ __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
   else st0[(tile_v * 5 + 4) * a.Np + lane] = sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane];
 }
 
+// ---- the losses' total --------------------------------------------------------------------------------
+struct Total {
+  const float* loss;  // [N]
+  int64_t N;
+  float* out;  // {sum, mean over the rows that take part (0 without one), their number}, or NULL
+};
+// By the last workgroup of 256 threads that has written its rows' losses: which one it is does not
+// change the order of the sum.
+__device__ __forceinline__ void add_up(const Total& t, Meta* meta) {
+  __shared__ int last;
+  __shared__ double red[4];
+  if (!t.out) return;
+  __syncthreads();  // the workgroup's losses are written
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(&meta->done, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0;
+#pragma unroll 16
+  for (int64_t r = threadIdx.x; r < t.N; r += 256)
+    s += __hip_atomic_load(t.loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = red[0] + red[1] + red[2] + red[3];
+    const int rows = meta->rows;
+    t.out[0] = (float)s;
+    t.out[1] = rows > 0 ? (float)(s / rows) : 0.f;
+    t.out[2] = (float)rows;
+  }
+}
+__global__ void no_total_kernel(float* out) {  // of no rows
+  if (threadIdx.x < 3) out[threadIdx.x] = 0.f;
+}
+
 // ---- joining the tiles' statistics ------------------------------------------------------------------
 // 256 threads: 1 << rb_log rows, the rest of the threads along the tiles; each joins its tiles in order,
 // then pairs of threads join theirs, so the order is fixed.
 struct JoinArgs {
   const float* stats;
   const float* zlab;
-  const Meta* meta;
+  Meta* meta;
   const int32_t* src;
   const int32_t* lab;
   int64_t Np;
   int tiles, rb_log;
+  Total total;
   float* loss;     // [N]
   float* lse[2];   // [N]
   float* lsep[2];  // [Np], of the packed rows (or NULL)
   float* apart;    // [Np] the teacher's normaliser less the student's (or NULL)
 };
 enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
+template <int WHAT>
+__device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const Stat& s0, const Stat& s1) {
+  const int64_t r = a.src[p];
+  const float lse = (float)((double)s0.m + log((double)s0.s));
+  a.lse[0][r] = lse;
+  if (a.lsep[0]) a.lsep[0][p] = lse;
+  if constexpr (WHAT != JOIN_CE) {
+    const float lt = (float)((double)s1.m + log((double)s1.s));
+    a.lse[1][r] = lt;
+    if (a.lsep[1]) a.lsep[1][p] = lt;
+    // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
+    // would lose their common part
+    const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
+    if constexpr (WHAT == JOIN_KL) a.loss[r] = (float)((double)s1.c / s1.s - apart);
+    else a.apart[p] = (float)apart;
+  } else {
+    a.loss[r] = a.lab[p] < 0 ? __builtin_nanf("")
+                             : (float)((double)s0.m - a.zlab[p] + log((double)s0.s));
+  }
+}
+
 template <int WHAT>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   constexpr int PLANES = WHAT == JOIN_CE ? 2 : WHAT == JOIN_KL ? 5 : 4;
@@ -747,31 +810,14 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
     }
     // (the next round writes the lower half of what this one read)
   }
-  if (!live || sl != 0) return;
-  const int64_t r = a.src[p];
-  const float lse = (float)((double)s0.m + log((double)s0.s));
-  a.lse[0][r] = lse;
-  if (a.lsep[0]) a.lsep[0][p] = lse;
-  if constexpr (PLANES > 2) {
-    const float lt = (float)((double)s1.m + log((double)s1.s));
-    a.lse[1][r] = lt;
-    if (a.lsep[1]) a.lsep[1][p] = lt;
-    // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
-    // would lose their common part
-    const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
-    if constexpr (PLANES > 4) a.loss[r] = (float)((double)s1.c / s1.s - apart);
-    else a.apart[p] = (float)apart;
-  } else {
-    a.loss[r] = a.lab[p] < 0 ? __builtin_nanf("")
-                             : (float)((double)s0.m - a.zlab[p] + log((double)s0.s));
-  }
+  if (live && sl == 0) write_row<WHAT>(a, p, s0, s1);
+  if constexpr (WHAT != JOIN_LSE) add_up(a.total, a.meta);
 }
 
 // The loss of every row that takes part from its parts [parts][Np], in order
-__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ part, int parts,
-                                                   const Meta* __restrict__ meta,
+__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ part, int parts, Meta* meta,
                                                    const int32_t* __restrict__ src, int64_t Np,
-                                                   float* __restrict__ loss) {
+                                                   float* loss, Total total) {
   __shared__ double sh[256];
   const int rl = threadIdx.x & 7, sl = threadIdx.x >> 3;  // 8 rows
   const int64_t p = (int64_t)blockIdx.x * 8 + rl;
@@ -783,30 +829,11 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
   }
   sh[threadIdx.x] = s;
   __syncthreads();
-  if (!live || sl != 0) return;
-  for (int k = 1; k < 32; ++k) s += sh[k * 8 + rl];
-  loss[src[p]] = (float)s;
-}
-
-// out = {sum, mean over the rows that take part (0 without one), their number}
-__global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ loss, int64_t N,
-                                                     const Meta* __restrict__ meta,
-                                                     float* __restrict__ out) {
-  __shared__ double red[16];
-  double s = 0;
-  for (int64_t r = threadIdx.x; r < N; r += 1024) s += loss[r];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s = 0;
-    for (int w = 0; w < 16; ++w) s += red[w];
-    const int rows = N > 0 ? meta->rows : 0;
-    out[0] = (float)s;
-    out[1] = rows > 0 ? (float)(s / rows) : 0.f;
-    out[2] = (float)rows;
+  if (live && sl == 0) {
+    for (int k = 1; k < 32; ++k) s += sh[k * 8 + rl];
+    loss[src[p]] = (float)s;
   }
+  add_up(total, meta);
 }
 
 // ---- dz of tiles that were kept ----------------------------------------------------------------------
@@ -1113,11 +1140,6 @@ static int64_t piece_words(int64_t N, int64_t V, int64_t H, int bytes) {
   const int64_t pieces = (tiles + most - 1) / most;
   return (tiles + pieces - 1) / pieces * TILE;
 }
-// Floats of dx's parts: the splits that all rows would take
-static int64_t part_floats(int64_t N, int64_t words, int64_t H) {
-  return (int64_t)dx_splits(N, words, H, cu_count()) * N * H;
-}
-
 // The workspace, carved in order; p = NULL: sizes only.
 struct Carve {
   char* p;
@@ -1142,7 +1164,7 @@ struct Ws {
   float* g;
   uint16_t* dzt;
   float* part;
-  int64_t words;  // of a piece
+  int64_t words, part_floats;  // of a piece
 };
 enum { WS_FWD, WS_BWD, WS_STEP };
 // Whether the tiles are those of few rows
@@ -1178,7 +1200,11 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
     w.kl = c.take<float>((size_t)(Vp / 32 / finish_per(N, Vp)) * Np);
   }
   w.dzt = c.take<uint16_t>((size_t)w.words * Np);
-  if (grad_x) w.part = c.take<float>((size_t)part_floats(N, w.words, H));
+  if (grad_x) {
+    // dx's parts: the splits that all rows would take
+    w.part_floats = (int64_t)dx_splits(N, w.words, H, cu_count()) * N * H;
+    w.part = c.take<float>((size_t)w.part_floats);
+  }
   return w;
 }
 // Whether the forward of so many rows may keep what the gradients are made of
@@ -1232,14 +1258,10 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
     a.x[1] = s.tx; a.xp[1] = w.xp[1]; a.H[1] = s.Ht;
   }
   a.meta = w.meta; a.pos = w.pos; a.src = w.src; a.lab = w.lab;
+  a.words = w.words; a.z_floats = w.part_floats; a.cus = cu_count();
   a.inv_t = s.inv_t;
   a.reduction = PLZ_REDUCE_NONE;
   return a;
-}
-static void set_splits(PackArgs& p, const Sides& s, int64_t words) {
-  p.words = words;
-  p.z_floats = part_floats(s.N, words, s.H);
-  p.cus = cu_count();
 }
 static int pack(const PackArgs& a, hipStream_t st, const char* what) {
   hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows + BK / kPackRows)),
@@ -1304,8 +1326,8 @@ struct Products {
     }
     if (grad_x) {
       const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add};
-      // at most z tiles of rows: z rows H <= the parts' floats, and 64 splits of a tile that is not full
-      const int64_t items = (part_floats(s.N, panel, s.H) / s.H / TILE + 64) * tiles_h;
+      // z tiles of rows: z rows H <= the parts' floats, and a split each of a tile that is not full
+      const int64_t items = (w.part_floats / s.H / TILE + kMaxSplits) * tiles_h;
       hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
       if (int rc = check_launch(what)) return rc;
     }
@@ -1353,21 +1375,21 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
       return PLZ_EUNSUPPORTED;
     }
   }
-  Carve need{nullptr};
-  carve(need, use, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
-  if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
   Carve c{reinterpret_cast<char*>(ws)};
   const Ws w = carve(c, use, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  if (int rc = check_ws(ws, ws_bytes, c.used, what)) return rc;
   const int64_t Np = up(s.N, TILE), Vp = up(s.V, TILE);
+  const Total sums = {loss, s.N, total};
+  if (s.N == 0 && total) {
+    hipLaunchKernelGGL(no_total_kernel, dim3(1), dim3(64), 0, st, total);
+    return check_launch(what);
+  }
   if (s.N > 0) {
     PackArgs p = pack_args(s, w);
     p.zero[0] = loss;
     p.zero[1] = lse;
     if (KL) p.zero[2] = lse + s.N;
-    if (STEP) {
-      p.reduction = reduction;
-      if (grad_x) set_splits(p, s, Vp);
-    }
+    if (STEP) p.reduction = reduction;
     if (int rc = pack(p, st, what)) return rc;
     LogitArgs l = logit_args(s, w);
     l.planes = !KL ? 2 : STEP ? 4 : 5;
@@ -1394,6 +1416,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.lsep[0] = w.lse[0];
     j.lsep[1] = w.lse[1];
     j.apart = w.apart;
+    j.total = sums;
     hipLaunchKernelGGL(join_kernel<!KL ? JOIN_CE : STEP ? JOIN_LSE : JOIN_KL>,
                        dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)), dim3(256), 0, st, j);
     if (int rc = check_launch(what)) return rc;
@@ -1404,13 +1427,9 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     if (int rc = finish<KL>(f, st, what)) return rc;
     if (KL) {
       hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((s.N + 7) / 8)), dim3(256), 0, st, w.kl,
-                         (int)(Vp / 32 / f.per), w.meta, w.src, Np, loss);
+                         (int)(Vp / 32 / f.per), w.meta, w.src, Np, loss, sums);
       if (int rc = check_launch(what)) return rc;
     }
-  }
-  if (total) {
-    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, s.N, w.meta, total);
-    if (int rc = check_launch(what)) return rc;
   }
   if (!STEP || (!grad_x && !grad_w)) return PLZ_OK;
   const Products prod = {s, w, grad_x, grad_w, Vp, st, what};
@@ -1432,17 +1451,14 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
     if (grad_w) zero_async(grad_w, (size_t)s.V * s.H * 2, st);
     return check_launch(what);
   }
-  Carve need{nullptr};
-  carve(need, WS_BWD, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
-  if (int rc = check_ws(ws, ws_bytes, need.used, what)) return rc;
   Carve c{reinterpret_cast<char*>(ws)};
   const Ws w = carve(c, WS_BWD, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
+  if (int rc = check_ws(ws, ws_bytes, c.used, what)) return rc;
   const int64_t words = w.words;
   PackArgs p = pack_args(s, w);
   p.grad = grad;
   p.reduction = reduction;
   if (reduction == PLZ_REDUCE_NONE) p.g = w.g;
-  if (grad_x) set_splits(p, s, words);
   for (int k = 0; k < (KL ? 2 : 1); ++k) {
     p.lse_in[k] = lse + k * s.N;
     p.lse[k] = w.lse[k];

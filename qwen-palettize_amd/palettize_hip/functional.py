@@ -205,8 +205,14 @@ def soft_lut_linear(x, palette, logits, noise, tau, bias=None, lora_a=None, lora
 # ---- losses over a large vocabulary --------------------------------------------------------------
 def _rows(t, width):
     """[..., width] as contiguous rows on 16 bytes, as the kernels read them."""
-    t = t.reshape(-1, width).contiguous()
+    if t.dim() != 2 or not t.is_contiguous():
+        t = t.reshape(-1, width).contiguous()
     return t.clone() if t.data_ptr() % 16 else t
+
+
+def _keys(t):
+    """Labels or a mask as the kernels read them."""
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 class _VocabLossFunction(torch.autograd.Function):
@@ -237,7 +243,7 @@ class _VocabLossFunction(torch.autograd.Function):
         lse, *args = ctx.saved_tensors
         grads, ctx.grads = ctx.grads, None
         if grads is not None:
-            ops.scale_grads([g for g in grads if g is not None], grad.contiguous())
+            ops._scale_fresh(grads, grad)
         else:
             grads = ctx.calls[2](*args, lse, grad.contiguous(), ctx.reduction, *ctx.needs_input_grad[3:5])
         return None, None, None, *grads, *[None] * (len(args) - 2)
@@ -261,7 +267,7 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean")
     if not ops.vocab_step_fits(labels.numel(), weight.shape[0], H):
         calls = calls[0], None, calls[2]
     loss = _VocabLossFunction.apply(calls, torch.is_grad_enabled(), reduction, _rows(x, H),
-                                    _rows(weight, weight.shape[-1]), labels.reshape(-1).contiguous())
+                                    _rows(weight, weight.shape[-1]), _keys(labels))
     return loss.reshape(labels.shape) if reduction == "none" else loss
 
 
@@ -286,6 +292,6 @@ def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=
         calls = calls[0], None, calls[2]
     loss = _VocabLossFunction.apply(
         calls, torch.is_grad_enabled(), reduction, _rows(x, H), _rows(weight, weight.shape[-1]),
-        _rows(teacher_x.detach(), Ht), _rows(teacher_weight.detach(), teacher_weight.shape[-1]),
-        None if mask is None else mask.reshape(-1).contiguous())
+        *(_rows(t.detach() if t.requires_grad else t, t.shape[-1]) for t in (teacher_x, teacher_weight)),
+        None if mask is None else _keys(mask))
     return loss.reshape(x.shape[:-1]) if reduction == "none" else loss

@@ -14,6 +14,8 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
+from array import array
 
 import torch
 
@@ -1213,16 +1215,22 @@ def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     dev = _one_device("linear_ce_fwd", x, weight, labels)
     loss, lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
-    ws = _workspace(query("plz_vocab_loss_workspace", N, V, H, 0), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, 0), x.device)
     _on(dev, "plz_linear_ce_fwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
         _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H)
     return loss, lse, out
 
 
+# sizes that come again each step: looked up once
+@functools.lru_cache(maxsize=256)
+def _vocab_workspace(which, *sizes):
+    return query(which, *sizes)
+
+
 def vocab_step_fits(N, V, H, H_teacher=0) -> bool:
     """Whether linear_ce_step (linear_kl_step with H_teacher) takes N rows: it keeps 2 (10) bytes a logit
     for the length of the call, 4 (8) GiB at most."""
-    return query("plz_vocab_loss_step_workspace", N, V, H, H_teacher, 0) > 0
+    return _vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, H_teacher, 0) > 0
 
 
 def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_x=True, grad_weight=True):
@@ -1235,7 +1243,7 @@ def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(query("plz_vocab_loss_step_workspace", N, V, H, 0, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, 0, int(grad_x)), x.device)
     _on(dev, "plz_linear_ce_step", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index), mode,
         _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
     return loss, lse, total, gx, gw
@@ -1252,7 +1260,7 @@ def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-
     dev = _one_device("linear_ce_bwd", x, weight, labels, lse, grad)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(query("plz_vocab_loss_bwd_workspace", N, V, H, 0, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_bwd_workspace", N, V, H, 0, int(grad_x)), x.device)
     _on(dev, "plz_linear_ce_bwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
         _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
     return gx, gw
@@ -1270,7 +1278,7 @@ def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
     lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
-    ws = _workspace(query("plz_vocab_loss_workspace", N, V, H, Ht), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, Ht), x.device)
     _on(dev, "plz_linear_kl_fwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H, Ht)
     return loss, lse, out
@@ -1288,7 +1296,7 @@ def linear_kl_step(x, weight, teacher_x, teacher_weight, reduction="mean", mask=
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(query("plz_vocab_loss_step_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, Ht, int(grad_x)), x.device)
     _on(dev, "plz_linear_kl_step", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, mode, _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws),
         ws.numel(), N, V, H, Ht)
@@ -1306,7 +1314,7 @@ def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="me
     dev = _one_device("linear_kl_bwd", x, weight, teacher_x, teacher_weight, mask, lse, grad)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(query("plz_vocab_loss_bwd_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace("plz_vocab_loss_bwd_workspace", N, V, H, Ht, int(grad_x)), x.device)
     _on(dev, "plz_linear_kl_bwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V,
         H, Ht)
@@ -1315,17 +1323,17 @@ def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="me
 
 # ---- gradient norm and clipping --------------------------------------------------------------------
 _Tensor = torch.Tensor
+_dtype_of = operator.attrgetter("dtype")
 
 
 def _grad_table(name, tensors):
-    """(addresses, values, dtypes) of contiguous GPU tensors of one device, as arrays of the C ABI."""
-    n = len(tensors)
+    """(addresses, values, dtypes, device) of contiguous GPU tensors of one device; arrays of the C ABI."""
     # one pass of C calls for each property: 0.2 us a tensor in all, a loop over checks 1.5
     try:
         devices = set(map(_Tensor.get_device, tensors))
         dense = all(map(_Tensor.is_contiguous, tensors))
-        kinds = [_DT[t.dtype] for t in tensors]
-    except (TypeError, KeyError):
+        kinds = array("i", map(_DT.__getitem__, map(_dtype_of, tensors)))
+    except (TypeError, KeyError, AttributeError):
         raise TypeError(f"{name}: bf16, fp16 or fp32 tensors expected") from None
     if -1 in devices:
         raise RuntimeError(f"{name}: GPU tensors expected (palettize_hip has no CPU path)")
@@ -1333,8 +1341,13 @@ def _grad_table(name, tensors):
         raise ValueError(f"{name}: the tensors are on different devices")
     if not dense:
         raise ValueError(f"{name}: the tensors must be contiguous")
-    return ((C.c_void_p * n)(*map(_Tensor.data_ptr, tensors)),
-            (C.c_int64 * n)(*map(_Tensor.numel, tensors)), (C.c_int32 * n)(*kinds), devices.pop())
+    return (array("Q", map(_Tensor.data_ptr, tensors)), array("q", map(_Tensor.numel, tensors)), kinds,
+            devices.pop())
+
+
+def _at(a):
+    """The address of an array's values (which lives as long as the array)."""
+    return a.buffer_info()[0]
 
 
 def grad_norm(grads):
@@ -1346,9 +1359,18 @@ def grad_norm(grads):
     ptrs, sizes, kinds, dev = _grad_table("grad_norm", grads)
     _no_backward("grad_norm", *grads)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    ws = _workspace(query("plz_grad_norm_workspace", sizes, len(grads)), norm.device)
-    _on(dev, "plz_grad_norm", ptrs, sizes, kinds, len(grads), _ptr(norm), _ptr(ws), ws.numel())
+    ws = _workspace(query("plz_grad_norm_workspace", _at(sizes), len(grads)), norm.device)
+    _on(dev, "plz_grad_norm", _at(ptrs), _at(sizes), _at(kinds), len(grads), _ptr(norm), _ptr(ws), ws.numel())
     return norm
+
+
+def _scale_fresh(grads, factor):
+    """scale_grads of up to two bf16 gradients that this package has just made (or None)."""
+    grads = [g for g in grads if g is not None]
+    n = len(grads)
+    factor = factor.contiguous()
+    _on(factor.get_device(), "plz_scale_grads", (C.c_void_p * n)(*(g.data_ptr() for g in grads)),
+        (C.c_int64 * n)(*(g.numel() for g in grads)), (C.c_int32 * n)(), n, _ptr(factor))
 
 
 def scale_grads(grads, factor):
@@ -1364,7 +1386,7 @@ def scale_grads(grads, factor):
     _no_backward("scale_grads", *grads, factor)
     if len({a for a, n in zip(ptrs, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("scale_grads: a tensor is written twice")
-    _on(dev, "plz_scale_grads", ptrs, sizes, kinds, len(grads), _ptr(factor))
+    _on(dev, "plz_scale_grads", _at(ptrs), _at(sizes), _at(kinds), len(grads), _ptr(factor))
 
 
 def clip_grads(grads, max_norm, out=None):
@@ -1400,9 +1422,9 @@ def clip_grads(grads, max_norm, out=None):
             if j is not None and (ptrs[i] != to[i] or kinds[i] != to_kinds[i]):
                 raise ValueError("clip_grads: an output is another gradient, or of another type in place")
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    ws = _workspace(query("plz_grad_norm_workspace", sizes, len(grads)), norm.device)
-    _on(dev, "plz_clip_grads", ptrs, sizes, kinds, to, to_kinds, len(grads), max_norm, _ptr(norm),
-        _ptr(ws), ws.numel())
+    ws = _workspace(query("plz_grad_norm_workspace", _at(sizes), len(grads)), norm.device)
+    _on(dev, "plz_clip_grads", _at(ptrs), _at(sizes), _at(kinds), _at(to), _at(to_kinds), len(grads),
+        max_norm, _ptr(norm), _ptr(ws), ws.numel())
     return norm
 
 

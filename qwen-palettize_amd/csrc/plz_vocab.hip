@@ -82,7 +82,7 @@ __host__ __device__ inline float dx_us(int z, int64_t rows, int64_t words, int64
   const int tiles = (int)((rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE));
   const int len = ((int)words + z * BK - 1) / (z * BK);
   if (z > 1 && (len < 3 || z * rows * H > floats)) return INFINITY;
-  const float part = 8.f * (float)rows * (float)H / 5.0e6f;
+  const float part = 16.f * (float)rows * (float)H / 5.0e6f;
   return (float)(((int64_t)tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
 }
 constexpr int kMaxSplits = 64;
@@ -286,7 +286,28 @@ __device__ __forceinline__ void logits_tile(lds_u8* lbase, const uint16_t* w, co
   }
 }
 
-template <int MODE>
+// A lane's offsets of a Row tile's copies of rows ld apart, from the tile's first row. Rows past the
+// last are past the resource's end, which the hardware checks.
+__device__ __forceinline__ void row_offsets(uint32_t (&off)[COPY_INSTS], int64_t ld) {
+#pragma unroll
+  for (int it = 0; it < COPY_INSTS; ++it) {
+    const int pch = it * NTHR + threadIdx.x, row = pch >> 3;
+    off[it] = (uint32_t)((row * ld + ((pch & 7) ^ row_swz(row)) * 8) * 2);
+  }
+}
+struct Operands {
+  BufRsrc w, x;
+  uint32_t off[COPY_INSTS];
+};
+__device__ __forceinline__ void copy_operands(const Operands& o, int kt, lds_u8* as) {
+  tile_copy(as, TileDma{o.w, {o.off[0], o.off[1], o.off[2], o.off[3]}}, (uint32_t)(kt * BK * 2));
+  tile_copy(as + TILE_BYTES, TileDma{o.x, {o.off[0], o.off[1], o.off[2], o.off[3]}}, (uint32_t)(kt * BK * 2));
+}
+
+// STREAM: the stages of all the workgroup's tiles follow each other through the two slots without a
+// break: the last two stages of a tile copy the first two of the next one, which are on their way
+// during the epilogue. For widths of whole stages, two at least.
+template <int MODE, bool STREAM>
 __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
@@ -299,13 +320,73 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   // the other
   const int xcd = blockIdx.x % 8, step = gridDim.x / 8;
   const int64_t begin = total * xcd / 8, run = total * (xcd + 1) / 8 - begin;
-  for (int64_t at = blockIdx.x / 8; at < run * a.sides; at += step) {
-    const int side = MODE == Z_KEEP && at >= run ? 1 : 0;
-    int tile_i, tile_j;
-    tile_coords(4, tiles_i, tiles_j, (int)(begin + at - side * run), tile_i, tile_j);
-    const int64_t i0 = a.v0 + (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
+  struct Tile {
+    int side, tile_i, tile_j;
+    int64_t i0, j0;
+  };
+  auto tile_at = [&](int64_t at) {
+    Tile t;
+    t.side = MODE == Z_KEEP && at >= run ? 1 : 0;
+    tile_coords(4, tiles_i, tiles_j, (int)(begin + at - t.side * run), t.tile_i, t.tile_j);
+    t.i0 = a.v0 + (int64_t)t.tile_i * TILE;
+    t.j0 = (int64_t)t.tile_j * TILE;
+    return t;
+  };
+  const int64_t ends = run * a.sides;
+  int64_t at = blockIdx.x / 8;
+  if (at >= ends) return;
+  Tile t = tile_at(at);
+  Operands o;
+  auto operands = [&](const Tile& t) {
+    const int64_t H = a.H[t.side];
+    o.w = make_rsrc(a.w[t.side] + t.i0 * H, (uint32_t)(min((int64_t)TILE, a.v1 - t.i0) * H * 2));
+    o.x = make_rsrc(a.x[t.side] + t.j0 * H, (uint32_t)(TILE * H * 2));
+    row_offsets(o.off, H);
+  };
+  int slot = 0;  // of the next stage
+  bf16x8 fa[WT_I], fb[WT_J];
+  auto slot_at = [&](int k) { return lbase + (k & 1) * 2 * TILE_BYTES; };
+  if constexpr (STREAM) {
+    operands(t);
+    copy_operands(o, 0, slot_at(0));
+    copy_operands(o, 1, slot_at(1));
+    wait_vmcnt<2 * COPY_INSTS>();  // stage 0 has landed; stage 1 may be in flight
+    stage_barrier();
+    load_frags<false, false>(slot_at(0), slot_at(0) + TILE_BYTES, 0, wi, wj, lane, fa, fb);
+  }
+  for (;;) {
+    const int side = t.side, tile_i = t.tile_i, tile_j = t.tile_j;
+    const int64_t i0 = t.i0, j0 = t.j0;
     f32x16 acc[WT_I][WT_J];
-    logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
+    const int64_t next = at + step;
+    if constexpr (STREAM) {
+#pragma unroll
+      for (int i = 0; i < WT_I; ++i)
+#pragma unroll
+        for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
+      const int nfull = (int)(a.H[side] / BK);
+      auto stages = [&](int from, int to, int skip) {
+        for (int kt = from; kt < to; ++kt, ++slot) {
+          lds_u8* const cs = slot_at(slot);
+          const lds_u8* const ns = slot_at(slot + 1);
+          mma_stage_pipe<false, false>(
+              cs, cs + TILE_BYTES, ns, ns + TILE_BYTES, cs, cs + TILE_BYTES, acc, wi, wj, lane, fa, fb,
+              [&] {
+                wait_vmcnt<0>();  // this wave's copies of the next stage
+                stage_barrier();
+              },
+              [&](lds_u8* da, lds_u8*) { copy_operands(o, kt + 2 - skip, da); });
+        }
+      };
+      stages(0, nfull - 2, 0);
+      // behind the last tile its first stages are copied once more, and not used
+      if (next < ends) t = tile_at(next);
+      operands(t);
+      stages(nfull - 2, nfull, nfull);
+    } else {
+      logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
+      if (next < ends) t = tile_at(next);
+    }
 
     // This lane's word of block ti and register e is vl + 32 ti + 8 (e / 4) + e % 4, from the tile's
     // first one; of the tile's words, nw exist.
@@ -440,7 +521,10 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
       }
       __syncthreads();
     }
+    at = next;
+    if (at >= ends) break;
   }
+  __builtin_amdgcn_s_waitcnt(0);  // the copies past the last tile
 }
 
 // ---- tiles of logits of few rows ------------------------------------------------------------------------
@@ -841,10 +925,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
 // (cross entropy, in place) or 10 bytes a logit. The cross entropy's block of exponentials lies where
 // its dz goes, and is in registers before any of that is written. A distillation's blocks also add up
 // their words' share of the loss.
+// (Blocks of a workgroup: a distillation's parts of the loss are read again, 2 of 1, 2, 4 and 8 measured;
+// 4 or 8 cost the cross entropy a tenth.)
+constexpr int kFinishKl = 2;
 struct FinishArgs {
   uint16_t* dzt;
   int64_t words, n, Np;  // of the panels, of the piece
-  int per;               // blocks of a workgroup: 1, 2, 4 or 8 of a tile
+  int per;               // blocks of a workgroup, of one tile
   int stat_log;          // words of a statistic: 7 or 8
   const Meta* meta;
   const int32_t* lab;
@@ -1170,11 +1257,6 @@ enum { WS_FWD, WS_BWD, WS_STEP };
 // Whether the tiles are those of few rows
 static bool few(int64_t N) { return N <= 128; }
 static int stat_words(int64_t N) { return few(N) ? kFewWords : TILE; }
-// Blocks of 32 words that a workgroup of the finishing pass takes: a tile where there are many
-static int finish_per(int64_t N, int64_t words) {
-  const int64_t tiles = up(N, TILE) / TILE * (words / TILE);
-  return tiles >= 4096 ? 8 : tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
-}
 static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
   Ws w = {};
   const int64_t Np = up(N, TILE), Vp = up(V, TILE);
@@ -1197,7 +1279,7 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
   if (use == WS_BWD) w.g = c.take<float>(Np);
   if (use == WS_STEP && Ht) {
     w.apart = c.take<float>(Np);
-    w.kl = c.take<float>((size_t)(Vp / 32 / finish_per(N, Vp)) * Np);
+    w.kl = c.take<float>((size_t)(Vp / 32 / kFinishKl) * Np);
   }
   w.dzt = c.take<uint16_t>((size_t)w.words * Np);
   if (grad_x) {
@@ -1298,9 +1380,12 @@ static int logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* wha
       return N <= 32 ? few_logits<MODE, 1>(a, N, st, what)
              : N <= 64 ? few_logits<MODE, 2>(a, N, st, what) : few_logits<MODE, 4>(a, N, st, what);
   }
-  static uint64_t done = 0;
-  auto kern = logits_kernel<MODE>;
-  if (int rc = reserve_lds((const void*)kern, kLdsLogits, done, what)) return rc;
+  const bool stream = MODE != CE_GRAD && a.H[0] % BK == 0 && a.H[0] >= 2 * BK &&
+                      (a.sides < 2 || (a.H[1] % BK == 0 && a.H[1] >= 2 * BK));
+  static uint64_t done[2] = {0, 0};
+  // (a gradient's epilogue stages the tile where the next one's stages would go)
+  auto kern = stream ? logits_kernel<MODE, MODE != CE_GRAD> : logits_kernel<MODE, false>;
+  if (int rc = reserve_lds((const void*)kern, kLdsLogits, done[stream], what)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)(cu_count() / 8 * 8)), dim3(NTHR), kLdsLogits, st, a);
   return check_launch(what);
 }
@@ -1344,7 +1429,7 @@ struct Products {
 static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   FinishArgs f = {};
   f.dzt = w.dzt; f.words = w.words; f.n = n; f.Np = up(s.N, TILE);
-  f.per = finish_per(s.N, w.words);
+  f.per = s.Ht ? kFinishKl : 1;
   f.stat_log = few(s.N) ? 7 : 8;
   f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;

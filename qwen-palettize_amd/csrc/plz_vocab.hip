@@ -38,7 +38,7 @@ constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dz, and of the logits of 
 constexpr size_t kKeepBytes = (size_t)8 << 30;   // of what a step keeps
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
-constexpr int kPackRows = 4;
+constexpr int kPackMost = 64;  // rows of a packing workgroup, at most
 
 enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
 // What a launch over tiles of logits leaves: their statistics, the gradients of the logits, the
@@ -55,6 +55,7 @@ struct Meta {
 struct PackArgs {
   const void* key;  // labels or mask
   int kind;
+  int per;  // rows of a workgroup, a divisor of BK
   int64_t ignore, V, N;
   const uint16_t* x[2];  // student, teacher
   uint16_t* xp[2];
@@ -102,15 +103,15 @@ __device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
   }
 }
 
-// A workgroup packs kPackRows rows behind all that take part before them, which it counts itself (the
-// keys of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come BK / kPackRows that clear
+// A workgroup packs a.per rows behind all that take part before them, which it counts itself (the keys
+// of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come BK / a.per that clear
 // the packed rows up to the next whole stage of the dW product, whose reduction runs over them; the
 // first of them writes meta, a split of dx a lane.
 __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   __shared__ int red[4];
-  __shared__ int at[kPackRows];
-  const int64_t r0 = min((int64_t)blockIdx.x * kPackRows, a.N);
-  const int pad = (int)(blockIdx.x - (a.N + kPackRows - 1) / kPackRows);  // < 0: rows
+  __shared__ int at[kPackMost];
+  const int64_t r0 = min((int64_t)blockIdx.x * a.per, a.N);
+  const int pad = (int)(blockIdx.x - (a.N + a.per - 1) / a.per);  // < 0: rows
   int before = (int)r0;
   if (a.kind != KEY_NONE) {
     int c = 0;
@@ -123,8 +124,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
     before = red[0] + red[1] + red[2] + red[3];
   }
   if (pad >= 0) {
-    const int rows = before, first = rows + pad * kPackRows;
-    const int end = min(first + kPackRows, (rows + BK - 1) / BK * BK);
+    const int rows = before, first = rows + pad * a.per;
+    const int end = min(first + a.per, (rows + BK - 1) / BK * BK);
     for (int k = 0; k < 2; ++k) {
       if (!a.x[k] || first >= end) continue;
       const int64_t c8 = a.H[k] / 8;
@@ -152,12 +153,12 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
     }
     return;
   }
-  const int n = (int)min((int64_t)kPackRows, a.N - r0);
+  const int n = (int)min((int64_t)a.per, a.N - r0);
   if (threadIdx.x < 64) {
     const int i = threadIdx.x;
     const bool on = i < n && takes_part(a, r0 + i);
     const uint64_t all = __ballot(on);
-    if (i < kPackRows) at[i] = on ? before + __popcll(all & ((1ull << i) - 1)) : -1;
+    if (i < a.per) at[i] = on ? before + __popcll(all & ((1ull << i) - 1)) : -1;
     if (i < n) {
       const int64_t r = r0 + i;
       const int p = at[i];
@@ -286,27 +287,39 @@ __device__ __forceinline__ void logits_tile(lds_u8* lbase, const uint16_t* w, co
   }
 }
 
-// A lane's offsets of a Row tile's copies of rows ld apart, from the tile's first row. Rows past the
-// last are past the resource's end, which the hardware checks.
-__device__ __forceinline__ void row_offsets(uint32_t (&off)[COPY_INSTS], int64_t ld) {
-#pragma unroll
-  for (int it = 0; it < COPY_INSTS; ++it) {
-    const int pch = it * NTHR + threadIdx.x, row = pch >> 3;
-    off[it] = (uint32_t)((row * ld + ((pch & 7) ^ row_swz(row)) * 8) * 2);
-  }
-}
+// The two operands of a tile of logits: a lane's offsets of the copies of a stage, 64 rows apart, and the
+// bit that takes its chunk of a last stage that is not whole out of the buffer. What is out of the
+// buffer, rows past the last too, is zero in LDS: the hardware checks the range.
 struct Operands {
   BufRsrc w, x;
-  uint32_t off[COPY_INSTS];
+  uint32_t off[COPY_INSTS], past;
+  int stages;
 };
+__device__ __forceinline__ Operands operands_of(const uint16_t* w, const uint16_t* x, int64_t H, int64_t nw) {
+  Operands o;
+  o.w = make_rsrc(w, (uint32_t)(nw * H * 2));
+  o.x = make_rsrc(x, (uint32_t)(TILE * H * 2));
+  const int row = threadIdx.x >> 3, c = (threadIdx.x & 7) ^ row_swz(row);  // of every 64 rows the same
+#pragma unroll
+  for (int it = 0; it < COPY_INSTS; ++it) o.off[it] = (uint32_t)(((64 * it + row) * H + c * 8) * 2);
+  o.stages = (int)((H + BK - 1) / BK);
+  o.past = H % BK && c * 8 >= H % BK ? kBufOob : 0;
+  return o;
+}
 __device__ __forceinline__ void copy_operands(const Operands& o, int kt, lds_u8* as) {
-  tile_copy(as, TileDma{o.w, {o.off[0], o.off[1], o.off[2], o.off[3]}}, (uint32_t)(kt * BK * 2));
-  tile_copy(as + TILE_BYTES, TileDma{o.x, {o.off[0], o.off[1], o.off[2], o.off[3]}}, (uint32_t)(kt * BK * 2));
+  const uint32_t past = kt == o.stages - 1 ? o.past : 0;
+  TileDma d;
+#pragma unroll
+  for (int it = 0; it < COPY_INSTS; ++it) d.off[it] = o.off[it] | past;
+  d.r = o.w;
+  tile_copy(as, d, (uint32_t)(kt * BK * 2));
+  d.r = o.x;
+  tile_copy(as + TILE_BYTES, d, (uint32_t)(kt * BK * 2));
 }
 
 // STREAM: the stages of all the workgroup's tiles follow each other through the two slots without a
 // break: the last two stages of a tile copy the first two of the next one, which are on their way
-// during the epilogue. For widths of whole stages, two at least.
+// during the epilogue. For two stages at least.
 template <int MODE, bool STREAM>
 __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   extern __shared__ uint4 smem[];
@@ -339,9 +352,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   Operands o;
   auto operands = [&](const Tile& t) {
     const int64_t H = a.H[t.side];
-    o.w = make_rsrc(a.w[t.side] + t.i0 * H, (uint32_t)(min((int64_t)TILE, a.v1 - t.i0) * H * 2));
-    o.x = make_rsrc(a.x[t.side] + t.j0 * H, (uint32_t)(TILE * H * 2));
-    row_offsets(o.off, H);
+    o = operands_of(a.w[t.side] + t.i0 * H, a.x[t.side] + t.j0 * H, H, min((int64_t)TILE, a.v1 - t.i0));
   };
   int slot = 0;  // of the next stage
   bf16x8 fa[WT_I], fb[WT_J];
@@ -364,7 +375,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
       for (int i = 0; i < WT_I; ++i)
 #pragma unroll
         for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
-      const int nfull = (int)(a.H[side] / BK);
+      const int n = o.stages;
       auto stages = [&](int from, int to, int skip) {
         for (int kt = from; kt < to; ++kt, ++slot) {
           lds_u8* const cs = slot_at(slot);
@@ -378,11 +389,11 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
               [&](lds_u8* da, lds_u8*) { copy_operands(o, kt + 2 - skip, da); });
         }
       };
-      stages(0, nfull - 2, 0);
+      stages(0, n - 2, 0);
       // behind the last tile its first stages are copied once more, and not used
       if (next < ends) t = tile_at(next);
       operands(t);
-      stages(nfull - 2, nfull, nfull);
+      stages(n - 2, n, n);
     } else {
       logits_tile(lbase, a.w[side], a.x[side], a.H[side], i0, a.v1, j0, acc, wi, wj, lane);
       if (next < ends) t = tile_at(next);
@@ -550,66 +561,49 @@ __device__ __forceinline__ void few_tile(lds_u8* lbase, const uint16_t* w, const
   uint32_t ow[4], ox[NB];
   const int row = threadIdx.x >> 3, ch = (threadIdx.x & 7) ^ row_swz(row);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ow[i] = (uint32_t)((min(32 * i + row, nw - 1) * H + ch * 8) * 2);
+  for (int i = 0; i < 4; ++i) ow[i] = (uint32_t)(((32 * i + row) * H + ch * 8) * 2);
 #pragma unroll
   for (int i = 0; i < NB; ++i) ox[i] = (uint32_t)(((32 * i + row) * H + ch * 8) * 2);
+  // a last stage that is not whole: chunks past the width are out of the buffer and zero (Operands)
+  const int nst = (int)((H + BK - 1) / BK);
+  const uint32_t out = H % BK && ch * 8 >= H % BK ? kBufOob : 0;
   const int wbase = __builtin_amdgcn_readfirstlane(wave * 1024);
   auto copy = [&](int kt, int slot) {
     lds_u8* d = lbase + slot * STAGE + wbase;
+    const uint32_t past = kt == nst - 1 ? out : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, d + i * 4096, 16, ow[i], kt * (BK * 2), 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, d + i * 4096, 16, ow[i] | past, kt * (BK * 2), 0, 0);
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, d + (4 + i) * 4096, 16, ox[i], kt * (BK * 2), 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, d + (4 + i) * 4096, 16, ox[i] | past, kt * (BK * 2), 0, 0);
   };
 #pragma unroll
   for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
-  auto stage = [&](const lds_u8* s, int nks) {
+  // Stage kt is waited for with the SLOTS - 2 stages behind it still on their way; the barrier also
+  // frees the slot of stage kt - 1, which stage kt + SLOTS - 1 goes to. Past the last stage the copies
+  // repeat it, so that every stage waits for as many.
+#pragma unroll
+  for (int k = 0; k < SLOTS - 1; ++k) copy(min(k, nst - 1), k);
+  int slot = 0;
+  for (int kt = 0; kt < nst; ++kt) {
+    wait_vmcnt<(SLOTS - 2) * COPIES>();
+    stage_barrier();
+    copy(min(kt + SLOTS - 1, nst - 1), slot == 0 ? SLOTS - 1 : slot - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const lds_u8* s = lbase + slot * STAGE;
 #pragma unroll
     for (int ks = 0; ks < BK / 16; ++ks) {
-      if (ks >= nks) break;
       const bf16x8 fa = frag_row((const uint4*)s, 32 * wave, ks, lane);
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             fa, frag_row((const uint4*)(s + 16384), 32 * i, ks, lane), acc[i], 0, 0, 0);
     }
-  };
-  // Stage kt is waited for with the SLOTS - 2 stages behind it still on their way; the barrier also
-  // frees the slot of stage kt - 1, which stage kt + SLOTS - 1 goes to. Past the last stage the copies
-  // repeat it, so that every stage waits for as many.
-  const int nfull = (int)(H / BK);
-  if (nfull > 0) {
-#pragma unroll
-    for (int k = 0; k < SLOTS - 1; ++k) copy(min(k, nfull - 1), k);
-    int slot = 0;
-    for (int kt = 0; kt < nfull; ++kt) {
-      wait_vmcnt<(SLOTS - 2) * COPIES>();
-      stage_barrier();
-      copy(min(kt + SLOTS - 1, nfull - 1), slot == 0 ? SLOTS - 1 : slot - 1);
-      __builtin_amdgcn_sched_barrier(0);
-      stage(lbase + slot * STAGE, BK / 16);
-      slot = slot == SLOTS - 1 ? 0 : slot + 1;
-    }
+    slot = slot == SLOTS - 1 ? 0 : slot + 1;
   }
   __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
   __syncthreads();
-  if (H % BK) {
-    const int64_t r0 = (int64_t)nfull * BK;
-    const int c = threadIdx.x & 7;
-#pragma unroll
-    for (int i = 0; i < 4 + NB; ++i) {
-      const int r = 32 * i + row;  // of the words, then of the rows
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r0 + 8 * c < H && (i >= 4 || r < nw))
-        v = *reinterpret_cast<const uint4*>((i < 4 ? w + r * H : x + (r - kFewWords) * H) + r0 + 8 * c);
-      reinterpret_cast<lds_u32x4*>(lbase)[row_chunk(r, c)] = u32x4{v.x, v.y, v.z, v.w};
-    }
-    __syncthreads();
-    stage(lbase, (int)((H % BK + 15) / 16));
-    __syncthreads();
-  }
 }
 
 template <int MODE, int NB>
@@ -1131,27 +1125,16 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   for (int i = 0; i < WT_I; ++i)
 #pragma unroll
     for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
-  const int64_t len = rend > rbeg ? rend - rbeg : 0;
-  const int nfull = (int)(len / BK);
-  const uint16_t* dz = a.dzt + tile_i * a.panel * TILE;
-  const TileDma dA = col_tile_dma(dz, TILE, 0, TILE, a.words);
-  const TileDma dB = col_tile_dma(a.w, a.H, j0, a.H, a.words);
-  col_stages<true>(lbase, nfull, acc, wi, wj, lane, [&](bool is_a, int kt, lds_u8* dst) {
+  // whole stages: words past the last are past both buffers and zero (Operands)
+  const int nst = rend > rbeg ? (int)((rend - rbeg + BK - 1) / BK) : 0;
+  const TileDma dA = col_tile_dma(a.dzt + tile_i * a.panel * TILE, TILE, 0, TILE, rend);
+  const TileDma dB = col_tile_dma(a.w, a.H, j0, a.H, rend);
+  col_stages<true>(lbase, nst, acc, wi, wj, lane, [&](bool is_a, int kt, lds_u8* dst) {
     const int64_t r0 = rbeg + (int64_t)kt * BK;
     if (is_a) tile_copy(dst, dA, (uint32_t)(r0 * TILE * 2));
     else tile_copy(dst, dB, (uint32_t)(r0 * a.H * 2));
   });
   __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
-  __syncthreads();
-  if (len % BK) {
-    const int64_t r0 = rbeg + (int64_t)nfull * BK;
-    copy_col_tile_masked((uint4*)lbase, dz, TILE, 0, TILE, r0, rend);
-    copy_col_tile_masked((uint4*)(lbase + TILE_BYTES), a.w, a.H, j0, a.H, r0, rend);
-    __syncthreads();
-    mma_stage_sync<true, true>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane,
-                               (int)((len % BK + 15) / 16));
-    __syncthreads();
-  }
   // from the tile's first row: a lane's address and a uniform one of its register's row
   const int nr = min(rows - (int)i0, TILE);
   const BufRsrc part = make_rsrc(a.part + ((int64_t)zsl * rows + i0) * a.H, (uint32_t)(nr * a.H * 4));
@@ -1312,8 +1295,8 @@ static int check(const Sides& s, bool kl, const char* what) {
   PLZ_REQUIRE(s.H % 8 == 0 && s.Ht % 8 == 0, "%s: hidden widths must be multiples of 8", what);
   const int64_t lim = (int64_t)1 << 31;
   if (up(s.N, TILE) * s.H >= lim || up(s.N, TILE) * s.Ht >= lim || s.V >= lim - TILE ||
-      s.N >= ((int64_t)1 << 22) || up(s.N, TILE) / TILE * (up(s.V, TILE) / TILE) >= lim) {
-    set_error("%s: 2^31 values of x, words or tiles, or 2^22 rows, or more", what);
+      s.N >= ((int64_t)1 << 22) || std::max(s.H, s.Ht) >= ((int64_t)1 << 22) || up(s.N, TILE) / TILE * (up(s.V, TILE) / TILE) >= lim) {
+    set_error("%s: 2^31 values of x, words or tiles, 2^22 rows or a width of 2^22, or more", what);
     return PLZ_EUNSUPPORTED;
   }
   PLZ_REQUIRE(s.w && (s.x || s.N == 0) && (!kl || (s.tw && (s.tx || s.N == 0))),
@@ -1340,14 +1323,16 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
     a.x[1] = s.tx; a.xp[1] = w.xp[1]; a.H[1] = s.Ht;
   }
   a.meta = w.meta; a.pos = w.pos; a.src = w.src; a.lab = w.lab;
+  // (every workgroup counts: with 4 rows each, 2^20 keys would be read 2^17 times)
+  a.per = s.N <= 16384 ? 4 : kPackMost;
   a.words = w.words; a.z_floats = w.part_floats; a.cus = cu_count();
   a.inv_t = s.inv_t;
   a.reduction = PLZ_REDUCE_NONE;
   return a;
 }
 static int pack(const PackArgs& a, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + kPackRows - 1) / kPackRows + BK / kPackRows)),
-                     dim3(256), 0, st, a);
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + a.per - 1) / a.per + BK / a.per)), dim3(256), 0,
+                     st, a);
   return check_launch(what);
 }
 static LogitArgs logit_args(const Sides& s, const Ws& w) {
@@ -1380,8 +1365,7 @@ static int logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* wha
       return N <= 32 ? few_logits<MODE, 1>(a, N, st, what)
              : N <= 64 ? few_logits<MODE, 2>(a, N, st, what) : few_logits<MODE, 4>(a, N, st, what);
   }
-  const bool stream = MODE != CE_GRAD && a.H[0] % BK == 0 && a.H[0] >= 2 * BK &&
-                      (a.sides < 2 || (a.H[1] % BK == 0 && a.H[1] >= 2 * BK));
+  const bool stream = MODE != CE_GRAD && a.H[0] > BK && (a.sides < 2 || a.H[1] > BK);
   static uint64_t done[2] = {0, 0};
   // (a gradient's epilogue stages the tile where the next one's stages would go)
   auto kern = stream ? logits_kernel<MODE, MODE != CE_GRAD> : logits_kernel<MODE, false>;

@@ -1237,9 +1237,15 @@ struct Ws {
   int64_t words, part_floats;  // of a piece
 };
 enum { WS_FWD, WS_BWD, WS_STEP };
-// Whether the tiles are those of few rows
-static bool few(int64_t N) { return N <= 128; }
-static int stat_words(int64_t N) { return few(N) ? kFewWords : TILE; }
+// Whether the tiles are those of few rows: one row of them (where half of a 256x256 tile's rows do not
+// exist: 128 rows of 151936 x 2560 215 us, 129 by the other tiles 241), or two workgroups a CU for all of
+// them (us here and by the other tiles: 256 rows of 32000 x 1024 / 2560 31.6 / 55.7 and 38.3 / 63.6, 768 of
+// 8000 x 2560 51 and 65; 384 of 32000 x 1024 43.9 and 41.1, 256 of 151936 x 2560 299 and 249).
+static bool few(int64_t N, int64_t V, int64_t Ht) {
+  const int64_t tiles = up(V, kFewWords) / kFewWords * (up(N, 128) / 128) * (Ht ? 2 : 1);
+  return N <= 128 || tiles <= 2 * cu_count();
+}
+static int stat_words(int64_t N, int64_t V, int64_t Ht) { return few(N, V, Ht) ? kFewWords : TILE; }
 static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, bool grad_x) {
   Ws w = {};
   const int64_t Np = up(N, TILE), Vp = up(V, TILE);
@@ -1256,7 +1262,7 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
     w.zlab = c.take<float>(Np);
   }
   if (Ht || use != WS_BWD)
-    w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / stat_words(N)) * (Ht ? 5 : 2) * Np);
+    w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / stat_words(N, V, Ht)) * (Ht ? 5 : 2) * Np);
   if (use == WS_FWD) return w;
   for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
   if (use == WS_BWD) w.g = c.take<float>(Np);
@@ -1359,9 +1365,10 @@ static int few_logits(const LogitArgs& a, int64_t N, hipStream_t st, const char*
   return check_launch(what);
 }
 template <int MODE>
-static int logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* what) {
+static int logits(const LogitArgs& a, const Sides& s, hipStream_t st, const char* what) {
+  const int64_t N = s.N;
   if constexpr (MODE != CE_GRAD) {
-    if (few(N))
+    if (few(N, s.V, s.Ht))
       return N <= 32 ? few_logits<MODE, 1>(a, N, st, what)
              : N <= 64 ? few_logits<MODE, 2>(a, N, st, what) : few_logits<MODE, 4>(a, N, st, what);
   }
@@ -1414,7 +1421,7 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   FinishArgs f = {};
   f.dzt = w.dzt; f.words = w.words; f.n = n; f.Np = up(s.N, TILE);
   f.per = s.Ht ? kFinishKl : 1;
-  f.stat_log = few(s.N) ? 7 : 8;
+  f.stat_log = few(s.N, s.V, s.Ht) ? 7 : 8;
   f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
   f.kept = w.kept; f.kept_side = f.Np * w.words;
@@ -1448,6 +1455,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
   const Ws w = carve(c, use, s.N, s.V, s.H, s.Ht, grad_x != nullptr);
   if (int rc = check_ws(ws, ws_bytes, c.used, what)) return rc;
   const int64_t Np = up(s.N, TILE), Vp = up(s.V, TILE);
+  const int stat = stat_words(s.N, s.V, s.Ht);
   const Total sums = {loss, s.N, total};
   if (s.N == 0 && total) {
     hipLaunchKernelGGL(no_total_kernel, dim3(1), dim3(64), 0, st, total);
@@ -1465,10 +1473,10 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     for (int64_t v0 = 0; v0 < s.V; v0 += KL ? w.words : s.V) {
       l.v0 = v0;
       l.v1 = KL ? std::min(s.V, v0 + w.words) : s.V;
-      l.tile0 = (int)(v0 / stat_words(s.N));
-      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, s.N, st, what)) return rc;
+      l.tile0 = (int)(v0 / stat);
+      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, s, st, what)) return rc;
       if (KL && !STEP) {
-        const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1, few(s.N)};
+        const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1, stat < TILE};
         hipLaunchKernelGGL(cross_kernel, dim3((unsigned)(Np / TILE * (up(l.v1 - l.v0, TILE) / TILE) * 4)),
                            dim3(256), 0, st, x);
         if (int rc = check_launch(what)) return rc;
@@ -1477,7 +1485,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     JoinArgs j = {};
     j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
     j.Np = Np;
-    j.tiles = (int)(up(s.V, stat_words(s.N)) / stat_words(s.N));
+    j.tiles = (int)(up(s.V, stat) / stat);
     j.rb_log = s.N >= 4096 ? 4 : s.N >= 512 ? 2 : 0;
     j.loss = loss;
     j.lse[0] = lse;
@@ -1540,7 +1548,7 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   for (int64_t v0 = 0; v0 < s.V; v0 += words) {
     l.v0 = v0;
     l.v1 = std::min(s.V, v0 + words);
-    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, s.N, st, what)) return rc;
+    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, s, st, what)) return rc;
     if (KL) {
       FinishArgs f = finish_args(s, w, l.v1 - l.v0);
       f.g = p.g;

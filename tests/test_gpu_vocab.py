@@ -216,6 +216,28 @@ def test_step_captured_and_replayed(ops, kind):
             assert torch.equal(a, b)
 
 
+# ---- more tiles than a CU has workgroups for: 256 x 256 of them ------------------------------------------
+WIDE = [(300, 40001, 136), (129, 70000, 72), (257, 33000, 64), (700, 17003, 200), (1025, 15000, 576)]
+
+
+@pytest.mark.parametrize("N,V,H", WIDE)
+def test_wide_ce(F, ops, N, V, H):
+    x, w, labels = inputs(N, V, H, seed=N, ignored=0.2)
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+    check(run_ce(F, x, w, labels, "none"), reference(x, w, labels, reduction="none"))
+    check(two_calls_ce(ops, x, w, labels), reference(x, w, labels, kept=False))
+
+
+@pytest.mark.parametrize("N,V,H", WIDE)
+@pytest.mark.parametrize("Ht", [64, 328])
+def test_wide_kl(F, N, V, H, Ht):
+    x, w, tx, tw, mask = kl_inputs(N, V, H, Ht, N, 0.2)
+    check(run_kl(F, x, w, tx, tw, mask=mask, temperature=1.3),
+          reference(x, w, tx=tx, tw=tw, mask=mask, T=1.3))
+    check(run_kl(F, x, w, tx, tw, "none", mask=mask),
+          reference(x, w, tx=tx, tw=tw, mask=mask, reduction="none"))
+
+
 # ---- what takes no part -------------------------------------------------------------------------------
 @pytest.mark.parametrize("N", [1, 40, 300])
 def test_ce_no_row_takes_part(F, N):

@@ -77,11 +77,12 @@ struct PackArgs {
 };
 
 // Modelled time of dx over the words of a piece for `rows` rows in z splits: whole waves of workgroups
-// at 1.9 us a stage and 4 stages of prologue and epilogue, 8 bytes an element and split written and read
-// at 5 TB/s; infinite for splits of less than 3 stages or parts of more than `floats`.
+// at 1.9 us a stage and 4 stages of prologue and epilogue, the fp32 parts (8 bytes an element and split
+// written and read) at half of 5 TB/s; infinite for splits of less than 3 stages or parts of more than
+// `floats`.
 __host__ __device__ inline float dx_us(int z, int64_t rows, int64_t words, int64_t H, int C, int64_t floats) {
   const int tiles = (int)((rows + TILE - 1) / TILE * ((H + TILE - 1) / TILE));
-  const int len = ((int)words + z * BK - 1) / (z * BK);
+  const int len = (int)((words + z * BK - 1) / (z * BK));
   if (z > 1 && (len < 3 || z * rows * H > floats)) return INFINITY;
   const float part = 16.f * (float)rows * (float)H / 5.0e6f;
   return (float)(((int64_t)tiles * z + C - 1) / C) * ((float)len + 4.f) * 1.9f + (float)z * part;
@@ -478,8 +479,8 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
               sum += p[e];
             }
             if constexpr (MODE == CE_KEEP) {
-              // relative to the tile's maximum, fp16: off by 2^-12, an eighth of a step of the bf16
-              // that dz is rounded to, or by 2^-25 of that maximum
+              // relative to the tile's maximum, fp16: off by 2^-11 of the value, an eighth of what the
+              // rounding of dz to bf16 may be off, or by 2^-25 of that maximum
               u32x4 v;
 #pragma unroll
               for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);

@@ -240,13 +240,13 @@ class _VocabLossFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        lse, *args = ctx.saved_tensors
         grads, ctx.grads = ctx.grads, None
         if grads is not None:
             ops._scale_fresh(grads, grad)
         else:
+            lse, *args = ctx.saved_tensors
             grads = ctx.calls[2](*args, lse, grad.contiguous(), ctx.reduction, *ctx.needs_input_grad[3:5])
-        return None, None, None, *grads, *[None] * (len(args) - 2)
+        return None, None, None, *grads, *[None] * (len(ctx.needs_input_grad) - 5)
 
 
 def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean"):

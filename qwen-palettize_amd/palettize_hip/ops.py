@@ -1213,7 +1213,7 @@ def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     N, V, H = _head(x, weight)
     size = _labels(labels, N)
     dev = _one_device("linear_ce_fwd", x, weight, labels)
-    loss, lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    loss, lse = (torch.empty(N, dtype=torch.float32, device=x.device) for _ in range(2))
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
     ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, 0), x.device)
     _on(dev, "plz_linear_ce_fwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
@@ -1239,7 +1239,7 @@ def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_
     N, V, H = _head(x, weight)
     size, mode = _labels(labels, N), _reduction(reduction)
     dev = _one_device("linear_ce_step", x, weight, labels)
-    loss, lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    loss, lse = (torch.empty(N, dtype=torch.float32, device=x.device) for _ in range(2))
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
@@ -1367,10 +1367,9 @@ def grad_norm(grads):
 def _scale_fresh(grads, factor):
     """scale_grads of up to two bf16 gradients that this package has just made (or None)."""
     grads = [g for g in grads if g is not None]
-    n = len(grads)
-    factor = factor.contiguous()
-    _on(factor.get_device(), "plz_scale_grads", (C.c_void_p * n)(*(g.data_ptr() for g in grads)),
-        (C.c_int64 * n)(*(g.numel() for g in grads)), (C.c_int32 * n)(), n, _ptr(factor))
+    ptrs, sizes = (array("q", [f(g) for g in grads]) for f in (_Tensor.data_ptr, _Tensor.numel))
+    kinds, factor = array("i", [_lib.PLZ_DT_BF16] * len(grads)), factor.contiguous()
+    _on(factor.get_device(), "plz_scale_grads", _at(ptrs), _at(sizes), _at(kinds), len(grads), _ptr(factor))
 
 
 def scale_grads(grads, factor):

@@ -496,3 +496,52 @@ def test_refusals(F, ops):
         ops.linear_ce_bwd(x, w, labels, torch.zeros(10, device="cuda"), torch.ones(2, device="cuda"))
     with pytest.raises(ValueError, match="lse"):
         ops.linear_ce_bwd(x, w, labels, torch.zeros(9, device="cuda"), torch.ones(1, device="cuda"))
+
+
+# ---- as they are used together --------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_last_layer_through_the_head(F, kind):
+    """A palettized layer trained through the model's final norm and frozen head: the loss over the
+    vocabulary, its gradient at the layer's output, the layer's own gradients clipped and applied."""
+    from palettize_hip import layer
+    from palettize_hip.optim import FusedAdamW, clip_grad_norm_
+    cfg = layer.LayerConfig(hidden=512, heads=4, kv_heads=2, head_dim=128, intermediate=1024,
+                            lora_rank=16)
+    student = layer.PalettizedDecoderLayer(cfg, seed=0, device="cuda", lora_b_std=0.02)
+    teacher = layer.DenseDecoderLayer(cfg, seed=1, device="cuda")
+    norm = layer.RMSNorm(512, cfg.eps, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    head = (torch.randn(3001, 512, generator=g, device="cuda") * 0.1).bfloat16()
+    hs = torch.randn(2, 96, 512, generator=g, device="cuda").bfloat16()
+    labels = torch.randint(0, 3001, (2, 96), generator=g, device="cuda")
+    labels[:, 70:] = -100
+    cos, sin = layer.rope_tables(96, 128, cfg.rope_theta, "cuda")
+    out = norm(student(hs, cos, sin))
+    out.retain_grad()
+    with torch.no_grad():
+        t_out = norm(teacher(hs, cos, sin))
+    if kind == "ce":
+        loss = F.linear_cross_entropy(out, head, labels)
+        ref = reference(out.detach().view(-1, 512), head, labels.flatten())
+    else:
+        loss = F.linear_distill(out, head, t_out, head, mask=labels != -100)
+        ref = reference(out.detach().view(-1, 512), head, tx=t_out.view(-1, 512), tw=head,
+                        mask=(labels != -100).flatten())
+    loss.backward()
+    close(loss.detach(), ref["loss"], ref["loss_tol"], "loss")
+    close(out.grad.view(-1, 512), ref["gx"], ref["gx_tol"], "gradient of the layer's output")
+    params = [p for lin in student.linears() for p in (lin.palette, lin.lora_a, lin.lora_b, lin.index_logits)]
+    grads = [p.grad.clone() for p in params]
+    assert all(torch.isfinite(v).all() and v.any() for v in grads)
+    total = float(sum(v.double().pow(2).sum() for v in grads)) ** 0.5
+    got = clip_grad_norm_(params, total / 2)
+    assert abs(float(got) - total) <= 2.0 ** -22 * total
+    for p, v in zip(params, grads):
+        # half, but for the roundings of the factor and of the value
+        want = v.double() * (total / 2 / (total + 1e-6))
+        eps = torch.finfo(v.dtype).eps / 2
+        assert bool(((p.grad.double() - want).abs() <= (eps + 2.0 ** -21) * want.abs() + 2.0 ** -133).all())
+    before = [p.detach().clone() for p in params]
+    FusedAdamW([{"params": params, "lr": 1e-3}]).step()
+    assert all(torch.isfinite(p).all() for p in params)
+    assert any(not torch.equal(p, b) for p, b in zip(params, before))

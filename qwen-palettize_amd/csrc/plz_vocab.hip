@@ -55,7 +55,7 @@ struct Meta {
 struct PackArgs {
   const void* key;  // labels or mask
   int kind;
-  int per;  // rows of a workgroup, a divisor of BK
+  int per;  // rows of a workgroup, a divisor of TILE
   int64_t ignore, V, N;
   const uint16_t* x[2];  // student, teacher
   uint16_t* xp[2];
@@ -105,9 +105,10 @@ __device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
 }
 
 // A workgroup packs a.per rows behind all that take part before them, which it counts itself (the keys
-// of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come BK / a.per that clear
-// the packed rows up to the next whole stage of the dW product, whose reduction runs over them; the
-// first of them writes meta, a split of dx a lane.
+// of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come TILE / a.per that clear the
+// packed rows up to the next whole tile: dW's reduction runs over those of the last stage, and
+// multiplying zeros takes less power than what was there. The first of them writes meta, a split of dx
+// a lane.
 __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   __shared__ int red[4];
   __shared__ int at[kPackMost];
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   }
   if (pad >= 0) {
     const int rows = before, first = rows + pad * a.per;
-    const int end = min(first + a.per, (rows + BK - 1) / BK * BK);
+    const int end = min(first + a.per, (rows + TILE - 1) / TILE * TILE);
     for (int k = 0; k < 2; ++k) {
       if (!a.x[k] || first >= end) continue;
       const int64_t c8 = a.H[k] / 8;
@@ -1036,6 +1037,18 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
   }
 }
 
+// A Col tile's copies of p[r][H] whose columns past H are out of the buffer, and so zero, as the rows
+// past rtotal
+__device__ __forceinline__ TileDma col_tile_zero(const uint16_t* p, int64_t H, int64_t col0, int64_t rtotal) {
+  TileDma d = col_tile_dma(p, H, col0, H, rtotal);
+#pragma unroll
+  for (int it = 0; it < COPY_INSTS; ++it) {
+    const int pch = it * NTHR + threadIdx.x;
+    if (col0 + (((pch & 31) ^ col_swz(pch >> 5)) * 8) >= H) d.off[it] = kBufOob;
+  }
+  return d;
+}
+
 // ---- dW of a piece: dz^T [words, rows] x [rows, H] ----------------------------------------------------
 struct DwArgs {
   const uint16_t* dzt;
@@ -1065,7 +1078,7 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
   // (row_tile_dma bounds the copies by its rows: here by all panels)
   TileDma dA = row_tile_dma(a.dzt + i0 * TILE, TILE, 0, TILE);
   dA.r = make_rsrc(a.dzt + i0 * TILE, (uint32_t)((a.Np / TILE * a.panel - i0) * TILE * 2));
-  const TileDma dB = col_tile_dma(a.x, a.H, j0, a.H, a.Np);
+  const TileDma dB = col_tile_zero(a.x, a.H, j0, a.Np);
   const uint32_t panel = (uint32_t)(a.panel * TILE * 2);
   dense_stages<false, true>(lbase, nst, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
     tile_copy(As, dA, (uint32_t)(kt / (TILE / BK)) * panel + (uint32_t)(kt % (TILE / BK)) * (BK * 2));
@@ -1129,7 +1142,7 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   // whole stages: words past the last are past both buffers and zero (Operands)
   const int nst = rend > rbeg ? (int)((rend - rbeg + BK - 1) / BK) : 0;
   const TileDma dA = col_tile_dma(a.dzt + tile_i * a.panel * TILE, TILE, 0, TILE, rend);
-  const TileDma dB = col_tile_dma(a.w, a.H, j0, a.H, rend);
+  const TileDma dB = col_tile_zero(a.w, a.H, j0, rend);
   col_stages<true>(lbase, nst, acc, wi, wj, lane, [&](bool is_a, int kt, lds_u8* dst) {
     const int64_t r0 = rbeg + (int64_t)kt * BK;
     if (is_a) tile_copy(dst, dA, (uint32_t)(r0 * TILE * 2));
@@ -1338,7 +1351,7 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
   return a;
 }
 static int pack(const PackArgs& a, hipStream_t st, const char* what) {
-  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + a.per - 1) / a.per + BK / a.per)), dim3(256), 0,
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)((a.N + a.per - 1) / a.per + TILE / a.per)), dim3(256), 0,
                      st, a);
   return check_launch(what);
 }

@@ -781,20 +781,24 @@ struct Total {
   int64_t N;
   float* out;  // {sum, mean over the rows that take part (0 without one), their number}, or NULL
 };
+// A row's loss goes past the XCD's L2 (agent scope), and the barrier in add_up waits until it has: no
+// fence, which would write the L2 back once a workgroup (5 us of a launch of 256).
+__device__ __forceinline__ void put_loss(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 // By the last workgroup of 256 threads that has written its rows' losses: which one it is does not
 // change the order of the sum.
 __device__ __forceinline__ void add_up(const Total& t, Meta* meta) {
   __shared__ int last;
   __shared__ double red[4];
   if (!t.out) return;
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();  // the workgroup's losses are written
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(&meta->done, 1) == (int)gridDim.x - 1;
-  }
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(&meta->done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           (int)gridDim.x - 1;
   __syncthreads();
   if (!last) return;
-  __threadfence();
   double s = 0;
 #pragma unroll 16
   for (int64_t r = threadIdx.x; r < t.N; r += 256)
@@ -846,11 +850,11 @@ __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const St
     // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
     // would lose their common part
     const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
-    if constexpr (WHAT == JOIN_KL) a.loss[r] = (float)((double)s1.c / s1.s - apart);
+    if constexpr (WHAT == JOIN_KL) put_loss(a.loss + r, (float)((double)s1.c / s1.s - apart));
     else a.apart[p] = (float)apart;
   } else {
-    a.loss[r] = a.lab[p] < 0 ? __builtin_nanf("")
-                             : (float)((double)s0.m - a.zlab[p] + log((double)s0.s));
+    put_loss(a.loss + r, a.lab[p] < 0 ? __builtin_nanf("")
+                                      : (float)((double)s0.m - a.zlab[p] + log((double)s0.s)));
   }
 }
 
@@ -911,7 +915,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
   __syncthreads();
   if (live && sl == 0) {
     for (int k = 1; k < 32; ++k) s += sh[k * 8 + rl];
-    loss[src[p]] = (float)s;
+    put_loss(loss + src[p], (float)s);
   }
   add_up(total, meta);
 }
@@ -1344,7 +1348,7 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
   }
   a.meta = w.meta; a.pos = w.pos; a.src = w.src; a.lab = w.lab;
   // (every workgroup counts: with 4 rows each, 2^20 keys would be read 2^17 times)
-  a.per = s.N <= 16384 ? 4 : kPackMost;
+  a.per = s.N <= 2048 ? 4 : s.N <= 16384 ? 8 : kPackMost;
   a.words = w.words; a.z_floats = w.part_floats; a.cus = cu_count();
   a.inv_t = s.inv_t;
   a.reduction = PLZ_REDUCE_NONE;

@@ -255,7 +255,7 @@ __device__ __forceinline__ void store16(void* base, uint32_t off, u32x4 v) {
   typedef __attribute__((address_space(1))) u32x4 gu32x4;
   uint64_t p = reinterpret_cast<uint64_t>(base);
   asm volatile("" : "+s"(p));
-  *reinterpret_cast<gu32x4*>(reinterpret_cast<gchar*>(p) + off) = v;
+  __builtin_nontemporal_store(v, reinterpret_cast<gu32x4*>(reinterpret_cast<gchar*>(p) + off));
 }
 
 typedef __attribute__((address_space(3))) float lds_f32;

@@ -545,3 +545,103 @@ def test_last_layer_through_the_head(F, kind):
     FusedAdamW([{"params": params, "lr": 1e-3}]).step()
     assert all(torch.isfinite(p).all() for p in params)
     assert any(not torch.equal(p, b) for p, b in zip(params, before))
+
+
+# ---- calls beside each other, captured, past 32 bits -------------------------------------------------------
+def test_two_calls_at_once(F):
+    """Steps on two streams, each with a workspace of its own."""
+    sides = []
+    for k in range(2):
+        x, w, labels = inputs(300 + 200 * k, 20000, 320, seed=40 + k, ignored=0.1 * k)
+        sides.append((x, w, labels, run_ce(F, x, w, labels), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for k, (x, w, labels, _, s) in enumerate(sides):
+            with torch.cuda.stream(s):
+                got[k].append(run_ce(F, x, w, labels))
+    torch.cuda.synchronize()
+    for k, (_, _, _, want, _) in enumerate(sides):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_autograd_captured_and_replayed(F, kind, reduction):
+    """Loss and backward through autograd in a graph; no eager graph of its leaves is alive meanwhile."""
+    N, V, H = 200, 2500, 136
+    x, w, labels = inputs(N, V, H, seed=50)
+    tx = x.flip(0).contiguous()
+
+    def step(x, w):
+        if kind == "ce":
+            loss = F.linear_cross_entropy(x, w, labels, reduction=reduction)
+        else:
+            loss = F.linear_distill(x, w, tx, w.detach(), mask=labels != -100, reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), torch.full_like(loss, 1.5)))
+
+    cx, cw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(cx, cw)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cx, cw)
+    for seed in range(3):
+        nx, nw, nl = inputs(N, V, H, seed=60 + seed, ignored=0.3 * seed)
+        with torch.no_grad():
+            cx.copy_(nx)
+            cw.copy_(nw)
+        labels.copy_(nl)
+        tx.copy_(nx.flip(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step(nx.clone().requires_grad_(), nw.clone().requires_grad_())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_many_rows_of_few_words(F):
+    """More rows than are packed four or eight a workgroup, long runs of them without part."""
+    x, w, labels = inputs(20011, 301, 64, seed=51, ignored=0.3)
+    labels[5000:9000] = -100
+    check(run_ce(F, x, w, labels), reference(x, w, labels))
+    check(run_ce(F, x, w, labels, "none"), reference(x, w, labels, reduction="none"))
+
+
+def test_head_of_more_than_two_to_the_31_values(F, ops):
+    """Offsets into the head and its gradient pass 32 bits; pieces of the vocabulary, no step."""
+    N, V, H = 3, 900001, 2400
+    assert V * H > 2 ** 31 and not ops.vocab_step_fits(N, V, H)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(V, H, dtype=torch.bfloat16, device="cuda").normal_(0, 0.05, generator=g).requires_grad_()
+    x = torch.randn(N, H, generator=g, device="cuda").bfloat16().requires_grad_()
+    labels = torch.tensor([5, V - 1, V // 2 + 77], device="cuda")
+    loss = F.linear_cross_entropy(x, w, labels, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    with torch.no_grad():
+        cuts = range(0, V, 100000)
+        part = [x.double() @ w[c:c + 100000].double().T for c in cuts]
+        z = torch.cat(part, 1)
+        # logits of 2400 products of about 1 * 0.05 each, off by at most this
+        off = (H + 4) * 2.0 ** -24 * float((x.double().abs().sum(1) * float(w.abs().max())).max())
+        dz = torch.softmax(z, 1)
+        lse = torch.logsumexp(z, 1)
+        rows = lse - z[torch.arange(3), labels]
+        tol = 2 * off + (200 + V // 128) * 2.0 ** -24 + 8 * 2.0 ** -24 * lse.abs()
+        assert abs(float(loss) - float(rows.sum())) <= float(tol.sum())
+        dz[torch.arange(3), labels] -= 1
+        # rounding to bf16, and the logits' and normalisers' errors
+        dz_tol = dz.abs() * (2.0 ** -8 + 3 * off + 2 * tol.max())
+        want, bound = torch.zeros_like(x, dtype=torch.float64), torch.zeros_like(x, dtype=torch.float64)
+        for c in cuts:
+            d, t, wd = dz[:, c:c + 100000], dz_tol[:, c:c + 100000], w[c:c + 100000].double()
+            want += d @ wd
+            bound += (t + V * 2.0 ** -24 * d.abs()) @ wd.abs()
+            e = d.T @ x.double()
+            te = (t + 67 * 2.0 ** -24 * d.abs()).T @ x.double().abs()
+            close(gw[c:c + 100000], e, te + (2.0 ** -8 + 2.0 ** -20) * (e.abs() + te), f"grad_weight from {c}")
+        close(gx, want, bound + (2.0 ** -8 + 2.0 ** -20) * (want.abs() + bound), "grad_x")

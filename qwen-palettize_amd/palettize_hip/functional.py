@@ -235,7 +235,8 @@ class _VocabLossFunction(torch.autograd.Function):
         else:
             loss, lse, total = fwd(*args, reduction != "none")
         ctx.save_for_backward(lse, *args)
-        return loss if total is None else total[0 if reduction == "sum" else 1]
+        # (.data: a user may divide the loss in place, which autograd refuses for a function's views)
+        return loss if total is None else total[0 if reduction == "sum" else 1].data
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -249,6 +250,12 @@ class _VocabLossFunction(torch.autograd.Function):
         return None, None, None, *grads, *[None] * (len(ctx.needs_input_grad) - 5)
 
 
+def _two_dims(**weights):
+    for name, w in weights.items():
+        if w.dim() != 2:
+            raise ValueError(f"{name} must have 2 dimensions, got {tuple(w.shape)}")
+
+
 def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean"):
     """Cross entropy of labels under softmax(x weight^T): torch's cross_entropy of those logits in fp32,
     without them. x bf16 [..., H], weight bf16 [V, H] (H a multiple of 8), labels int64 or int32 [...].
@@ -256,6 +263,7 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean")
     labels outside [0, V) give NaN. Returns fp32: the mean over the rows that take part (0 without
     one), the sum, or every row's loss in the labels' shape. Gradients of x and weight are bf16."""
     ops._reduction(reduction)
+    _two_dims(weight=weight)
     if labels.shape != x.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not match x {tuple(x.shape)}")
     ignore, H = int(ignore_index), x.shape[-1]
@@ -279,6 +287,7 @@ def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=
     [...]: rows that it leaves out take no part (whatever they hold; their gradient is 0). Returns as
     linear_cross_entropy does; the loss is not multiplied by temperature^2."""
     ops._reduction(reduction)
+    _two_dims(weight=weight, teacher_weight=teacher_weight)
     if teacher_x.shape[:-1] != x.shape[:-1] or (mask is not None and mask.shape != x.shape[:-1]):
         raise ValueError("x, teacher_x and mask differ in their leading dimensions")
     N, H, Ht, T = x.shape[:-1].numel(), x.shape[-1], teacher_x.shape[-1], float(temperature)

@@ -482,6 +482,10 @@ def test_refusals(F, ops):
         F.linear_cross_entropy(x[:, :60].contiguous(), w[:, :60].contiguous(), labels)
     with pytest.raises(ValueError, match="word"):
         F.linear_cross_entropy(x, w[:0], labels)
+    with pytest.raises(ValueError, match="2 dimensions"):
+        F.linear_cross_entropy(x, w.reshape(2, 25, 64), labels)
+    with pytest.raises(ValueError, match="2 dimensions"):
+        F.linear_distill(x, w, x, w.reshape(2, 25, 64))
     with pytest.raises(RuntimeError, match="GPU tensor"):
         F.linear_cross_entropy(x.cpu(), w, labels)
     with pytest.raises(ValueError, match="temperature"):
@@ -645,3 +649,23 @@ def test_head_of_more_than_two_to_the_31_values(F, ops):
             te = (t + 67 * 2.0 ** -24 * d.abs()).T @ x.double().abs()
             close(gw[c:c + 100000], e, te + (2.0 ** -8 + 2.0 ** -20) * (e.abs() + te), f"grad_weight from {c}")
         close(gx, want, bound + (2.0 ** -8 + 2.0 ** -20) * (want.abs() + bound), "grad_x")
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_loss_divided_in_place(F, kind, reduction):
+    """As a loop over micro-batches does; 8 is a power of two, so nothing is rounded by it."""
+    x, w, labels = inputs(150, 1000, 96, seed=52)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    tx, tw = x.detach().flip(0).contiguous(), w.detach().flip(0).contiguous()
+
+    def loss():
+        if kind == "ce":
+            return F.linear_cross_entropy(x, w, labels, reduction=reduction)
+        return F.linear_distill(x, w, tx, tw, reduction=reduction)
+
+    whole, part = loss(), loss()
+    part /= 8
+    assert torch.equal(part * 8, whole)
+    for a, b in zip(torch.autograd.grad(part, (x, w)), torch.autograd.grad(whole, (x, w))):
+        assert torch.equal(a * 8, b)

@@ -36,6 +36,11 @@ using namespace g2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dz, and of the logits of a piece
 constexpr size_t kKeepBytes = (size_t)8 << 30;   // of what a step keeps
+// Exponentials relative to the tile's maximum are kept in fp16 times this: the greatest is then 2^15, and
+// those from 2^-29 on are normal, off by 2^-11 of their own value, an eighth of what the rounding of dz to
+// bf16 may be off (as they are, from 2^-14 on: beside a word of probability 1 those of 10^-6 were off by
+// 3%). Below, by 2^-40 of the tile's maximum.
+constexpr float kKeptScale = 32768.f;
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
 constexpr int kPackMost = 64;  // rows of a packing workgroup, at most
@@ -222,6 +227,11 @@ struct LogitArgs {
 // exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
 // distance from the maximum (or the normaliser), which is small wherever the exponential counts
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// two exponentials as a step keeps them
+__device__ __forceinline__ uint32_t kept2(float a, float b) {
+  return f2h(a * kKeptScale) | (f2h(b * kKeptScale) << 16);
+}
 
 // The statistics of a set of words: the maximum, the sum of exponentials relative to it and, for the
 // teacher, the sum of exponentials times (teacher - student).
@@ -480,11 +490,9 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
               sum += p[e];
             }
             if constexpr (MODE == CE_KEEP) {
-              // relative to the tile's maximum, fp16: off by 2^-11 of the value, an eighth of what the
-              // rounding of dz to bf16 may be off, or by 2^-25 of that maximum
               u32x4 v;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);
+              for (int e = 0; e < 4; ++e) v[e] = kept2(p[2 * e], p[2 * e + 1]);
               store16(exps + ti * 8192 + tj * 1024 + h * 512, wi * 65536 + wj * 4096 + lane * 16, v);
             }
           }
@@ -694,7 +702,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a) {
       if constexpr (MODE == CE_KEEP) {
         u32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = f2h(p[2 * e]) | (f2h(p[2 * e + 1]) << 16);
+        for (int e = 0; e < 4; ++e) v[e] = kept2(p[2 * e], p[2 * e + 1]);
         *reinterpret_cast<u32x4*>(exps + h * 512 + lane * 8) = v;
       }
     }
@@ -996,6 +1004,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
       } else {
         const int l = live ? a.lab[n] : 0;
         float f = live && v0 < a.n ? exp_of(a.stats[(int64_t)(v0 >> a.stat_log) * 2 * a.Np + n] - lse) : 0.f;
+        f *= 1.f / kKeptScale;
         if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

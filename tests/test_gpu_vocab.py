@@ -669,3 +669,32 @@ def test_loss_divided_in_place(F, kind, reduction):
     assert torch.equal(part * 8, whole)
     for a, b in zip(torch.autograd.grad(part, (x, w)), torch.autograd.grad(whole, (x, w))):
         assert torch.equal(a * 8, b)
+
+
+@pytest.mark.parametrize("N", [4, 300])
+def test_unlikely_words_beside_a_likely_one(F, N):
+    """Every row's label has a probability of about 1, the other words of its tile 10^-4 to 10^-8: their
+    rows of the weight's gradient are sums of those alone, and as exact as any."""
+    V, H = 256, 64
+    g = torch.Generator(device="cuda").manual_seed(53)
+    x = torch.zeros(N, H, device="cuda")
+    x[:, 0] = 1
+    x[:, 1:] = torch.rand(N, H - 1, generator=g, device="cuda")
+    w = torch.zeros(V, H, device="cuda")
+    w[:, 0] = -torch.linspace(9, 18, V, device="cuda")
+    w[100, 0] = 0
+    x, w = x.bfloat16(), w.bfloat16()
+    labels = torch.full((N,), 100, device="cuda")
+    ref = reference(x, w, labels)
+    check(run_ce(F, x, w, labels), ref)
+    some = ref["gw"].abs() > 0
+    assert float((ref["gw_tol"][some] / ref["gw"][some].abs()).median()) < 0.02
+
+
+def test_more_than_four_gib_of_logits_kept(F, ops):
+    """A distillation's step that keeps 6.6 GB of both sides' logits (N past the rows of a tile too)."""
+    N, V, H = 4100, 190000, 64
+    assert ops.vocab_step_fits(N, V, H, H)
+    x, w, _ = inputs(N, V, H, seed=54)
+    tx, tw, _ = inputs(N, V, H, seed=55)
+    check(run_kl(F, x, w, tx, tw), reference(x, w, tx=tx, tw=tw))

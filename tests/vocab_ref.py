@@ -52,8 +52,8 @@ def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None,
             rows_tol[r] = off + dz[i, l] + 4 * U32 * (lse.abs() + z[i, l].abs())
             d = q.clone()
             d[i, l] -= 1
-            if kept:  # half a step of fp16, or of its subnormals
-                q_tol = q_tol + 2.0 ** -11 * q + 2.0 ** -25 * q.max(1, keepdim=True).values
+            if kept:  # half a step of fp16, or of its subnormals (of 2^15 times the value)
+                q_tol = q_tol + 2.0 ** -11 * q + 2.0 ** -40 * q.max(1, keepdim=True).values
         else:
             zt, dzt = logits(tx[r], tw, T)
             lt = torch.logsumexp(zt, 1)

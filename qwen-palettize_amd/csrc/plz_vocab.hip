@@ -341,8 +341,12 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   const int rows = a.meta->rows;
   const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE), tiles_j = (rows + TILE - 1) / TILE;
   const int64_t total = (int64_t)tiles_i * tiles_j;
-  // every XCD walks a run of its own, four tiles of words at a time over the rows, of one side after
-  // the other
+  // Every XCD walks a run of its own, four tiles of words at a time over the rows, of one side after the
+  // other. Both sides' logits are stored: with 8 or 16 tiles of rows its 32 workgroups would then start
+  // and store their tiles in step, so there it is six (two sides of 2048 rows of 151936 x 2560 3.54 and
+  // 3.36 ms, 1024 rows 1.84 and 1.80, 4096 6.72 and 6.62; but of 1792 rows 2.88 and 2.95, of 2816 4.49 and
+  // 4.60, and a cross entropy's 4096 2.62 and 2.63).
+  const int group = MODE == Z_KEEP && tiles_j % 4 == 0 ? 6 : 4;
   const int xcd = blockIdx.x % 8, step = gridDim.x / 8;
   const int64_t begin = total * xcd / 8, run = total * (xcd + 1) / 8 - begin;
   struct Tile {
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   auto tile_at = [&](int64_t at) {
     Tile t;
     t.side = MODE == Z_KEEP && at >= run ? 1 : 0;
-    tile_coords(4, tiles_i, tiles_j, (int)(begin + at - t.side * run), t.tile_i, t.tile_j);
+    tile_coords(group, tiles_i, tiles_j, (int)(begin + at - t.side * run), t.tile_i, t.tile_j);
     t.i0 = a.v0 + (int64_t)t.tile_i * TILE;
     t.j0 = (int64_t)t.tile_j * TILE;
     return t;

@@ -109,6 +109,13 @@ __device__ __forceinline__ bool takes_part(const PackArgs& a, int64_t r) {
   }
 }
 
+__device__ __forceinline__ int label_of(const PackArgs& a, int64_t r) {
+  if (a.kind != KEY_INT64 && a.kind != KEY_INT32) return -1;
+  const int64_t l = a.kind == KEY_INT64 ? reinterpret_cast<const int64_t*>(a.key)[r]
+                                        : reinterpret_cast<const int32_t*>(a.key)[r];
+  return l >= 0 && l < a.V ? (int)l : -1;
+}
+
 // A workgroup packs a.per rows behind all that take part before them, which it counts itself (the keys
 // of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come TILE / a.per that clear the
 // packed rows up to the next whole tile: dW's reduction runs over those of the last stage, and
@@ -171,11 +178,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
       const int p = at[i];
       if (on) {
         a.src[p] = (int)r;
-        if (a.kind == KEY_INT64 || a.kind == KEY_INT32) {
-          const int64_t l = a.kind == KEY_INT64 ? reinterpret_cast<const int64_t*>(a.key)[r]
-                                                : reinterpret_cast<const int32_t*>(a.key)[r];
-          a.lab[p] = l >= 0 && l < a.V ? (int)l : -1;
-        }
+        if (a.kind == KEY_INT64 || a.kind == KEY_INT32) a.lab[p] = label_of(a, r);
         for (int k = 0; k < 2; ++k)
           if (a.lse_in[k]) a.lse[k][p] = a.lse_in[k][r];
         if (a.g) a.g[p] = a.grad[r];
@@ -565,19 +568,24 @@ constexpr int few_slots() { return NB == 1 ? 4 : NB == 2 ? 3 : 2; }
 template <int NB>
 constexpr int few_stage() { return (kFewWords + 32 * NB) * BK * 2; }
 
-// acc[word, row] of the wave's 32 words and 32 NB rows; of the tile's 128 words, nw exist
-template <int MODE, int NB>
+// acc[word, row] of the wave's 32 words and 32 NB rows of x, the copies' row i of 32 NB being
+// row_of(i) (none, < 0: zeros); of the tile's 128 words, nw exist, of x's rows nx
+template <int MODE, int NB, typename Row>
 __device__ __forceinline__ void few_tile(lds_u8* lbase, const uint16_t* w, const uint16_t* x, int64_t H,
-                                         int nw, f32x16 (&acc)[NB], int wave, int lane) {
+                                         int nw, int nx, Row&& row_of, f32x16 (&acc)[NB], int wave,
+                                         int lane) {
   constexpr int SLOTS = few_slots<NB>(), STAGE = few_stage<NB>(), COPIES = 4 + NB;
   // copies: a lane's chunk of 16 bytes of every 32 rows, swizzled as the core's row tiles
-  const BufRsrc rw = make_rsrc(w, (uint32_t)(nw * H * 2)), rx = make_rsrc(x, (uint32_t)(32 * NB * H * 2));
+  const BufRsrc rw = make_rsrc(w, (uint32_t)(nw * H * 2)), rx = make_rsrc(x, (uint32_t)(nx * H * 2));
   uint32_t ow[4], ox[NB];
   const int row = threadIdx.x >> 3, ch = (threadIdx.x & 7) ^ row_swz(row);
 #pragma unroll
   for (int i = 0; i < 4; ++i) ow[i] = (uint32_t)(((32 * i + row) * H + ch * 8) * 2);
 #pragma unroll
-  for (int i = 0; i < NB; ++i) ox[i] = (uint32_t)(((32 * i + row) * H + ch * 8) * 2);
+  for (int i = 0; i < NB; ++i) {
+    const int r = row_of(32 * i + row);
+    ox[i] = r < 0 ? kBufOob : (uint32_t)((r * H + ch * 8) * 2);
+  }
   // a last stage that is not whole: chunks past the width are out of the buffer and zero (Operands)
   const int nst = (int)((H + BK - 1) / BK);
   const uint32_t out = H % BK && ch * 8 >= H % BK ? kBufOob : 0;
@@ -620,12 +628,55 @@ __device__ __forceinline__ void few_tile(lds_u8* lbase, const uint16_t* w, const
   __syncthreads();
 }
 
-template <int MODE, int NB>
-__global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a) {
+// The row of x that is the k-th of those that take part: bit k of the set ones of two masks of 64 rows
+__device__ __forceinline__ int kth_row(uint64_t m0, uint64_t m1, int k) {
+  const int c0 = __popcll(m0);
+  uint64_t m = k < c0 ? m0 : m1;
+  int at = k < c0 ? 0 : 64;
+  k -= k < c0 ? 0 : c0;
+  if (k >= __popcll(m)) return -1;
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) {
+    const int c = __popcll(m & ((1ull << s) - 1));
+    if (k >= c) {
+      k -= c;
+      m >>= s;
+      at += s;
+    }
+  }
+  return at;
+}
+
+// GATHER (a forward of up to 128 rows, x as it came): every wave finds the rows that take part from the
+// keys itself and the copies pick them out, instead of a launch that packs them (17 rows of 32000 x 1024
+// 23.2 -> 20.9 us a call, 16 of 151936 x 2560 149 -> 142); the first workgroup leaves what the join needs.
+template <int MODE, int NB, bool GATHER>
+__global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, const PackArgs k) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rows = a.meta->rows;
+  uint64_t m0 = 0, m1 = 0;
+  if constexpr (GATHER) {
+    m0 = __ballot(lane < k.N && takes_part(k, lane));
+    m1 = __ballot(64 + lane < k.N && takes_part(k, 64 + lane));
+  }
+  const int rows = GATHER ? __popcll(m0) + __popcll(m1) : a.meta->rows;
+  if (GATHER && blockIdx.x == 0) {
+    const int r = threadIdx.x;
+    if (r == 0) *k.meta = Meta{rows, 0, 1.f, 1};
+    if (r < k.N) {
+      const uint64_t m = r < 64 ? m0 : m1;
+      if (m >> (r & 63) & 1) {
+        const int p = __popcll(m & ((1ull << (r & 63)) - 1)) + (r < 64 ? 0 : __popcll(m0));
+        k.src[p] = r;
+        k.lab[p] = label_of(k, r);
+      } else {
+#pragma unroll
+        for (int z = 0; z < 3; ++z)
+          if (k.zero[z]) k.zero[z][r] = 0.f;
+      }
+    }
+  }
   const int tiles_i = (int)((a.v1 - a.v0 + kFewWords - 1) / kFewWords);
   const int tiles_j = (rows + 32 * NB - 1) / (32 * NB);
   const int total = tiles_i * tiles_j;
@@ -642,7 +693,20 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a) {
   const int64_t i0 = a.v0 + (int64_t)tile_i * kFewWords, j0 = (int64_t)tile_j * (32 * NB), H = a.H[side];
   const int nw = (int)min((int64_t)kFewWords, a.v1 - i0);
   f32x16 acc[NB];
-  few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, acc, wave, lane);
+  int lab[NB];  // labels of the lane's rows
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int n = 32 * i + (lane & 31);
+    lab[i] = -1;
+    if (MODE != Z_KEEP && j0 + n < rows)
+      lab[i] = GATHER ? label_of(k, kth_row(m0, m1, n)) : a.lab[j0 + n];
+  }
+  if constexpr (GATHER)
+    few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side], H, nw, (int)k.N,
+                       [&](int i) { return kth_row(m0, m1, i); }, acc, wave, lane);
+  else
+    few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, 32 * NB,
+                       [](int i) { return i; }, acc, wave, lane);
 
   // The wave's 32 words of the panel's block, 16 a lane: word vl + 8 (e / 4) + e % 4 of the tile.
   const int vl = 32 * wave + 4 * (lane >> 5);
@@ -666,7 +730,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a) {
                                   ((wi * WAVES_J + (nb >> 1)) * 64 + lane) * 4) = v;
       }
     } else if (n < rows) {
-      const int lv = a.lab[n] - (int)i0 - vl;
+      const int lv = lab[i] - (int)i0 - vl;
       if (lv >= 0 && lv < 32 && (lv & 4) == 0) {
         float zl = 0.f;
 #pragma unroll
@@ -1384,23 +1448,31 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
   return a;
 }
-template <int MODE, int NB>
-static int few_logits(const LogitArgs& a, int64_t N, hipStream_t st, const char* what) {
+template <int MODE, int NB, bool GATHER>
+static int few_logits(const LogitArgs& a, const PackArgs& k, hipStream_t st, const char* what) {
   static uint64_t done = 0;
-  auto kern = few_kernel<MODE, NB>;
+  const int64_t N = k.N;
+  auto kern = few_kernel<MODE, NB, GATHER>;
   constexpr size_t lds = (size_t)few_slots<NB>() * few_stage<NB>();
   if (int rc = reserve_lds((const void*)kern, lds, done, what)) return rc;
   const int64_t items = up(a.v1 - a.v0, kFewWords) / kFewWords * (up(N, 32 * NB) / (32 * NB)) * a.sides;
-  hipLaunchKernelGGL(kern, dim3((unsigned)items), dim3(kFewThreads), lds, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)items), dim3(kFewThreads), lds, st, a, k);
   return check_launch(what);
 }
+template <int MODE, bool GATHER>
+static int few_logits(const LogitArgs& a, const PackArgs& k, hipStream_t st, const char* what) {
+  return k.N <= 32   ? few_logits<MODE, 1, GATHER>(a, k, st, what)
+         : k.N <= 64 ? few_logits<MODE, 2, GATHER>(a, k, st, what)
+                     : few_logits<MODE, 4, GATHER>(a, k, st, what);
+}
 template <int MODE>
-static int logits(const LogitArgs& a, const Sides& s, hipStream_t st, const char* what) {
-  const int64_t N = s.N;
+static int logits(const LogitArgs& a, const PackArgs& k, const Sides& s, hipStream_t st, const char* what) {
   if constexpr (MODE != CE_GRAD) {
-    if (few(N, s.V, s.Ht))
-      return N <= 32 ? few_logits<MODE, 1>(a, N, st, what)
-             : N <= 64 ? few_logits<MODE, 2>(a, N, st, what) : few_logits<MODE, 4>(a, N, st, what);
+    if (few(s.N, s.V, s.Ht)) {
+      // (a forward of up to 128 rows gathers them)
+      if constexpr (MODE == CE_STATS) return few_logits<MODE, 4, false>(a, k, st, what);
+      else return few_logits<MODE, false>(a, k, st, what);
+    }
   }
   const bool stream = MODE != CE_GRAD && a.H[0] > BK && (a.sides < 2 || a.H[1] > BK);
   static uint64_t done[2] = {0, 0};
@@ -1500,14 +1572,27 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
       p.reduction = reduction;
       p.grad_x = grad_x;
     }
-    if (int rc = pack(p, st, what)) return rc;
     LogitArgs l = logit_args(s, w);
     l.planes = !KL ? 2 : STEP ? 4 : 5;
+    // (a step's products read the packed rows; few() holds for up to 128)
+    const bool gather = !STEP && s.N <= 128;
+    if (gather) {
+      l.x[0] = s.x;
+      l.x[1] = s.tx;
+    } else if (int rc = pack(p, st, what)) {
+      return rc;
+    }
     for (int64_t v0 = 0; v0 < s.V; v0 += KL ? w.words : s.V) {
       l.v0 = v0;
       l.v1 = KL ? std::min(s.V, v0 + w.words) : s.V;
       l.tile0 = (int)(v0 / stat);
-      if (int rc = logits<KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS>(l, s, st, what)) return rc;
+      int rc = PLZ_OK;
+      constexpr int MODE = KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS;
+      if constexpr (!STEP) {
+        if (gather) rc = few_logits<MODE, true>(l, p, st, what);
+      }
+      if (!gather) rc = logits<MODE>(l, p, s, st, what);
+      if (rc) return rc;
       if (KL && !STEP) {
         const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1, stat < TILE};
         hipLaunchKernelGGL(cross_kernel, dim3((unsigned)(Np / TILE * (up(l.v1 - l.v0, TILE) / TILE) * 4)),
@@ -1582,7 +1667,7 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   for (int64_t v0 = 0; v0 < s.V; v0 += words) {
     l.v0 = v0;
     l.v1 = std::min(s.V, v0 + words);
-    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, s, st, what)) return rc;
+    if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, p, s, st, what)) return rc;
     if (KL) {
       FinishArgs f = finish_args(s, w, l.v1 - l.v0);
       f.g = p.g;

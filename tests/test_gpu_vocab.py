@@ -698,3 +698,28 @@ def test_more_than_four_gib_of_logits_kept(F, ops):
     x, w, _ = inputs(N, V, H, seed=54)
     tx, tw, _ = inputs(N, V, H, seed=55)
     check(run_kl(F, x, w, tx, tw), reference(x, w, tx=tx, tw=tw))
+
+
+@pytest.mark.parametrize("N", [1, 2, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129])
+@pytest.mark.parametrize("on", ["all", "odd", "first", "last", "late", "none"])
+def test_few_rows_that_take_part(ops, N, on):
+    """Forwards of few rows: any of them may take part, the others hold NaN."""
+    V, H = 700, 72
+    i = torch.arange(N, device="cuda")
+    keep = {"all": i >= 0, "odd": i % 2 == 1, "first": i == 0, "last": i == N - 1, "late": i >= 64,
+            "none": i < 0}[on]
+    x, w, labels = inputs(N, V, H, seed=56)
+    labels = torch.where(keep, labels, torch.full_like(labels, -100))
+    ref = reference(x, w, labels)
+    bad = torch.where(keep[:, None], x, torch.full_like(x, float("nan")))
+    for kind in (labels, labels.int()):
+        loss, lse, total = ops.linear_ce_fwd(bad, w, kind)
+        close(loss, ref["rows"], ref["rows_tol"], "loss")
+        close(total[1], ref["loss"], ref["loss_tol"], "mean")
+        assert float(total[2]) == int(keep.sum()) and not lse[~keep].any()
+    tx, tw, _ = inputs(N, V, 136, seed=57)
+    ref = reference(x, w, tx=tx, tw=tw, mask=keep)
+    loss, lse, total = ops.linear_kl_fwd(bad, w, torch.where(keep[:, None], tx, torch.full_like(tx, float("nan"))), tw, keep)
+    close(loss, ref["rows"], ref["rows_tol"], "loss")
+    close(total[1], ref["loss"], ref["loss_tol"], "mean")
+    assert float(total[2]) == int(keep.sum()) and not lse[:, ~keep].any()

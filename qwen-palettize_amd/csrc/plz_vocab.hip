@@ -116,11 +116,32 @@ __device__ __forceinline__ int label_of(const PackArgs& a, int64_t r) {
   return l >= 0 && l < a.V ? (int)l : -1;
 }
 
+// By one wave: a split of dx a lane, the fastest of the model
+__device__ __forceinline__ void write_meta(const PackArgs& a, int rows) {
+  const int lane = threadIdx.x & 63;
+  int z = lane + 1;
+  float us = a.z_floats ? dx_us(z, rows, a.words, a.H[0], a.cus, a.z_floats) : 0.f;
+#pragma unroll
+  for (int o = 1; o < kMaxSplits; o <<= 1) {
+    const float u = __shfl_xor(us, o);
+    const int v = __shfl_xor(z, o);
+    if (u < us || (u == us && v < z)) {
+      us = u;
+      z = v;
+    }
+  }
+  if (lane == 0) {
+    float alpha = a.inv_t;
+    if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
+    if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
+    *a.meta = Meta{rows, 0, alpha, z};
+  }
+}
+
 // A workgroup packs a.per rows behind all that take part before them, which it counts itself (the keys
 // of 16384 rows are 128 KB in the L2s). Behind the rows' workgroups come TILE / a.per that clear the
 // packed rows up to the next whole tile: dW's reduction runs over those of the last stage, and
-// multiplying zeros takes less power than what was there. The first of them writes meta, a split of dx
-// a lane.
+// multiplying zeros takes less power than what was there. The first of them writes meta.
 __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   __shared__ int red[4];
   __shared__ int at[kPackMost];
@@ -146,25 +167,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
       uint4* d = reinterpret_cast<uint4*>(a.xp[k]) + first * c8;
       for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) d[c] = make_uint4(0, 0, 0, 0);
     }
-    if (pad == 0 && threadIdx.x < 64) {
-      int z = threadIdx.x + 1;
-      float us = a.z_floats ? dx_us(z, rows, a.words, a.H[0], a.cus, a.z_floats) : 0.f;
-#pragma unroll
-      for (int o = 1; o < kMaxSplits; o <<= 1) {
-        const float u = __shfl_xor(us, o);
-        const int v = __shfl_xor(z, o);
-        if (u < us || (u == us && v < z)) {
-          us = u;
-          z = v;
-        }
-      }
-      if (threadIdx.x == 0) {
-        float alpha = a.inv_t;
-        if (a.grad && a.reduction != PLZ_REDUCE_NONE) alpha *= a.grad[0];
-        if (a.reduction == PLZ_REDUCE_MEAN && rows > 0) alpha /= (float)rows;
-        *a.meta = Meta{rows, 0, alpha, z};
-      }
-    }
+    if (pad == 0 && threadIdx.x < 64) write_meta(a, rows);
     return;
   }
   const int n = (int)min((int64_t)a.per, a.N - r0);
@@ -647,9 +650,10 @@ __device__ __forceinline__ int kth_row(uint64_t m0, uint64_t m1, int k) {
   return at;
 }
 
-// GATHER (a forward of up to 128 rows, x as it came): every wave finds the rows that take part from the
+// GATHER (up to 128 rows, x as it came, no dW): every wave finds the rows that take part from the
 // keys itself and the copies pick them out, instead of a launch that packs them (17 rows of 32000 x 1024
-// 23.2 -> 20.9 us a call, 16 of 151936 x 2560 149 -> 142); the first workgroup leaves what the join needs.
+// 23.2 -> 20.9 us a call, 16 of 151936 x 2560 149 -> 142); one workgroup
+// more leaves what the other kernels need.
 template <int MODE, int NB, bool GATHER>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, const PackArgs k) {
   extern __shared__ uint4 smem[];
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
   const int rows = GATHER ? __popcll(m0) + __popcll(m1) : a.meta->rows;
   if (GATHER && blockIdx.x == 0) {
     const int r = threadIdx.x;
-    if (r == 0) *k.meta = Meta{rows, 0, 1.f, 1};
+    if (r < 64) write_meta(k, rows);
     if (r < k.N) {
       const uint64_t m = r < 64 ? m0 : m1;
       if (m >> (r & 63) & 1) {
@@ -676,11 +680,20 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
           if (k.zero[z]) k.zero[z][r] = 0.f;
       }
     }
+    if (k.grad_x && rows < k.N) {
+      const int c8 = (int)(k.H[0] / 8);
+      for (int i = 0; i < (int)k.N; ++i) {
+        if ((i < 64 ? m0 >> i : m1 >> (i - 64)) & 1) continue;
+        uint4* d = reinterpret_cast<uint4*>(k.grad_x) + (int64_t)i * c8;
+        for (int c = threadIdx.x; c < c8; c += kFewThreads) d[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
   }
   const int tiles_i = (int)((a.v1 - a.v0 + kFewWords - 1) / kFewWords);
   const int tiles_j = (rows + 32 * NB - 1) / (32 * NB);
   const int total = tiles_i * tiles_j;
-  int at = (int)blockIdx.x, side = 0;
+  int at = (int)blockIdx.x - (GATHER ? 1 : 0), side = 0;
   if (MODE == Z_KEEP && at >= total) {
     at -= total;
     side = 1;
@@ -1456,7 +1469,7 @@ static int few_logits(const LogitArgs& a, const PackArgs& k, hipStream_t st, con
   constexpr size_t lds = (size_t)few_slots<NB>() * few_stage<NB>();
   if (int rc = reserve_lds((const void*)kern, lds, done, what)) return rc;
   const int64_t items = up(a.v1 - a.v0, kFewWords) / kFewWords * (up(N, 32 * NB) / (32 * NB)) * a.sides;
-  hipLaunchKernelGGL(kern, dim3((unsigned)items), dim3(kFewThreads), lds, st, a, k);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items + GATHER)), dim3(kFewThreads), lds, st, a, k);
   return check_launch(what);
 }
 template <int MODE, bool GATHER>
@@ -1574,8 +1587,8 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     }
     LogitArgs l = logit_args(s, w);
     l.planes = !KL ? 2 : STEP ? 4 : 5;
-    // (a step's products read the packed rows; few() holds for up to 128)
-    const bool gather = !STEP && s.N <= 128;
+    // (dW reads the packed rows; few() holds for up to 128)
+    const bool gather = s.N <= 128 && !grad_w;
     if (gather) {
       l.x[0] = s.x;
       l.x[1] = s.tx;
@@ -1586,12 +1599,8 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
       l.v0 = v0;
       l.v1 = KL ? std::min(s.V, v0 + w.words) : s.V;
       l.tile0 = (int)(v0 / stat);
-      int rc = PLZ_OK;
       constexpr int MODE = KL ? Z_KEEP : STEP ? CE_KEEP : CE_STATS;
-      if constexpr (!STEP) {
-        if (gather) rc = few_logits<MODE, true>(l, p, st, what);
-      }
-      if (!gather) rc = logits<MODE>(l, p, s, st, what);
+      const int rc = gather ? few_logits<MODE, true>(l, p, st, what) : logits<MODE>(l, p, s, st, what);
       if (rc) return rc;
       if (KL && !STEP) {
         const CrossArgs x = {l.kept, l.kept_side, w.meta, w.stats, Np, l.v0, l.v1, stat < TILE};

@@ -717,9 +717,18 @@ def test_few_rows_that_take_part(ops, N, on):
         close(loss, ref["rows"], ref["rows_tol"], "loss")
         close(total[1], ref["loss"], ref["loss_tol"], "mean")
         assert float(total[2]) == int(keep.sum()) and not lse[~keep].any()
+        _, _, total, gx, gw = ops.linear_ce_step(bad, w, kind, grad_weight=False)
+        close(total[1], ref["loss"], ref["loss_tol"], "mean")
+        close(gx, ref["gx"], ref["gx_tol"], "grad_x")
+        assert gw is None and not gx[~keep].any()
     tx, tw, _ = inputs(N, V, 136, seed=57)
     ref = reference(x, w, tx=tx, tw=tw, mask=keep)
-    loss, lse, total = ops.linear_kl_fwd(bad, w, torch.where(keep[:, None], tx, torch.full_like(tx, float("nan"))), tw, keep)
+    bad_tx = torch.where(keep[:, None], tx, torch.full_like(tx, float("nan")))
+    loss, lse, total = ops.linear_kl_fwd(bad, w, bad_tx, tw, keep)
     close(loss, ref["rows"], ref["rows_tol"], "loss")
     close(total[1], ref["loss"], ref["loss_tol"], "mean")
     assert float(total[2]) == int(keep.sum()) and not lse[:, ~keep].any()
+    _, _, total, gx, gw = ops.linear_kl_step(bad, w, bad_tx, tw, mask=keep, grad_weight=False)
+    close(total[1], ref["loss"], ref["loss_tol"], "mean")
+    close(gx, ref["gx"], ref["gx_tol"], "grad_x")
+    assert gw is None and not gx[~keep].any()

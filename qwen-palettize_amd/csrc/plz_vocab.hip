@@ -44,6 +44,12 @@ constexpr float kKeptScale = 32768.f;
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
 constexpr int kPackMost = 64;  // rows of a packing workgroup, at most
+// Up to so many rows, dz is two bf16, the second the first's rounding: row n's lies kTwo rows behind it, in
+// the half of the 256-row tile that would be empty. The products' fp32 sums add both, so that rounding dz
+// does not show: in one bf16 it is off by as much as the gradient's own rounding, more or less by the
+// rows' chance where few are summed (a distillation's gradients of 16 rows 1.3 to 1.9 times the error of
+// those from dz in fp32, of 900 rows 1.4 to 1.5). dx's products are the same, dW's stages twice as many.
+constexpr int kTwo = 128;
 
 enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
 // What a launch over tiles of logits leaves: their statistics, the gradients of the logits, the
@@ -78,6 +84,7 @@ struct PackArgs {
   float* g;       // [Np], reduction none
   float inv_t;
   int64_t words, z_floats;  // of a piece, and of dx's parts: 0 without dx
+  int two;  // kTwo: packed twice
   int cus;
 };
 
@@ -160,12 +167,15 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   }
   if (pad >= 0) {
     const int rows = before, first = rows + pad * a.per;
-    const int end = min(first + a.per, (rows + TILE - 1) / TILE * TILE);
+    const int end = min(first + a.per, a.two ? kTwo : (rows + TILE - 1) / TILE * TILE);
     for (int k = 0; k < 2; ++k) {
       if (!a.x[k] || first >= end) continue;
       const int64_t c8 = a.H[k] / 8;
       uint4* d = reinterpret_cast<uint4*>(a.xp[k]) + first * c8;
-      for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) d[c] = make_uint4(0, 0, 0, 0);
+      for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) {
+        d[c] = make_uint4(0, 0, 0, 0);
+        if (a.two) d[kTwo * c8 + c] = make_uint4(0, 0, 0, 0);
+      }
     }
     if (pad == 0 && threadIdx.x < 64) write_meta(a, rows);
     return;
@@ -201,8 +211,10 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
 #pragma unroll 4
     for (int j = threadIdx.x; j < n * c8; j += 256) {
       const int i = j / c8, p = at[i];
-      if (p >= 0) to[(int64_t)p * c8 + (j - i * c8)] = from[j];
-      else if (k == 0 && a.grad_x) reinterpret_cast<uint4*>(a.grad_x + r0 * H)[j] = make_uint4(0, 0, 0, 0);
+      if (p >= 0) {
+        to[(int64_t)p * c8 + (j - i * c8)] = from[j];
+        if (a.two) to[(int64_t)(p + kTwo) * c8 + (j - i * c8)] = from[j];
+      } else if (k == 0 && a.grad_x) reinterpret_cast<uint4*>(a.grad_x + r0 * H)[j] = make_uint4(0, 0, 0, 0);
     }
   }
 }
@@ -228,11 +240,18 @@ struct LogitArgs {
   int64_t words;  // of a piece, whole tiles
   float* kept;    // logits over T, [side][tile of the launch][256 * 256] in the accumulators' order
   int64_t kept_side;  // floats of a side
+  int two;  // dz's rows up to kTwo in two parts
 };
 
 // exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
 // distance from the maximum (or the normaliser), which is small wherever the exponential counts
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// d and what rounding it leaves, in bf16
+__device__ __forceinline__ uint16_t low_part(float d, uint16_t high) {
+  const float l = d - bf2f(high);
+  return fabsf(l) < INFINITY ? (uint16_t)f2bf(l) : 0;  // else the first part is infinite or NaN
+}
 
 // two exponentials as a step keeps them
 __device__ __forceinline__ uint32_t kept2(float a, float b) {
@@ -529,14 +548,23 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float d = live ? exp_of(acc[ti][tj][e] - lse) * g : 0.f;
-            *reinterpret_cast<lds_u16t*>(lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS +
-                                         nl * 2) = (uint16_t)f2bf(d);
+            const uint16_t high = (uint16_t)f2bf(d);
+            lds_u8* const at = lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS + nl * 2;
+            if (!a.two) {
+              *reinterpret_cast<lds_u16t*>(at) = high;
+            } else if (nl < kTwo) {
+              *reinterpret_cast<lds_u16t*>(at) = high;
+              *reinterpret_cast<lds_u16t*>(at + kTwo * 2) = low_part(d, high);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (live && holds(l))
-          *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) =
-              (uint16_t)f2bf((exp_of(zl - lse) - 1.f) * g);
+        if (live && holds(l)) {
+          const float d = (exp_of(zl - lse) - 1.f) * g;
+          const uint16_t high = (uint16_t)f2bf(d);
+          *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) = high;
+          if (a.two) *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + (nl + kTwo) * 2) = low_part(d, high);
+        }
       }
     }
     if constexpr (MODE == CE_GRAD) {
@@ -1032,6 +1060,7 @@ struct FinishArgs {
   const float* kept;
   int64_t kept_side;
   float* loss;  // [words / 32 / per][Np], or NULL
+  int two;      // dz's rows up to kTwo in two parts
 };
 template <bool KL>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
@@ -1107,8 +1136,15 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int row = 8 * (e >> 2) + (e & 3);
-        *reinterpret_cast<uint16_t*>(st + (row + 4 * (lane >> 5)) * EPI_RS + nl * 2) =
-            (uint16_t)f2bf(live && row < left ? d[e] : 0.f);
+        const float v = live && row < left ? d[e] : 0.f;
+        const uint16_t high = (uint16_t)f2bf(v);
+        uint16_t* const to = reinterpret_cast<uint16_t*>(st + (row + 4 * (lane >> 5)) * EPI_RS) + nl;
+        if (!a.two) {
+          *to = high;
+        } else if (nl < kTwo) {
+          *to = high;
+          to[kTwo] = low_part(v, high);
+        }
       }
     }
     __syncthreads();
@@ -1151,6 +1187,7 @@ struct DwArgs {
   int64_t Np, H, words;
   const Meta* meta;
   uint16_t* out;  // [words][H]
+  int two;        // dz's rows up to kTwo in two parts
 };
 __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
   extern __shared__ uint4 smem[];
@@ -1168,13 +1205,14 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
 #pragma unroll
     for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
   // whole stages: the packed rows past the last one are cleared, and so is dz there
-  const int nst = (a.meta->rows + BK - 1) / BK;
+  const int part = (a.meta->rows + BK - 1) / BK, nst = a.two ? 2 * part : part;
   // (row_tile_dma bounds the copies by its rows: here by all panels)
   TileDma dA = row_tile_dma(a.dzt + i0 * TILE, TILE, 0, TILE);
   dA.r = make_rsrc(a.dzt + i0 * TILE, (uint32_t)((a.Np / TILE * a.panel - i0) * TILE * 2));
   const TileDma dB = col_tile_zero(a.x, a.H, j0, a.Np);
   const uint32_t panel = (uint32_t)(a.panel * TILE * 2);
   dense_stages<false, true>(lbase, nst, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
+    if (a.two && kt >= part) kt += kTwo / BK - part;  // the second parts
     tile_copy(As, dA, (uint32_t)(kt / (TILE / BK)) * panel + (uint32_t)(kt % (TILE / BK)) * (BK * 2));
     tile_copy(Bs, dB, (uint32_t)((int64_t)kt * BK * a.H * 2));
   });
@@ -1211,6 +1249,7 @@ struct DxArgs {
   const Meta* meta;
   float* part;  // [z][rows / 4][H][4]
   int add;      // to what earlier pieces left
+  int two;      // dz's rows up to kTwo in two parts
 };
 __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   extern __shared__ uint4 smem[];
@@ -1244,6 +1283,32 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
     else tile_copy(dst, dB, (uint32_t)(r0 * a.H * 2));
   });
   __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
+  if (a.two) {
+    // the waves of rows kTwo .. hand the second parts' sums to those of the same columns
+    __syncthreads();
+    typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+    lds_f32x4* ex = reinterpret_cast<lds_f32x4*>(lbase) + (threadIdx.x & (NTHR / 2 - 1));
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (wi == 1 - half) {
+#pragma unroll
+        for (int i = 0; i < WT_I * WT_J * 4; ++i) {
+          f32x16& t = acc[i / (WT_J * 4)][i / 4 % WT_J];
+          const int e = i % 4 * 4;
+          if (half == 0) {
+            ex[i * (NTHR / 2)] = f32x4{t[e], t[e + 1], t[e + 2], t[e + 3]};
+          } else {
+            const f32x4 v = ex[i * (NTHR / 2)];
+            t[e] += v[0];
+            t[e + 1] += v[1];
+            t[e + 2] += v[2];
+            t[e + 3] += v[3];
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
   // Four rows of a column are four registers: their sums lie together. From the tile's first four rows a
   // lane's offset and a uniform one of its registers.
   const int64_t quads = (rows + 3) / 4;
@@ -1428,6 +1493,8 @@ static int check_ws(const void* ws, size_t have, size_t need, const char* what) 
   return PLZ_OK;
 }
 
+static int two_parts(int64_t N) { return N <= kTwo; }
+
 static PackArgs pack_args(const Sides& s, const Ws& w) {
   PackArgs a = {};
   a.key = s.key; a.kind = s.kind; a.ignore = s.ignore; a.V = s.V; a.N = s.N;
@@ -1440,6 +1507,7 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
   a.per = s.N <= 2048 ? 4 : s.N <= 16384 ? 8 : kPackMost;
   a.words = w.words; a.z_floats = w.part_floats; a.cus = cu_count();
   a.inv_t = s.inv_t;
+  a.two = two_parts(s.N);
   a.reduction = PLZ_REDUCE_NONE;
   return a;
 }
@@ -1459,6 +1527,7 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.lse = w.lse[0];
   a.dzt = w.dzt; a.words = w.words;
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
+  a.two = two_parts(s.N);
   return a;
 }
 template <int MODE, int NB, bool GATHER>
@@ -1510,13 +1579,14 @@ struct Products {
     if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
     const int64_t tiles_h = up(s.H, TILE) / TILE;
     if (grad_w) {
-      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H};
+      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H,
+                        two_parts(s.N)};
       hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
                          kLdsLogits, st, d);
       if (int rc = check_launch(what)) return rc;
     }
     if (grad_x) {
-      const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add};
+      const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add, two_parts(s.N)};
       // z tiles of rows: z rows H <= the parts' floats, and a split each of a tile that is not full
       const int64_t items = (w.part_floats / s.H / TILE + kMaxSplits) * tiles_h;
       hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
@@ -1540,6 +1610,7 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
   f.kept = w.kept; f.kept_side = f.Np * w.words;
+  f.two = two_parts(s.N);
   return f;
 }
 template <bool KL>

@@ -67,14 +67,18 @@ def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None,
             d = (q - p) / T
             q_tol = q_tol / T
         d, q_tol = d * g[r][:, None], q_tol * g[r][:, None].abs()
-        # rounded to bf16 (a value below the type's range, 2^-133, is not met), then fp32 sums
-        d_tol = U16 * d.abs() + 2 * q_tol + 8 * U32 * d.abs()
+        # rounded to bf16 (a value below the type's range, 2^-133, is not met), of up to 128 rows to two,
+        # then fp32 sums
+        d_tol = (U16 * U16 if N <= 128 else U16) * d.abs() + 2 * q_tol + 8 * U32 * d.abs()
         gx[r] = d @ w.double()
         gx_tol[r] = (d_tol + (V + 64) * U32 * d.abs()) @ w.double().abs()
         gw += d.T @ x[r].double()
         gw_tol += (d_tol + (N + 64) * U32 * d.abs()).T @ x[r].double().abs()
-    gx_tol += (U16 + 4 * U32) * (gx.abs() + gx_tol)
-    gw_tol += (U16 + 4 * U32) * (gw.abs() + gw_tol)
+    # rounded to bf16; a sum's or mean's that the forward computed is multiplied by an upstream gradient
+    # afterwards and rounded once more: r(r(g) u) is off by (1 + 2^-8)^2 - 1 = 2 * 2^-8 + 2^-16 of g u
+    last = U16 if upstream is None or reduction == "none" else 2 * U16 + U16 * U16
+    gx_tol += (last + 4 * U32) * (gx.abs() + gx_tol)
+    gw_tol += (last + 4 * U32) * (gw.abs() + gw_tol)
     loss, tol = rows, rows_tol
     if reduction != "none":
         k = n if reduction == "mean" else 1

@@ -950,20 +950,29 @@ struct JoinArgs {
   Total total;
   float* loss;     // [N]
   float* lse[2];   // [N]
-  float* lsep[2];  // [Np], of the packed rows (or NULL)
+  float* lsep[2];  // [Np], of the packed rows (or NULL), and what rounding them leaves
+  float* rest[2];
   float* apart;    // [Np] the teacher's normaliser less the student's (or NULL)
 };
 enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
 template <int WHAT>
 __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const Stat& s0, const Stat& s1) {
   const int64_t r = a.src[p];
-  const float lse = (float)((double)s0.m + log((double)s0.s));
+  const double exact = (double)s0.m + log((double)s0.s);
+  const float lse = (float)exact;
   a.lse[0][r] = lse;
-  if (a.lsep[0]) a.lsep[0][p] = lse;
+  if (a.lsep[0]) {
+    a.lsep[0][p] = lse;
+    a.rest[0][p] = (float)(exact - lse);
+  }
   if constexpr (WHAT != JOIN_CE) {
-    const float lt = (float)((double)s1.m + log((double)s1.s));
+    const double exact_t = (double)s1.m + log((double)s1.s);
+    const float lt = (float)exact_t;
     a.lse[1][r] = lt;
-    if (a.lsep[1]) a.lsep[1][p] = lt;
+    if (a.lsep[1]) {
+      a.lsep[1][p] = lt;
+      a.rest[1][p] = (float)(exact_t - lt);
+    }
     // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
     // would lose their common part
     const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
@@ -1054,7 +1063,9 @@ struct FinishArgs {
   const int32_t* lab;
   const float* stats;
   const float* zlab;
-  const float* lse[2];  // [Np]
+  // [Np] normalisers, and what rounding them left (or NULL): where a word holds nearly all, its gradient
+  // is a small difference, and the rounding of a normaliser of 16 (10^-6) would be 1% of 10^-4
+  const float *lse[2], *rest[2];
   const float* apart;   // [Np]
   const float* g;       // [Np] or NULL
   const float* kept;
@@ -1090,11 +1101,12 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     for (int tj = 0; tj < WT_J; ++tj) {
       const int nl = wj * 64 + 32 * tj + (lane & 31), n = tile_j * TILE + nl;
       const bool live = n < rows;
-      const float lse = live ? a.lse[0][n] : 0.f;
+      const float lse = live ? a.lse[0][n] : 0.f, rest = live && a.rest[0] ? a.rest[0][n] : 0.f;
       const int left = (int)(a.n - v0) - 4 * (lane >> 5);  // words from the lane's first one
       float d[16];
       if constexpr (KL) {
-        const float lt = live ? a.lse[1][n] : 0.f, apart = live && a.loss ? a.apart[n] : 0.f;
+        const float lt = live ? a.lse[1][n] : 0.f, rest_t = live && a.rest[1] ? a.rest[1][n] : 0.f;
+        const float apart = live && a.loss ? a.apart[n] : 0.f;
         const float g = live && a.g ? a.g[n] : 1.f;
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
@@ -1105,7 +1117,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
               __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.kept + a.kept_side) + o);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float q = exp_of(zs[e] - lse), p = exp_of(zt[e] - lt);
+            const float q = exp_of((zs[e] - lse) - rest), p = exp_of((zt[e] - lt) - rest_t);
             d[4 * e4 + e] = (q - p) * g;
             // a word without weight counts for nothing, however far the two sides are
             if (8 * e4 + e < left && p != 0.f) kl[tj] += p * ((zt[e] - zs[e]) - apart);
@@ -1113,8 +1125,9 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         }
       } else {
         const int l = live ? a.lab[n] : 0;
-        float f = live && v0 < a.n ? exp_of(a.stats[(int64_t)(v0 >> a.stat_log) * 2 * a.Np + n] - lse) : 0.f;
-        f *= 1.f / kKeptScale;
+        float f = 0.f;
+        if (live && v0 < a.n)
+          f = exp_of((a.stats[(int64_t)(v0 >> a.stat_log) * 2 * a.Np + n] - lse) - rest) * (1.f / kKeptScale);
         if (l < 0) f = __builtin_nanf("");  // no such word: nothing to learn from
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -1128,7 +1141,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         // the label's word from the logit itself
         const int lv = l - v0 - 4 * (lane >> 5);
         if (live && lv >= 0 && lv < 32 && (lv & 4) == 0) {
-          const float dl = exp_of(a.zlab[n] - lse) - 1.f;
+          const float dl = expm1f((a.zlab[n] - lse) - rest);
 #pragma unroll
           for (int e = 0; e < 16; ++e) d[e] = lv == 8 * (e >> 2) + (e & 3) ? dl : d[e];
         }
@@ -1401,7 +1414,7 @@ struct Ws {
   float* zlab;
   float* stats;
   float* kept;
-  float* lse[2];
+  float *lse[2], *rest[2];
   float* apart;
   float* kl;
   float* g;
@@ -1436,7 +1449,10 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
   if (Ht || use != WS_BWD)
     w.stats = c.take<float>((size_t)((use == WS_BWD ? w.words : Vp) / stat_words(N, V, Ht)) * (Ht ? 5 : 2) * Np);
   if (use == WS_FWD) return w;
-  for (int k = 0; k < (Ht ? 2 : 1); ++k) w.lse[k] = c.take<float>(Np);
+  for (int k = 0; k < (Ht ? 2 : 1); ++k) {
+    w.lse[k] = c.take<float>(Np);
+    if (use == WS_STEP) w.rest[k] = c.take<float>(Np);
+  }
   if (use == WS_BWD) w.g = c.take<float>(Np);
   if (use == WS_STEP && Ht) {
     w.apart = c.take<float>(Np);
@@ -1609,6 +1625,7 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   f.stat_log = few(s.N, s.V, s.Ht) ? 7 : 8;
   f.meta = w.meta; f.lab = w.lab; f.stats = w.stats; f.zlab = w.zlab;
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
+  f.rest[0] = w.rest[0]; f.rest[1] = w.rest[1];
   f.kept = w.kept; f.kept_side = f.Np * w.words;
   f.two = two_parts(s.N);
   return f;
@@ -1690,6 +1707,8 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.lse[1] = lse + s.N;
     j.lsep[0] = w.lse[0];
     j.lsep[1] = w.lse[1];
+    j.rest[0] = w.rest[0];
+    j.rest[1] = w.rest[1];
     j.apart = w.apart;
     j.total = sums;
     hipLaunchKernelGGL(join_kernel<!KL ? JOIN_CE : STEP ? JOIN_LSE : JOIN_KL>,

@@ -732,3 +732,26 @@ def test_few_rows_that_take_part(ops, N, on):
     close(total[1], ref["loss"], ref["loss_tol"], "mean")
     close(gx, ref["gx"], ref["gx_tol"], "grad_x")
     assert gw is None and not gx[~keep].any()
+
+
+@pytest.mark.parametrize("others", [5.1875, 5.90625, 6.1875, 6.40625])
+def test_a_word_that_holds_nearly_all(F, others):
+    """Its gradient is a small difference, of logits that are exact here: 20, the last of its lane, and
+    others. The sum of exponentials is 1 and little more from there on: six more additions (a half wave,
+    three waves, two joins) of at most 2^-24 each, then the rounding of the result. (A normaliser of 20
+    rounded to fp32 is off by 8.5 to 9.5 times 10^-7 with these others.)"""
+    V, H, at = 40, 8, 27
+    x = torch.zeros(1, H, device="cuda")
+    x[0, 0] = 1
+    w, tw = torch.zeros(V, H, device="cuda"), torch.zeros(V, H, device="cuda")
+    w[:, 0], tw[:, 0] = others, others + 0.25
+    w[at, 0] = tw[at, 0] = 20
+    x, w, tw = x.bfloat16(), w.bfloat16(), tw.bfloat16()
+    q, p = (1 - torch.softmax(t[:, 0].double(), 0)[at] for t in (w, tw))
+    wg = w.clone().requires_grad_()
+    labels = torch.full((1,), at, device="cuda")
+    (got,) = torch.autograd.grad(F.linear_cross_entropy(x, wg, labels), wg)
+    assert abs(got[at, 0].double() + q) <= (2.0 ** -8 + 2.0 ** -12) * q + 7 * 2.0 ** -24
+    # both sides' sums, and their exponentials: two steps of 2^-24 each
+    (got,) = torch.autograd.grad(F.linear_distill(x, wg, x, tw), wg)
+    assert abs(got[at, 0].double() - (p - q)) <= (2.0 ** -8 + 2.0 ** -12) * (p - q).abs() + 16 * 2.0 ** -24

@@ -953,6 +953,7 @@ struct JoinArgs {
   float* lsep[2];  // [Np], of the packed rows (or NULL), and what rounding them leaves
   float* rest[2];
   float* apart;    // [Np] the teacher's normaliser less the student's (or NULL)
+  int32_t* best[2];  // [Np] the tile of each side's maximum (or NULL)
 };
 enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
 template <int WHAT>
@@ -988,6 +989,8 @@ template <int WHAT>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   constexpr int PLANES = WHAT == JOIN_CE ? 2 : WHAT == JOIN_KL ? 5 : 4;
   __shared__ float sh[PLANES][256];
+  __shared__ int sh_best[WHAT == JOIN_LSE ? 2 : 1][256];
+  int best0 = 0, best1 = 0;
   const int RB = 1 << a.rb_log, slices = 256 >> a.rb_log;
   const int rl = threadIdx.x & (RB - 1), sl = threadIdx.x >> a.rb_log;
   const int64_t p = (int64_t)blockIdx.x * RB + rl;
@@ -997,6 +1000,10 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
 #pragma unroll 4
     for (int t = sl; t < a.tiles; t += slices) {
       const float* v = a.stats + (int64_t)t * PLANES * a.Np + p;
+      if constexpr (WHAT == JOIN_LSE) {
+        if (v[0] > s0.m) best0 = t;
+        if (v[2 * a.Np] > s1.m) best1 = t;
+      }
       s0 = join(s0, Stat{v[0], v[a.Np], 0.f});
       if constexpr (PLANES > 2)
         s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], PLANES > 4 ? v[4 * a.Np] : 0.f});
@@ -1011,16 +1018,30 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
         sh[3][threadIdx.x] = s1.s;
         if constexpr (PLANES > 4) sh[4][threadIdx.x] = s1.c;
       }
+      if constexpr (WHAT == JOIN_LSE) {
+        sh_best[0][threadIdx.x] = best0;
+        sh_best[1][threadIdx.x] = best1;
+      }
     }
     __syncthreads();
     if (sl < half) {
       const int i = threadIdx.x + half * RB;
+      if constexpr (WHAT == JOIN_LSE) {
+        if (sh[0][i] > s0.m) best0 = sh_best[0][i];
+        if (sh[2][i] > s1.m) best1 = sh_best[1][i];
+      }
       s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
       if constexpr (PLANES > 2) s1 = join(s1, Stat{sh[2][i], sh[3][i], PLANES > 4 ? sh[4][i] : 0.f});
     }
     // (the next round writes the lower half of what this one read)
   }
-  if (live && sl == 0) write_row<WHAT>(a, p, s0, s1);
+  if (live && sl == 0) {
+    write_row<WHAT>(a, p, s0, s1);
+    if (WHAT == JOIN_LSE && a.best[0]) {
+      a.best[0][p] = best0;
+      a.best[1][p] = best1;
+    }
+  }
   if constexpr (WHAT != JOIN_LSE) add_up(a.total, a.meta);
 }
 
@@ -1044,6 +1065,63 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
     put_loss(loss + src[p], (float)s);
   }
   add_up(total, meta);
+}
+
+// ---- the word whose gradient is the greatest -----------------------------------------------------------
+// One word often holds nearly all of a row's dz (97% of its squares where teacher and student lean to other
+// words), and rounding that one to bf16 is then what the gradients are off by, as much as by their own
+// rounding. So what the rounding leaves of it is added to the products' sums: the word is looked for in the
+// tiles of both sides' maxima, a row a wave, 4 words a lane, with dz as finish_kernel forms it.
+struct TopArgs {
+  const float* kept;
+  int64_t kept_side;
+  int64_t n;  // words
+  int best_shift;  // best counts tiles of 256 words >> best_shift
+  const Meta* meta;
+  const int32_t* best[2];
+  const float *lse[2], *rest[2];
+  int32_t* word;  // [Np], -1: none
+  float* low;     // [Np]
+};
+__global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
+  const int lane = threadIdx.x & 63, p = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (p >= a.meta->rows) return;
+  const int tiles_i = (int)((a.n + TILE - 1) / TILE);
+  const int half = lane & 1, e4 = (lane >> 1) & 3, ti = (lane >> 3) & 3, wi = lane >> 5;
+  const int nl = p % TILE, wj = nl / 64, tj = nl / 32 % 2;
+  const float lse = a.lse[0][p], lt = a.lse[1][p], rest = a.rest[0][p], rest_t = a.rest[1][p];
+  float most = 0.f;
+  int word = -1;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const int t = a.best[side][p] >> a.best_shift;
+    const int64_t o = ((int64_t)(p / TILE) * tiles_i + t) * (TILE * TILE / 4) +
+                      ((ti * WT_J + tj) * 4 + e4) * NTHR + (wi * WAVES_J + wj) * 64 + nl % 32 + 32 * half;
+    const f32x4 zs = reinterpret_cast<const f32x4*>(a.kept)[o];
+    const f32x4 zt = reinterpret_cast<const f32x4*>(a.kept + a.kept_side)[o];
+    const int v = t * TILE + (wi * 4 + ti) * 32 + 8 * e4 + 4 * half;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float d = exp_of((zs[e] - lse) - rest) - exp_of((zt[e] - lt) - rest_t);
+      if (v + e < a.n && fabsf(d) > fabsf(most)) {
+        most = d;
+        word = v + e;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float d = __shfl_xor(most, o);
+    const int w = __shfl_xor(word, o);
+    if (fabsf(d) > fabsf(most) || (fabsf(d) == fabsf(most) && w > word)) {
+      most = d;
+      word = w;
+    }
+  }
+  if (lane == 0) {
+    a.word[p] = word;
+    a.low[p] = most - bf2f(f2bf(most));
+  }
 }
 
 // ---- dz of tiles that were kept ----------------------------------------------------------------------
@@ -1201,7 +1279,65 @@ struct DwArgs {
   const Meta* meta;
   uint16_t* out;  // [words][H]
   int two;        // dz's rows up to kTwo in two parts
+  const int32_t* top;  // [Np] words, or NULL
+  const float* low;    // [Np] what rounding their dz left
 };
+// acc += the remainders of dz of the tile's words i0 .. times their rows of x, 64 rows a stage
+__device__ __forceinline__ void dw_remainders(lds_u8* lbase, const DwArgs& a, int64_t i0, int64_t j0,
+                                              f32x16 (&acc)[WT_I][WT_J], int wi, int wj, int lane) {
+  typedef __attribute__((address_space(3))) int lds_int;
+  lds_int* const list = reinterpret_cast<lds_int*>(lbase + 4 * TILE_BYTES);  // up to 63 + 512 rows
+  lds_int* const counts = list + 1024;
+  const int rows = a.meta->rows, wave = threadIdx.x >> 6;
+  int have = 0;
+  for (int base = 0; base < rows; base += NTHR) {
+    const int r = base + (int)threadIdx.x;
+    const int w = r < rows ? a.top[r] : -1;
+    const bool mine = w >= i0 && w < i0 + TILE;
+    const uint64_t all = __ballot(mine);
+    if (lane == 0) counts[wave] = __popcll(all);
+    __syncthreads();
+    int at = have;
+#pragma unroll
+    for (int k = 0; k < NTHR / 64; ++k) {
+      const int c = counts[k];
+      at += k < wave ? c : 0;
+      have += c;
+    }
+    if (mine) list[at + __popcll(all & ((1ull << lane) - 1))] = r;
+    __syncthreads();
+    while (have >= BK || (have > 0 && base + NTHR >= rows)) {
+      const int n = min(have, BK);
+      // A: zeros but for a remainder a column; B: the rows' x
+      uint4* const as = (uint4*)lbase;
+      uint4* const bs = (uint4*)(lbase + TILE_BYTES);
+#pragma unroll
+      for (int it = 0; it < COPY_INSTS; ++it) {
+        const int ch = it * NTHR + threadIdx.x;
+        as[ch] = make_uint4(0, 0, 0, 0);
+        const int kr = ch >> 5, c = ch & 31;
+        const int64_t h = j0 + 8 * c;
+        bs[col_chunk(kr, c)] = kr < n && h < a.H
+                                   ? *reinterpret_cast<const uint4*>(a.x + (int64_t)list[kr] * a.H + h)
+                                   : make_uint4(0, 0, 0, 0);
+      }
+      const int left = have - n;
+      const int moved = (int)threadIdx.x < left ? list[n + threadIdx.x] : 0;
+      const int row = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+      __syncthreads();
+      if ((int)threadIdx.x < n) {
+        const int k = (int)threadIdx.x;
+        *reinterpret_cast<lds_u16t*>(lbase + row_chunk((int)(a.top[row] - i0), k >> 3) * 16 + (k & 7) * 2) =
+            (uint16_t)f2bf(a.low[row]);
+      }
+      if ((int)threadIdx.x < left) list[threadIdx.x] = moved;
+      __syncthreads();
+      mma_stage_sync<false, true>(lbase, lbase + TILE_BYTES, acc, wi, wj, lane, (n + 15) / 16);
+      __syncthreads();
+      have = left;
+    }
+  }
+}
 __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
   extern __shared__ uint4 smem[];
   lds_u8* lbase = (lds_u8*)smem;
@@ -1229,6 +1365,7 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
     tile_copy(As, dA, (uint32_t)(kt / (TILE / BK)) * panel + (uint32_t)(kt % (TILE / BK)) * (BK * 2));
     tile_copy(Bs, dB, (uint32_t)((int64_t)kt * BK * a.H * 2));
   });
+  if (a.top) dw_remainders(lbase, a, i0, j0, acc, wi, wj, lane);
   const float alpha = a.meta->alpha;
 #pragma unroll
   for (int ti = 0; ti < WT_I; ++ti)
@@ -1352,7 +1489,10 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
 __global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ part,
                                                      const int32_t* __restrict__ src,
                                                      const Meta* __restrict__ meta, int H,
-                                                     uint16_t* __restrict__ out) {
+                                                     uint16_t* __restrict__ out,
+                                                     const int32_t* __restrict__ top,
+                                                     const float* __restrict__ low,
+                                                     const uint16_t* __restrict__ w) {
   const int hb = (H + 255) / 256;  // workgroups of four rows
   const int64_t q = (int)blockIdx.x / hb;
   const int h = (int)blockIdx.x % hb * 256 + threadIdx.x;
@@ -1366,6 +1506,13 @@ __global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ p
   const f32x4* v = reinterpret_cast<const f32x4*>(part) + q * H + h;
 #pragma unroll 8
   for (int k = 0; k < z; ++k, v += quads * H) a += *v;
+  if (top) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = at[i] >= 0 ? top[4 * q + i] : -1;
+      if (t >= 0) a[i] += low[4 * q + i] * bf2f(w[(int64_t)t * H + h]);
+    }
+  }
   const float alpha = meta->alpha;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -1396,6 +1543,7 @@ static int64_t piece_words(int64_t N, int64_t V, int64_t H, int bytes) {
   const int64_t pieces = (tiles + most - 1) / most;
   return (tiles + pieces - 1) / pieces * TILE;
 }
+static int two_parts(int64_t N) { return N <= kTwo; }
 // The workspace, carved in order; p = NULL: sizes only.
 struct Carve {
   char* p;
@@ -1416,6 +1564,8 @@ struct Ws {
   float* kept;
   float *lse[2], *rest[2];
   float* apart;
+  int32_t *best[2], *top;  // of a step's distillation of more than kTwo rows
+  float* low;
   float* kl;
   float* g;
   uint16_t* dzt;
@@ -1456,6 +1606,11 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
   if (use == WS_BWD) w.g = c.take<float>(Np);
   if (use == WS_STEP && Ht) {
     w.apart = c.take<float>(Np);
+    if (!two_parts(N)) {
+      for (int k = 0; k < 2; ++k) w.best[k] = c.take<int32_t>(Np);
+      w.top = c.take<int32_t>(Np);
+      w.low = c.take<float>(Np);
+    }
     w.kl = c.take<float>((size_t)(Vp / 32 / kFinishKl) * Np);
   }
   w.dzt = c.take<uint16_t>((size_t)w.words * Np);
@@ -1508,8 +1663,6 @@ static int check_ws(const void* ws, size_t have, size_t need, const char* what) 
   PLZ_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace must be 16-byte aligned", what);
   return PLZ_OK;
 }
-
-static int two_parts(int64_t N) { return N <= kTwo; }
 
 static PackArgs pack_args(const Sides& s, const Ws& w) {
   PackArgs a = {};
@@ -1596,7 +1749,7 @@ struct Products {
     const int64_t tiles_h = up(s.H, TILE) / TILE;
     if (grad_w) {
       const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H,
-                        two_parts(s.N)};
+                        two_parts(s.N), w.top, w.low};
       hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
                          kLdsLogits, st, d);
       if (int rc = check_launch(what)) return rc;
@@ -1613,7 +1766,7 @@ struct Products {
   int sum() const {
     if (!grad_x) return PLZ_OK;
     hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)(up(s.N, 4) / 4 * (up(s.H, 256) / 256))),
-                       dim3(256), 0, st, w.part, w.src, w.meta, (int)s.H, grad_x);
+                       dim3(256), 0, st, w.part, w.src, w.meta, (int)s.H, grad_x, w.top, w.low, s.w);
     return check_launch(what);
   }
 };
@@ -1710,6 +1863,8 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.rest[0] = w.rest[0];
     j.rest[1] = w.rest[1];
     j.apart = w.apart;
+    j.best[0] = w.best[0];
+    j.best[1] = w.best[1];
     j.total = sums;
     hipLaunchKernelGGL(join_kernel<!KL ? JOIN_CE : STEP ? JOIN_LSE : JOIN_KL>,
                        dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)), dim3(256), 0, st, j);
@@ -1718,6 +1873,12 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
   if (STEP && (KL || grad_x || grad_w)) {
     FinishArgs f = finish_args(s, w, s.V);
     f.loss = w.kl;
+    if (w.top) {
+      const TopArgs t = {w.kept, f.kept_side, s.V, stat < TILE, w.meta, {w.best[0], w.best[1]},
+                         {w.lse[0], w.lse[1]}, {w.rest[0], w.rest[1]}, w.top, w.low};
+      hipLaunchKernelGGL(top_kernel, dim3((unsigned)((s.N + 3) / 4)), dim3(256), 0, st, t);
+      if (int rc = check_launch(what)) return rc;
+    }
     if (int rc = finish<KL>(f, st, what)) return rc;
     if (KL) {
       hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((s.N + 7) / 8)), dim3(256), 0, st, w.kl,

@@ -755,3 +755,25 @@ def test_a_word_that_holds_nearly_all(F, others):
     # both sides' sums, and their exponentials: two steps of 2^-24 each
     (got,) = torch.autograd.grad(F.linear_distill(x, wg, x, tw), wg)
     assert abs(got[at, 0].double() - (p - q)) <= (2.0 ** -8 + 2.0 ** -12) * (p - q).abs() + 16 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("N,V,H,Ht,words", [(129, 300, 64, 64, 300), (400, 5003, 200, 136, 5003),
+                                            (1300, 2048, 72, 64, 3), (900, 40000, 128, 128, 40000)])
+def test_the_word_that_dominates(F, N, V, H, Ht, words):
+    """A distillation of more than 128 rows whose sides lean to different words: what rounding the
+    greatest gradient of a row's logits leaves is added. words: the sides lean to the first ones (of 3: many
+    rows share one)."""
+    x, w, labels = inputs(N, V, H, seed=58, lean=0.0)
+    tx, tw, _ = inputs(N, V, Ht, seed=59, lean=0.0)
+    g = torch.Generator(device="cuda").manual_seed(60)
+    a = torch.randint(0, words, (N,), generator=g, device="cuda")
+    b = (a + 1) % words
+    x = (x.float() + 1.5 * w[a].float()).bfloat16()
+    tx = (tx.float() + 1.5 * tw[b].float()).bfloat16()
+    q, p = (torch.softmax(s.double() @ t.double().T, 1) for s, t in ((x, w), (tx, tw)))
+    most = (q - p).abs().argmax(1)
+    some = torch.zeros(N, V, dtype=torch.bool, device="cuda")
+    for side in (q, p):  # the tiles that are looked at
+        some |= torch.arange(V, device="cuda") // 256 == (side.argmax(1) // 256)[:, None]
+    assert bool(some.gather(1, most[:, None]).all())
+    check(run_kl(F, x, w, tx, tw), reference(x, w, tx=tx, tw=tw, top=True))

@@ -14,11 +14,12 @@ def logits(x, w, T=1.0):
 
 
 def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None, T=1.0,
-              reduction="mean", upstream=None, kept=None):
+              reduction="mean", upstream=None, kept=None, top=False):
     """A dict of the loss and gradients of `reduction` in 64 bits and the bounds of their errors
     (loss_tol, gx_tol, gw_tol), and every row's loss (rows, rows_tol). upstream: the gradient of the
     loss, a number or one of every row. kept: the gradient is of a cross entropy that kept its
-    exponentials in fp16, relative to the greatest of 256 words (a sum or mean of linear_cross_entropy)."""
+    exponentials in fp16, relative to the greatest of 256 words (a sum or mean of linear_cross_entropy).
+    top: the greatest gradient of each row's logits is in two bf16."""
     kept = labels is not None and reduction != "none" if kept is None else kept
     N, V = x.shape[0], w.shape[0]
     dev = x.device
@@ -69,7 +70,10 @@ def reference(x, w, labels=None, ignore_index=-100, tx=None, tw=None, mask=None,
         d, q_tol = d * g[r][:, None], q_tol * g[r][:, None].abs()
         # rounded to bf16 (a value below the type's range, 2^-133, is not met), of up to 128 rows to two,
         # then fp32 sums
-        d_tol = (U16 * U16 if N <= 128 else U16) * d.abs() + 2 * q_tol + 8 * U32 * d.abs()
+        part = torch.full_like(d, U16 * U16 if N <= 128 else U16)
+        if top:
+            part.scatter_(1, d.abs().argmax(1, keepdim=True), U16 * U16)
+        d_tol = part * d.abs() + 2 * q_tol + 8 * U32 * d.abs()
         gx[r] = d @ w.double()
         gx_tol[r] = (d_tol + (V + 64) * U32 * d.abs()) @ w.double().abs()
         gw += d.T @ x[r].double()

@@ -718,8 +718,9 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
  *                  q = softmax(z / T), over teacher_x [N, H_teacher] and teacher_w [V, H_teacher];
  *                  mask uint8 [N]: rows of 0 take no part (NULL: all do).
  * Rows that take no part have loss and lse 0 and gradient 0, and nothing of them, a NaN neither,
- * reaches another output. loss fp32 [N]; lse fp32 [N] (cross entropy) or [2][N] (distillation: the
- * student's, then the teacher's, of z / T), which the backward takes; total (NULL: not wanted) fp32
+ * reaches another output. loss fp32 [N]; lse fp32 [2][N] (cross entropy: the normalisers, then
+ * what rounding them to fp32 left) or [4][N] (distillation: the student's and the teacher's, of z / T,
+ * then what rounding those left), which the backward takes; total (NULL: not wanted) fp32
  * [3] = {sum, mean over the rows that take part (0 without one), their number}.
  * The backward takes grad fp32: [N] of every row's loss (PLZ_REDUCE_NONE), or [1] of the sum
  * (PLZ_REDUCE_SUM) or of the mean (PLZ_REDUCE_MEAN). grad_x bf16 [N, H] and grad_w bf16 [V, H]; NULL:

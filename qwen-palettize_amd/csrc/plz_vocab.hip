@@ -74,11 +74,11 @@ struct PackArgs {
   Meta* meta;
   int32_t* src;    // [Np] the row of a packed row
   int32_t* lab;    // [Np] labels, -1: no word
-  float* zero[3];  // forward: outputs that are 0 for rows that take no part (or NULL)
+  float* zero[5];  // forward: outputs that are 0 for rows that take no part (or NULL)
   uint16_t* grad_x;  // gradients of x, which are 0 for them (or NULL)
   // backward
-  const float* lse_in[2];
-  float* lse[2];  // [Np]
+  const float *lse_in[2], *rest_in[2];
+  float *lse[2], *rest[2];  // [Np]
   const float* grad;
   int reduction;  // PLZ_REDUCE_*
   float* g;       // [Np], reduction none
@@ -193,10 +193,13 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
         a.src[p] = (int)r;
         if (a.kind == KEY_INT64 || a.kind == KEY_INT32) a.lab[p] = label_of(a, r);
         for (int k = 0; k < 2; ++k)
-          if (a.lse_in[k]) a.lse[k][p] = a.lse_in[k][r];
+          if (a.lse_in[k]) {
+            a.lse[k][p] = a.lse_in[k][r];
+            a.rest[k][p] = a.rest_in[k][r];
+          }
         if (a.g) a.g[p] = a.grad[r];
       } else {
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < 5; ++k)
           if (a.zero[k]) a.zero[k][r] = 0.f;
       }
     }
@@ -229,7 +232,7 @@ struct LogitArgs {
   int64_t Np;
   const Meta* meta;
   const int32_t* lab;
-  const float* lse;  // [Np]
+  const float *lse, *rest;  // [Np]
   const float* g;    // [Np] or NULL
   float inv_t;
   float* stats;  // [tile of words][planes][Np]: maximum and sum of the student, of the teacher
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         __syncthreads();
       } else {
         // dz of this row's words, bf16, into the tile staged in LDS [word][row]
-        const float lse = live ? a.lse[n] : 0.f;
+        const float lse = live ? a.lse[n] : 0.f, rest = live ? a.rest[n] : 0.f;
         float g = live && a.g ? a.g[n] : 1.f;
         int l = live ? a.lab[n] : 0;
         if (l < 0) g = __builtin_nanf("");  // no such word: nothing to learn from
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
         for (int ti = 0; ti < WT_I; ++ti) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float d = live ? exp_of(acc[ti][tj][e] - lse) * g : 0.f;
+            const float d = live ? exp_of((acc[ti][tj][e] - lse) - rest) * g : 0.f;
             const uint16_t high = (uint16_t)f2bf(d);
             lds_u8* const at = lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS + nl * 2;
             if (!a.two) {
@@ -560,7 +563,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
         if (live && holds(l)) {
-          const float d = (exp_of(zl - lse) - 1.f) * g;
+          const float d = expm1f((zl - lse) - rest) * g;
           const uint16_t high = (uint16_t)f2bf(d);
           *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) = high;
           if (a.two) *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + (nl + kTwo) * 2) = low_part(d, high);
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
         k.lab[p] = label_of(k, r);
       } else {
 #pragma unroll
-        for (int z = 0; z < 3; ++z)
+        for (int z = 0; z < 5; ++z)
           if (k.zero[z]) k.zero[z][r] = 0.f;
       }
     }
@@ -949,7 +952,8 @@ struct JoinArgs {
   int tiles, rb_log;
   Total total;
   float* loss;     // [N]
-  float* lse[2];   // [N]
+  float* lse[2];   // [N], and what rounding them leaves
+  float* rest_out[2];
   float* lsep[2];  // [Np], of the packed rows (or NULL), and what rounding them leaves
   float* rest[2];
   float* apart;    // [Np] the teacher's normaliser less the student's (or NULL)
@@ -962,6 +966,7 @@ __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const St
   const double exact = (double)s0.m + log((double)s0.s);
   const float lse = (float)exact;
   a.lse[0][r] = lse;
+  a.rest_out[0][r] = (float)(exact - lse);
   if (a.lsep[0]) {
     a.lsep[0][p] = lse;
     a.rest[0][p] = (float)(exact - lse);
@@ -970,6 +975,7 @@ __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const St
     const double exact_t = (double)s1.m + log((double)s1.s);
     const float lt = (float)exact_t;
     a.lse[1][r] = lt;
+    a.rest_out[1][r] = (float)(exact_t - lt);
     if (a.lsep[1]) {
       a.lsep[1][p] = lt;
       a.rest[1][p] = (float)(exact_t - lt);
@@ -1141,7 +1147,7 @@ struct FinishArgs {
   const int32_t* lab;
   const float* stats;
   const float* zlab;
-  // [Np] normalisers, and what rounding them left (or NULL): where a word holds nearly all, its gradient
+  // [Np] normalisers, and what rounding them left: where a word holds nearly all, its gradient
   // is a small difference, and the rounding of a normaliser of 16 (10^-6) would be 1% of 10^-4
   const float *lse[2], *rest[2];
   const float* apart;   // [Np]
@@ -1179,11 +1185,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     for (int tj = 0; tj < WT_J; ++tj) {
       const int nl = wj * 64 + 32 * tj + (lane & 31), n = tile_j * TILE + nl;
       const bool live = n < rows;
-      const float lse = live ? a.lse[0][n] : 0.f, rest = live && a.rest[0] ? a.rest[0][n] : 0.f;
+      const float lse = live ? a.lse[0][n] : 0.f, rest = live ? a.rest[0][n] : 0.f;
       const int left = (int)(a.n - v0) - 4 * (lane >> 5);  // words from the lane's first one
       float d[16];
       if constexpr (KL) {
-        const float lt = live ? a.lse[1][n] : 0.f, rest_t = live && a.rest[1] ? a.rest[1][n] : 0.f;
+        const float lt = live ? a.lse[1][n] : 0.f, rest_t = live ? a.rest[1][n] : 0.f;
         const float apart = live && a.loss ? a.apart[n] : 0.f;
         const float g = live && a.g ? a.g[n] : 1.f;
 #pragma unroll
@@ -1601,7 +1607,7 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
   if (use == WS_FWD) return w;
   for (int k = 0; k < (Ht ? 2 : 1); ++k) {
     w.lse[k] = c.take<float>(Np);
-    if (use == WS_STEP) w.rest[k] = c.take<float>(Np);
+    w.rest[k] = c.take<float>(Np);
   }
   if (use == WS_BWD) w.g = c.take<float>(Np);
   if (use == WS_STEP && Ht) {
@@ -1694,6 +1700,7 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.meta = w.meta; a.lab = w.lab; a.inv_t = s.inv_t;
   a.stats = w.stats; a.zlab = w.zlab;
   a.lse = w.lse[0];
+  a.rest = w.rest[0];
   a.dzt = w.dzt; a.words = w.words;
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
   a.two = two_parts(s.N);
@@ -1821,7 +1828,11 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     PackArgs p = pack_args(s, w);
     p.zero[0] = loss;
     p.zero[1] = lse;
-    if (KL) p.zero[2] = lse + s.N;
+    p.zero[2] = lse + s.N;
+    if (KL) {
+      p.zero[3] = lse + 2 * s.N;
+      p.zero[4] = lse + 3 * s.N;
+    }
     if (STEP) {
       p.reduction = reduction;
       p.grad_x = grad_x;
@@ -1858,6 +1869,8 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.loss = loss;
     j.lse[0] = lse;
     j.lse[1] = lse + s.N;
+    j.rest_out[0] = lse + (KL ? 2 : 1) * s.N;
+    j.rest_out[1] = lse + 3 * s.N;
     j.lsep[0] = w.lse[0];
     j.lsep[1] = w.lse[1];
     j.rest[0] = w.rest[0];
@@ -1917,7 +1930,9 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
   p.grad_x = grad_x;
   for (int k = 0; k < (KL ? 2 : 1); ++k) {
     p.lse_in[k] = lse + k * s.N;
+    p.rest_in[k] = lse + ((KL ? 2 : 1) + k) * s.N;
     p.lse[k] = w.lse[k];
+    p.rest[k] = w.rest[k];
   }
   if (int rc = pack(p, st, what)) return rc;
   LogitArgs l = logit_args(s, w);

@@ -1207,13 +1207,14 @@ def _kept(t, name, *shape):
 
 def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     """Cross entropy of labels (int64 or int32 [N]) under softmax(x weight^T), x bf16 [N, H], weight
-    bf16 [V, H], without the logits: (loss fp32 [N], lse fp32 [N] for the backward, total fp32 [3] =
-    sum, mean over the rows that take part (0 without one) and their number, or None). Rows whose label
+    bf16 [V, H], without the logits: (loss fp32 [N], lse fp32 [2, N] for the backward (the normalisers and
+    what rounding them to fp32 left), total fp32 [3] = sum, mean over the rows that take part (0 without one) and their number, or None). Rows whose label
     is ignore_index take no part: loss 0. Another label outside [0, V) gives NaN."""
     N, V, H = _head(x, weight)
     size = _labels(labels, N)
     dev = _one_device("linear_ce_fwd", x, weight, labels)
-    loss, lse = (torch.empty(N, dtype=torch.float32, device=x.device) for _ in range(2))
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
     ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, 0), x.device)
     _on(dev, "plz_linear_ce_fwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
@@ -1239,7 +1240,8 @@ def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_
     N, V, H = _head(x, weight)
     size, mode = _labels(labels, N), _reduction(reduction)
     dev = _one_device("linear_ce_step", x, weight, labels)
-    loss, lse = (torch.empty(N, dtype=torch.float32, device=x.device) for _ in range(2))
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
@@ -1255,7 +1257,7 @@ def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-
     of its mean or sum (fp32, one value) or of every row's (fp32 [N], reduction "none")."""
     N, V, H = _head(x, weight)
     size, mode = _labels(labels, N), _reduction(reduction)
-    _kept(lse, "lse", N)
+    _kept(lse, "lse", 2, N)
     _upstream(grad, mode, N)
     dev = _one_device("linear_ce_bwd", x, weight, labels, lse, grad)
     gx = torch.empty_like(x) if grad_x else None
@@ -1269,14 +1271,15 @@ def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-
 def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, total=True):
     """Distillation over the vocabulary, sum_v p_v (log p_v - log q_v) with p the teacher's
     softmax(teacher_x teacher_weight^T / temperature) and q the student's, without the logits: (loss
-    fp32 [N], lse fp32 [2, N] for the backward, total as linear_ce_fwd's). mask bool [N]: rows that it
+    fp32 [N], lse fp32 [4, N] for the backward (both sides' normalisers, then what rounding those left),
+    total as linear_ce_fwd's). mask bool [N]: rows that it
     leaves out take no part."""
     N, V, H, Ht = _two_heads(x, weight, teacher_x, teacher_weight)
     _mask(mask, N)
     inv = _inv_temperature(temperature)
     dev = _one_device("linear_kl_fwd", x, weight, teacher_x, teacher_weight, mask)
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
-    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(4, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
     ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, Ht), x.device)
     _on(dev, "plz_linear_kl_fwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
@@ -1292,7 +1295,7 @@ def linear_kl_step(x, weight, teacher_x, teacher_weight, reduction="mean", mask=
     mode, inv = _reduction(reduction), _inv_temperature(temperature)
     dev = _one_device("linear_kl_step", x, weight, teacher_x, teacher_weight, mask)
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
-    lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(4, N, dtype=torch.float32, device=x.device)
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
@@ -1309,7 +1312,7 @@ def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="me
     N, V, H, Ht = _two_heads(x, weight, teacher_x, teacher_weight)
     _mask(mask, N)
     mode, inv = _reduction(reduction), _inv_temperature(temperature)
-    _kept(lse, "lse", 2, N)
+    _kept(lse, "lse", 4, N)
     _upstream(grad, mode, N)
     dev = _one_device("linear_kl_bwd", x, weight, teacher_x, teacher_weight, mask, lse, grad)
     gx = torch.empty_like(x) if grad_x else None

@@ -497,9 +497,9 @@ def test_refusals(F, ops):
     with pytest.raises(ValueError, match="words"):
         F.linear_distill(x, w, x, w[:49])
     with pytest.raises(ValueError, match="grad"):
-        ops.linear_ce_bwd(x, w, labels, torch.zeros(10, device="cuda"), torch.ones(2, device="cuda"))
+        ops.linear_ce_bwd(x, w, labels, torch.zeros(2, 10, device="cuda"), torch.ones(2, device="cuda"))
     with pytest.raises(ValueError, match="lse"):
-        ops.linear_ce_bwd(x, w, labels, torch.zeros(9, device="cuda"), torch.ones(1, device="cuda"))
+        ops.linear_ce_bwd(x, w, labels, torch.zeros(2, 9, device="cuda"), torch.ones(1, device="cuda"))
 
 
 # ---- as they are used together --------------------------------------------------------------------------
@@ -716,7 +716,7 @@ def test_few_rows_that_take_part(ops, N, on):
         loss, lse, total = ops.linear_ce_fwd(bad, w, kind)
         close(loss, ref["rows"], ref["rows_tol"], "loss")
         close(total[1], ref["loss"], ref["loss_tol"], "mean")
-        assert float(total[2]) == int(keep.sum()) and not lse[~keep].any()
+        assert float(total[2]) == int(keep.sum()) and not lse[:, ~keep].any()
         _, _, total, gx, gw = ops.linear_ce_step(bad, w, kind, grad_weight=False)
         close(total[1], ref["loss"], ref["loss_tol"], "mean")
         close(gx, ref["gx"], ref["gx_tol"], "grad_x")
@@ -735,7 +735,8 @@ def test_few_rows_that_take_part(ops, N, on):
 
 
 @pytest.mark.parametrize("others", [5.1875, 5.90625, 6.1875, 6.40625])
-def test_a_word_that_holds_nearly_all(F, others):
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_word_that_holds_nearly_all(F, others, reduction):
     """Its gradient is a small difference, of logits that are exact here: 20, the last of its lane, and
     others. The sum of exponentials is 1 and little more from there on: six more additions (a half wave,
     three waves, two joins) of at most 2^-24 each, then the rounding of the result. (A normaliser of 20
@@ -750,10 +751,12 @@ def test_a_word_that_holds_nearly_all(F, others):
     q, p = (1 - torch.softmax(t[:, 0].double(), 0)[at] for t in (w, tw))
     wg = w.clone().requires_grad_()
     labels = torch.full((1,), at, device="cuda")
-    (got,) = torch.autograd.grad(F.linear_cross_entropy(x, wg, labels), wg)
+    loss = F.linear_cross_entropy(x, wg, labels, reduction=reduction)
+    (got,) = torch.autograd.grad(loss, wg, torch.ones_like(loss))
     assert abs(got[at, 0].double() + q) <= (2.0 ** -8 + 2.0 ** -12) * q + 7 * 2.0 ** -24
     # both sides' sums, and their exponentials: two steps of 2^-24 each
-    (got,) = torch.autograd.grad(F.linear_distill(x, wg, x, tw), wg)
+    loss = F.linear_distill(x, wg, x, tw, reduction=reduction)
+    (got,) = torch.autograd.grad(loss, wg, torch.ones_like(loss))
     assert abs(got[at, 0].double() - (p - q)) <= (2.0 ** -8 + 2.0 ** -12) * (p - q).abs() + 16 * 2.0 ** -24
 
 

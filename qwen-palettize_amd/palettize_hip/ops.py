@@ -1353,6 +1353,12 @@ def _at(a):
     return a.buffer_info()[0]
 
 
+# Told of tensors that a kernel wrote by their addresses: autograd refuses a backward that saved one of
+# them, and who keeps what a gradient was made into (LayerTrainer's squared sums) sees that it has changed.
+# 0.1 us a tensor.
+_written = torch.autograd.graph.increment_version
+
+
 def grad_norm(grads):
     """The 2-norm of all values of a sequence of tensors (bf16, fp16 or fp32, of one device, at least
     one), squared and summed in 64 bits: fp32, no dimensions."""
@@ -1389,6 +1395,7 @@ def scale_grads(grads, factor):
     if len({a for a, n in zip(ptrs, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("scale_grads: a tensor is written twice")
     _on(dev, "plz_scale_grads", _at(ptrs), _at(sizes), _at(kinds), len(grads), _ptr(factor))
+    _written(grads)
 
 
 def clip_grads(grads, max_norm, out=None):
@@ -1427,6 +1434,7 @@ def clip_grads(grads, max_norm, out=None):
     ws = _workspace(query("plz_grad_norm_workspace", _at(sizes), len(grads)), norm.device)
     _on(dev, "plz_clip_grads", _at(ptrs), _at(sizes), _at(kinds), _at(to), _at(to_kinds), len(grads),
         max_norm, _ptr(norm), _ptr(ws), ws.numel())
+    _written(grads if out is None else out)
     return norm
 
 

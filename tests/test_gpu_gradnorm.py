@@ -230,3 +230,44 @@ def test_refusals(ops):
     with pytest.raises(ValueError, match="outputs"):
         ops.clip_grads([a], 1.0, out=[])
     assert torch.equal(a, torch.ones_like(a))
+
+
+# ---- what else knows of the gradients -----------------------------------------------------------------
+def test_autograd_sees_what_was_written(ops):
+    """A tensor that a graph saved and that is clipped or scaled before the backward: refused, as after any
+    in-place operation. A gradient that is only read may still be used."""
+    def saved(t):
+        leaf = torch.ones(16, device="cuda", requires_grad=True)
+        return (leaf * t).sum()
+
+    one = torch.full((), 0.5, device="cuda")
+    read, written = torch.full((16,), 2.0, device="cuda"), torch.full((16,), 2.0, device="cuda")
+    for call, t in ((lambda: ops.clip_grads([written], 1.0), written),
+                    (lambda: ops.clip_grads([read], 1.0, out=[written]), written),
+                    (lambda: ops.scale_grads([written], one), written)):
+        loss, other, before = saved(t), saved(read), t._version
+        call()
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        other.backward()
+
+
+def test_clipped_between_backward_and_update(ops):
+    """The trainer's update takes the squared sums that the backward wrote beside the gradients only while
+    those are as they were: of clipped ones it reports the norm of what they are now."""
+    from palettize_hip import layer
+    from palettize_hip.optim import clip_grad_norm_
+    cfg = layer.LayerConfig(hidden=512, heads=4, kv_heads=2, head_dim=128, intermediate=1024, lora_rank=16)
+    tr = layer.LayerTrainer(cfg, "cuda", seed=0, lora_b_std=0.02)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tr.forward_backward(torch.randn(2, 64, 512, generator=g, device="cuda").bfloat16())
+    before = norm_of([p.grad for p in tr.logits])
+    clip_grad_norm_(tr.logits, before / 8)
+    want = [norm_of([p.grad for p in params]) for params in (tr.logits, tr.others)]
+    assert want[0] < before / 4
+    tr.update()
+    for got, w in zip(tr.opt.last_norms.tolist(), want):
+        # the optimizer's own sum, in fp32, of positive terms: a thread's 32 squares (64 roundings), then
+        # fewer than 64 additions of partial sums
+        assert abs(got - w) <= 128 * 2.0 ** -24 * w

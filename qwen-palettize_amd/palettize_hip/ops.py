@@ -1425,10 +1425,10 @@ def clip_grads(grads, max_norm, out=None):
     if len({to[i] for i in live}) != len(live):
         raise ValueError("clip_grads: a tensor is written twice")
     if out is not None:
-        where = {ptrs[i]: i for i in live}
-        for i in live:
-            j = where.get(to[i])
-            if j is not None and (ptrs[i] != to[i] or kinds[i] != to_kinds[i]):
+        mine = {to[i]: i for i in live}
+        for i in live:  # (a gradient given twice has two readers)
+            j = mine.get(ptrs[i])
+            if j is not None and (i != j or kinds[i] != to_kinds[i]):
                 raise ValueError("clip_grads: an output is another gradient, or of another type in place")
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
     ws = _workspace(query("plz_grad_norm_workspace", _at(sizes), len(grads)), norm.device)

@@ -57,3 +57,23 @@ def test_workspace(lib):
     assert 8 * (10 ** 9 // 32768) < lib.plz_grad_norm_workspace(s, n) < 8 * (10 ** 9 // 32768) + 1024
     assert lib.plz_grad_norm_workspace(None, 0) >= 256
     assert lib.plz_grad_norm_workspace(None, 2) == 0
+
+
+def test_a_gradient_read_beside_its_own_clipping_is_refused(monkeypatch):
+    """Tensors given twice, once or both times in place: refused before anything is launched. (The table's
+    addresses are of the CPU's memory, and no call gets past the checks.)"""
+    import torch
+    from palettize_hip import ops
+    launched = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(ops, "_on", lambda dev, name, *args: launched.append(name))
+    monkeypatch.setattr(ops, "query", lambda *args: 256)
+    g, h, b, c = (torch.ones(64) for _ in range(4))
+    for grads, out in (([g, g], [g, b]), ([g, g], [b, g]), ([g, h, g], [b, h, g]), ([g, h], [h, b]),
+                       ([g, g, h], [c, b, g])):
+        with pytest.raises(ValueError, match="another gradient"):
+            ops.clip_grads(grads, 1.0, out=out)
+    assert not launched
+    for grads, out in (([g, g], [b, c]), ([g, h], [g, b]), ([g, h], [g, h]), ([g, h], [b, c])):
+        ops.clip_grads(grads, 1.0, out=out)
+    assert launched == ["plz_clip_grads"] * 4

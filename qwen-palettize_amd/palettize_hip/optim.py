@@ -24,10 +24,19 @@ def clip_grad_norm_(parameters, max_norm):
     if not live:
         return torch.zeros((), dtype=torch.float32,
                            device=parameters[0].device if parameters else None)
-    for p in live:
-        if not p.grad.is_contiguous():
-            p.grad = p.grad.contiguous()
-    return ops.clip_grads([p.grad for p in live], max_norm)
+    # in place in memory of another order too: who holds the gradient (a bucket's view) holds the clipped
+    # one. An expanded gradient has no memory of its own and gets some.
+    grads = [p.grad for p in live]
+    dense = [g.contiguous() for g in grads]
+    norm = ops.clip_grads(dense, max_norm)
+    for p, g, d in zip(live, grads, dense):
+        if d is g:
+            continue
+        if any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+            p.grad = d
+        else:
+            g.copy_(d)
+    return norm
 
 
 class NextBuild:

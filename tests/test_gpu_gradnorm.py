@@ -271,3 +271,25 @@ def test_clipped_between_backward_and_update(ops):
         # the optimizer's own sum, in fp32, of positive terms: a thread's 32 squares (64 roundings), then
         # fewer than 64 additions of partial sums
         assert abs(got - w) <= 128 * 2.0 ** -24 * w
+
+
+def test_clip_grad_norm_keeps_the_gradients_memory(ops):
+    """Gradients of other orders and strides are scaled where they are: who holds them, or what they are
+    views of, holds the clipped values, and what lies between them stays."""
+    from palettize_hip.optim import clip_grad_norm_
+    bucket = torch.randn(40, 24, device="cuda")
+    turned = torch.randn(24, 40, device="cuda").bfloat16()
+    params = [torch.nn.Parameter(torch.zeros(40, 12, device="cuda")),
+              torch.nn.Parameter(torch.zeros(40, 24, device="cuda", dtype=torch.bfloat16)),
+              torch.nn.Parameter(torch.zeros(7, device="cuda")),
+              torch.nn.Parameter(torch.zeros(5, 3, device="cuda"))]
+    held = [bucket[:, ::2], turned.t(), torch.randn(7, device="cuda"), torch.ones(3, device="cuda").expand(5, 3)]
+    for p, g in zip(params, held):
+        p.grad = g
+    before, rest = [g.clone() for g in held], bucket[:, 1::2].clone()
+    check_norm(clip_grad_norm_(params, 0.25), before)
+    check_clipped([p.grad for p in params], before, 0.25)
+    for p, g in zip(params[:3], held):
+        assert p.grad is g
+    check_clipped([bucket[:, ::2], turned.t()], before[:2], norm_of(before[:2]) * 0.25 / norm_of(before))
+    assert torch.equal(bucket[:, 1::2], rest)

@@ -1216,22 +1216,31 @@ def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
     lse = torch.empty(2, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, 0), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_workspace", N, V, H, 0), x.device)
     _on(dev, "plz_linear_ce_fwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
         _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H)
     return loss, lse, out
 
 
-# sizes that come again each step: looked up once
+# sizes that come again each step: looked up once, on the device of the call (dx's splits and the tiles of
+# few rows go by its CUs)
 @functools.lru_cache(maxsize=256)
-def _vocab_workspace(which, *sizes):
-    return query(which, *sizes)
+def _vocab_workspace(dev, which, *sizes):
+    if torch._C._cuda_getDevice() == dev:
+        return query(which, *sizes)
+    with torch.cuda.device(dev):
+        return query(which, *sizes)
 
 
 def vocab_step_fits(N, V, H, H_teacher=0) -> bool:
     """Whether linear_ce_step (linear_kl_step with H_teacher) takes N rows: it keeps 2 (10) bytes a logit
     for the length of the call, 4 (8) GiB at most."""
-    return _vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, H_teacher, 0) > 0
+    return _vocab_step_fits(N, V, H, H_teacher)
+
+
+@functools.lru_cache(maxsize=256)
+def _vocab_step_fits(*sizes):  # the same on every device
+    return query("plz_vocab_loss_step_workspace", *sizes, 0) > 0
 
 
 def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_x=True, grad_weight=True):
@@ -1245,7 +1254,7 @@ def linear_ce_step(x, weight, labels, reduction="mean", ignore_index=-100, grad_
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, 0, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_step_workspace", N, V, H, 0, int(grad_x)), x.device)
     _on(dev, "plz_linear_ce_step", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index), mode,
         _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
     return loss, lse, total, gx, gw
@@ -1262,7 +1271,7 @@ def linear_ce_bwd(x, weight, labels, lse, grad, reduction="mean", ignore_index=-
     dev = _one_device("linear_ce_bwd", x, weight, labels, lse, grad)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_bwd_workspace", N, V, H, 0, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_bwd_workspace", N, V, H, 0, int(grad_x)), x.device)
     _on(dev, "plz_linear_ce_bwd", _ptr(x), _ptr(weight), _ptr(labels), size, int(ignore_index),
         _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V, H)
     return gx, gw
@@ -1281,7 +1290,7 @@ def linear_kl_fwd(x, weight, teacher_x, teacher_weight, mask=None, temperature=1
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
     lse = torch.empty(4, N, dtype=torch.float32, device=x.device)
     out = torch.empty(3, dtype=torch.float32, device=x.device) if total else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_workspace", N, V, H, Ht), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_workspace", N, V, H, Ht), x.device)
     _on(dev, "plz_linear_kl_fwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, _ptr(loss), _ptr(lse), _ptr(out), _ptr(ws), ws.numel(), N, V, H, Ht)
     return loss, lse, out
@@ -1299,7 +1308,7 @@ def linear_kl_step(x, weight, teacher_x, teacher_weight, reduction="mean", mask=
     total = torch.empty(3, dtype=torch.float32, device=x.device)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_step_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_step_workspace", N, V, H, Ht, int(grad_x)), x.device)
     _on(dev, "plz_linear_kl_step", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, mode, _ptr(loss), _ptr(lse), _ptr(total), _ptr(gx), _ptr(gw), _ptr(ws),
         ws.numel(), N, V, H, Ht)
@@ -1317,7 +1326,7 @@ def linear_kl_bwd(x, weight, teacher_x, teacher_weight, lse, grad, reduction="me
     dev = _one_device("linear_kl_bwd", x, weight, teacher_x, teacher_weight, mask, lse, grad)
     gx = torch.empty_like(x) if grad_x else None
     gw = torch.empty_like(weight) if grad_weight else None
-    ws = _workspace(_vocab_workspace("plz_vocab_loss_bwd_workspace", N, V, H, Ht, int(grad_x)), x.device)
+    ws = _workspace(_vocab_workspace(dev, "plz_vocab_loss_bwd_workspace", N, V, H, Ht, int(grad_x)), x.device)
     _on(dev, "plz_linear_kl_bwd", _ptr(x), _ptr(weight), _ptr(teacher_x), _ptr(teacher_weight),
         _ptr(mask), inv, _ptr(lse), _ptr(grad), mode, _ptr(gx), _ptr(gw), _ptr(ws), ws.numel(), N, V,
         H, Ht)

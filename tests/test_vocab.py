@@ -88,3 +88,51 @@ def test_steps_that_fit(lib):
     for kw, word in ((dict(mode=0), b"reduction"), (dict(mode=7), b"reduction"),
                      (dict(gx=C.c_void_p(8)), b"aligned"), (dict(gw=C.c_void_p(2)), b"aligned")):
         assert call(64, **kw) == 1 and word in lib.plz_last_error()
+
+
+def test_a_workspace_is_sized_on_the_device_of_its_call(monkeypatch):
+    """Devices of other CU counts need other workspaces for the same sizes; whether a step fits does not go
+    by the device, and is not asked of one."""
+    import functools
+
+    import torch
+    from palettize_hip import ops
+    now = [0]
+    # a cache of its own: what is looked up here is not the library's
+    monkeypatch.setattr(ops, "_vocab_workspace", functools.lru_cache(ops._vocab_workspace.__wrapped__))
+
+    class On:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.dev
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    class Sized(Exception):
+        pass
+
+    def workspace(nbytes, device):
+        raise Sized(nbytes)
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(ops, "query", lambda which, *sizes: 1000 * (now[0] + 1))
+    monkeypatch.setattr(ops, "_need", lambda t, *_: t)
+    monkeypatch.setattr(ops, "_workspace", workspace)
+    x, w, labels = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
+    lse = torch.zeros(2, 3)
+    calls = (lambda: ops.linear_ce_fwd(x, w, labels), lambda: ops.linear_ce_step(x, w, labels),
+             lambda: ops.linear_ce_bwd(x, w, labels, lse, torch.ones(1)),
+             lambda: ops.linear_kl_fwd(x, w, x, w), lambda: ops.linear_kl_step(x, w, x, w),
+             lambda: ops.linear_kl_bwd(x, w, x, w, torch.zeros(4, 3), torch.ones(1)))
+    for current in (0, 1):
+        now[0] = current
+        for dev in (1, 0, 2, 1):
+            monkeypatch.setattr(ops, "_one_device", lambda *_: dev)
+            for call in calls:
+                with pytest.raises(Sized) as got:
+                    call()
+                assert got.value.args == (1000 * (dev + 1),) and now[0] == current

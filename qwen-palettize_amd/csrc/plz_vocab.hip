@@ -261,17 +261,24 @@ __device__ __forceinline__ uint32_t kept2(float a, float b) {
   return f2h(a * kKeptScale) | (f2h(b * kKeptScale) << 16);
 }
 
-// The statistics of a set of words: the maximum, the sum of exponentials relative to it and, for the
-// teacher, the sum of exponentials times (teacher - student).
+// The statistics of a set of words: the maximum and the sum of exponentials relative to it.
 struct Stat {
-  float m, s, c;
+  float m, s;
 };
 __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
   const float M = fmaxf(a.m, b.m);
   // no word above -inf on either side: nothing to scale (inf - inf is not 0)
-  if (M == -INFINITY) return Stat{M, a.s + b.s, a.c + b.c};
-  const float fa = exp_of(a.m - M), fb = exp_of(b.m - M);
-  return Stat{M, a.s * fa + b.s * fb, a.c * fa + b.c * fb};
+  if (M == -INFINITY) return Stat{M, a.s + b.s};
+  return Stat{M, a.s * exp_of(a.m - M) + b.s * exp_of(b.m - M)};
+}
+// A set of words' sum of the teacher's exponentials times ((teacher - its maximum) - (student - its
+// maximum)), relative to the maxima Mt and Ms of more words. (Without weight there it is nothing, also
+// where the student's logits were -inf and it was infinite.)
+__device__ __forceinline__ float cross_of(float c, const Stat& student, const Stat& teacher, float Ms, float Mt) {
+  const float f = teacher.m == -INFINITY ? 0.f : exp_of(teacher.m - Mt);
+  if (f == 0.f) return 0.f;
+  const float moved = student.m == -INFINITY ? 0.f : student.m - Ms;
+  return f * (c + teacher.s * ((teacher.m - Mt) - moved));
 }
 // over lanes l and l ^ 32
 __device__ __forceinline__ float swap32_max(float v) {
@@ -836,9 +843,11 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
   }
 }
 
-// Sum of p (t - s) over the words of each tile of a launch that kept both sides' logits, with the
-// weights relative to the teacher's maximum of the tile: the fifth plane of the statistics. HBM-bound, 8
-// bytes a logit. A workgroup takes a tile's column of 64 rows, wave w its words 64 w .. 64 w + 63.
+// Sum of p ((t - max t) - (s - max s)) over the words of each tile of a launch that kept both sides'
+// logits, with the maxima and the weights relative to the teacher's of the tile: the fifth plane of the
+// statistics. What all logits of a row have in common is no part of the loss, and is none of the sum's
+// rounding either. HBM-bound, 8 bytes a logit. A workgroup takes a tile's column of 64 rows, wave w its
+// words 64 w .. 64 w + 63.
 struct CrossArgs {
   const float* kept;
   int64_t kept_side;
@@ -864,8 +873,9 @@ __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
 #pragma unroll
   for (int tj = 0; tj < WT_J; ++tj) {
     const int n = 32 * tj + (lane & 31);
-    const float m = (!a.halves || nw > 128 * wi) && tile_j * TILE + wj * 64 + n < rows ? st[2 * a.Np + n] : 0.f;
-    const float m0 = m == -INFINITY ? 0.f : m;
+    const bool any = (!a.halves || nw > 128 * wi) && tile_j * TILE + wj * 64 + n < rows;
+    const float ms = any ? st[n] : 0.f, mt = any ? st[2 * a.Np + n] : 0.f;
+    const float ms0 = ms == -INFINITY ? 0.f : ms, mt0 = mt == -INFINITY ? 0.f : mt;
     float c = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -880,9 +890,9 @@ __global__ __launch_bounds__(256) void cross_kernel(const CrossArgs a) {
         const float zs[4] = {z.x, z.y, z.z, z.w}, zt[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp_of(zt[e] - m0);
+          const float p = exp_of(zt[e] - mt0);
           // a word without weight counts for nothing, however far the two sides are
-          if (8 * e4 + e < left && p != 0.f) c += p * (zt[e] - zs[e]);
+          if (8 * e4 + e < left && p != 0.f) c += p * ((zt[e] - mt0) - (zs[e] - ms0));
         }
       }
     }
@@ -961,7 +971,7 @@ struct JoinArgs {
 };
 enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
 template <int WHAT>
-__device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const Stat& s0, const Stat& s1) {
+__device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const Stat& s0, const Stat& s1, float c) {
   const int64_t r = a.src[p];
   const double exact = (double)s0.m + log((double)s0.s);
   const float lse = (float)exact;
@@ -980,11 +990,11 @@ __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const St
       a.lsep[1][p] = lt;
       a.rest[1][p] = (float)(exact_t - lt);
     }
-    // from the maxima's difference and the sums' quotient: as a difference of two rounded normalisers it
+    // from the sums' quotient (and the maxima's difference): as a difference of two rounded normalisers it
     // would lose their common part
-    const double apart = ((double)s1.m - s0.m) + log((double)s1.s / s0.s);
-    if constexpr (WHAT == JOIN_KL) put_loss(a.loss + r, (float)((double)s1.c / s1.s - apart));
-    else a.apart[p] = (float)apart;
+    const double quotient = log((double)s1.s / s0.s);
+    if constexpr (WHAT == JOIN_KL) put_loss(a.loss + r, (float)((double)c / s1.s - quotient));
+    else a.apart[p] = (float)(((double)s1.m - s0.m) + quotient);
   } else {
     put_loss(a.loss + r, a.lab[p] < 0 ? __builtin_nanf("")
                                       : (float)((double)s0.m - a.zlab[p] + log((double)s0.s)));
@@ -1001,7 +1011,19 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   const int rl = threadIdx.x & (RB - 1), sl = threadIdx.x >> a.rb_log;
   const int64_t p = (int64_t)blockIdx.x * RB + rl;
   const bool live = p < a.meta->rows;
-  Stat s0{-INFINITY, 0.f, 0.f}, s1{-INFINITY, 0.f, 0.f};
+  Stat s0{-INFINITY, 0.f}, s1{-INFINITY, 0.f};
+  float c = 0.f;
+  // both sides' words, and with the fifth plane theirs in common
+  auto add = [&](const Stat& t0, const Stat& t1, float tc) {
+    const Stat m0 = join(s0, t0);
+    if constexpr (PLANES > 2) {
+      const Stat m1 = join(s1, t1);
+      if constexpr (PLANES > 4)
+        c = cross_of(c, s0, s1, m0.m, m1.m) + cross_of(tc, t0, t1, m0.m, m1.m);
+      s1 = m1;
+    }
+    s0 = m0;
+  };
   if (live) {
 #pragma unroll 4
     for (int t = sl; t < a.tiles; t += slices) {
@@ -1010,9 +1032,8 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
         if (v[0] > s0.m) best0 = t;
         if (v[2 * a.Np] > s1.m) best1 = t;
       }
-      s0 = join(s0, Stat{v[0], v[a.Np], 0.f});
-      if constexpr (PLANES > 2)
-        s1 = join(s1, Stat{v[2 * a.Np], v[3 * a.Np], PLANES > 4 ? v[4 * a.Np] : 0.f});
+      add(Stat{v[0], v[a.Np]}, PLANES > 2 ? Stat{v[2 * a.Np], v[3 * a.Np]} : Stat{},
+          PLANES > 4 ? v[4 * a.Np] : 0.f);
     }
   }
   for (int half = slices / 2; half >= 1; half >>= 1) {
@@ -1022,7 +1043,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
       if constexpr (PLANES > 2) {
         sh[2][threadIdx.x] = s1.m;
         sh[3][threadIdx.x] = s1.s;
-        if constexpr (PLANES > 4) sh[4][threadIdx.x] = s1.c;
+        if constexpr (PLANES > 4) sh[4][threadIdx.x] = c;
       }
       if constexpr (WHAT == JOIN_LSE) {
         sh_best[0][threadIdx.x] = best0;
@@ -1036,13 +1057,13 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
         if (sh[0][i] > s0.m) best0 = sh_best[0][i];
         if (sh[2][i] > s1.m) best1 = sh_best[1][i];
       }
-      s0 = join(s0, Stat{sh[0][i], sh[1][i], 0.f});
-      if constexpr (PLANES > 2) s1 = join(s1, Stat{sh[2][i], sh[3][i], PLANES > 4 ? sh[4][i] : 0.f});
+      if constexpr (PLANES == 2) add(Stat{sh[0][i], sh[1][i]}, Stat{}, 0.f);
+      else add(Stat{sh[0][i], sh[1][i]}, Stat{sh[2][i], sh[3][i]}, PLANES > 4 ? sh[PLANES - 1][i] : 0.f);
     }
     // (the next round writes the lower half of what this one read)
   }
   if (live && sl == 0) {
-    write_row<WHAT>(a, p, s0, s1);
+    write_row<WHAT>(a, p, s0, s1, c);
     if (WHAT == JOIN_LSE && a.best[0]) {
       a.best[0][p] = best0;
       a.best[1][p] = best1;

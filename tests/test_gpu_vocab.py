@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from vocab_ref import close, inputs, reference
+from vocab_ref import close, inputs, logits, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -780,3 +780,51 @@ def test_the_word_that_dominates(F, N, V, H, Ht, words):
         some |= torch.arange(V, device="cuda") // 256 == (side.argmax(1) // 256)[:, None]
     assert bool(some.gather(1, most[:, None]).all())
     check(run_kl(F, x, w, tx, tw), reference(x, w, tx=tx, tw=tw, top=True))
+
+
+# ---- a distillation's loss alone ----------------------------------------------------------------------
+def exact_inputs(N, V, H, seed):
+    """x, w of multiples of 1/4 up to 2: logits, and those moved by up to 2^16, are exact in fp32."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return tuple((torch.randint(-8, 9, (n, H), generator=g, device="cuda") / 4).bfloat16() for n in (N, V))
+
+
+@pytest.mark.parametrize("N,V", [(3, 700), (130, 1003), (300, 40001), (16384, 33333)])
+@pytest.mark.parametrize("shift", [2.0 ** 10, -2.0 ** 14])
+def test_what_all_logits_of_a_row_share_is_no_part_of_a_distillation(ops, N, V, shift):
+    """The student's logits moved by the same amount: exact ones, so every difference is the same and the loss
+    is the same to the last bit. (Of 16384 rows the words come in pieces.)"""
+    x, w = exact_inputs(N, V, 16, 70)
+    tx, tw = exact_inputs(N, V, 16, 71)
+    x[:, -1] = 1
+    w[:, -1] = 0
+    want = ops.linear_kl_fwd(x, w, tx, tw)[0]
+    w[:, -1] = shift
+    assert torch.equal(ops.linear_kl_fwd(x, w, tx, tw)[0], want)
+    # a teacher that is the student but for that
+    same, ws = x.clone(), w.clone()
+    ws[:, -1] = 0
+    assert not ops.linear_kl_fwd(x, w, same, ws)[0].any()
+
+
+@pytest.mark.parametrize("N", [3, 150, 700])
+def test_words_that_cannot_be_distilled(ops, N):
+    """Logits of minus infinity, of whole tiles too: where the teacher's are, the words count for nothing;
+    where only the student's are, the loss is infinite."""
+    V, H = 1100, 64
+    x, w, _ = inputs(N, V, H, seed=72)
+    tx, tw, _ = inputs(N, V, H, seed=73)
+    x[:, 0] = tx[:, 0] = 1
+    i = torch.arange(V, device="cuda")
+    dead = (i < 131) | ((i >= 256) & (i < 512)) | (i == V - 1)
+    kill = lambda t: torch.where(dead[:, None], torch.where(torch.arange(H, device="cuda") == 0,
+                                                            -float("inf"), 0.0), t.float()).bfloat16()
+    both = reference(x, w[~dead], tx=tx, tw=tw[~dead], reduction="none")
+    close(ops.linear_kl_fwd(x, kill(w), tx, kill(tw))[0], both["rows"], both["rows_tol"], "of neither side")
+    # the student's probabilities are of all words: its normaliser is another
+    got = ops.linear_kl_fwd(x, w, tx, kill(tw))[0]
+    z, dz = logits(x, w)
+    apart = torch.logsumexp(z, 1) - torch.logsumexp(z[:, ~dead], 1)
+    tol = both["rows_tol"] + 2 * dz.max(1).values + 256 * 2.0 ** -24
+    close(got, both["rows"] + apart, tol, "of the teacher's words alone")
+    assert bool((ops.linear_kl_fwd(x, kill(w), tx, tw)[0] == float("inf")).all())

@@ -44,12 +44,14 @@ constexpr float kKeptScale = 32768.f;
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
 constexpr int kPackMost = 64;  // rows of a packing workgroup, at most
-// Up to so many rows, dz is two bf16, the second the first's rounding: row n's lies kTwo rows behind it, in
-// the half of the 256-row tile that would be empty. The products' fp32 sums add both, so that rounding dz
-// does not show: in one bf16 it is off by as much as the gradient's own rounding, more or less by the
-// rows' chance where few are summed (a distillation's gradients of 16 rows 1.3 to 1.9 times the error of
-// those from dz in fp32, of 900 rows 1.4 to 1.5). dx's products are the same, dW's stages twice as many.
+// Where no more rows than these take part, dz is two bf16, the second the first's rounding: row n's lies kTwo
+// rows behind it, in the half of the 256-row tile that would be empty. The products' fp32 sums add both, so
+// that rounding dz does not show: in one bf16 it is off by as much as the gradient's own rounding, more or
+// less by the rows' chance where few are summed (a distillation's gradients of 16 rows 1.3 to 1.9 times the
+// error of those from dz in fp32, of 900 rows 1.4 to 1.5). dx's products are the same, dW's stages twice as
+// many, each reading the rows of x once more.
 constexpr int kTwo = 128;
+__host__ __device__ constexpr bool two_parts(int64_t rows) { return rows <= kTwo; }
 
 enum { KEY_NONE = 0, KEY_INT64 = 1, KEY_INT32 = 2, KEY_MASK = 3 };
 // What a launch over tiles of logits leaves: their statistics, the gradients of the logits, the
@@ -84,7 +86,6 @@ struct PackArgs {
   float* g;       // [Np], reduction none
   float inv_t;
   int64_t words, z_floats;  // of a piece, and of dx's parts: 0 without dx
-  int two;  // kTwo: packed twice
   int cus;
 };
 
@@ -167,15 +168,12 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
   }
   if (pad >= 0) {
     const int rows = before, first = rows + pad * a.per;
-    const int end = min(first + a.per, a.two ? kTwo : (rows + TILE - 1) / TILE * TILE);
+    const int end = min(first + a.per, (rows + TILE - 1) / TILE * TILE);
     for (int k = 0; k < 2; ++k) {
       if (!a.x[k] || first >= end) continue;
       const int64_t c8 = a.H[k] / 8;
       uint4* d = reinterpret_cast<uint4*>(a.xp[k]) + first * c8;
-      for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) {
-        d[c] = make_uint4(0, 0, 0, 0);
-        if (a.two) d[kTwo * c8 + c] = make_uint4(0, 0, 0, 0);
-      }
+      for (int64_t c = threadIdx.x; c < (end - first) * c8; c += 256) d[c] = make_uint4(0, 0, 0, 0);
     }
     if (pad == 0 && threadIdx.x < 64) write_meta(a, rows);
     return;
@@ -214,10 +212,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
 #pragma unroll 4
     for (int j = threadIdx.x; j < n * c8; j += 256) {
       const int i = j / c8, p = at[i];
-      if (p >= 0) {
-        to[(int64_t)p * c8 + (j - i * c8)] = from[j];
-        if (a.two) to[(int64_t)(p + kTwo) * c8 + (j - i * c8)] = from[j];
-      } else if (k == 0 && a.grad_x) reinterpret_cast<uint4*>(a.grad_x + r0 * H)[j] = make_uint4(0, 0, 0, 0);
+      if (p >= 0) to[(int64_t)p * c8 + (j - i * c8)] = from[j];
+      else if (k == 0 && a.grad_x) reinterpret_cast<uint4*>(a.grad_x + r0 * H)[j] = make_uint4(0, 0, 0, 0);
     }
   }
 }
@@ -243,7 +239,6 @@ struct LogitArgs {
   int64_t words;  // of a piece, whole tiles
   float* kept;    // logits over T, [side][tile of the launch][256 * 256] in the accumulators' order
   int64_t kept_side;  // floats of a side
-  int two;  // dz's rows up to kTwo in two parts
 };
 
 // exp(d) as 2^(d log2 e): d is formed first, so its rounding and the product's are relative to the
@@ -374,6 +369,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave / WAVES_J, wj = wave % WAVES_J;
   const int rows = a.meta->rows;
+  const bool two = two_parts(rows);
   const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE), tiles_j = (rows + TILE - 1) / TILE;
   const int64_t total = (int64_t)tiles_i * tiles_j;
   // Every XCD walks a run of its own, four tiles of words at a time over the rows, of one side after the
@@ -560,7 +556,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
             const float d = live ? exp_of((acc[ti][tj][e] - lse) - rest) * g : 0.f;
             const uint16_t high = (uint16_t)f2bf(d);
             lds_u8* const at = lbase + (vl + 32 * ti + 8 * (e >> 2) + (e & 3)) * EPI_RS + nl * 2;
-            if (!a.two) {
+            if (!two) {
               *reinterpret_cast<lds_u16t*>(at) = high;
             } else if (nl < kTwo) {
               *reinterpret_cast<lds_u16t*>(at) = high;
@@ -573,7 +569,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
           const float d = expm1f((zl - lse) - rest) * g;
           const uint16_t high = (uint16_t)f2bf(d);
           *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) = high;
-          if (a.two) *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + (nl + kTwo) * 2) = low_part(d, high);
+          if (two) *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + (nl + kTwo) * 2) = low_part(d, high);
         }
       }
     }
@@ -1176,7 +1172,6 @@ struct FinishArgs {
   const float* kept;
   int64_t kept_side;
   float* loss;  // [words / 32 / per][Np], or NULL
-  int two;      // dz's rows up to kTwo in two parts
 };
 template <bool KL>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
@@ -1186,6 +1181,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
   const int64_t tile = (int64_t)blockIdx.x / of;
   const int tile_j = (int)(tile / tiles_i), tile_i = (int)(tile % tiles_i);
   const int rows = a.meta->rows;
+  const bool two = two_parts(rows);
   if (tile_j * TILE >= rows) return;
   const int part = (int)blockIdx.x % of;
   float kl[WT_J] = {0.f, 0.f};
@@ -1257,7 +1253,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         const float v = live && row < left ? d[e] : 0.f;
         const uint16_t high = (uint16_t)f2bf(v);
         uint16_t* const to = reinterpret_cast<uint16_t*>(st + (row + 4 * (lane >> 5)) * EPI_RS) + nl;
-        if (!a.two) {
+        if (!two) {
           *to = high;
         } else if (nl < kTwo) {
           *to = high;
@@ -1305,7 +1301,6 @@ struct DwArgs {
   int64_t Np, H, words;
   const Meta* meta;
   uint16_t* out;  // [words][H]
-  int two;        // dz's rows up to kTwo in two parts
   const int32_t* top;  // [Np] words, or NULL
   const float* low;    // [Np] what rounding their dz left
 };
@@ -1381,18 +1376,20 @@ __global__ __launch_bounds__(NTHR) void dw_kernel(const DwArgs a) {
 #pragma unroll
     for (int j = 0; j < WT_J; ++j) acc[i][j] = f32x16{};
   // whole stages: the packed rows past the last one are cleared, and so is dz there
-  const int part = (a.meta->rows + BK - 1) / BK, nst = a.two ? 2 * part : part;
+  const bool two = two_parts(a.meta->rows);
+  const int part = (a.meta->rows + BK - 1) / BK, nst = two ? 2 * part : part;
   // (row_tile_dma bounds the copies by its rows: here by all panels)
   TileDma dA = row_tile_dma(a.dzt + i0 * TILE, TILE, 0, TILE);
   dA.r = make_rsrc(a.dzt + i0 * TILE, (uint32_t)((a.Np / TILE * a.panel - i0) * TILE * 2));
   const TileDma dB = col_tile_zero(a.x, a.H, j0, a.Np);
   const uint32_t panel = (uint32_t)(a.panel * TILE * 2);
   dense_stages<false, true>(lbase, nst, acc, wi, wj, lane, [&](int kt, lds_u8* As, lds_u8* Bs) {
-    if (a.two && kt >= part) kt += kTwo / BK - part;  // the second parts
-    tile_copy(As, dA, (uint32_t)(kt / (TILE / BK)) * panel + (uint32_t)(kt % (TILE / BK)) * (BK * 2));
-    tile_copy(Bs, dB, (uint32_t)((int64_t)kt * BK * a.H * 2));
+    const bool second = two && kt >= part;  // the second parts, times the same rows of x
+    const int ka = second ? kt + kTwo / BK - part : kt, kb = second ? kt - part : kt;
+    tile_copy(As, dA, (uint32_t)(ka / (TILE / BK)) * panel + (uint32_t)(ka % (TILE / BK)) * (BK * 2));
+    tile_copy(Bs, dB, (uint32_t)((int64_t)kb * BK * a.H * 2));
   });
-  if (a.top) dw_remainders(lbase, a, i0, j0, acc, wi, wj, lane);
+  if (a.top && !two) dw_remainders(lbase, a, i0, j0, acc, wi, wj, lane);
   const float alpha = a.meta->alpha;
 #pragma unroll
   for (int ti = 0; ti < WT_I; ++ti)
@@ -1426,7 +1423,6 @@ struct DxArgs {
   const Meta* meta;
   float* part;  // [z][rows / 4][H][4]
   int add;      // to what earlier pieces left
-  int two;      // dz's rows up to kTwo in two parts
 };
 __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   extern __shared__ uint4 smem[];
@@ -1460,7 +1456,7 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
     else tile_copy(dst, dB, (uint32_t)(r0 * a.H * 2));
   });
   __builtin_amdgcn_s_waitcnt(0);  // the repeated copies past the last stage
-  if (a.two) {
+  if (two_parts(rows)) {
     // the waves of rows kTwo .. hand the second parts' sums to those of the same columns
     __syncthreads();
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
@@ -1533,7 +1529,7 @@ __global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ p
   const f32x4* v = reinterpret_cast<const f32x4*>(part) + q * H + h;
 #pragma unroll 8
   for (int k = 0; k < z; ++k, v += quads * H) a += *v;
-  if (top) {
+  if (top && !two_parts(rows)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = at[i] >= 0 ? top[4 * q + i] : -1;
@@ -1570,7 +1566,6 @@ static int64_t piece_words(int64_t N, int64_t V, int64_t H, int bytes) {
   const int64_t pieces = (tiles + most - 1) / most;
   return (tiles + pieces - 1) / pieces * TILE;
 }
-static int two_parts(int64_t N) { return N <= kTwo; }
 // The workspace, carved in order; p = NULL: sizes only.
 struct Carve {
   char* p;
@@ -1703,7 +1698,6 @@ static PackArgs pack_args(const Sides& s, const Ws& w) {
   a.per = s.N <= 2048 ? 4 : s.N <= 16384 ? 8 : kPackMost;
   a.words = w.words; a.z_floats = w.part_floats; a.cus = cu_count();
   a.inv_t = s.inv_t;
-  a.two = two_parts(s.N);
   a.reduction = PLZ_REDUCE_NONE;
   return a;
 }
@@ -1724,7 +1718,6 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.rest = w.rest[0];
   a.dzt = w.dzt; a.words = w.words;
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
-  a.two = two_parts(s.N);
   return a;
 }
 template <int MODE, int NB, bool GATHER>
@@ -1776,14 +1769,14 @@ struct Products {
     if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
     const int64_t tiles_h = up(s.H, TILE) / TILE;
     if (grad_w) {
-      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H,
-                        two_parts(s.N), w.top, w.low};
+      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H, w.top,
+                        w.low};
       hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
                          kLdsLogits, st, d);
       if (int rc = check_launch(what)) return rc;
     }
     if (grad_x) {
-      const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add, two_parts(s.N)};
+      const DxArgs d = {w.dzt, panel, s.w + v0 * s.H, s.H, n, w.meta, w.part, add};
       // z tiles of rows: z rows H <= the parts' floats, and a split each of a tile that is not full
       const int64_t items = (w.part_floats / s.H / TILE + kMaxSplits) * tiles_h;
       hipLaunchKernelGGL(dx_kernel, dim3((unsigned)items), dim3(NTHR), kLdsRing, st, d);
@@ -1808,7 +1801,6 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
   f.rest[0] = w.rest[0]; f.rest[1] = w.rest[1];
   f.kept = w.kept; f.kept_side = f.Np * w.words;
-  f.two = two_parts(s.N);
   return f;
 }
 template <bool KL>

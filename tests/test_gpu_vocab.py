@@ -828,3 +828,47 @@ def test_words_that_cannot_be_distilled(ops, N):
     tol = both["rows_tol"] + 2 * dz.max(1).values + 256 * 2.0 ** -24
     close(got, both["rows"] + apart, tol, "of the teacher's words alone")
     assert bool((ops.linear_kl_fwd(x, kill(w), tx, tw)[0] == float("inf")).all())
+
+
+# ---- what rounding the logits' gradients may leave -------------------------------------------------------
+def single_terms(N, D, at, seed):
+    """Inputs whose gradients are one product each: the rows `at` hold one value each, in a column of its own,
+    and the head's words too, so that neither gradient sums over words or rows and the roundings of the
+    logits' gradient and of the result show as they are. The other rows hold NaN and take no part."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    k = torch.arange(at.numel(), device="cuda")
+    x, tx = (torch.full((N, D), float("nan"), device="cuda") for _ in range(2))
+    keep = torch.zeros(N, dtype=torch.bool, device="cuda")
+    keep[at] = True
+    w, tw = (torch.diag(0.5 + 1.5 * torch.rand(D, generator=g, device="cuda")).bfloat16() for _ in range(2))
+    for t in (x, tx):
+        t[at] = 0
+        t[at, k] = 6 * torch.rand(at.numel(), generator=g, device="cuda")
+    labels = torch.full((N,), -100, device="cuda")
+    labels[at] = k
+    return x.bfloat16(), w, tx.bfloat16(), tw, labels, keep
+
+
+def check_rows(got, ref, at):
+    """check() of gradients of which only the rows `at` took part, against a reference of those alone."""
+    loss, gx, gw = got
+    close(loss if loss.dim() == 0 else loss[at], ref["loss"], ref["loss_tol"], "loss")
+    close(gx[at], ref["gx"], ref["gx_tol"], "grad_x")
+    close(gw, ref["gw"], ref["gw_tol"], "grad_weight")
+
+
+@pytest.mark.parametrize("N,part,D", [(300, 13, 64), (1000, 100, 128), (200, 128, 136), (4099, 3, 64)])
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_rows_of_many_take_part(F, N, part, D, kind, reduction):
+    """Where up to 128 rows take part, the logits' gradients are in two bf16 however many rows were given."""
+    at = torch.randperm(N, generator=torch.Generator().manual_seed(N))[:part].sort().values.cuda()
+    x, w, tx, tw, labels, keep = single_terms(N, D, at, N + part)
+    up = None
+    if reduction == "none":
+        up = torch.rand(N, device="cuda") + 0.5
+    kw = dict(reduction=reduction, upstream=None if up is None else up[at])
+    if kind == "ce":
+        check_rows(run_ce(F, x, w, labels, reduction, up), reference(x[at], w, labels[at], **kw), at)
+    else:
+        check_rows(run_kl(F, x, w, tx, tw, reduction, up, mask=keep), reference(x[at], w, tx=tx[at], tw=tw, **kw), at)

@@ -237,6 +237,7 @@ struct LogitArgs {
   // [tile of rows][word of the piece, whole tiles][256 rows]: dz, or the exponentials kept for it
   uint16_t* dzt;
   int64_t words;  // of a piece, whole tiles
+  float* low;     // CE_GRAD: [Np] what rounding the labels' dz left (or NULL)
   float* kept;    // logits over T, [side][tile of the launch][256 * 256] in the accumulators' order
   int64_t kept_side;  // floats of a side
 };
@@ -245,11 +246,12 @@ struct LogitArgs {
 // distance from the maximum (or the normaliser), which is small wherever the exponential counts
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-// d and what rounding it leaves, in bf16
-__device__ __forceinline__ uint16_t low_part(float d, uint16_t high) {
+// What rounding d to bf16 (high) leaves, and that in bf16
+__device__ __forceinline__ float left_of(float d, uint16_t high) {
   const float l = d - bf2f(high);
-  return fabsf(l) < INFINITY ? (uint16_t)f2bf(l) : 0;  // else the first part is infinite or NaN
+  return fabsf(l) < INFINITY ? l : 0.f;  // else the first part is infinite or NaN
 }
+__device__ __forceinline__ uint16_t low_part(float d, uint16_t high) { return (uint16_t)f2bf(left_of(d, high)); }
 
 // two exponentials as a step keeps them
 __device__ __forceinline__ uint32_t kept2(float a, float b) {
@@ -570,6 +572,7 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
           const uint16_t high = (uint16_t)f2bf(d);
           *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + nl * 2) = high;
           if (two) *reinterpret_cast<lds_u16t*>(lbase + l * EPI_RS + (nl + kTwo) * 2) = low_part(d, high);
+          if (a.low) a.low[n] = left_of(d, high);
         }
       }
     }
@@ -1093,8 +1096,9 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
 // ---- the word whose gradient is the greatest -----------------------------------------------------------
 // One word often holds nearly all of a row's dz (97% of its squares where teacher and student lean to other
 // words), and rounding that one to bf16 is then what the gradients are off by, as much as by their own
-// rounding. So what the rounding leaves of it is added to the products' sums: the word is looked for in the
-// tiles of both sides' maxima, a row a wave, 4 words a lane, with dz as finish_kernel forms it.
+// rounding. So what the rounding leaves of it is added to the products' sums. Of a cross entropy it is the
+// label's word: 1 - q is the sum of all others' q. Of a distillation it is looked for in the tiles of both
+// sides' maxima, a row a wave, 4 words a lane, with dz as finish_kernel forms it.
 struct TopArgs {
   const float* kept;
   int64_t kept_side;
@@ -1143,7 +1147,7 @@ __global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
   }
   if (lane == 0) {
     a.word[p] = word;
-    a.low[p] = most - bf2f(f2bf(most));
+    a.low[p] = left_of(most, (uint16_t)f2bf(most));
   }
 }
 
@@ -1172,6 +1176,7 @@ struct FinishArgs {
   const float* kept;
   int64_t kept_side;
   float* loss;  // [words / 32 / per][Np], or NULL
+  float* low;   // cross entropy: [Np] what rounding the labels' dz left (or NULL)
 };
 template <bool KL>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
@@ -1243,6 +1248,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         const int lv = l - v0 - 4 * (lane >> 5);
         if (live && lv >= 0 && lv < 32 && (lv & 4) == 0) {
           const float dl = expm1f((a.zlab[n] - lse) - rest);
+          if (a.low) a.low[n] = left_of(dl, (uint16_t)f2bf(dl));
 #pragma unroll
           for (int e = 0; e < 16; ++e) d[e] = lv == 8 * (e >> 2) + (e & 3) ? dl : d[e];
         }
@@ -1300,6 +1306,7 @@ struct DwArgs {
   const uint16_t* x;
   int64_t Np, H, words;
   const Meta* meta;
+  int64_t v0;     // the piece's first word
   uint16_t* out;  // [words][H]
   const int32_t* top;  // [Np] words, or NULL
   const float* low;    // [Np] what rounding their dz left
@@ -1315,7 +1322,7 @@ __device__ __forceinline__ void dw_remainders(lds_u8* lbase, const DwArgs& a, in
   for (int base = 0; base < rows; base += NTHR) {
     const int r = base + (int)threadIdx.x;
     const int w = r < rows ? a.top[r] : -1;
-    const bool mine = w >= i0 && w < i0 + TILE;
+    const bool mine = w >= a.v0 + i0 && w < a.v0 + i0 + TILE;
     const uint64_t all = __ballot(mine);
     if (lane == 0) counts[wave] = __popcll(all);
     __syncthreads();
@@ -1349,7 +1356,8 @@ __device__ __forceinline__ void dw_remainders(lds_u8* lbase, const DwArgs& a, in
       __syncthreads();
       if ((int)threadIdx.x < n) {
         const int k = (int)threadIdx.x;
-        *reinterpret_cast<lds_u16t*>(lbase + row_chunk((int)(a.top[row] - i0), k >> 3) * 16 + (k & 7) * 2) =
+        const int word = (int)(a.top[row] - a.v0 - i0);
+        *reinterpret_cast<lds_u16t*>(lbase + row_chunk(word, k >> 3) * 16 + (k & 7) * 2) =
             (uint16_t)f2bf(a.low[row]);
       }
       if ((int)threadIdx.x < left) list[threadIdx.x] = moved;
@@ -1586,7 +1594,9 @@ struct Ws {
   float* kept;
   float *lse[2], *rest[2];
   float* apart;
-  int32_t *best[2], *top;  // of a step's distillation of more than kTwo rows
+  // of more than kTwo rows: each row's word whose dz is the greatest and what rounding that left, and of a
+  // distillation's step the tiles that it is looked for in
+  int32_t *best[2], *top;
   float* low;
   float* kl;
   float* g;
@@ -1626,6 +1636,10 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
     w.rest[k] = c.take<float>(Np);
   }
   if (use == WS_BWD) w.g = c.take<float>(Np);
+  if (!two_parts(N) && !Ht) {
+    w.top = w.lab;
+    w.low = c.take<float>(Np);
+  }
   if (use == WS_STEP && Ht) {
     w.apart = c.take<float>(Np);
     if (!two_parts(N)) {
@@ -1716,7 +1730,7 @@ static LogitArgs logit_args(const Sides& s, const Ws& w) {
   a.stats = w.stats; a.zlab = w.zlab;
   a.lse = w.lse[0];
   a.rest = w.rest[0];
-  a.dzt = w.dzt; a.words = w.words;
+  a.dzt = w.dzt; a.words = w.words; a.low = w.low;
   a.kept = w.kept; a.kept_side = up(s.N, TILE) * w.words;
   return a;
 }
@@ -1769,8 +1783,8 @@ struct Products {
     if (int rc = reserve_lds((const void*)dx_kernel, kLdsRing, done_x, what)) return rc;
     const int64_t tiles_h = up(s.H, TILE) / TILE;
     if (grad_w) {
-      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, grad_w + v0 * s.H, w.top,
-                        w.low};
+      const DwArgs d = {w.dzt, panel, w.xp[0], up(s.N, TILE), s.H, n, w.meta, v0, grad_w + v0 * s.H,
+                        w.top, w.low};
       hipLaunchKernelGGL(dw_kernel, dim3((unsigned)(up(n, TILE) / TILE * tiles_h)), dim3(NTHR),
                          kLdsLogits, st, d);
       if (int rc = check_launch(what)) return rc;
@@ -1801,6 +1815,7 @@ static FinishArgs finish_args(const Sides& s, const Ws& w, int64_t n) {
   f.lse[0] = w.lse[0]; f.lse[1] = w.lse[1]; f.apart = w.apart;
   f.rest[0] = w.rest[0]; f.rest[1] = w.rest[1];
   f.kept = w.kept; f.kept_side = f.Np * w.words;
+  f.low = w.low;
   return f;
 }
 template <bool KL>
@@ -1899,7 +1914,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
   if (STEP && (KL || grad_x || grad_w)) {
     FinishArgs f = finish_args(s, w, s.V);
     f.loss = w.kl;
-    if (w.top) {
+    if (KL && w.top) {
       const TopArgs t = {w.kept, f.kept_side, s.V, stat < TILE, w.meta, {w.best[0], w.best[1]},
                          {w.lse[0], w.lse[1]}, {w.rest[0], w.rest[1]}, w.top, w.low};
       hipLaunchKernelGGL(top_kernel, dim3((unsigned)((s.N + 3) / 4)), dim3(256), 0, st, t);

@@ -872,3 +872,17 @@ def test_few_rows_of_many_take_part(F, N, part, D, kind, reduction):
         check_rows(run_ce(F, x, w, labels, reduction, up), reference(x[at], w, labels[at], **kw), at)
     else:
         check_rows(run_kl(F, x, w, tx, tw, reduction, up, mask=keep), reference(x[at], w, tx=tx[at], tw=tw, **kw), at)
+
+
+@pytest.mark.parametrize("N,part,D", [(200, 200, 200), (300, 150, 152), (520, 520, 520), (1500, 1100, 1104)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_the_label_s_gradient_in_two_parts(F, ops, N, part, D, reduction):
+    """Of more than 128 rows, what rounding the greatest gradient of a row's logits leaves, the label's, is
+    added to both products; in a step, and where the backward computes the logits again."""
+    at = torch.randperm(N, generator=torch.Generator().manual_seed(N)).sort().values[-part:].cuda()
+    x, w, _, _, labels, _ = single_terms(N, D, at, N + part)
+    up = torch.rand(N, device="cuda") + 0.5 if reduction == "none" else None
+    ref = reference(x[at], w, labels[at], reduction=reduction, top=True, upstream=None if up is None else up[at])
+    check_rows(run_ce(F, x, w, labels, reduction, up), ref, at)
+    if reduction != "none":
+        check_rows(two_calls_ce(ops, x, w, labels, reduction), ref, at)

@@ -724,9 +724,10 @@ int plz_distill_loss_bwd(const uint16_t* student, const uint16_t* teacher, const
  * [3] = {sum, mean over the rows that take part (0 without one), their number}.
  * The backward takes grad fp32: [N] of every row's loss (PLZ_REDUCE_NONE), or [1] of the sum
  * (PLZ_REDUCE_SUM) or of the mean (PLZ_REDUCE_MEAN). grad_x bf16 [N, H] and grad_w bf16 [V, H]; NULL:
- * not wanted. The gradient of the logits is rounded to bf16 before its products with x and w (where no
- * more than 128 rows take part to a sum of two bf16, as the greatest of a row in a distillation's step).
- * The teacher has no gradient. H_teacher = 0 in the workspace queries: cross entropy.
+ * not wanted. The gradient of the logits is rounded to bf16 before its products with x and w, the greatest
+ * of each row (and, where no more than 128 rows take part, every one) to a sum of two bf16. (The greatest of
+ * a distillation: of those in the tiles of 256 words of both sides' greatest logits.) The teacher has no
+ * gradient. H_teacher = 0 in the workspace queries: cross entropy.
  * A step is the forward with the gradients of the sum or mean (reduction) for an upstream gradient of
  * 1: it keeps what the gradients of the logits are made of for the length of the call (2 bytes a logit,
  * a distillation 10) instead of computing the logits twice. Its workspace query returns 0 where N V

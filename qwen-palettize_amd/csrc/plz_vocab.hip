@@ -969,7 +969,8 @@ struct JoinArgs {
   int32_t* best[2];  // [Np] the tile of each side's maximum (or NULL)
   float* low;        // cross entropy: [Np] what rounding the labels' dz will leave (or NULL)
 };
-enum { JOIN_CE, JOIN_KL, JOIN_LSE };  // JOIN_LSE: both sides' normalisers, the loss comes later
+// JOIN_LSE: both sides' normalisers, the loss comes later; JOIN_BEST: the tiles of the maxima alone
+enum { JOIN_CE, JOIN_KL, JOIN_LSE, JOIN_BEST };
 template <int WHAT>
 __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const Stat& s0, const Stat& s1, float c) {
   const int64_t r = a.src[p];
@@ -1008,8 +1009,9 @@ __device__ __forceinline__ void write_row(const JoinArgs& a, int64_t p, const St
 template <int WHAT>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   constexpr int PLANES = WHAT == JOIN_CE ? 2 : WHAT == JOIN_KL ? 5 : 4;
+  constexpr bool BEST = WHAT == JOIN_LSE || WHAT == JOIN_BEST;
   __shared__ float sh[PLANES][256];
-  __shared__ int sh_best[WHAT == JOIN_LSE ? 2 : 1][256];
+  __shared__ int sh_best[BEST ? 2 : 1][256];
   int best0 = 0, best1 = 0;
   const int RB = 1 << a.rb_log, slices = 256 >> a.rb_log;
   const int rl = threadIdx.x & (RB - 1), sl = threadIdx.x >> a.rb_log;
@@ -1032,7 +1034,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
 #pragma unroll 4
     for (int t = sl; t < a.tiles; t += slices) {
       const float* v = a.stats + (int64_t)t * PLANES * a.Np + p;
-      if constexpr (WHAT == JOIN_LSE) {
+      if constexpr (BEST) {
         if (v[0] > s0.m) best0 = t;
         if (v[2 * a.Np] > s1.m) best1 = t;
       }
@@ -1049,7 +1051,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
         sh[3][threadIdx.x] = s1.s;
         if constexpr (PLANES > 4) sh[4][threadIdx.x] = c;
       }
-      if constexpr (WHAT == JOIN_LSE) {
+      if constexpr (BEST) {
         sh_best[0][threadIdx.x] = best0;
         sh_best[1][threadIdx.x] = best1;
       }
@@ -1057,7 +1059,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
     __syncthreads();
     if (sl < half) {
       const int i = threadIdx.x + half * RB;
-      if constexpr (WHAT == JOIN_LSE) {
+      if constexpr (BEST) {
         if (sh[0][i] > s0.m) best0 = sh_best[0][i];
         if (sh[2][i] > s1.m) best1 = sh_best[1][i];
       }
@@ -1067,13 +1069,13 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
     // (the next round writes the lower half of what this one read)
   }
   if (live && sl == 0) {
-    write_row<WHAT>(a, p, s0, s1, c);
-    if (WHAT == JOIN_LSE && a.best[0]) {
+    if constexpr (WHAT != JOIN_BEST) write_row<WHAT>(a, p, s0, s1, c);
+    if (BEST && a.best[0]) {
       a.best[0][p] = best0;
       a.best[1][p] = best1;
     }
   }
-  if constexpr (WHAT != JOIN_LSE) add_up(a.total, a.meta);
+  if constexpr (!BEST) add_up(a.total, a.meta);
 }
 
 // The loss of every row that takes part from its parts [parts][Np], in order
@@ -1103,17 +1105,21 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ par
 // words), and rounding that one to bf16 is then what the gradients are off by, as much as by their own
 // rounding. So what the rounding leaves of it is added to the products' sums. Of a cross entropy it is the
 // label's word: 1 - q is the sum of all others' q. Of a distillation it is looked for in the tiles of both
-// sides' maxima, a row a wave, 4 words a lane, with dz as finish_kernel forms it.
+// sides' maxima, a row a wave, 4 words a lane, with dz as finish_kernel forms it. Of a vocabulary in pieces
+// every piece has its own, which its dW adds; dx adds the greatest of all pieces.
 struct TopArgs {
   const float* kept;
   int64_t kept_side;
-  int64_t n;  // words
+  int64_t n, v0;  // words, and the first of them
   int best_shift;  // best counts tiles of 256 words >> best_shift
   const Meta* meta;
   const int32_t* best[2];
   const float *lse[2], *rest[2];
-  int32_t* word;  // [Np], -1: none
-  float* low;     // [Np]
+  const float* g;  // [Np] or NULL
+  int32_t* word;   // [Np], -1: none
+  float* low;      // [Np]
+  int32_t* x_word;  // of the pieces so far (or NULL)
+  float *x_low, *x_most;
 };
 __global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
   const int lane = threadIdx.x & 63, p = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -1122,6 +1128,7 @@ __global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
   const int half = lane & 1, e4 = (lane >> 1) & 3, ti = (lane >> 3) & 3, wi = lane >> 5;
   const int nl = p % TILE, wj = nl / 64, tj = nl / 32 % 2;
   const float lse = a.lse[0][p], lt = a.lse[1][p], rest = a.rest[0][p], rest_t = a.rest[1][p];
+  const float g = a.g ? a.g[p] : 1.f;
   float most = 0.f;
   int word = -1;
 #pragma unroll
@@ -1134,7 +1141,7 @@ __global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
     const int v = t * TILE + (wi * 4 + ti) * 32 + 8 * e4 + 4 * half;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float d = exp_of((zs[e] - lse) - rest) - exp_of((zt[e] - lt) - rest_t);
+      const float d = (exp_of((zs[e] - lse) - rest) - exp_of((zt[e] - lt) - rest_t)) * g;
       if (v + e < a.n && fabsf(d) > fabsf(most)) {
         most = d;
         word = v + e;
@@ -1151,8 +1158,15 @@ __global__ __launch_bounds__(256) void top_kernel(const TopArgs a) {
     }
   }
   if (lane == 0) {
+    const float low = left_of(most, (uint16_t)f2bf(most));
+    word = word < 0 ? -1 : (int)a.v0 + word;
     a.word[p] = word;
-    a.low[p] = left_of(most, (uint16_t)f2bf(most));
+    a.low[p] = low;
+    if (a.x_word && (a.v0 == 0 || fabsf(most) > a.x_most[p])) {
+      a.x_word[p] = word;
+      a.x_low[p] = low;
+      a.x_most[p] = fabsf(most);
+    }
   }
 }
 
@@ -1627,10 +1641,10 @@ struct Ws {
   float* kept;
   float *lse[2], *rest[2];
   float* apart;
-  // of more than kTwo rows: each row's word whose dz is the greatest and what rounding that left, and of a
-  // distillation's step the tiles that it is looked for in
-  int32_t *best[2], *top;
-  float* low;
+  // of more than kTwo rows: each row's word whose dz is the greatest and what rounding that left; of a
+  // distillation the tiles that it is looked for in, and of its backward that of all pieces so far
+  int32_t *best[2], *top, *x_top;
+  float *low, *x_low, *x_most;
   float* kl;
   float* g;
   uint16_t* dzt;
@@ -1669,17 +1683,18 @@ static Ws carve(Carve& c, int use, int64_t N, int64_t V, int64_t H, int64_t Ht, 
     w.rest[k] = c.take<float>(Np);
   }
   if (use == WS_BWD) w.g = c.take<float>(Np);
-  if (!two_parts(N) && !Ht) {
-    w.top = w.lab;
-    w.low = c.take<float>(Np);
+  if (!two_parts(N)) {
+    for (int k = 0; k < (Ht ? 2 : 0); ++k) w.best[k] = c.take<int32_t>(Np);
+    w.top = w.x_top = Ht ? c.take<int32_t>(Np) : w.lab;
+    w.low = w.x_low = c.take<float>(Np);
+    if (Ht && use == WS_BWD) {
+      w.x_top = c.take<int32_t>(Np);
+      w.x_low = c.take<float>(Np);
+      w.x_most = c.take<float>(Np);
+    }
   }
   if (use == WS_STEP && Ht) {
     w.apart = c.take<float>(Np);
-    if (!two_parts(N)) {
-      for (int k = 0; k < 2; ++k) w.best[k] = c.take<int32_t>(Np);
-      w.top = c.take<int32_t>(Np);
-      w.low = c.take<float>(Np);
-    }
     w.kl = c.take<float>((size_t)(Vp / 32 / kFinishKl) * Np);
   }
   w.dzt = c.take<uint16_t>((size_t)w.words * Np);
@@ -1834,7 +1849,8 @@ struct Products {
   int sum() const {
     if (!grad_x) return PLZ_OK;
     hipLaunchKernelGGL(dx_sum_kernel, dim3((unsigned)(up(s.N, 4) / 4 * (up(s.H, 256) / 256))),
-                       dim3(256), 0, st, w.part, w.src, w.meta, (int)s.H, grad_x, w.top, w.low, s.w);
+                       dim3(256), 0, st, w.part, w.src, w.meta, (int)s.H, grad_x, w.x_top, w.x_low,
+                       s.w);
     return check_launch(what);
   }
 };
@@ -1854,6 +1870,24 @@ template <bool KL>
 static int finish(const FinishArgs& f, hipStream_t st, const char* what) {
   hipLaunchKernelGGL(finish_kernel<KL>, dim3((unsigned)(f.Np / TILE * (up(f.n, TILE) / TILE) * (8 / f.per))),
                      dim3(256), 0, st, f);
+  return check_launch(what);
+}
+
+// Workgroups of a join and the rows of each
+static unsigned join_grid(int64_t N, int& rb_log) {
+  rb_log = N >= 4096 ? 4 : N >= 512 ? 2 : 0;
+  return (unsigned)((N + (1 << rb_log) - 1) >> rb_log);
+}
+// Each row's word whose dz is the greatest of the n words from v0 on, whose logits are kept
+static int top(const Sides& s, const Ws& w, int64_t n, int64_t v0, const float* g, hipStream_t st,
+               const char* what) {
+  const bool halves = stat_words(s.N, s.V, s.Ht) < TILE;
+  TopArgs t = {w.kept, up(s.N, TILE) * w.words, n, v0, halves, w.meta, {w.best[0], w.best[1]},
+               {w.lse[0], w.lse[1]}, {w.rest[0], w.rest[1]}, g, w.top, w.low};
+  if (w.x_most) {
+    t.x_word = w.x_top; t.x_low = w.x_low; t.x_most = w.x_most;
+  }
+  hipLaunchKernelGGL(top_kernel, dim3((unsigned)((s.N + 3) / 4)), dim3(256), 0, st, t);
   return check_launch(what);
 }
 
@@ -1925,7 +1959,7 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.stats = w.stats; j.zlab = w.zlab; j.meta = w.meta; j.src = w.src; j.lab = w.lab;
     j.Np = Np;
     j.tiles = (int)(up(s.V, stat) / stat);
-    j.rb_log = s.N >= 4096 ? 4 : s.N >= 512 ? 2 : 0;
+    const unsigned joins = join_grid(s.N, j.rb_log);
     j.loss = loss;
     j.lse[0] = lse;
     j.lse[1] = lse + s.N;
@@ -1941,18 +1975,14 @@ static int forward(const Sides& s, int reduction, float* loss, float* lse, float
     j.low = KL ? nullptr : w.low;
     j.total = sums;
     hipLaunchKernelGGL(join_kernel<!KL ? JOIN_CE : STEP ? JOIN_LSE : JOIN_KL>,
-                       dim3((unsigned)((s.N + (1 << j.rb_log) - 1) >> j.rb_log)), dim3(256), 0, st, j);
+                       dim3(joins), dim3(256), 0, st, j);
     if (int rc = check_launch(what)) return rc;
   }
   if (STEP && (KL || grad_x || grad_w)) {
     FinishArgs f = finish_args(s, w, s.V);
     f.loss = w.kl;
-    if (KL && w.top) {
-      const TopArgs t = {w.kept, f.kept_side, s.V, stat < TILE, w.meta, {w.best[0], w.best[1]},
-                         {w.lse[0], w.lse[1]}, {w.rest[0], w.rest[1]}, w.top, w.low};
-      hipLaunchKernelGGL(top_kernel, dim3((unsigned)((s.N + 3) / 4)), dim3(256), 0, st, t);
-      if (int rc = check_launch(what)) return rc;
-    }
+    if (KL && w.top)
+      if (int rc = top(s, w, s.V, 0, nullptr, st, what)) return rc;
     if (int rc = finish<KL>(f, st, what)) return rc;
     if (KL) {
       hipLaunchKernelGGL(rows_kernel, dim3((unsigned)((s.N + 7) / 8)), dim3(256), 0, st, w.kl,
@@ -2005,6 +2035,17 @@ static int backward(const Sides& s, const float* lse, const float* grad, int red
     l.v1 = std::min(s.V, v0 + words);
     if (int rc = logits<KL ? Z_KEEP : CE_GRAD>(l, p, s, st, what)) return rc;
     if (KL) {
+      if (w.top) {
+        const int stat = stat_words(s.N, s.V, s.Ht);
+        JoinArgs j = {};
+        j.stats = w.stats; j.meta = w.meta; j.Np = l.Np;
+        j.tiles = (int)(up(l.v1 - l.v0, stat) / stat);
+        j.best[0] = w.best[0]; j.best[1] = w.best[1];
+        const unsigned joins = join_grid(s.N, j.rb_log);
+        hipLaunchKernelGGL(join_kernel<JOIN_BEST>, dim3(joins), dim3(256), 0, st, j);
+        if (int rc = check_launch(what)) return rc;
+        if (int rc = top(s, w, l.v1 - l.v0, l.v0, p.g, st, what)) return rc;
+      }
       FinishArgs f = finish_args(s, w, l.v1 - l.v0);
       f.g = p.g;
       if (int rc = finish<true>(f, st, what)) return rc;

@@ -886,3 +886,44 @@ def test_the_label_s_gradient_in_two_parts(F, ops, N, part, D, reduction):
     check_rows(run_ce(F, x, w, labels, reduction, up), ref, at)
     if reduction != "none":
         check_rows(two_calls_ce(ops, x, w, labels, reduction), ref, at)
+
+
+@pytest.mark.parametrize("N,part,D", [(200, 200, 200), (300, 150, 152), (520, 520, 520), (1500, 1100, 1104)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_distillation_s_backward_adds_what_its_step_adds(F, ops, N, part, D, reduction):
+    """Of more than 128 rows, what rounding the greatest gradient of a row's logits leaves is added, whether a
+    step or a backward of its own computes them."""
+    at = torch.randperm(N, generator=torch.Generator().manual_seed(N)).sort().values[-part:].cuda()
+    x, w, tx, tw, _, keep = single_terms(N, D, at, N + part)
+    up = torch.rand(N, device="cuda") - 0.5 if reduction == "none" else None
+    ref = reference(x[at], w, tx=tx[at], tw=tw, reduction=reduction, top=True, upstream=None if up is None else up[at])
+    check_rows(run_kl(F, x, w, tx, tw, reduction, up, mask=keep), ref, at)
+    if reduction != "none":
+        check_rows(two_calls_kl(ops, x, w, tx, tw, keep), ref, at)
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_the_greatest_gradients_over_pieces(ops, kind):
+    """As those, of a vocabulary in four pieces: a piece's dW adds its own, dx the greatest of all. 200 words
+    anywhere hold one value each, in a column of its own; the other words' logits are 0."""
+    N, part, V, H = 16384, 200, 25011, 200
+    g = torch.Generator(device="cuda").manual_seed(80)
+    at = torch.randperm(N, generator=torch.Generator().manual_seed(81))[:part].sort().values.cuda()
+    _, dw, _, dtw, _, keep = single_terms(N, H, at, 82)
+    words = torch.randperm(V, generator=torch.Generator().manual_seed(83))[:H].cuda()
+    x, tx = (torch.full((N, H), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    w, tw = (torch.zeros(V, H, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    k = torch.arange(part, device="cuda")
+    # the sides lean to other words, of other pieces
+    for t, d, m, l in ((x, dw, w, k), (tx, dtw, tw, (k + 77) % part)):
+        t[at] = 0
+        t[at, l] = (9 + 3 * torch.rand(part, generator=g, device="cuda")).bfloat16()
+        m[words] = d
+    labels = torch.full((N,), -100, device="cuda")
+    labels[at] = words[k]
+    if kind == "ce":
+        ref = reference(x[at], w, labels[at], kept=False, top=True)
+        check_rows(two_calls_ce(ops, x, w, labels), ref, at)
+    else:
+        ref = reference(x[at], w, tx=tx[at], tw=tw, top=True)
+        check_rows(two_calls_kl(ops, x, w, tx, tw, keep), ref, at)

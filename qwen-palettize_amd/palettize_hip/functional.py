@@ -12,7 +12,7 @@
       W_soft = sum_c P_c pal_c without the 1/tau factor unless scale_by_inv_tau.
 
   linear_cross_entropy(x, weight, labels), linear_distill(x, weight, teacher_x, teacher_weight)
-      losses over a large vocabulary from hidden states and head weights, the logits never kept.
+      losses over a large vocabulary from hidden states and head weights, no logits kept beyond a call.
 
 Inputs are 2-D ([M, K]); callers flatten leading dimensions.
 """
@@ -256,12 +256,19 @@ def _two_dims(**weights):
             raise ValueError(f"{name} must have 2 dimensions, got {tuple(w.shape)}")
 
 
-def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean"):
+def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean", recompute=False):
     """Cross entropy of labels under softmax(x weight^T): torch's cross_entropy of those logits in fp32,
     without them. x bf16 [..., H], weight bf16 [V, H] (H a multiple of 8), labels int64 or int32 [...].
     Rows whose label is ignore_index take no part (whatever x holds there; their gradient is 0); other
     labels outside [0, V) give NaN. Returns fp32: the mean over the rows that take part (0 without
-    one), the sum, or every row's loss in the labels' shape. Gradients of x and weight are bf16."""
+    one), the sum, or every row's loss in the labels' shape. Gradients of x and weight are bf16.
+
+    Where gradients are on, the forward of a mean or sum computes them too where it can
+    (ops.vocab_step_fits), with 2 bytes a logit for the length of its call, and holds them for the
+    backward, which rounds them again where its upstream gradient is not 1 or a power of two. recompute:
+    the forward computes the loss alone and holds 8 bytes a row, and the backward computes the logits
+    again, in pieces of 1 GiB: less memory, one rounding, no gradients of a loss that is only looked at,
+    for one product more beside a step's three."""
     ops._reduction(reduction)
     _two_dims(weight=weight)
     if labels.shape != x.shape[:-1]:
@@ -272,20 +279,22 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction="mean")
         lambda x, w, labels, reduction, gx, gw: ops.linear_ce_step(x, w, labels, reduction, ignore, gx, gw),
         lambda x, w, labels, lse, grad, reduction, gx, gw: ops.linear_ce_bwd(
             x, w, labels, lse, grad, reduction, ignore, gx, gw))
-    if not ops.vocab_step_fits(labels.numel(), weight.shape[0], H):
+    if recompute or not ops.vocab_step_fits(labels.numel(), weight.shape[0], H):
         calls = calls[0], None, calls[2]
     loss = _VocabLossFunction.apply(calls, torch.is_grad_enabled(), reduction, _rows(x, H),
                                     _rows(weight, weight.shape[-1]), _keys(labels))
     return loss.reshape(labels.shape) if reduction == "none" else loss
 
 
-def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, reduction="mean"):
+def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=1.0, reduction="mean",
+                   recompute=False):
     """Distillation on the teacher's distribution over the vocabulary: KL(p, q) with
     p = softmax(teacher_x teacher_weight^T / temperature), q = softmax(x weight^T / temperature), without
     the logits. x bf16 [..., H], weight bf16 [V, H]; teacher_x bf16 [..., Ht], teacher_weight bf16
     [V, Ht], which get no gradient (a frozen head that both sides share is given twice); mask bool
     [...]: rows that it leaves out take no part (whatever they hold; their gradient is 0). Returns as
-    linear_cross_entropy does; the loss is not multiplied by temperature^2."""
+    linear_cross_entropy does; the loss is not multiplied by temperature^2. recompute: as there; the
+    forward of a mean or sum takes 10 bytes a logit without it, a piece of 1 GiB with it."""
     ops._reduction(reduction)
     _two_dims(weight=weight, teacher_weight=teacher_weight)
     if teacher_x.shape[:-1] != x.shape[:-1] or (mask is not None and mask.shape != x.shape[:-1]):
@@ -297,7 +306,7 @@ def linear_distill(x, weight, teacher_x, teacher_weight, mask=None, temperature=
             x, w, tx, tw, reduction, mask, T, gx, gw),
         lambda x, w, tx, tw, mask, lse, grad, reduction, gx, gw: ops.linear_kl_bwd(
             x, w, tx, tw, lse, grad, reduction, mask, T, gx, gw))
-    if not ops.vocab_step_fits(N, weight.shape[0], H, Ht):
+    if recompute or not ops.vocab_step_fits(N, weight.shape[0], H, Ht):
         calls = calls[0], None, calls[2]
     loss = _VocabLossFunction.apply(
         calls, torch.is_grad_enabled(), reduction, _rows(x, H), _rows(weight, weight.shape[-1]),

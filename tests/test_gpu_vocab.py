@@ -927,3 +927,61 @@ def test_the_greatest_gradients_over_pieces(ops, kind):
     else:
         ref = reference(x[at], w, tx=tx[at], tw=tw, top=True)
         check_rows(two_calls_kl(ops, x, w, tx, tw, keep), ref, at)
+
+
+# ---- the logits computed again instead of what a step keeps ----------------------------------------------
+@pytest.mark.parametrize("N,part,D", [(13, 13, 64), (300, 200, 200), (700, 520, 520)])
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_recompute_rounds_once(F, N, part, D, kind):
+    """Gradients for an upstream gradient of 0.37: those of every row's loss times 0.37 over the rows, rounded
+    once (what the forward computed would be rounded before, too)."""
+    at = torch.randperm(N, generator=torch.Generator().manual_seed(N)).sort().values[-part:].cuda()
+    x, w, tx, tw, labels, keep = single_terms(N, D, at, N + part)
+    up = torch.full((part,), 0.37 / part, device="cuda", dtype=torch.float64)
+    kw = dict(labels=labels[at]) if kind == "ce" else dict(tx=tx[at], tw=tw)
+    ref = reference(x[at], w, reduction="none", upstream=up, top=True, **kw)
+    mean = reference(x[at], w, **kw)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    if kind == "ce":
+        loss = F.linear_cross_entropy(a, b, labels, recompute=True)
+    else:
+        loss = F.linear_distill(a, b, tx, tw, mask=keep, recompute=True)
+    close(loss.detach(), mean["loss"], mean["loss_tol"], "loss")
+    for _ in range(2):  # a second backward is the same
+        gx, gw = torch.autograd.grad(loss, (a, b), torch.tensor(0.37, device="cuda"), retain_graph=True)
+        # (0.37 in fp32, and over the rows: two roundings more)
+        close(gx[at], ref["gx"], ref["gx_tol"] + 2.0 ** -22 * ref["gx"].abs(), "grad_x")
+        close(gw, ref["gw"], ref["gw_tol"] + 2.0 ** -22 * ref["gw"].abs(), "grad_weight")
+
+
+@pytest.mark.parametrize("kind", ["ce", "kl"])
+def test_recompute_takes_a_piece_of_memory(F, ops, kind):
+    """4096 rows of 150000 words: 1.1 GiB kept by a step (5.7 a distillation's), 1 GiB in pieces, and nothing
+    but the rows' normalisers from the forward to the backward."""
+    N, V, H = 4096, 150000, 64
+    x, w, labels = inputs(N, V, H, seed=90, ignored=0.1)
+    tx = x.flip(0).contiguous()
+    assert ops.vocab_step_fits(N, V, H, 0 if kind == "ce" else H)
+
+    def peaks(recompute):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        if kind == "ce":
+            loss = F.linear_cross_entropy(a, b, labels, recompute=recompute)
+        else:
+            loss = F.linear_distill(a, b, tx, w, mask=labels != -100, recompute=recompute)
+        forward = torch.cuda.max_memory_allocated() - before
+        held = torch.cuda.memory_allocated() - before
+        grads = torch.autograd.grad(loss, (a, b))
+        return (loss.detach(), *grads), forward, held, torch.cuda.max_memory_allocated() - before
+
+    want, forward, held, _ = peaks(False)
+    got, less, row, peak = peaks(True)
+    gib = 2 ** 30
+    assert forward > (1.1 if kind == "ce" else 5.7) * gib and held > 2 * (w.numel() + x.numel())
+    assert less < (0.1 if kind == "ce" else 1.1) * gib and row < 64 * N and peak < 1.2 * gib
+    ref = dict(labels=labels) if kind == "ce" else dict(tx=tx, tw=w, mask=labels != -100)
+    check(want, reference(x, w, **ref))
+    check(got, reference(x, w, kept=False, **ref))

@@ -985,3 +985,17 @@ def test_recompute_takes_a_piece_of_memory(F, ops, kind):
     ref = dict(labels=labels) if kind == "ce" else dict(tx=tx, tw=w, mask=labels != -100)
     check(want, reference(x, w, **ref))
     check(got, reference(x, w, kept=False, **ref))
+
+
+def test_a_loss_beyond_a_step_s_limit(F, ops):
+    """The mean and sum of a distillation of more rows than a step keeps: pieces of the vocabulary through
+    autograd, for an upstream gradient that is no power of two."""
+    N, V, H = 16384, 60001, 64
+    assert not ops.vocab_step_fits(N, V, H, H)
+    x, w, labels = inputs(N, V, H, seed=91, ignored=0.3)
+    tx, mask = (x.float() * 0.8).bfloat16(), labels != -100
+    for reduction, up in (("mean", 3.0), ("sum", 0.37)):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = F.linear_distill(a, b, tx, w, mask=mask, reduction=reduction)
+        grads = torch.autograd.grad(loss, (a, b), torch.tensor(up, device="cuda"))
+        check((loss.detach(), *grads), reference(x, w, tx=tx, tw=w, mask=mask, reduction=reduction, upstream=up))

@@ -61,7 +61,7 @@ __device__ __forceinline__ float h2f(uint32_t b) {
 // Raw buffer loads: a resource covering [p, p + bytes); a lane whose offset is out of range
 // reads zeros (the hardware range check), which replaces per-lane branches.
 typedef __amdgpu_buffer_rsrc_t BufRsrc;
-constexpr uint32_t kBufOob = 0x80000000u;  // an offset past any buffer this library builds
+constexpr uint32_t kBufOob = 0x80000000u;  // an offset past any buffer of up to 2 GiB
 __device__ __forceinline__ BufRsrc make_rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes,
                                            0x00020000);

@@ -1305,13 +1305,15 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
 }
 
 // A Col tile's copies of p[r][H] whose columns past H are out of the buffer, and so zero, as the rows
-// past rtotal
+// past rtotal. p may be of up to 4 GiB (less 16 bytes: rows are of whole 16), which kBufOob lies within.
+// (Only the power goes by it: what the columns past H give is stored nowhere.)
+constexpr uint32_t kPastAll = 0xfffffff0u;
 __device__ __forceinline__ TileDma col_tile_zero(const uint16_t* p, int64_t H, int64_t col0, int64_t rtotal) {
   TileDma d = col_tile_dma(p, H, col0, H, rtotal);
 #pragma unroll
   for (int it = 0; it < COPY_INSTS; ++it) {
     const int pch = it * NTHR + threadIdx.x;
-    if (col0 + (((pch & 31) ^ col_swz(pch >> 5)) * 8) >= H) d.off[it] = kBufOob;
+    if (col0 + (((pch & 31) ^ col_swz(pch >> 5)) * 8) >= H) d.off[it] = kPastAll;
   }
   return d;
 }

@@ -987,15 +987,53 @@ def test_recompute_takes_a_piece_of_memory(F, ops, kind):
     check(got, reference(x, w, kept=False, **ref))
 
 
-def test_a_loss_beyond_a_step_s_limit(F, ops):
-    """The mean and sum of a distillation of more rows than a step keeps: pieces of the vocabulary through
-    autograd, for an upstream gradient that is no power of two."""
-    N, V, H = 16384, 60001, 64
-    assert not ops.vocab_step_fits(N, V, H, H)
+@pytest.mark.parametrize("kind,N,V", [("kl", 16384, 60001), ("ce", 33000, 66001)])
+def test_a_loss_beyond_a_step_s_limit(F, ops, kind, N, V):
+    """The mean and sum of more logits than a step keeps: pieces of the vocabulary through autograd, for an
+    upstream gradient that is no power of two."""
+    H = 64
+    assert not ops.vocab_step_fits(N, V, H, H if kind == "kl" else 0)
     x, w, labels = inputs(N, V, H, seed=91, ignored=0.3)
     tx, mask = (x.float() * 0.8).bfloat16(), labels != -100
     for reduction, up in (("mean", 3.0), ("sum", 0.37)):
         a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
-        loss = F.linear_distill(a, b, tx, w, mask=mask, reduction=reduction)
+        if kind == "kl":
+            loss, ref = F.linear_distill(a, b, tx, w, mask=mask, reduction=reduction), dict(tx=tx, tw=w, mask=mask)
+        else:
+            loss, ref = F.linear_cross_entropy(a, b, labels, reduction=reduction), dict(labels=labels, kept=False)
         grads = torch.autograd.grad(loss, (a, b), torch.tensor(up, device="cuda"))
-        check((loss.detach(), *grads), reference(x, w, tx=tx, tw=w, mask=mask, reduction=reduction, upstream=up))
+        check((loss.detach(), *grads), reference(x, w, reduction=reduction, upstream=up, **ref))
+
+
+def test_a_step_of_a_head_past_two_gib(F, ops):
+    """Offsets of the head's copies pass 31 bits, and its last tile of columns is not whole."""
+    N, V, H = 130, 240007, 4504
+    assert V * H * 2 > 2 ** 31 and H % 256 and ops.vocab_step_fits(N, V, H)
+    g = torch.Generator(device="cuda").manual_seed(92)
+    w = torch.empty(V, H, dtype=torch.bfloat16, device="cuda").normal_(0, 0.03, generator=g).requires_grad_()
+    x = torch.randn(N, H, generator=g, device="cuda").bfloat16().requires_grad_()
+    labels = torch.randint(0, V, (N,), generator=g, device="cuda")
+    labels[-1] = V - 1
+    loss = F.linear_cross_entropy(x, w, labels, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    with torch.no_grad():
+        cuts = range(0, V, 40000)
+        z = torch.cat([x.double() @ w[c:c + 40000].double().T for c in cuts], 1)
+        # of a logit: products of magnitudes of at most this sum, and the normaliser's
+        off = (H + 4) * 2.0 ** -24 * float((x.double().abs().sum(1) * float(w.abs().max())).max())
+        lse = torch.logsumexp(z, 1)
+        rows = lse - z[torch.arange(N), labels]
+        tol = 2 * off + (200 + V // 128) * 2.0 ** -24 + 8 * 2.0 ** -24 * lse.abs()
+        assert abs(float(loss) - float(rows.sum())) <= float(tol.sum()) + 2 * 2.0 ** -24 * float(rows.sum())
+        dz = torch.exp(z - lse[:, None])
+        dz[torch.arange(N), labels] -= 1
+        # rounded to bf16, kept in fp16 before, from logits and normalisers that are off
+        dz_tol = dz.abs() * (2.0 ** -8 + 2.0 ** -11 + 3 * off + 2 * float(tol.max())) + 2.0 ** -40
+        want, bound = (torch.zeros_like(x, dtype=torch.float64) for _ in range(2))
+        for c in cuts:
+            d, t, wd = dz[:, c:c + 40000], dz_tol[:, c:c + 40000], w[c:c + 40000].double()
+            want += d @ wd
+            bound += (t + V * 2.0 ** -24 * d.abs()) @ wd.abs()
+            e, te = d.T @ x.double(), (t + (N + 64) * 2.0 ** -24 * d.abs()).T @ x.double().abs()
+            close(gw[c:c + 40000], e, te + (2.0 ** -8 + 2.0 ** -20) * (e.abs() + te), f"grad_weight from {c}")
+        close(gx, want, bound + (2.0 ** -8 + 2.0 ** -20) * (want.abs() + bound), "grad_x")

@@ -1,4 +1,4 @@
-// Losses over a large vocabulary from hidden states and head weights, without keeping the logits:
+// Losses over a large vocabulary from hidden states and head weights, no logits kept beyond a call:
 //
 //   z = x W^T                               x bf16 [N, H], W bf16 [V, H], fp32 sums
 //   cross entropy   loss_n = log sum_v exp z_nv - z_n,label
@@ -15,8 +15,9 @@
 // (8 bytes a row and 256 words) and joins them in a second kernel, in 64 bits. The backward computes
 // the logits of a piece of the vocabulary again, now with the rows' normalisers at hand, rounds dz to
 // bf16 into a workspace dz^T [words, rows] of at most kPieceBytes, and multiplies it with x (dW of the
-// piece) and with W (dx, its fp32 parts summed over pieces and splits in a fixed order). The scale of
-// a mean and of its gradient is applied to the fp32 sums, not to dz: it would be rounded with it.
+// piece) and with W (dx, its fp32 parts summed over pieces and splits in a fixed order). What rounding
+// the greatest dz of each row leaves, of few rows every dz, is added to both products. The scale of a
+// mean and of its gradient is applied to the fp32 sums, not to dz: it would be rounded with it.
 //
 // A sum or mean whose logits are few enough has its gradients with the forward (step): the tiles keep
 // what dz is made of and a memory-bound pass makes dz of it once the normalisers are known, instead of
@@ -37,9 +38,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dz, and of the logits of a piece
 constexpr size_t kKeepBytes = (size_t)8 << 30;   // of what a step keeps
 // Exponentials relative to the tile's maximum are kept in fp16 times this: the greatest is then 2^15, and
-// those from 2^-29 on are normal, off by 2^-11 of their own value, an eighth of what the rounding of dz to
-// bf16 may be off (as they are, from 2^-14 on: beside a word of probability 1 those of 10^-6 were off by
-// 3%). Below, by 2^-40 of the tile's maximum.
+// those from 2^-29 on are normal, off by 2^-11 of their own value, an eighth of what rounding dz, or the
+// gradient, to bf16 may be off (as they are, from 2^-14 on: beside a word of probability 1 those of 10^-6
+// were off by 3%). Below, by 2^-40 of the tile's maximum. (The label's dz comes from its logit in fp32.)
 constexpr float kKeptScale = 32768.f;
 constexpr size_t kLdsLogits = 2 * 2 * TILE_BYTES + 8192;  // two stages and the statistics' exchange
 constexpr size_t kLdsRing = RING_SLOTS * TILE_BYTES;
@@ -375,10 +376,15 @@ __global__ __launch_bounds__(NTHR) void logits_kernel(const LogitArgs a) {
   const int tiles_i = (int)((a.v1 - a.v0 + TILE - 1) / TILE), tiles_j = (rows + TILE - 1) / TILE;
   const int64_t total = (int64_t)tiles_i * tiles_j;
   // Every XCD walks a run of its own, four tiles of words at a time over the rows, of one side after the
-  // other. Both sides' logits are stored: with 8 or 16 tiles of rows its 32 workgroups would then start
-  // and store their tiles in step, so there it is six (two sides of 2048 rows of 151936 x 2560 3.54 and
-  // 3.36 ms, 1024 rows 1.84 and 1.80, 4096 6.72 and 6.62; but of 1792 rows 2.88 and 2.95, of 2816 4.49 and
-  // 4.60, and a cross entropy's 4096 2.62 and 2.63).
+  // other. Both sides' logits are stored: with 4, 8 or 16 tiles of rows its 32 workgroups would then start
+  // and store their tiles in step, so there it is six. With four and with six, ms of both sides' logits and
+  // the pass over them:  151936 x 2560  151936 x 1024  50257 x 1600  32000 x 2560  128256 x 4096
+  //   1024 rows           1.80  1.75     1.04  0.97     0.440  0.438  0.360  0.357   2.12   2.13
+  //   2048                3.53  3.36     2.08  1.91     0.846  0.814  0.721  0.710   4.07   4.08
+  //   4096                6.69  6.63     3.90  3.78     1.61   1.56   1.41   1.39    7.91   7.88
+  //   1280                2.12  2.13     1.24  1.25     0.533  0.532  0.448  0.453   2.59   2.60
+  //   1792                2.88  2.94     1.64  1.70     0.711  0.725  0.619  0.624   3.52   3.63
+  // (2560 rows would be 0 to 4% faster with six, and a cross entropy's 4096 are not: 2.62 and 2.63.)
   const int group = MODE == Z_KEEP && tiles_j % 4 == 0 ? 6 : 4;
   const int xcd = blockIdx.x % 8, step = gridDim.x / 8;
   const int64_t begin = total * xcd / 8, run = total * (xcd + 1) / 8 - begin;
@@ -610,7 +616,7 @@ constexpr int few_stage() { return (kFewWords + 32 * NB) * BK * 2; }
 
 // acc[word, row] of the wave's 32 words and 32 NB rows of x, the copies' row i of 32 NB being
 // row_of(i) (none, < 0: zeros); of the tile's 128 words, nw exist, of x's rows nx
-template <int MODE, int NB, typename Row>
+template <int NB, typename Row>
 __device__ __forceinline__ void few_tile(lds_u8* lbase, const uint16_t* w, const uint16_t* x, int64_t H,
                                          int nw, int nx, Row&& row_of, f32x16 (&acc)[NB], int wave,
                                          int lane) {
@@ -688,9 +694,9 @@ __device__ __forceinline__ int kth_row(uint64_t m0, uint64_t m1, int k) {
 }
 
 // GATHER (up to 128 rows, x as it came, no dW): every wave finds the rows that take part from the
-// keys itself and the copies pick them out, instead of a launch that packs them (17 rows of 32000 x 1024
-// 23.2 -> 20.9 us a call, 16 of 151936 x 2560 149 -> 142); one workgroup
-// more leaves what the other kernels need.
+// keys itself and the copies pick them out, instead of a launch that packs them (losses alone of 17 rows of
+// 32000 x 1024 23.2 -> 20.9 us a call, of 16 of 151936 x 2560 149 -> 142); one workgroup more leaves what
+// the other kernels need.
 template <int MODE, int NB, bool GATHER>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, const PackArgs k) {
   extern __shared__ uint4 smem[];
@@ -752,10 +758,10 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
       lab[i] = GATHER ? label_of(k, kth_row(m0, m1, n)) : a.lab[j0 + n];
   }
   if constexpr (GATHER)
-    few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side], H, nw, (int)k.N,
+    few_tile<NB>(lbase, a.w[side] + i0 * H, a.x[side], H, nw, (int)k.N,
                        [&](int i) { return kth_row(m0, m1, i); }, acc, wave, lane);
   else
-    few_tile<MODE, NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, 32 * NB,
+    few_tile<NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, 32 * NB,
                        [](int i) { return i; }, acc, wave, lane);
 
   // The wave's 32 words of the panel's block, 16 a lane: word vl + 8 (e / 4) + e % 4 of the tile.
@@ -1492,7 +1498,8 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
   const Item item = map_item(T, false, 0, 1, (int)blockIdx.x % T, (int)blockIdx.x / T, z);
   const int zsl = item.zsl;
   int tile_i, tile_j;
-  // (two tiles of rows at a time: 2.67 ms for 3890 rows of 151936 x 2560, 1 2.72, 3 2.67, 4 2.70, 5 2.71)
+  // (two tiles of rows at a time; 1, 2 and 4 are within 1% of each other at six shapes of 1000 to 3890 rows
+  // and 32000 x 1024 to 128256 x 4096)
   tile_coords(2, tiles_i, tiles_j, item.bid, tile_i, tile_j);
   const int64_t i0 = (int64_t)tile_i * TILE, j0 = (int64_t)tile_j * TILE;
   const int64_t rbeg = (int64_t)zsl * split, rend = min(a.words, rbeg + split);
@@ -1618,8 +1625,9 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // the copies of dx address, the pieces of one size but for the last tiles.
 static int64_t piece_words(int64_t N, int64_t V, int64_t H, int bytes) {
   const int64_t tiles = up(V, TILE) / TILE;
-  int64_t most = std::min((int64_t)(kPieceBytes / bytes) / std::max(up(N, TILE), (int64_t)1), (((int64_t)1 << 31) - 1) / H) / TILE;
-  most = std::max(most, (int64_t)1);
+  const int64_t held = (int64_t)(kPieceBytes / bytes) / std::max(up(N, TILE), (int64_t)1);
+  const int64_t addressed = (((int64_t)1 << 31) - 1) / H;
+  const int64_t most = std::max(std::min(held, addressed) / TILE, (int64_t)1);
   const int64_t pieces = (tiles + most - 1) / most;
   return (tiles + pieces - 1) / pieces * TILE;
 }
@@ -1730,7 +1738,8 @@ static int check(const Sides& s, bool kl, const char* what) {
   PLZ_REQUIRE(s.H % 8 == 0 && s.Ht % 8 == 0, "%s: hidden widths must be multiples of 8", what);
   const int64_t lim = (int64_t)1 << 31;
   if (up(s.N, TILE) * s.H >= lim || up(s.N, TILE) * s.Ht >= lim || s.V >= lim - TILE ||
-      s.N >= ((int64_t)1 << 22) || std::max(s.H, s.Ht) >= ((int64_t)1 << 22) || up(s.N, TILE) / TILE * (up(s.V, TILE) / TILE) >= lim) {
+      s.N >= ((int64_t)1 << 22) || std::max(s.H, s.Ht) >= ((int64_t)1 << 22) ||
+      up(s.N, TILE) / TILE * (up(s.V, TILE) / TILE) >= lim) {
     set_error("%s: 2^31 values of x, words or tiles, 2^22 rows or a width of 2^22, or more", what);
     return PLZ_EUNSUPPORTED;
   }

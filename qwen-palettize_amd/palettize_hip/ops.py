@@ -1208,8 +1208,9 @@ def _kept(t, name, *shape):
 def linear_ce_fwd(x, weight, labels, ignore_index=-100, total=True):
     """Cross entropy of labels (int64 or int32 [N]) under softmax(x weight^T), x bf16 [N, H], weight
     bf16 [V, H], without the logits: (loss fp32 [N], lse fp32 [2, N] for the backward (the normalisers and
-    what rounding them to fp32 left), total fp32 [3] = sum, mean over the rows that take part (0 without one) and their number, or None). Rows whose label
-    is ignore_index take no part: loss 0. Another label outside [0, V) gives NaN."""
+    what rounding them to fp32 left), total fp32 [3] = sum, mean over the rows that take part (0 without
+    one) and their number, or None). Rows whose label is ignore_index take no part: loss 0. Another label
+    outside [0, V) gives NaN."""
     N, V, H = _head(x, weight)
     size = _labels(labels, N)
     dev = _one_device("linear_ce_fwd", x, weight, labels)

@@ -1534,10 +1534,10 @@ __global__ __launch_bounds__(NTHR) void dx_kernel(const DxArgs a) {
             ex[i * (NTHR / 2)] = f32x4{t[e], t[e + 1], t[e + 2], t[e + 3]};
           } else {
             const f32x4 v = ex[i * (NTHR / 2)];
-            t[e] += v[0];
-            t[e + 1] += v[1];
-            t[e + 2] += v[2];
-            t[e + 3] += v[3];
+            // Of an infinite weight the second part, 0 or of the other sign, would make NaN of the first's
+            // infinity; there the first has it all.
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[e + k] += fabsf(v[k]) < INFINITY ? v[k] : 0.f;
           }
         }
       }
@@ -1592,7 +1592,8 @@ __global__ __launch_bounds__(256) void dx_sum_kernel(const float* __restrict__ p
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = at[i] >= 0 ? top[4 * q + i] : -1;
-      if (t >= 0) left[i] = low[4 * q + i] * bf2f(w[(int64_t)t * H + h]);
+      const float l = t >= 0 ? low[4 * q + i] * bf2f(w[(int64_t)t * H + h]) : 0.f;
+      left[i] = fabsf(l) < INFINITY ? l : 0.f;  // (as dx_kernel's second parts)
     }
   }
   f32x4 a = {};

@@ -1037,3 +1037,44 @@ def test_a_step_of_a_head_past_two_gib(F, ops):
             e, te = d.T @ x.double(), (t + (N + 64) * 2.0 ** -24 * d.abs()).T @ x.double().abs()
             close(gw[c:c + 40000], e, te + (2.0 ** -8 + 2.0 ** -20) * (e.abs() + te), f"grad_weight from {c}")
         close(gx, want, bound + (2.0 ** -8 + 2.0 ** -20) * (want.abs() + bound), "grad_x")
+
+
+@pytest.mark.parametrize("N,part", [(5, 5), (100, 100), (300, 90), (300, 300)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_label_that_cannot_be(F, N, part, reduction):
+    """A label whose logit is minus infinity, of one row: its loss and its gradient along the infinite weight
+    are infinite, as the formula's are (dz is -1 there and 0 elsewhere; 0 times infinity is NaN in the other
+    rows, as it is in any product)."""
+    V, H, dead, row = 700, 64, 301, 3
+    x, w, labels = inputs(N, V, H, seed=95)
+    labels[part:] = -100
+    x[:, 0] = 1
+    labels[labels == dead] = 5
+    labels[row] = dead
+    w[dead] = 0
+    w[dead, 0] = -float("inf")
+    loss, gx, gw = run_ce(F, x, w, labels, reduction)
+    assert float(loss if reduction == "mean" else loss[row]) == float("inf")
+    assert float(gx[row, 0]) == float("inf") and torch.isfinite(gx[row, 1:]).all()
+    others = torch.arange(part, device="cuda") != row
+    assert torch.isnan(gx[:part][others][:, 0]).all() and torch.isfinite(gx[:part, 1:]).all()
+    assert torch.isfinite(gw).all()
+
+
+@pytest.mark.parametrize("N,part", [(5, 5), (100, 100), (300, 90), (300, 300)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_word_that_only_the_student_cannot_say(F, N, part, reduction):
+    """Its logit is minus infinity, the teacher's is not: infinite losses, and gradients of -p times minus
+    infinity along the infinite weight."""
+    V, H, dead = 700, 64, 301
+    x, w, _ = inputs(N, V, H, seed=96)
+    tx, tw, _ = inputs(N, V, H, seed=97)
+    mask = torch.arange(N, device="cuda") < part
+    x[:, 0] = 1
+    w[dead] = 0
+    w[dead, 0] = -float("inf")
+    tx[:, 1], tw[dead, 1] = 1, 8.0  # the teacher's likeliest word, so the greatest gradient of each row
+    loss, gx, gw = run_kl(F, x, w, tx, tw, reduction, mask=mask)
+    assert bool((loss if reduction == "mean" else loss[:part] == float("inf")).all())
+    assert bool((gx[:part, 0] == float("inf")).all()) and torch.isfinite(gx[:part, 1:]).all()
+    assert torch.isfinite(gw).all() and not gx[part:].any()

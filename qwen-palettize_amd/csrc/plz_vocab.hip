@@ -759,10 +759,10 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(const LogitArgs a, con
   }
   if constexpr (GATHER)
     few_tile<NB>(lbase, a.w[side] + i0 * H, a.x[side], H, nw, (int)k.N,
-                       [&](int i) { return kth_row(m0, m1, i); }, acc, wave, lane);
+                 [&](int i) { return kth_row(m0, m1, i); }, acc, wave, lane);
   else
     few_tile<NB>(lbase, a.w[side] + i0 * H, a.x[side] + j0 * H, H, nw, 32 * NB,
-                       [](int i) { return i; }, acc, wave, lane);
+                 [](int i) { return i; }, acc, wave, lane);
 
   // The wave's 32 words of the panel's block, 16 a lane: word vl + 8 (e / 4) + e % 4 of the tile.
   const int vl = 32 * wave + 4 * (lane >> 5);
